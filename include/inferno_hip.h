@@ -441,6 +441,149 @@ int ihip_spec_commit_state(void *state_dev, const void *snap_dev, size_t bytes,
 int ihip_spec_advance_len(int32_t *len_dev, const int32_t *n_accepted_dev,
                           int steps, void *stream);
 
+/* ---- token mixers: what stands between the projections of a layer
+ *      (csrc/rope.hip, csrc/attn.hip, csrc/delta.hip) ---- */
+
+/* Types of a KV cache (GGML ids, src/GGUF.jl:25-60). */
+#define IHIP_F16   1
+#define IHIP_BF16 30
+
+/* A KV cache: n_seq sequences of `capacity` entries, n_kv heads of head_dim
+ * values of `type`. Entry t of head h of sequence s starts seq_stride s +
+ * tok_stride t + head_stride h values behind k (and behind v); an entry's
+ * values are contiguous. k and v are 16-byte aligned, the strides multiples
+ * of 8 values; they may be of either order ([S, cap, heads, D] or [S, heads,
+ * cap, D]) and pass 32 bits. The reference keeps an fp32 cache per layer
+ * (src/ModelCPU.jl:234-258). */
+typedef struct ihip_kv {
+    int type;            /* IHIP_F16 / IHIP_BF16 */
+    int n_seq, n_kv, head_dim;
+    int64_t capacity;
+    void *k, *v;         /* device */
+    int64_t seq_stride, tok_stride, head_stride;
+} ihip_kv;
+
+/* Rotary positions (the reference's partial RoPE: src/ModelCPU.jl:125-231).
+ * The first rot_dim values of a head are rotated by pairs, pair i by the
+ * angle pos theta_i, theta_i = base^(-2 i / rot_dim): values (i, i + rot_dim /
+ * 2), or (2 i, 2 i + 1) with `interleaved`; both results are multiplied by
+ * mscale, and the values past rot_dim are left as they are. Scaled positions:
+ *   IHIP_ROPE_LINEAR:   theta_i / factor;
+ *   IHIP_ROPE_BY_PARTS: r = orig_len theta_i / (2 pi) turns over the length
+ *     the model was trained on; keep = clamp((r - beta_slow) / (beta_fast -
+ *     beta_slow), 0, 1); theta_i' = theta_i (keep + (1 - keep) / factor).
+ * freq_factors_dev (a device array [rot_dim / 2], NULL: none; a GGUF file's
+ * rope_freqs) divides each theta_i; not with IHIP_ROPE_BY_PARTS.
+ * Angles are formed in fp64 and reduced to a turn before sine and cosine, so
+ * far positions lose nothing. ihip_rope_init fills the caller's ihip_rope
+ * (host memory, kept with the model; no GPU work); the calls below copy it
+ * into the kernel's arguments. rot_dim is even, 2 .. min(head_dim, 256). */
+#define IHIP_ROPE_PLAIN    0
+#define IHIP_ROPE_LINEAR   1
+#define IHIP_ROPE_BY_PARTS 2
+typedef struct ihip_rope {
+    int head_dim, rot_dim, interleaved;
+    float mscale;
+    const float *freq_factors; /* device, or NULL */
+    double turns[128];         /* theta_i' / (2 pi) */
+} ihip_rope;
+int ihip_rope_init(ihip_rope *rope, int head_dim, int rot_dim, int interleaved,
+                   double base, int scaling, double factor, double orig_len,
+                   double beta_fast, double beta_slow, double mscale,
+                   const float *freq_factors_dev);
+
+/* y[t, h] = x[t, h] rotated to position pos_dev[t], t < tokens, h < heads:
+ * fp32 rows of heads x head_dim values, ldx / ldy values between rows. In
+ * place where y == x and ldy == ldx; else the rows do not overlap. */
+int ihip_rope_apply(const ihip_rope *rope, const float *x_dev, int64_t ldx,
+                    float *y_dev, int64_t ldy, int heads,
+                    const int32_t *pos_dev, int tokens, void *stream);
+
+/* The new tokens' [q; k; v] rows (row s M + m: token m of sequence s; n_q +
+ * 2 n_kv heads of head_dim, ld values between rows): q rotated into q_out
+ * (rows of n_q heads, ldq values apart; q_out == qkv with ldq == ld rotates
+ * in place), k rotated and v as it is into the cache's entry len_dev[s] + m,
+ * rounded once to its type. The position is pos_dev[s M + m], or pos0 +
+ * len_dev[s] + m with pos_dev NULL (pos0: the length of a shared prefix).
+ * A sequence with len_dev[s] < 0 is idle: its rows and cache stay as they
+ * were. One whose M entries do not fit its capacity gets NaN rows of q_out,
+ * and its cache stays as it was (the lengths are read on the device, so that
+ * a captured step can follow ihip_spec_advance_len). Counts of rows x heads
+ * and pointers as in ihip_kv; the KV write of src/ModelCPU.jl:245-258. */
+int ihip_rope_append(const ihip_rope *rope, const float *qkv_dev, int64_t ld,
+                     float *q_out_dev, int64_t ldq, int n_q,
+                     const ihip_kv *cache, const int32_t *len_dev,
+                     const int32_t *pos_dev, int pos0, int M, void *stream);
+
+/* Attention of each sequence's M new tokens (rows s M + m of q and out: n_q
+ * heads of the cache's head_dim, fp32, ldq / ldo values between rows; query
+ * head h reads key head h / (n_q / n_kv)) over
+ *   every entry of `prefix` (NULL: none): one sequence that all share, whose
+ *     capacity is its length; it is read once for all rows, not once each;
+ *   the entries [0, len_dev[s]) of the sequence's own cache;
+ *   the new entries len_dev[s] + j (already appended): j <= m, or, with
+ *     tree_mask_dev [n_seq x M] (M <= 64), those whose bit j is set in
+ *     tree_mask_dev[s M + m] (a draft tree: the node's ancestors and itself).
+ * out = sum_j p_j v_j, p the softmax of scale q.k_j over the entries seen, in
+ * fp32 accuracy: the queries and probabilities meet the 16-bit cache as two
+ * (f16) or three (bf16) limbs on the matrix cores, statistics and sums are
+ * fp32. A row that sees nothing is zero. Entries a row does not see have no
+ * effect on it, NaN and infinities included; a row that sees a non-finite
+ * score or value gets a non-finite result there. A sequence with len_dev[s]
+ * < 0 is idle (its rows of out stay as they were); one with len_dev[s] + M >
+ * capacity gets NaN rows. head_dim 64, 128 or 256. q and out 16-byte aligned,
+ * ldq and ldo multiples of 4. Results do not depend on what runs beside the
+ * call (no atomics). ws: ihip_attn_prefix_ws_bytes, 16-byte aligned, not
+ * shared by calls that overlap in time. Replaces the cached attention of
+ * src/ModelCPU.jl:730-856 for the tokens of a verify step. */
+int ihip_attn_prefix_ws_bytes(int n_q, int M, const ihip_kv *cache,
+                              const ihip_kv *prefix, size_t *bytes);
+int ihip_attn_prefix(const float *q_dev, int64_t ldq, float *out_dev,
+                     int64_t ldo, int n_q, int M, const ihip_kv *cache,
+                     const int32_t *len_dev, const ihip_kv *prefix,
+                     const uint64_t *tree_mask_dev, float scale, void *ws,
+                     size_t ws_bytes, void *stream);
+
+/* The gated delta rule (the recurrent layers of the hybrid model,
+ * src/ModelCPU.jl:476-700) for T tokens of each of n_seq sequences. Per value
+ * head, S [dk x dv] its state, for t = 0 .. T-1:
+ *   S  = exp(g_t) S
+ *   S += k_t (beta_t (v_t - S^T k_t))^T
+ *   o_t = scale S^T q_t
+ * with the q and k of key head h / (n_v / n_k); with IHIP_DELTA_L2NORM q and k
+ * are first divided by sqrt(sum x^2 + 1e-6). Row s T + t holds token t of
+ * sequence s: heads of dk (q, k) or dv (v, o) values, ldq .. ldo values
+ * between rows; g and beta one value a head, ldg and ldb between rows. The
+ * states [n_seq][n_v][dk][dv] are contiguous: state_in (NULL: zeros),
+ * state_out (the last one; NULL: not kept; may be state_in), snap_out [n_seq]
+ * [T][n_v][dk][dv] (the state after every token, what ihip_spec_commit_state
+ * picks from; NULL: not kept; T <= 64). len_dev (NULL: T for all): tokens of
+ * each sequence, clamped to T; o and snapshots past them are left as they
+ * were, and with 0 or less state_out is state_in. All fp32. dk 64 or 128, dv
+ * a multiple of 4 up to 512; pointers 16-byte aligned (g and beta: 4), ld's
+ * multiples of 4 (ldg, ldb: any). o may not overlap the inputs. ws:
+ * ihip_delta_ws_bytes, 16-byte aligned, not shared by calls that overlap in
+ * time. Few tokens (and every call with snapshots) go one by one; many go in
+ * chunks of 64 on the matrix cores, where each chunk's tokens become one
+ * triangular system (fp32 accuracy both ways). */
+#define IHIP_DELTA_L2NORM 1
+typedef struct ihip_delta {
+    const float *q, *k, *v, *g, *beta;
+    int64_t ldq, ldk, ldv, ldg, ldb;
+    float *o;
+    int64_t ldo;
+    const float *state_in;
+    float *state_out, *snap_out;
+    const int32_t *len;
+    int n_seq, T, n_k, n_v, dk, dv;
+    float scale;
+    int flags;
+} ihip_delta;
+int ihip_delta_ws_bytes(int n_seq, int T, int n_k, int n_v, int dk, int dv,
+                        int snapshots, size_t *bytes);
+int ihip_gated_delta_rule(const ihip_delta *a, void *ws, size_t ws_bytes,
+                          void *stream);
+
 /* ---- draft-side sampler (csrc/sample.hip) ---- */
 
 /* softmax_sample (src/ModelCPU.jl:1123-1200) on each row of logits

@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -13,6 +14,7 @@
 
 #include "../../include/inferno_hip.h"
 #include "chain.h"
+#include "mixer.h"
 
 // kernels (gemm.hip, dequant.hip, accept.hip, misc.hip)
 hipError_t launch_gemm(int qt, const void *W, const float *X, float *Y, int M, int N, int K, int flags, void *ws,
@@ -68,6 +70,12 @@ hipError_t launch_gemm_chain_ex(int qt, const void *W, const float *X, int ldx, 
 size_t q8k_block_bytes();
 hipError_t launch_quantize_q8k(const float *x, void *y, int64_t k, hipStream_t st);
 hipError_t launch_vec_dot_q8k(int qt, const void *x, const void *y, int nb, float *out, hipStream_t st);
+// token mixers (rope.hip, attn.hip, delta.hip)
+hipError_t launch_rope(const RopeArgs &a, const RopeTable &tab, int64_t rows, bool vec, hipStream_t st);
+size_t attn_ws(const AttnArgs &a);
+hipError_t launch_attn(const AttnArgs &a, void *ws, hipStream_t st);
+size_t delta_ws(const DeltaArgs &a, bool snapshots);
+hipError_t launch_delta(const DeltaArgs &a, void *ws, hipStream_t st);
 size_t noalloc_scratch_bytes();
 hipError_t noalloc_scratch(void **out);
 hipError_t noalloc_prepare(int device);
@@ -977,6 +985,231 @@ int ihip_spec_advance_len(int32_t *len_dev, const int32_t *n_accepted_dev, int s
     if (steps < 1) return fail(IHIP_EINVAL, "ihip_spec_advance_len: steps=%d", steps);
     hipError_t e = launch_advance_len(len_dev, n_accepted_dev, steps, S(stream));
     return e == hipSuccess ? ok() : hip_fail(e, "ihip_spec_advance_len");
+}
+
+// ---- token mixers ----
+
+namespace {
+
+bool is_finite(double v) { return std::isfinite(v); }
+
+int check_rope(const char *name, const ihip_rope *r) {
+    if (!r) return fail(IHIP_EFAULT, "%s: NULL pointer", name);
+    if (r->head_dim < 2 || r->rot_dim < 2 || (r->rot_dim & 1) || r->rot_dim > r->head_dim || r->rot_dim > 256)
+        return fail(IHIP_EINVAL, "%s: rot_dim=%d of head_dim=%d (even, 2 .. min(head_dim, 256))", name, r->rot_dim,
+                    r->head_dim);
+    if (r->head_dim > 65536 || !is_finite(r->mscale))
+        return fail(IHIP_EINVAL, "%s: head_dim=%d mscale=%g", name, r->head_dim, r->mscale);
+    return IHIP_OK;
+}
+
+int check_kv(const char *name, const char *what, const ihip_kv *c) {
+    if (!c || !c->k || !c->v) return fail(IHIP_EFAULT, "%s: NULL pointer in %s", name, what);
+    if (c->type != IHIP_F16 && c->type != IHIP_BF16) return fail(IHIP_EINVAL, "%s: %s of type %d", name, what, c->type);
+    if (c->n_seq < 1 || c->n_seq > 65535 || c->n_kv < 1 || c->n_kv > 4096 || c->head_dim < 8 || (c->head_dim & 7) ||
+        c->head_dim > 65536 || c->capacity < 1 || c->capacity > 0x7fffffff)
+        return fail(IHIP_EINVAL, "%s: %s of n_seq=%d n_kv=%d head_dim=%d capacity=%lld", name, what, c->n_seq, c->n_kv,
+                    c->head_dim, (long long)c->capacity);
+    if (!aligned16(c->k) || !aligned16(c->v) || ((c->seq_stride | c->tok_stride | c->head_stride) & 7))
+        return fail(IHIP_EINVAL, "%s: %s must be 16-byte aligned with strides of multiples of 8 values", name, what);
+    // entries may not overlap: the two inner axes in either order, sequences apart (128 bits: the products may pass 64)
+    typedef __int128 wide;
+    const wide cap = c->capacity, heads = c->n_kv, D = c->head_dim, ts = c->tok_stride, hs = c->head_stride;
+    const bool bad_sign = c->seq_stride < 0 || ts < 0 || hs < 0;
+    const bool tok_inner = (cap == 1 || ts >= D) && (heads == 1 || hs >= (cap - 1) * ts + D);
+    const bool head_inner = (heads == 1 || hs >= D) && (cap == 1 || ts >= (heads - 1) * hs + D);
+    const wide extent = (cap - 1) * ts + (heads - 1) * hs + D;
+    if (bad_sign || !(tok_inner || head_inner) || (c->n_seq > 1 && c->seq_stride < extent))
+        return fail(IHIP_EINVAL, "%s: %s strides %lld %lld %lld overlap", name, what, (long long)c->seq_stride,
+                    (long long)c->tok_stride, (long long)c->head_stride);
+    return IHIP_OK;
+}
+
+int fill_attn(const char *name, AttnArgs &a, int n_q, int M, const ihip_kv *cache, const ihip_kv *prefix) {
+    int rc = check_kv(name, "cache", cache);
+    if (rc != IHIP_OK) return rc;
+    if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256)
+        return fail(IHIP_EINVAL, "%s: head_dim=%d (64, 128 or 256)", name, cache->head_dim);
+    if (n_q < 1 || n_q % cache->n_kv || n_q > 65535 || M < 1 || (int64_t)M * cache->n_seq * n_q > 0x7fffffff)
+        return fail(IHIP_EINVAL, "%s: n_q=%d over n_kv=%d, M=%d", name, n_q, cache->n_kv, M);
+    a = AttnArgs{};
+    a.n_q = n_q, a.M = M, a.n_seq = cache->n_seq, a.n_kv = cache->n_kv, a.head_dim = cache->head_dim;
+    a.type = cache->type, a.k = cache->k, a.v = cache->v, a.capacity = cache->capacity;
+    a.seq_stride = cache->seq_stride, a.tok_stride = cache->tok_stride, a.head_stride = cache->head_stride;
+    if (prefix) {
+        rc = check_kv(name, "prefix", prefix);
+        if (rc != IHIP_OK) return rc;
+        if (prefix->n_seq != 1 || prefix->n_kv != cache->n_kv || prefix->head_dim != cache->head_dim ||
+            prefix->type != cache->type)
+            return fail(IHIP_EINVAL, "%s: the prefix is one sequence of the cache's type, n_kv and head_dim", name);
+        a.pk = prefix->k, a.pv = prefix->v, a.P = prefix->capacity;
+        a.p_tok_stride = prefix->tok_stride, a.p_head_stride = prefix->head_stride;
+    }
+    return IHIP_OK;
+}
+
+int check_delta_shape(const char *name, int n_seq, int T, int n_k, int n_v, int dk, int dv) {
+    if (n_seq < 1 || n_seq > 65535 || T < 1 || (int64_t)n_seq * T > 0x7fffffff)
+        return fail(IHIP_EINVAL, "%s: n_seq=%d T=%d", name, n_seq, T);
+    if (n_k < 1 || n_v < 1 || n_v % n_k || n_v > 4096) return fail(IHIP_EINVAL, "%s: n_k=%d n_v=%d", name, n_k, n_v);
+    if ((dk != 64 && dk != 128) || dv < 4 || (dv & 3) || dv > 512)
+        return fail(IHIP_EINVAL, "%s: dk=%d (64 or 128) dv=%d (a multiple of 4 up to 512)", name, dk, dv);
+    return IHIP_OK;
+}
+
+}  // namespace
+
+int ihip_rope_init(ihip_rope *rope, int head_dim, int rot_dim, int interleaved, double base, int scaling,
+                   double factor, double orig_len, double beta_fast, double beta_slow, double mscale,
+                   const float *freq_factors_dev) {
+    if (!rope) return fail(IHIP_EFAULT, "ihip_rope_init: NULL pointer");
+    ihip_rope r{};
+    r.head_dim = head_dim, r.rot_dim = rot_dim, r.interleaved = interleaved ? 1 : 0;
+    r.mscale = (float)mscale, r.freq_factors = freq_factors_dev;
+    const int rc = check_rope("ihip_rope_init", &r);
+    if (rc != IHIP_OK) return rc;
+    if (!(base > 0) || !is_finite(base)) return fail(IHIP_EINVAL, "ihip_rope_init: base=%g", base);
+    if (scaling != IHIP_ROPE_PLAIN && (scaling < 0 || scaling > IHIP_ROPE_BY_PARTS))
+        return fail(IHIP_EINVAL, "ihip_rope_init: scaling %d", scaling);
+    if (scaling != IHIP_ROPE_PLAIN && (!(factor > 0) || !is_finite(factor)))
+        return fail(IHIP_EINVAL, "ihip_rope_init: factor=%g", factor);
+    if (scaling == IHIP_ROPE_BY_PARTS) {
+        if (!(orig_len > 0) || !is_finite(orig_len) || !(beta_fast > beta_slow) || !(beta_slow >= 0) || !is_finite(beta_fast))
+            return fail(IHIP_EINVAL, "ihip_rope_init: orig_len=%g beta_fast=%g beta_slow=%g", orig_len, beta_fast, beta_slow);
+        if (freq_factors_dev) return fail(IHIP_EINVAL, "ihip_rope_init: frequency factors with scaling by parts");
+    }
+    for (int i = 0; i < rot_dim / 2; i++) {
+        double t = std::pow(base, -2.0 * i / rot_dim) / 6.283185307179586476925;
+        if (scaling == IHIP_ROPE_LINEAR) t /= factor;
+        if (scaling == IHIP_ROPE_BY_PARTS) {
+            const double keep = std::min(1.0, std::max(0.0, (orig_len * t - beta_slow) / (beta_fast - beta_slow)));
+            t *= keep + (1.0 - keep) / factor;
+        }
+        r.turns[i] = t;
+    }
+    *rope = r;
+    return ok();
+}
+
+static void rope_args(RopeArgs &a, RopeTable &tab, const ihip_rope *r) {
+    a.head_dim = r->head_dim, a.rot_dim = r->rot_dim, a.interleaved = r->interleaved, a.mscale = r->mscale;
+    a.freq_factors = r->freq_factors;
+    memcpy(tab.turns, r->turns, sizeof tab.turns);
+}
+
+// 16-byte accesses: whole vectors in every part of a head, aligned rows
+static bool rope_vec(const RopeArgs &a) {
+    return a.head_dim % 4 == 0 && a.rot_dim % (a.interleaved ? 4 : 8) == 0 && a.ldx % 4 == 0 && a.ldy % 4 == 0 &&
+           aligned16(a.x) && aligned16(a.y);
+}
+
+int ihip_rope_apply(const ihip_rope *rope, const float *x_dev, int64_t ldx, float *y_dev, int64_t ldy, int heads,
+                    const int32_t *pos_dev, int tokens, void *stream) {
+    if (!x_dev || !y_dev || !pos_dev) return fail(IHIP_EFAULT, "ihip_rope_apply: NULL pointer");
+    const int rc = check_rope("ihip_rope_apply", rope);
+    if (rc != IHIP_OK) return rc;
+    const int64_t width = (int64_t)heads * rope->head_dim;
+    if (heads < 1 || heads > 65536 || width > (1 << 24) || tokens < 1 || ldx < width || ldy < width)
+        return fail(IHIP_EINVAL, "ihip_rope_apply: heads=%d tokens=%d ldx=%lld ldy=%lld", heads, tokens, (long long)ldx,
+                    (long long)ldy);
+    if (x_dev == y_dev && ldx != ldy) return fail(IHIP_EINVAL, "ihip_rope_apply: in place needs ldy = ldx");
+    RopeArgs a{};
+    RopeTable tab;
+    rope_args(a, tab, rope);
+    a.x = x_dev, a.y = y_dev, a.ldx = ldx, a.ldy = ldy, a.pos = pos_dev, a.n_q = heads, a.M = 1;
+    const hipError_t e = launch_rope(a, tab, tokens, rope_vec(a), S(stream));
+    return e == hipSuccess ? ok() : hip_fail(e, "ihip_rope_apply");
+}
+
+int ihip_rope_append(const ihip_rope *rope, const float *qkv_dev, int64_t ld, float *q_out_dev, int64_t ldq, int n_q,
+                     const ihip_kv *cache, const int32_t *len_dev, const int32_t *pos_dev, int pos0, int M,
+                     void *stream) {
+    if (!qkv_dev || !q_out_dev || !len_dev) return fail(IHIP_EFAULT, "ihip_rope_append: NULL pointer");
+    int rc = check_rope("ihip_rope_append", rope);
+    if (rc == IHIP_OK) rc = check_kv("ihip_rope_append", "cache", cache);
+    if (rc != IHIP_OK) return rc;
+    if (rope->head_dim != cache->head_dim)
+        return fail(IHIP_EINVAL, "ihip_rope_append: head_dim %d and the cache's %d", rope->head_dim, cache->head_dim);
+    const int64_t D = cache->head_dim, width = ((int64_t)n_q + 2 * cache->n_kv) * D;
+    if (n_q < 1 || n_q > 65536 || width > (1 << 24) || M < 1 || (int64_t)M * cache->n_seq > 0x7fffffff || ld < width ||
+        ldq < n_q * D)
+        return fail(IHIP_EINVAL, "ihip_rope_append: n_q=%d M=%d ld=%lld ldq=%lld", n_q, M, (long long)ld, (long long)ldq);
+    if (qkv_dev == q_out_dev && ld != ldq) return fail(IHIP_EINVAL, "ihip_rope_append: in place needs ldq = ld");
+    RopeArgs a{};
+    RopeTable tab;
+    rope_args(a, tab, rope);
+    a.x = qkv_dev, a.y = q_out_dev, a.ldx = ld, a.ldy = ldq, a.pos = pos_dev, a.len = len_dev, a.pos0 = pos0, a.M = M;
+    a.k = cache->k, a.v = cache->v, a.type = cache->type, a.capacity = cache->capacity;
+    a.seq_stride = cache->seq_stride, a.tok_stride = cache->tok_stride, a.head_stride = cache->head_stride;
+    a.n_q = n_q, a.n_k = a.n_v = cache->n_kv;
+    const hipError_t e = launch_rope(a, tab, (int64_t)M * cache->n_seq, rope_vec(a), S(stream));
+    return e == hipSuccess ? ok() : hip_fail(e, "ihip_rope_append");
+}
+
+int ihip_attn_prefix_ws_bytes(int n_q, int M, const ihip_kv *cache, const ihip_kv *prefix, size_t *bytes) {
+    if (!bytes) return fail(IHIP_EFAULT, "ihip_attn_prefix_ws_bytes: NULL pointer");
+    AttnArgs a;
+    const int rc = fill_attn("ihip_attn_prefix_ws_bytes", a, n_q, M, cache, prefix);
+    if (rc != IHIP_OK) return rc;
+    *bytes = attn_ws(a);
+    return ok();
+}
+
+int ihip_attn_prefix(const float *q_dev, int64_t ldq, float *out_dev, int64_t ldo, int n_q, int M, const ihip_kv *cache,
+                     const int32_t *len_dev, const ihip_kv *prefix, const uint64_t *tree_mask_dev, float scale, void *ws,
+                     size_t ws_bytes, void *stream) {
+    if (!q_dev || !out_dev || !len_dev || !ws) return fail(IHIP_EFAULT, "ihip_attn_prefix: NULL pointer");
+    AttnArgs a;
+    const int rc = fill_attn("ihip_attn_prefix", a, n_q, M, cache, prefix);
+    if (rc != IHIP_OK) return rc;
+    const int64_t width = (int64_t)n_q * a.head_dim;
+    if (ldq < width || ldo < width || (ldq & 3) || (ldo & 3) || !aligned16(q_dev) || !aligned16(out_dev))
+        return fail(IHIP_EINVAL, "ihip_attn_prefix: rows of %lld values at ldq=%lld ldo=%lld (multiples of 4, 16-byte "
+                                 "aligned)", (long long)width, (long long)ldq, (long long)ldo);
+    if (tree_mask_dev && M > 64) return fail(IHIP_EINVAL, "ihip_attn_prefix: a tree of M=%d nodes (up to 64)", M);
+    if (!is_finite(scale)) return fail(IHIP_EINVAL, "ihip_attn_prefix: scale %g", scale);
+    if (!aligned16(ws)) return fail(IHIP_EINVAL, "ihip_attn_prefix: workspace must be 16-byte aligned");
+    if (ws_bytes < attn_ws(a))
+        return fail(IHIP_ENOMEM, "ihip_attn_prefix: workspace %zu < %zu bytes", ws_bytes, attn_ws(a));
+    a.q = q_dev, a.out = out_dev, a.ldq = ldq, a.ldo = ldo, a.len = len_dev, a.mask = tree_mask_dev, a.scale = scale;
+    const hipError_t e = launch_attn(a, ws, S(stream));
+    return e == hipSuccess ? ok() : hip_fail(e, "ihip_attn_prefix");
+}
+
+int ihip_delta_ws_bytes(int n_seq, int T, int n_k, int n_v, int dk, int dv, int snapshots, size_t *bytes) {
+    if (!bytes) return fail(IHIP_EFAULT, "ihip_delta_ws_bytes: NULL pointer");
+    const int rc = check_delta_shape("ihip_delta_ws_bytes", n_seq, T, n_k, n_v, dk, dv);
+    if (rc != IHIP_OK) return rc;
+    DeltaArgs a{};
+    a.n_seq = n_seq, a.T = T, a.n_k = n_k, a.n_v = n_v, a.dk = dk, a.dv = dv;
+    *bytes = delta_ws(a, snapshots != 0);
+    return ok();
+}
+
+int ihip_gated_delta_rule(const ihip_delta *d, void *ws, size_t ws_bytes, void *stream) {
+    if (!d || !d->q || !d->k || !d->v || !d->g || !d->beta || !d->o || !ws)
+        return fail(IHIP_EFAULT, "ihip_gated_delta_rule: NULL pointer");
+    int rc = check_delta_shape("ihip_gated_delta_rule", d->n_seq, d->T, d->n_k, d->n_v, d->dk, d->dv);
+    if (rc != IHIP_OK) return rc;
+    const int64_t wk = (int64_t)d->n_k * d->dk, wv = (int64_t)d->n_v * d->dv;
+    if (d->ldq < wk || d->ldk < wk || d->ldv < wv || d->ldo < wv || d->ldg < d->n_v || d->ldb < d->n_v ||
+        ((d->ldq | d->ldk | d->ldv | d->ldo) & 3))
+        return fail(IHIP_EINVAL, "ihip_gated_delta_rule: rows at ldq=%lld ldk=%lld ldv=%lld ldo=%lld ldg=%lld ldb=%lld",
+                    (long long)d->ldq, (long long)d->ldk, (long long)d->ldv, (long long)d->ldo, (long long)d->ldg,
+                    (long long)d->ldb);
+    if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->o) || !aligned16(d->state_in) ||
+        !aligned16(d->state_out) || !aligned16(d->snap_out) || !aligned16(ws))
+        return fail(IHIP_EINVAL, "ihip_gated_delta_rule: pointers must be 16-byte aligned");
+    if (d->snap_out && d->T > 64) return fail(IHIP_EINVAL, "ihip_gated_delta_rule: snapshots of T=%d tokens (up to 64)", d->T);
+    if ((d->flags & ~IHIP_DELTA_L2NORM) || !is_finite(d->scale))
+        return fail(IHIP_EINVAL, "ihip_gated_delta_rule: flags 0x%x scale %g", d->flags, d->scale);
+    DeltaArgs a{d->q, d->k, d->v, d->g, d->beta, d->ldq, d->ldk, d->ldv, d->ldg, d->ldb, d->o, d->ldo, d->state_in,
+                d->state_out, d->snap_out, d->len, d->n_seq, d->T, d->n_k, d->n_v, d->dk, d->dv, d->scale,
+                (d->flags & IHIP_DELTA_L2NORM) ? 1 : 0};
+    const size_t need = delta_ws(a, d->snap_out != nullptr);
+    if (ws_bytes < need) return fail(IHIP_ENOMEM, "ihip_gated_delta_rule: workspace %zu < %zu bytes", ws_bytes, need);
+    const hipError_t e = launch_delta(a, ws, S(stream));
+    return e == hipSuccess ? ok() : hip_fail(e, "ihip_gated_delta_rule");
 }
 
 int ihip_sample(const float *logits_dev, int rows, int V, float T, int top_k, float top_p, float min_p,

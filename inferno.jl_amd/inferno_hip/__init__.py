@@ -7,6 +7,8 @@ lib/libinferno_hip.so. There is no CPU fallback.
 """
 from . import formats, gguf, synth
 from ._lib import HipError, load
+from .mixers import (KVCache, RopeParams, attn_prefix, attn_prefix_ws_bytes, gated_delta_rule, gated_delta_rule_ws_bytes,
+                     rope, rope_append)
 from .quantized_kernels import (ACT_PLAIN, ACT_RMSNORM, ACT_SILU_MUL, EPI_GATE, EPI_RESID, EPI_STATS, EPI_STORE,
                                 GEMM_ACCUM, GEMM_AUTO, GEMM_F32, GEMM_HALF, GEMM_DEFER, GEMM_PACKED, GEMM_REUSE, GEMM_SUM_OUT,
                                 chain_buffers, chain_in, chain_operand_bytes, chain_out, dequant, gemm_partials, gemm_q, gemm_q_chain,
@@ -25,4 +27,6 @@ __all__ = [
     "chain_out", "chain_buffers", "chain_operand_bytes", "gemm_q_chain", "pack_weights_gated", "MODE_REFERENCE", "MODE_STANDARD", "SpeculativeStats",
     "greedy_verify", "mtp_verify_step", "n_tokens", "softmax_stats", "spec_accept", "tree_accept",
     "softmax_sample", "sample_ws_bytes", "apply_penalties_", "commit_state_", "advance_len_",
+    "KVCache", "RopeParams", "rope", "rope_append", "attn_prefix", "attn_prefix_ws_bytes", "gated_delta_rule",
+    "gated_delta_rule_ws_bytes",
 ]

@@ -16,7 +16,7 @@ HEADER_PATH = os.path.join(os.path.dirname(PKG_ROOT), "include", "inferno_hip.h"
 IHIP_OK = 0
 STATUS_NAMES = {0: "OK", -14: "EFAULT", -22: "EINVAL", -12: "ENOMEM", -19: "ENODEV", -1000: "EHIP"}
 
-_vp, _i, _i64, _u64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_size_t
+_vp, _i, _i64, _u64, _f, _d, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_double, C.c_size_t
 
 
 class _NotPlain(Exception):
@@ -86,6 +86,13 @@ SIGNATURES = {
     "ihip_tree_accept": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ihip_spec_commit_state": (_i, [_vp, _vp, _sz, _i64, _i, _vp, _i, _i64, _i64, _vp]),
     "ihip_spec_advance_len": (_i, [_vp, _vp, _i, _vp]),
+    "ihip_rope_init": (_i, [_vp, _i, _i, _i, _d, _i, _d, _d, _d, _d, _d, _vp]),
+    "ihip_rope_apply": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _vp, _i, _vp]),
+    "ihip_rope_append": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i, _i, _vp]),
+    "ihip_attn_prefix_ws_bytes": (_i, [_i, _i, _vp, _vp, C.POINTER(_sz)]),
+    "ihip_attn_prefix": (_i, [_vp, _i64, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _f, _vp, _sz, _vp]),
+    "ihip_delta_ws_bytes": (_i, [_i, _i, _i, _i, _i, _i, _i, C.POINTER(_sz)]),
+    "ihip_gated_delta_rule": (_i, [_vp, _vp, _sz, _vp]),
     "ihip_sample": (_i, [_vp, _i, _i, _f, _i, _f, _f, _vp, _vp, _vp]),
     "ihip_sample_ws_bytes": (_i, [_i, _i, C.POINTER(_sz)]),
     "ihip_sample_ex": (_i, [_vp, _i, _i, _f, _i, _f, _f, _vp, _vp, _vp, _sz, _vp]),
@@ -125,6 +132,26 @@ class ChainOut(C.Structure):
     """struct ihip_chain_out"""
     _fields_ = [("epi", _i), ("y", _vp), ("ldy", _i), ("norm_w", _vp), ("consumer_qtype", _i), ("operand", _vp),
                 ("tile_sum", _vp), ("sum_stride", _i), ("tile_ssq", _vp), ("stat_rows", _i)]
+
+
+class Rope(C.Structure):
+    """struct ihip_rope"""
+    _fields_ = [("head_dim", _i), ("rot_dim", _i), ("interleaved", _i), ("mscale", _f), ("freq_factors", _vp),
+                ("turns", _d * 128)]
+
+
+class Kv(C.Structure):
+    """struct ihip_kv"""
+    _fields_ = [("type", _i), ("n_seq", _i), ("n_kv", _i), ("head_dim", _i), ("capacity", _i64), ("k", _vp),
+                ("v", _vp), ("seq_stride", _i64), ("tok_stride", _i64), ("head_stride", _i64)]
+
+
+class Delta(C.Structure):
+    """struct ihip_delta"""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("g", _vp), ("beta", _vp), ("ldq", _i64), ("ldk", _i64),
+                ("ldv", _i64), ("ldg", _i64), ("ldb", _i64), ("o", _vp), ("ldo", _i64), ("state_in", _vp),
+                ("state_out", _vp), ("snap_out", _vp), ("len", _vp), ("n_seq", _i), ("T", _i), ("n_k", _i),
+                ("n_v", _i), ("dk", _i), ("dv", _i), ("scale", _f), ("flags", _i)]
 
 
 class HipError(RuntimeError):
