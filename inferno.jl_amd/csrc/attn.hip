@@ -1,69 +1,545 @@
 // Attention of a batch's new tokens over a shared prefix, their own cached
 // entries and each other (src/ModelCPU.jl:730-856).
+//
+// For a key head, the rows of its query heads (all sequences' for the prefix,
+// one sequence's for its own entries) meet a range of keys in one workgroup:
+//   S^T = K Q^T, P^T = 2^(S^T c - m), O^T += V^T P^T
+// on 16x16x32 MFMAs, 32 keys at a time. Transposed, a lane's accumulators of
+// S^T belong to one query row (lane & 15), so the running maximum and sum are a
+// number a lane, and they are already the B operand of the second product (its
+// sum over keys takes any order of them: lane group g holds keys 4 g .. 4 g + 3
+// of either half): P never leaves the registers. V^T is read from the row-major
+// tile in LDS with transposing loads.
+//
+// fp32 accuracy from 16-bit matrix cores: K and V are 16-bit already and enter
+// as they are; q (times scale log2 e, and for f16 a power of two per row) and P
+// are split into limbs, two of f16 (22 bits) or three of bf16 (24 bits), each
+// product summed in fp32.
+//
+// Ranges of keys (splits) are joined by a last kernel in their order, so results
+// do not depend on what runs when.
 #include "common.h"
 #include "mixer.h"
 
 namespace {
 
-template <int TYPE> __device__ __forceinline__ float kv_at(const void *p, int64_t i) {
-    if constexpr (TYPE == KV_F16) return (float)((const _Float16 *)p)[i];
-    else return (float)((const __bf16 *)p)[i];
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+template <int TYPE> struct Kv;
+template <> struct Kv<KV_F16> {
+    typedef _Float16 t;
+    typedef h8 v8;
+    static constexpr int LIMBS = 2;
+    static constexpr float BIAS = 8.f;  // P is 2^BIAS too large: its second limb then reaches 2^-33 of a row's largest
+    static __device__ __forceinline__ f4 mfma(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Kv<KV_BF16> {
+    typedef __bf16 t;
+    typedef b8 v8;
+    static constexpr int LIMBS = 3;
+    static constexpr float BIAS = 0.f;
+    static __device__ __forceinline__ f4 mfma(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// x = l[0] + l[1] (+ l[2]), each limb the rest rounded to its type
+template <int TYPE> __device__ __forceinline__ void limbs(const float *x, typename Kv<TYPE>::v8 *l) {
+    typedef typename Kv<TYPE>::t t;
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < Kv<TYPE>::LIMBS; n++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const t h = (t)r[i];
+            l[n][i] = h;
+            r[i] -= (float)h;
+        }
 }
 
-// One wave a query row and head, entry by entry with the running maximum m and
-// sum l of its softmax; lane i holds values i, i + 64, .. of the head.
-template <int TYPE, int D> __global__ __launch_bounds__(64) void attn_row_kernel(AttnArgs a) {
-    constexpr int E = D / 64;
-    const int64_t row = blockIdx.x;
-    const int h = blockIdx.y, lane = threadIdx.x, s = (int)(row / a.M), r = (int)(row - (int64_t)s * a.M);
-    const int n = a.len[s];
-    if (n < 0) return;
-    float *out = a.out + row * a.ldo + (int64_t)h * D;
-    if ((int64_t)n + a.M > a.capacity) {
-        for (int e = 0; e < E; e++) out[lane + 64 * e] = __builtin_nanf("");
-        return;
+__device__ __forceinline__ float max_groups(float v) {  // over the four lane groups of a row
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const uint32_t y = __float_as_uint(m);
+    const auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const float m = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const uint32_t y = __float_as_uint(m);
+    const auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Byte of 16-byte chunk c of row r in a tile of D values a row. The chunks of a row are permuted by its number so that
+// neither the operand loads of K (16 rows, one chunk each) nor the transposing loads of V (4 rows, two chunks each)
+// meet in a bank: a row of 128 or 256 values starts at the same bank as the next.
+template <int D> __device__ __forceinline__ int tile_at(int r, int c) {
+    const int x = D == 64 ? ((r >> 1) & 3) * 2 : (r & 7) * 2;
+    return r * (D * 2) + ((c ^ x) << 4);
+}
+
+struct AttnSplit {
+    int rows;      // query rows of a key head in this launch's unit (all sequences, or one)
+    int blocks;    // row blocks
+    int splits;    // ranges of keys
+    int first;     // this launch's first part
+    int64_t per;   // keys of a split (prefix)
+};
+
+// WR x WK waves: wave (wr, wk) takes rows [16 RT wr, ..) of the block and every WK-th 32 keys of a tile of KB keys; the
+// tile is loaded to registers one round ahead and goes through NBUF buffers in LDS.
+template <int TYPE, int D, int RT, int WR, int WK, int KB, int NBUF, bool OWN>
+__global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, AttnSplit sp, float *__restrict__ opart,
+                                                              float2 *__restrict__ ml) {
+    typedef Kv<TYPE> X;
+    typedef typename X::t T;
+    typedef typename X::v8 v8;
+    constexpr int NT = WR * WK * 64, C = D / 8, STEPS = D / 32, DT = D / 16, ROWS = WR * RT * 16;
+    constexpr int TILE = KB * D * 2, NLD = KB * C / NT;
+    static_assert(KB % (32 * WK) == 0 && KB * C % NT == 0, "tile shape");
+    static_assert(WK == 1 || NBUF * 2 * TILE >= WR * WK * RT * 16 * D * 4, "the waves' results meet in the tile buffers");
+    __shared__ __align__(16) char lds[NBUF * 2 * TILE];  // NBUF x (K tile, V tile)
+    __shared__ int bad[2];
+    __shared__ float2 wml[WR * WK][RT * 16];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave / WK, wk = wave % WK, g = lane >> 4, col = lane & 15;
+    const int G = a.n_q / a.n_kv;
+
+    // the block's unit: which sequence, key head, rows and keys
+    int s = 0, hk, rb, split, n = 0;
+    int64_t begin, end;
+    const T *K, *V;
+    int64_t kstride;
+    if constexpr (OWN) {
+        int id = blockIdx.x;
+        split = id % sp.splits, id /= sp.splits;
+        rb = id % sp.blocks, id /= sp.blocks;
+        hk = id % a.n_kv, s = id / a.n_kv;
+        n = a.len[s];
+        if (n < 0 || (int64_t)n + a.M > a.capacity) return;
+        const int64_t all = (int64_t)n + a.M, per = ((all + sp.splits - 1) / sp.splits + 31) / 32 * 32;
+        begin = split * per;
+        end = begin + per < all ? begin + per : all;
+        kstride = a.tok_stride;
+        K = (const T *)a.k + s * a.seq_stride + hk * a.head_stride;
+        V = (const T *)a.v + s * a.seq_stride + hk * a.head_stride;
+    } else {
+        // row blocks of one range of keys go to one XCD (consecutive workgroups to the eight in turn), whose L2 then
+        // holds the range for all of them
+        const int id = blockIdx.x, x = id & 7, y = id >> 3;
+        rb = y % sp.blocks;
+        const int pair = (y / sp.blocks) * 8 + x;
+        if (pair >= sp.splits * a.n_kv) return;
+        hk = pair / sp.splits, split = pair % sp.splits;
+        begin = split * sp.per;
+        end = begin + sp.per < a.P ? begin + sp.per : a.P;
+        kstride = a.p_tok_stride;
+        K = (const T *)a.pk + hk * a.p_head_stride;
+        V = (const T *)a.pv + hk * a.p_head_stride;
     }
-    const int hk = h / (a.n_q / a.n_kv);
-    float q[E], acc[E], m = -__builtin_inff(), l = 0.f;
-    for (int e = 0; e < E; e++) {
-        q[e] = a.q[row * a.ldq + (int64_t)h * D + lane + 64 * e] * a.scale;
-        acc[e] = 0.f;
+    const int r0 = rb * ROWS + wr * RT * 16;
+
+    // this lane's query rows (one a row tile): the token row, its place in the sequence, its head
+    auto token = [&](int r) { return (int64_t)s * a.M + r / G; };
+    v8 q[RT][STEPS][X::LIMBS];
+    float c[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int r = r0 + t * 16 + col;
+        const bool in = r < sp.rows;
+        const float *src = a.q + (in ? token(r) * a.ldq + (int64_t)(hk * G + r % G) * D : 0) + 8 * g;
+        float x[STEPS][8], top = 0.f;
+        const float k2 = a.scale * 1.44269504088896341f;
+#pragma unroll
+        for (int u = 0; u < STEPS; u++) {
+            *(f4 *)(x[u]) = in ? *(const f4 *)(src + 32 * u) : f4{0, 0, 0, 0};
+            *(f4 *)(x[u] + 4) = in ? *(const f4 *)(src + 32 * u + 4) : f4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[u][i] *= k2, top = fmaxf(top, fabsf(x[u][i]));
+        }
+        float up = 1.f;
+        c[t] = 1.f;
+        if constexpr (TYPE == KV_F16) {  // the row's largest to [2^13, 2^14)
+            top = max_groups(top);
+            int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+            e = e < -100 ? -100 : e > 110 ? 110 : e;
+            up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+            c[t] = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+        }
+#pragma unroll
+        for (int u = 0; u < STEPS; u++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[u][i] *= up;
+            limbs<TYPE>(x[u], q[t][u]);
+        }
     }
-    auto take = [&](const void *k, const void *v, int64_t at) {
-        float z = 0.f;
-        for (int e = 0; e < E; e++) z = __builtin_fmaf(q[e], kv_at<TYPE>(k, at + lane + 64 * e), z);
-        z = wave_sum(z);
-        const float top = fmaxf(m, z);
-        const float base = top == -__builtin_inff() ? 0.f : top;
-        const float keep = expf(m - base), p = expf(z - base);
-        l = l * keep + p;
-        for (int e = 0; e < E; e++) acc[e] = acc[e] * keep + p * kv_at<TYPE>(v, at + lane + 64 * e);
-        m = top;
+
+    f4 o[RT][DT];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        m[t] = -__builtin_inff(), l[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[t][d] = f4{0, 0, 0, 0};
+    }
+    // new entry j (of the sequence's M) seen by this lane's row of tile t
+    auto sees = [&](int64_t key, int r) {
+        if (key < n) return true;
+        const int j = (int)(key - n), mine = r / G;
+        if (r >= sp.rows || j >= a.M) return false;
+        return a.mask ? ((a.mask[(int64_t)s * a.M + mine] >> j) & 1) != 0 : j <= mine;
     };
-    for (int64_t j = 0; j < a.P; j++) take(a.pk, a.pv, j * a.p_tok_stride + hk * a.p_head_stride);
-    const int64_t own = s * a.seq_stride + hk * a.head_stride;
-    for (int j = 0; j < n; j++) take(a.k, a.v, own + j * a.tok_stride);
-    for (int j = 0; j < a.M; j++)
-        if (a.mask ? (a.mask[row] >> j) & 1 : j <= r) take(a.k, a.v, own + ((int64_t)n + j) * a.tok_stride);
-    for (int e = 0; e < E; e++) out[lane + 64 * e] = l == 0.f ? 0.f : acc[e] / l;
+
+    uint4 sk[NLD], sv[NLD];
+    auto fetch = [&](int64_t k0) {
+#pragma unroll
+        for (int i = 0; i < NLD; i++) {
+            const int idx = tid + i * NT, r = idx / C, ch = idx % C;
+            const bool in = k0 + r < end;
+            const int64_t at = (k0 + r) * kstride + ch * 8;
+            sk[i] = in ? *(const uint4 *)(K + at) : uint4{0, 0, 0, 0};
+            sv[i] = in ? *(const uint4 *)(V + at) : uint4{0, 0, 0, 0};
+        }
+    };
+    auto put = [&](int64_t k0, int buf) {
+        char *tk = lds + buf * 2 * TILE, *tv = tk + TILE;
+        if constexpr (OWN) {
+            // non-finite values of new entries are taken out of the tile and added for the rows that see them
+            // (0 times infinity would reach the others)
+            if (k0 + KB > n) {
+                constexpr uint32_t E = TYPE == KV_F16 ? 0x7c00u : 0x7f80u;
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < NLD; i++) {
+                    uint32_t *w = (uint32_t *)&sv[i];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if ((w[j] & E) == E) w[j] &= 0xffff0000u, any = true;
+                        if ((w[j] & (E << 16)) == (E << 16)) w[j] &= 0xffffu, any = true;
+                    }
+                }
+                if (any) bad[buf] = 1;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NLD; i++) {
+            const int idx = tid + i * NT, r = idx / C, ch = idx % C;
+            *(uint4 *)(tk + tile_at<D>(r, ch)) = sk[i];
+            *(uint4 *)(tv + tile_at<D>(r, ch)) = sv[i];
+        }
+    };
+
+    auto compute = [&](int64_t k0, int buf) {
+        const char *tk = lds + buf * 2 * TILE, *tv = tk + TILE;
+        for (int sub = wk; sub < KB / 32; sub += WK) {
+            const int64_t key0 = k0 + sub * 32;
+            if (key0 >= end) break;
+            f4 z[RT][2];
+#pragma unroll
+            for (int t = 0; t < RT; t++) z[t][0] = z[t][1] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < STEPS; u++) {
+                v8 ka[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) ka[h] = *(const v8 *)(tk + tile_at<D>(sub * 32 + h * 16 + col, 4 * u + g));
+#pragma unroll
+                for (int x = 0; x < X::LIMBS; x++)
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) z[t][h] = X::mfma(ka[h], q[t][u][x], z[t][h]);
+            }
+            const bool partial = OWN ? key0 + 32 > n : key0 + 32 > end;
+            v8 p[RT][X::LIMBS];
+            float pf[RT][8];
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = z[t][i >> 2][i & 3] * c[t];
+                if (partial) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int64_t key = key0 + (i >> 2) * 16 + 4 * g + (i & 3);
+                        const bool on = key < end && (!OWN || sees(key, r0 + t * 16 + col));
+                        x[i] = on ? x[i] : -__builtin_inff();
+                    }
+                }
+                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                // the reference point moves only when a row's maximum passes it by 2^7 (P then still fits its type)
+                if (__any(top > m[t] + 7.f)) {
+                    top = fmaxf(m[t], max_groups(top));
+                    const float keep = m[t] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[t] - top);
+                    m[t] = top;
+                    l[t] *= keep;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[t][d] *= keep;
+                }
+                const float off = m[t] == -__builtin_inff() ? 0.f : m[t] - X::BIAS;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    pf[t][i] = __builtin_amdgcn_exp2f(x[i] - off);
+                    l[t] += pf[t][i];
+                }
+                limbs<TYPE>(pf[t], p[t]);
+            }
+            // transposing loads: 16 lanes read 4 keys x 16 values, lane i gets value i of the four
+            const int vr = (lane & 15) >> 2, vc = (lane & 3) >> 1, vb = (lane & 1) * 8;
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(tv + tile_at<D>(sub * 32 + 4 * g + vr, 2 * d + vc) + vb));
+                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(tv + tile_at<D>(sub * 32 + 16 + 4 * g + vr, 2 * d + vc) + vb));
+                typedef short s8 __attribute__((ext_vector_type(8)));
+                const v8 va = __builtin_bit_cast(v8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int x = 0; x < X::LIMBS; x++)
+#pragma unroll
+                    for (int t = 0; t < RT; t++) o[t][d] = X::mfma(va, p[t][x], o[t][d]);
+            }
+            if constexpr (OWN) {
+                if (k0 + KB > n && bad[buf]) {
+                    for (int j = 0; j < 32; j++) {
+                        const int64_t key = key0 + j;
+                        if (key >= end) break;
+#pragma unroll
+                        for (int t = 0; t < RT; t++) {
+                            float mine = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+                                if ((i >> 2) == (j >> 4) && (i & 3) == (j & 3)) mine = pf[t][i];
+                            const float w = __shfl(mine, ((j >> 2) & 3) * 16 + col);
+                            const bool on = sees(key, r0 + t * 16 + col);
+#pragma unroll
+                            for (int d = 0; d < DT; d++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    const float v = (float)V[key * kstride + d * 16 + 4 * g + i];
+                                    if (on && !(fabsf(v) < __builtin_inff())) o[t][d][i] += w * v;
+                                }
+                        }
+                    }
+                }
+            }
+        }
+    };
+
+    if (tid < 2) bad[tid] = 0;
+    if (begin < end) {
+        fetch(begin);
+        __syncthreads();
+        put(begin, 0);
+        if (begin + KB < end) fetch(begin + KB);
+        __syncthreads();
+        int buf = 0;
+        for (int64_t k0 = begin; k0 < end; k0 += KB) {
+            if constexpr (NBUF == 2) {
+                if (k0 + KB < end) put(k0 + KB, buf ^ 1);
+                if (k0 + 2 * KB < end) fetch(k0 + 2 * KB);
+                if (r0 < sp.rows) compute(k0, buf);
+                __syncthreads();
+                buf ^= 1;
+            } else {
+                if (r0 < sp.rows) compute(k0, 0);
+                __syncthreads();
+                if (k0 + KB < end) {
+                    put(k0 + KB, 0);
+                    if (k0 + 2 * KB < end) fetch(k0 + 2 * KB);
+                    __syncthreads();
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) l[t] = sum_groups(l[t]);
+
+    const int64_t all_rows = (int64_t)a.n_seq * a.M * a.n_q, part = (int64_t)(sp.first + split) * all_rows;
+    auto place = [&](int r) { return part + token(r) * a.n_q + hk * G + r % G; };
+    if constexpr (WK == 1) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int r = r0 + t * 16 + col;
+            if (r < sp.rows) {
+                const int64_t at = place(r);
+                if (g == 0) ml[at] = float2{m[t], l[t]};
+#pragma unroll
+                for (int d = 0; d < DT; d++) *(f4 *)(opart + at * D + d * 16 + 4 * g) = o[t][d];
+            }
+        }
+    } else {
+        // the waves of a row block that took different keys meet in LDS: [wave][row][value], 16-byte pieces permuted
+        f4 *const meet = (f4 *)lds;
+        constexpr int Q = D / 4;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int r = t * 16 + col;
+            if (g == 0) wml[wave][r] = float2{m[t], l[t]};
+#pragma unroll
+            for (int d = 0; d < DT; d++) meet[(wave * RT * 16 + r) * Q + ((d * 4 + g) ^ (r & 7))] = o[t][d];
+        }
+        __syncthreads();
+        for (int i = tid; i < ROWS * Q; i += NT) {
+            const int r = i / Q, ch = i % Q, w = r / (RT * 16), rr = r % (RT * 16), at_row = rb * ROWS + r;
+            if (at_row >= sp.rows) break;
+            float top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < WK; x++) top = fmaxf(top, wml[w * WK + x][rr].x);
+            f4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < WK; x++) {
+                const float2 e = wml[w * WK + x][rr];
+                const float keep = e.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(e.x - top);
+                sum += keep * e.y;
+                acc += keep * meet[((w * WK + x) * RT * 16 + rr) * Q + (ch ^ (rr & 7))];
+            }
+            const int64_t at = place(at_row);
+            if (ch == 0) ml[at] = float2{top, sum};
+            *(f4 *)(opart + at * D + ch * 4) = acc;
+        }
+    }
+}
+
+// A wave a row: the parts' results, each times 2^(its maximum - the largest), over their sum.
+template <int D> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int parts, const float *__restrict__ opart,
+                                                                       const float2 *__restrict__ ml) {
+    __shared__ float weight[4][256];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t rows = (int64_t)a.n_seq * a.M * a.n_q, row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= rows) return;
+    const int64_t tok = row / a.n_q;
+    const int h = (int)(row - tok * a.n_q), n = a.len[tok / a.M];
+    if (n < 0) return;
+    constexpr int E = D / 64;
+    float *out = a.out + tok * a.ldo + (int64_t)h * D + lane * E;
+    typedef float ve __attribute__((ext_vector_type(E)));
+    ve acc = (ve)0.f;
+    float sum = 0.f;
+    if ((int64_t)n + a.M <= a.capacity) {
+        float top = -__builtin_inff();
+        for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[(int64_t)i * rows + row].x);
+        top = wave_max(top);
+        for (int i = lane; i < parts; i += 64) {
+            const float2 e = ml[(int64_t)i * rows + row];
+            const float keep = e.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(e.x - top);
+            weight[wave][i] = keep;
+            sum += keep * e.y;
+        }
+        sum = wave_sum(sum);
+        __builtin_amdgcn_wave_barrier();
+        for (int i = 0; i < parts; i++) {
+            const float keep = weight[wave][i];
+            if (keep == 0.f) continue;
+            acc += keep * *(const ve *)(opart + ((int64_t)i * rows + row) * D + lane * E);
+        }
+        acc = sum == 0.f ? (ve)0.f : acc / sum;
+    } else {
+        acc = (ve)__builtin_nanf("");
+    }
+    *(ve *)out = acc;
+}
+
+// ---- launch shapes ----
+
+constexpr int MOST_PARTS = 256;
+
+// Row-block rows of the variant that serves `rows` query rows of a key head.
+int block_rows(int D, int64_t rows) {
+    if (D == 256) return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+}
+
+struct AttnPlan {
+    AttnSplit pre, own;
+    int parts, pre_rows, own_rows;
+};
+
+AttnPlan plan_of(const AttnArgs &a) {
+    AttnPlan p{};
+    const int64_t G = a.n_q / a.n_kv;
+    // one workgroup fills a CU: ranges of keys are added until there are about 256, none shorter than 64 keys
+    if (a.P > 0) {
+        const int64_t rows = (int64_t)a.n_seq * a.M * G;
+        p.pre_rows = block_rows(a.head_dim, rows);
+        p.pre.rows = (int)rows;
+        p.pre.blocks = (int)((rows + p.pre_rows - 1) / p.pre_rows);
+        int64_t splits = 256 / ((int64_t)p.pre.blocks * a.n_kv);
+        splits = splits < 1 ? 1 : splits > 128 ? 128 : splits;
+        const int64_t most = (a.P + 63) / 64;
+        splits = splits < most ? splits : most;
+        p.pre.per = ((a.P + splits - 1) / splits + 31) / 32 * 32;
+        p.pre.splits = (int)((a.P + p.pre.per - 1) / p.pre.per);
+    }
+    const int64_t rows = (int64_t)a.M * G;
+    p.own_rows = block_rows(a.head_dim, rows);
+    p.own.rows = (int)rows;
+    p.own.blocks = (int)((rows + p.own_rows - 1) / p.own_rows);
+    int64_t splits = 512 / ((int64_t)p.own.blocks * a.n_kv * a.n_seq);
+    splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
+    const int64_t most = (a.capacity + 127) / 128;
+    p.own.splits = (int)(splits < most ? splits : most);
+    p.own.first = p.pre.splits;
+    p.parts = p.pre.splits + p.own.splits;
+    return p;
+}
+
+template <int TYPE, int D, int RT, int WR, int WK, int KB, int NBUF, bool OWN>
+hipError_t launch_part(const AttnArgs &a, const AttnSplit &sp, float *opart, float2 *ml, hipStream_t st) {
+    const int64_t units = (int64_t)sp.splits * a.n_kv;
+    const int64_t grid = OWN ? units * sp.blocks * a.n_seq : (units + 7) / 8 * 8 * sp.blocks;
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    attn_part_kernel<TYPE, D, RT, WR, WK, KB, NBUF, OWN><<<(unsigned)grid, WR * WK * 64, 0, st>>>(a, sp, opart, ml);
+    return hipGetLastError();
+}
+
+template <int TYPE, int D, bool OWN>
+hipError_t launch_parts(const AttnArgs &a, const AttnSplit &sp, int rows, float *opart, float2 *ml, hipStream_t st) {
+    if constexpr (D == 256) {
+        if (rows == 16) return launch_part<TYPE, D, 1, 1, 4, 128, 1, OWN>(a, sp, opart, ml, st);
+        if (rows == 32) return launch_part<TYPE, D, 1, 2, 2, 64, 2, OWN>(a, sp, opart, ml, st);
+        if (rows == 64) return launch_part<TYPE, D, 1, 4, 2, 64, 2, OWN>(a, sp, opart, ml, st);
+        return launch_part<TYPE, D, 1, 8, 1, 64, 2, OWN>(a, sp, opart, ml, st);
+    } else {
+        if (rows == 16) return launch_part<TYPE, D, 1, 1, 4, 128, 2, OWN>(a, sp, opart, ml, st);
+        if (rows == 32) return launch_part<TYPE, D, 2, 1, 4, 128, 2, OWN>(a, sp, opart, ml, st);
+        if (rows == 64) return launch_part<TYPE, D, 2, 2, 4, 128, 2, OWN>(a, sp, opart, ml, st);
+        if (rows == 128) return launch_part<TYPE, D, 2, 4, 2, 128, 2, OWN>(a, sp, opart, ml, st);
+        return launch_part<TYPE, D, 2, 8, 1, 128, 2, OWN>(a, sp, opart, ml, st);
+    }
+}
+
+template <int TYPE, int D> hipError_t launch_all(const AttnArgs &a, const AttnPlan &p, void *ws, hipStream_t st) {
+    const int64_t rows = (int64_t)a.n_seq * a.M * a.n_q;
+    float2 *ml = (float2 *)ws;
+    float *opart = (float *)((char *)ws + ((size_t)p.parts * rows * sizeof(float2) + 255) / 256 * 256);
+    hipError_t e = hipSuccess;
+    if (a.P > 0) e = launch_parts<TYPE, D, false>(a, p.pre, p.pre_rows, opart, ml, st);
+    if (e == hipSuccess) e = launch_parts<TYPE, D, true>(a, p.own, p.own_rows, opart, ml, st);
+    if (e != hipSuccess) return e;
+    attn_join_kernel<D><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, p.parts, opart, ml);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-size_t attn_ws(const AttnArgs &) { return 16; }
+size_t attn_ws(const AttnArgs &a) {
+    const AttnPlan p = plan_of(a);
+    const size_t rows = (size_t)a.n_seq * a.M * a.n_q;
+    return (p.parts * rows * sizeof(float2) + 255) / 256 * 256 + p.parts * rows * a.head_dim * sizeof(float);
+}
 
-hipError_t launch_attn(const AttnArgs &a, void *, hipStream_t st) {
-    const dim3 grid((unsigned)(a.n_seq * a.M), (unsigned)a.n_q);
-#define ROWS(T, D) attn_row_kernel<T, D><<<grid, 64, 0, st>>>(a)
-    if (a.type == KV_F16) {
-        if (a.head_dim == 64) ROWS(KV_F16, 64);
-        else if (a.head_dim == 128) ROWS(KV_F16, 128);
-        else ROWS(KV_F16, 256);
-    } else {
-        if (a.head_dim == 64) ROWS(KV_BF16, 64);
-        else if (a.head_dim == 128) ROWS(KV_BF16, 128);
-        else ROWS(KV_BF16, 256);
-    }
-#undef ROWS
-    return hipGetLastError();
+hipError_t launch_attn(const AttnArgs &a, void *ws, hipStream_t st) {
+    const AttnPlan p = plan_of(a);
+    if (p.parts > MOST_PARTS) return hipErrorInvalidValue;
+    if (a.type == KV_F16)
+        return a.head_dim == 64    ? launch_all<KV_F16, 64>(a, p, ws, st)
+               : a.head_dim == 128 ? launch_all<KV_F16, 128>(a, p, ws, st)
+                                   : launch_all<KV_F16, 256>(a, p, ws, st);
+    return a.head_dim == 64    ? launch_all<KV_BF16, 64>(a, p, ws, st)
+           : a.head_dim == 128 ? launch_all<KV_BF16, 128>(a, p, ws, st)
+                               : launch_all<KV_BF16, 256>(a, p, ws, st);
 }
