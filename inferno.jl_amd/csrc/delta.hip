@@ -69,11 +69,521 @@ template <int DK> __global__ __launch_bounds__(64) void delta_token_kernel(Delta
     }
 }
 
+// ---- chunks of 64 tokens ----
+//
+// With G the running sum of g inside a chunk and S the state before it, the
+// chunk's writes X (row i: beta_i (v_i - S_i^T k_i), S_i the state token i
+// meets) solve (I + A) X = R, A_ij = beta_i e^(G_i - G_j) k_i.k_j below the
+// diagonal, R_i = beta_i (v_i - e^(G_i) S^T k_i); then
+//   o_i = scale (e^(G_i) S^T q_i + sum_{j<=i} e^(G_i - G_j) (q_i.k_j) x_j)
+//   S'  = e^(G_63) S + sum_j e^(G_63 - G_j) k_j x_j^T
+// Every exponent is <= 0 for g <= 0. What does not need the state is prepared
+// for all chunks at once (delta_prep_kernel): T = (I + A)^-1 by forward
+// substitution (the powers of A that a product form would need can be huge where
+// keys repeat), P_ij = e^(G_i - G_j) q_i.k_j, and q, k, T, P as fp16 operands.
+// Chunk after chunk (delta_chunk_kernel), a wave carries 16 columns of S in its
+// accumulators. The products run on 16x16x32 f16 MFMAs; an fp32 factor is two f16
+// limbs (22 bits) times a power of two - a row's for q, k and P, a column's for T
+// and for the state, R and X - and a product is hi hi + hi lo + lo hi.
+
+constexpr int CH = 64;
+constexpr int TP_BYTES = 6 * 2048;  // T or P: the six 16 x 32 blocks at or below the diagonal, two limbs
+constexpr int SCAL = 5 * CH + 16;   // floats: a, b, f, p, d per token, e^(G_63)
+
+__host__ __device__ constexpr int img_bytes(int dk) { return 2 * CH * dk * 2; }  // both limbs of 64 rows
+
+// byte of 16-byte chunk c of row r: chunks permuted so that 16 rows' loads of one chunk, and the transposing loads of 4
+// rows' two chunks, meet in no bank
+template <int DK> __device__ __forceinline__ int img_at(int r, int c) {
+    const int x = DK == 64 ? ((r >> 1) & 3) * 2 + ((r >> 3) & 1) : (r & 7) * 2 + ((r >> 3) & 1);
+    return r * (DK * 2) + ((c ^ x) << 4);
+}
+// 16 x 32 block (row tile t, columns 32 u ..) of T or P
+__device__ __forceinline__ int tp_block(int t, int u) { return t < 2 ? t : t * 2 - 2 + u; }
+
+// 2^e as a float, e in [-126, 127]
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// exponent of the power of two that brings a largest absolute value to [2^top, 2^(top + 1)); 0 for 0 and non-finite
+__device__ __forceinline__ int lift(float most, int top) {
+    const int b = (int)((__float_as_uint(most) >> 23) & 255);
+    if (b == 0 || b == 255) return 0;
+    const int e = top - (b - 127);
+    return e < -80 ? -80 : e > 80 ? 80 : e;
+}
+__device__ __forceinline__ float groups_max(float v) {
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const uint32_t y = __float_as_uint(m);
+    const auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ void split8(const float *x, float up, h8 &hi, h8 &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float v = x[i] * up;
+        const _Float16 h = (_Float16)v;
+        hi[i] = h;
+        lo[i] = (_Float16)(v - (float)h);
+    }
+}
+__device__ __forceinline__ f4 mma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mma3(h8 ah, h8 al, h8 bh, h8 bl, f4 c) { return mma(al, bh, mma(ah, bl, mma(ah, bh, c))); }
+
+struct DeltaWs {
+    char *img;    // [seq][key head][chunk]: q image, k image
+    char *tp;     // [seq][value head][chunk]: T, P
+    float *scal;  // [seq][value head][chunk][SCAL]
+    int chunks;
+};
+
+__device__ __forceinline__ int tokens_of(const DeltaArgs &a, int s) {
+    if (!a.len) return a.T;
+    const int w = a.len[s];
+    return w < 0 ? 0 : w < a.T ? w : a.T;
+}
+
+// One workgroup a chunk of a key head; its value heads two at a time.
+template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, DeltaWs w) {
+    constexpr int IMG = img_bytes(DK), LD = 68, U = DK / 32, PER = DK / 16;  // PER: 16-byte pieces of a row a thread takes
+    __shared__ __align__(16) char lds[2 * IMG > 4 * CH * LD * 4 ? 2 * IMG : 4 * CH * LD * 4];
+    __shared__ float ck[CH], cq[CH], beta[2][CH], colup[2][CH];
+    __shared__ double G[2][CH];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
+    const int c = blockIdx.x, hk = blockIdx.y, s = blockIdx.z, t0 = c * CH, n = tokens_of(a, s);
+    if (t0 >= n) return;
+    const int rep = a.n_v / a.n_k;
+
+    // rows of q (image 0) and k (image 1) to limbs: 4 threads a row
+    {
+        const int r = tid >> 2, part = tid & 3;
+        const bool in = t0 + r < n;
+        const int64_t row = (int64_t)s * a.T + t0 + r;
+        char *out = w.img + (((int64_t)s * a.n_k + hk) * w.chunks + c) * (2 * IMG);
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            const float *src = (m ? a.k + row * a.ldk : a.q + row * a.ldq) + (int64_t)hk * DK;
+            float x[PER / 2][8], sum = 0.f, most = 0.f;
+#pragma unroll
+            for (int i = 0; i < PER / 2; i++) {
+                const int ch = i * 4 + part;  // 8 values
+                *(f4 *)(x[i]) = in ? *(const f4 *)(src + ch * 8) : f4{0, 0, 0, 0};
+                *(f4 *)(x[i] + 4) = in ? *(const f4 *)(src + ch * 8 + 4) : f4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 8; j++) sum = __builtin_fmaf(x[i][j], x[i][j], sum), most = fmaxf(most, fabsf(x[i][j]));
+            }
+            sum += __shfl_xor(sum, 1);
+            most = fmaxf(most, __shfl_xor(most, 1));
+            sum += __shfl_xor(sum, 2);
+            most = fmaxf(most, __shfl_xor(most, 2));
+            const int e = lift(most, 13);
+            const float up = pow2(e);
+            if (part == 0) (m ? ck : cq)[r] = pow2(-e) * (a.l2norm ? 1.0f / sqrtf(sum + 1e-6f) : 1.0f);
+#pragma unroll
+            for (int i = 0; i < PER / 2; i++) {
+                h8 hi, lo;
+                split8(x[i], up, hi, lo);
+                const int at = m * IMG + img_at<DK>(r, i * 4 + part);
+                *(h8 *)(lds + at) = hi;
+                *(h8 *)(lds + at + IMG / 2) = lo;
+                *(h8 *)(out + at) = hi;
+                *(h8 *)(out + at + IMG / 2) = lo;
+            }
+        }
+    }
+    __syncthreads();
+    // wave t: row tile t of K K^T and Q K^T, columns up to its own tile
+    f4 kk[4], qk[4];
+    {
+        auto rows = [&](int m, int limb, int tile, int u) {
+            return *(const h8 *)(lds + m * IMG + limb * (IMG / 2) + img_at<DK>(tile * 16 + col, 4 * u + g));
+        };
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            kk[j] = qk[j] = f4{0, 0, 0, 0};
+            if (j <= wave) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const h8 bh = rows(1, 0, j, u), bl = rows(1, 1, j, u);
+                    kk[j] = mma3(rows(1, 0, wave, u), rows(1, 1, wave, u), bh, bl, kk[j]);
+                    qk[j] = mma3(rows(0, 0, wave, u), rows(0, 1, wave, u), bh, bl, qk[j]);
+                }
+            }
+        }
+    }
+    float *const M = (float *)lds;  // A of two heads, then P of two: [64][LD]
+    for (int h0 = 0; h0 < rep; h0 += 2) {
+        __syncthreads();  // (the images, or the pair before, are done with)
+        if (wave < 2 && h0 + wave < rep) {
+            const int hv = hk * rep + h0 + wave;
+            const bool in = t0 + lane < n;
+            const int64_t row = (int64_t)s * a.T + t0 + lane;
+            // fp64: a difference of two sums of the chunk keeps its digits however far both have fallen
+            double v = in ? (double)a.g[row * a.ldg + hv] : 0.0;
+            for (int o = 1; o < 64; o <<= 1) {
+                const double up = __shfl_up(v, o);
+                if (lane >= o) v += up;
+            }
+            G[wave][lane] = v;
+            beta[wave][lane] = in ? a.beta[row * a.ldb + hv] : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (h0 + h >= rep) break;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j > wave) continue;
+                const int cj = j * 16 + col;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int r = wave * 16 + 4 * g + i;
+                    const float e = cj <= r ? expf((float)(G[h][r] - G[h][cj])) * ck[cj] : 0.f;
+                    M[h * CH * LD + r * LD + cj] = cj < r ? beta[h][r] * e * (kk[j][i] * ck[r]) : 0.f;
+                    M[(2 + h) * CH * LD + r * LD + cj] = e * (qk[j][i] * (cq[r] * a.scale));
+                }
+            }
+        }
+        __syncthreads();
+        if (wave < 2 && h0 + wave < rep) {
+            // column `lane` of T: x_i = [i = lane] - sum_j A_ij x_j
+            float *const A = M + wave * CH * LD;
+            float x[CH], most = 1.f;
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                float v0 = lane == i ? 1.f : 0.f, v1 = 0.f;
+#pragma unroll
+                for (int j = 0; j < i; j += 4) {
+                    const f4 m = *(const f4 *)(A + i * LD + j);
+                    v0 = __builtin_fmaf(-m[0], x[j], v0);
+                    if (j + 1 < i) v1 = __builtin_fmaf(-m[1], x[j + 1], v1);
+                    if (j + 2 < i) v0 = __builtin_fmaf(-m[2], x[j + 2], v0);
+                    if (j + 3 < i) v1 = __builtin_fmaf(-m[3], x[j + 3], v1);
+                }
+                x[i] = v0 + v1;
+                most = fmaxf(most, fabsf(x[i]));
+            }
+            colup[wave][lane] = pow2(lift(most, 13));
+#pragma unroll
+            for (int i = 0; i < CH; i++) A[i * LD + lane] = x[i];
+        }
+        __syncthreads();
+        // operands: wave t takes row tile t of T and P of both heads
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (h0 + h >= rep) break;
+            const int64_t unit = ((int64_t)s * a.n_v + hk * rep + h0 + h) * w.chunks + c;
+            char *const out = w.tp + unit * (2 * TP_BYTES) + lane * 16;
+            const int r = wave * 16 + col;
+            const int us = wave < 2 ? 1 : 2;
+            float p[2][8], most = 0.f;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                if (u >= us) continue;
+                float t[8];
+                const float *src = M + h * CH * LD + r * LD + 32 * u + 4 * g;
+                *(f4 *)t = *(const f4 *)src, *(f4 *)(t + 4) = *(const f4 *)(src + 16);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int cj = 32 * u + 4 * g + (i & 3) + (i >> 2) * 16;
+                    // (past the row's tile nothing was written)
+                    t[i] = cj < (wave + 1) * 16 ? t[i] * colup[h][cj] : 0.f;
+                }
+                h8 hi, lo;
+                split8(t, 1.f, hi, lo);
+                char *to = out + tp_block(wave, u) * 2048;
+                *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
+                src += 2 * CH * LD;
+                *(f4 *)p[u] = *(const f4 *)src, *(f4 *)(p[u] + 4) = *(const f4 *)(src + 16);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int cj = 32 * u + 4 * g + (i & 3) + (i >> 2) * 16;
+                    if (cj >= (wave + 1) * 16) p[u][i] = 0.f;
+                    most = fmaxf(most, fabsf(p[u][i]));
+                }
+            }
+            const int e = lift(groups_max(most), 13);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                if (u >= us) continue;
+                h8 hi, lo;
+                split8(p[u], pow2(e), hi, lo);
+                char *to = out + TP_BYTES + tp_block(wave, u) * 2048;
+                *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
+            }
+            if (g == 0) {
+                float *sc = w.scal + unit * SCAL;
+                const float grown = expf((float)G[h][r]), left = expf((float)(G[h][CH - 1] - G[h][r]));
+                const float down = beta[h][r] / colup[h][r];
+                sc[r] = down;
+                sc[CH + r] = down * grown * ck[r];
+                sc[2 * CH + r] = a.scale * grown * cq[r] * pow2(e);
+                sc[3 * CH + r] = pow2(-e);
+                sc[4 * CH + r] = left * ck[r];
+                if (r == CH - 1) sc[5 * CH] = grown;
+            }
+        }
+    }
+}
+
+template <int N> struct Count {
+    static constexpr int value = N;
+};
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// NS pairs of waves, each pair 16 columns of the state. Wave A of a pair carries the state: R from K S, X = T R, the new
+// state; wave B forms the outputs from Q S and P X, and brings the next chunk's operands to LDS. The state's limbs and X's
+// go from A to B through LDS; two barriers a chunk.
+template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
+    constexpr int IMG = img_bytes(DK), U = DK / 32, R = DK / 16, NB = NS * 64;
+    constexpr int NK = IMG / 16 / NB, NTP = TP_BYTES / 16 / NB;  // pieces of an image, of T or P, a thread of B brings
+    static_assert(IMG % (16 * NB) == 0 && TP_BYTES % (16 * NB) == 0, "pieces");
+    __shared__ __align__(16) char kbuf[2][IMG], qbuf[IMG], tbuf[TP_BYTES], pbuf[TP_BYTES];
+    __shared__ __align__(16) char sbuf[NS][U * 2048], xbuf[NS][4096];
+    __shared__ __align__(16) float scal[2][SCAL];
+    __shared__ float sdown[NS][64], xdown[NS][64];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % NS;
+    const bool carries = wave < NS;
+    const int hv = blockIdx.y, s = blockIdx.z, hk = hv / (a.n_v / a.n_k), n = tokens_of(a, s), chunks = (n + CH - 1) / CH;
+    const int c0 = (blockIdx.x * NS + pair) * 16 + col;
+    const bool in = c0 < a.dv;
+    const int64_t head = ((int64_t)s * a.n_v + hv) * DK * a.dv + c0;
+
+    const char *img = w.img + ((int64_t)s * a.n_k + hk) * w.chunks * (2 * IMG);
+    const char *tp = w.tp + ((int64_t)s * a.n_v + hv) * w.chunks * (2 * TP_BYTES);
+    const float *sc = w.scal + ((int64_t)s * a.n_v + hv) * w.chunks * SCAL;
+
+    // operand of 16 rows: values 32 u + 4 g + 0..3 and 32 u + 16 + 4 g + 0..3 of row 16 t + col - the order in which the
+    // accumulators of two 16-row tiles, side by side, are a B operand
+    auto rows = [&](const char *im, int t, int u) __attribute__((always_inline)) {
+        const int r = t * 16 + col;
+        typedef _Float16 q4 __attribute__((ext_vector_type(4)));
+        const q4 x = *(const q4 *)(im + img_at<DK>(r, 4 * u + (g >> 1)) + (g & 1) * 8);
+        const q4 y = *(const q4 *)(im + img_at<DK>(r, 4 * u + 2 + (g >> 1)) + (g & 1) * 8);
+        return (h8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // operand of 16 columns 16 r .. as rows, tokens 32 u ..: transposing loads of 4 tokens x 16 values
+    auto cols = [&](const char *im, int r, int u) __attribute__((always_inline)) {
+        const int tok = 32 * u + 4 * g + (col >> 2), ch = 2 * r + ((col & 3) >> 1), b = (col & 1) * 8;
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(im + img_at<DK>(tok, ch) + b));
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(im + img_at<DK>(tok + 16, ch) + b));
+        return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto per_row = [&](int buf, int which, int t) __attribute__((always_inline)) { return *(const f4 *)(&scal[buf][which * CH + t * 16 + 4 * g]); };
+    // tiles v[0 .. 2 U2) of one column to limbs, its largest to [2^13, 2^14); returns what undoes the power of two
+    auto limbs_of = [&](const auto &v, auto &l, auto count) __attribute__((always_inline)) {
+        constexpr int U2 = decltype(count)::value;
+        float most = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2 * U2; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(v[t][i]));
+        const int e = lift(groups_max(most), 13);
+        const float up = pow2(e);
+#pragma unroll
+        for (int u = 0; u < U2; u++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = v[2 * u + (i >> 2)][i & 3];
+            split8(x, up, l[u][0], l[u][1]);
+        }
+        return pow2(-e);
+    };
+    typedef Count<U> CU;
+    typedef Count<2> C2;
+
+    u4 pk[NK], pq[NK], pt[NTP], pp[NTP];
+    const int bt = tid - NB;  // thread of the B waves
+    auto get = [&](auto &to, const char *from) __attribute__((always_inline)) {
+        constexpr int N = sizeof(to) / 16;
+#pragma unroll
+        for (int i = 0; i < N; i++) to[i] = *(const u4 *)(from + (bt + i * NB) * 16);
+    };
+    auto put = [&](char *to, const auto &from) __attribute__((always_inline)) {
+        constexpr int N = sizeof(from) / 16;
+#pragma unroll
+        for (int i = 0; i < N; i++) *(u4 *)(to + (bt + i * NB) * 16) = from[i];
+    };
+    auto put_scal = [&](int c) __attribute__((always_inline)) {
+        for (int i = bt; i < SCAL; i += NB) scal[c & 1][i] = sc[(int64_t)c * SCAL + i];
+    };
+
+    f4 S[R], v[4];
+    h8 Sl[U][2];
+    auto load_v = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int tok = c * CH + t * 16 + 4 * g + i;
+                v[t][i] = in && tok < n ? a.v[((int64_t)s * a.T + tok) * a.ldv + (int64_t)hv * a.dv + c0] : 0.f;
+            }
+    };
+    float Sdown = 1.f;
+    auto publish = [&]() __attribute__((always_inline)) {
+        Sdown = limbs_of(S, Sl, CU{});
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) *(h8 *)(sbuf[pair] + (u * 2 + x) * 1024 + lane * 16) = Sl[u][x];
+        sdown[pair][lane] = Sdown;
+    };
+    if (carries) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) S[r][i] = in && a.state_in ? a.state_in[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] : 0.f;
+        if (chunks) {
+            load_v(0);
+            publish();
+        }
+    } else if (chunks) {
+        get(pk, img + IMG), get(pq, img), get(pt, tp), get(pp, tp + TP_BYTES);
+        put(kbuf[0], pk), put(qbuf, pq), put(tbuf, pt);
+        put_scal(0);
+        if (chunks > 1) get(pk, img + 3 * IMG), get(pq, img + 2 * IMG), get(pt, tp + 2 * TP_BYTES);
+    }
+    __syncthreads();
+    for (int c = 0; c < chunks; c++) {
+        const int buf = c & 1;
+        const char *K = kbuf[buf];
+        f4 x[4];
+        if (carries) {
+            h8 Rl[2][2], Xl[2][2];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                x[t] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < U; u++) x[t] = mma3(rows(K, t, u), rows(K + IMG / 2, t, u), Sl[u][0], Sl[u][1], x[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[t] = per_row(buf, 0, t) * v[t] - (per_row(buf, 1, t) * Sdown) * x[t];
+            if (c + 1 < chunks) load_v(c + 1);
+            const float down = limbs_of(x, Rl, C2{});
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                x[t] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u <= t / 2; u++) {
+                    const char *T = tbuf + tp_block(t, u) * 2048 + lane * 16;
+                    x[t] = mma3(*(const h8 *)T, *(const h8 *)(T + 1024), Rl[u][0], Rl[u][1], x[t]);
+                }
+                x[t] *= down;
+            }
+            xdown[pair][lane] = limbs_of(x, Xl, C2{});
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) *(h8 *)(xbuf[pair] + (u * 2 + y) * 1024 + lane * 16) = Xl[u][y];
+        } else {
+            if (c + 1 < chunks) put(kbuf[buf ^ 1], pk), put_scal(c + 1);
+            put(pbuf, pp);
+            if (c + 2 < chunks) get(pk, img + (int64_t)(2 * c + 5) * IMG);
+            if (c + 1 < chunks) get(pp, tp + (int64_t)(2 * c + 3) * TP_BYTES);
+            h8 l[U][2];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) l[u][y] = *(const h8 *)(sbuf[pair] + (u * 2 + y) * 1024 + lane * 16);
+            const float down = sdown[pair][lane];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                x[t] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < U; u++) x[t] = mma3(rows(qbuf, t, u), rows(qbuf + IMG / 2, t, u), l[u][0], l[u][1], x[t]);
+                x[t] *= per_row(buf, 2, t) * down;
+            }
+        }
+        __syncthreads();
+        if (carries) {
+            h8 Xl[2][2];
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 4, t);
+            const float down = limbs_of(x, Xl, C2{}), grown = scal[buf][5 * CH];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                f4 y = {0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < 2; u++) y = mma3(cols(K, r, u), cols(K + IMG / 2, r, u), Xl[u][0], Xl[u][1], y);
+                S[r] = grown * S[r] + down * y;
+            }
+            publish();
+        } else {
+            if (c + 1 < chunks) put(qbuf, pq), put(tbuf, pt);
+            if (c + 2 < chunks) get(pq, img + (int64_t)(2 * c + 4) * IMG), get(pt, tp + (int64_t)(2 * c + 4) * TP_BYTES);
+            h8 l[2][2];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) l[u][y] = *(const h8 *)(xbuf[pair] + (u * 2 + y) * 1024 + lane * 16);
+            const float down = xdown[pair][lane], up = 1.0f / down;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                x[t] *= up;
+#pragma unroll
+                for (int u = 0; u <= t / 2; u++) {
+                    const char *P = pbuf + tp_block(t, u) * 2048 + lane * 16;
+                    x[t] = mma3(*(const h8 *)P, *(const h8 *)(P + 1024), l[u][0], l[u][1], x[t]);
+                }
+                x[t] *= per_row(buf, 3, t) * down;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int tok = c * CH + t * 16 + 4 * g + i;
+                    if (in && tok < n) a.o[((int64_t)s * a.T + tok) * a.ldo + (int64_t)hv * a.dv + c0] = x[t][i];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (carries && in && a.state_out) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) a.state_out[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] = S[r][i];
+    }
+}
+
+// Chunks from 32 tokens on, where no snapshots are asked for.
+bool chunked(const DeltaArgs &a, bool snapshots) { return !snapshots && a.T >= 32; }
+
+void ws_of(const DeltaArgs &a, char *ws, DeltaWs &w, size_t &bytes) {
+    w.chunks = (a.T + CH - 1) / CH;
+    const size_t img = (size_t)a.n_seq * a.n_k * w.chunks * 2 * img_bytes(a.dk);
+    const size_t tp = (size_t)a.n_seq * a.n_v * w.chunks * 2 * TP_BYTES;
+    w.img = ws, w.tp = ws + img, w.scal = (float *)(ws + img + tp);
+    bytes = img + tp + (size_t)a.n_seq * a.n_v * w.chunks * SCAL * sizeof(float);
+}
+
+template <int DK> hipError_t launch_chunked(const DeltaArgs &a, void *ws, hipStream_t st) {
+    DeltaWs w;
+    size_t bytes;
+    ws_of(a, (char *)ws, w, bytes);
+    delta_prep_kernel<DK><<<dim3((unsigned)w.chunks, (unsigned)a.n_k, (unsigned)a.n_seq), 256, 0, st>>>(a, w);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    constexpr int NS = 2;
+    delta_chunk_kernel<DK, NS><<<dim3((unsigned)((a.dv + 16 * NS - 1) / (16 * NS)), (unsigned)a.n_v, (unsigned)a.n_seq), NS * 128, 0, st>>>(a, w);
+    return hipGetLastError();
+}
+
 }  // namespace
 
-size_t delta_ws(const DeltaArgs &, bool) { return 16; }
+size_t delta_ws(const DeltaArgs &a, bool snapshots) {
+    if (!chunked(a, snapshots)) return 16;
+    DeltaWs w;
+    size_t bytes;
+    ws_of(a, nullptr, w, bytes);
+    return bytes;
+}
 
-hipError_t launch_delta(const DeltaArgs &a, void *, hipStream_t st) {
+hipError_t launch_delta(const DeltaArgs &a, void *ws, hipStream_t st) {
+    if (chunked(a, a.snap != nullptr)) return a.dk == 64 ? launch_chunked<64>(a, ws, st) : launch_chunked<128>(a, ws, st);
     const dim3 grid((unsigned)((a.dv + 31) / 32), (unsigned)a.n_v, (unsigned)a.n_seq);
     if (a.dk == 64) delta_token_kernel<64><<<grid, 64, 0, st>>>(a);
     else delta_token_kernel<128><<<grid, 64, 0, st>>>(a);
