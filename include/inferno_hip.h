@@ -453,7 +453,7 @@ int ihip_spec_advance_len(int32_t *len_dev, const int32_t *n_accepted_dev,
  * tok_stride t + head_stride h values behind k (and behind v); an entry's
  * values are contiguous. k and v are 16-byte aligned, the strides multiples
  * of 8 values; they may be of either order ([S, cap, heads, D] or [S, heads,
- * cap, D]) and pass 32 bits. The reference keeps an fp32 cache per layer
+ * cap, D]), tok_stride up to 2^24, the others past 32 bits. The reference keeps an fp32 cache per layer
  * (src/ModelCPU.jl:234-258). */
 typedef struct ihip_kv {
     int type;            /* IHIP_F16 / IHIP_BF16 */

@@ -24,6 +24,8 @@
 namespace {
 
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
 template <int TYPE> struct Kv;
@@ -188,26 +190,47 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
 #pragma unroll
         for (int d = 0; d < DT; d++) o[t][d] = f4{0, 0, 0, 0};
     }
-    // new entry j (of the sequence's M) seen by this lane's row of tile t
-    auto sees = [&](int64_t key, int r) {
-        if (key < n) return true;
-        const int j = (int)(key - n), mine = r / G;
-        if (r >= sp.rows || j >= a.M) return false;
-        return a.mask ? ((a.mask[(int64_t)s * a.M + mine] >> j) & 1) != 0 : j <= mine;
+    // which of the new entries this lane's rows see: those up to `last`, or the bits of a tree node
+    uint64_t bits[RT];
+    int last[RT];
+    if constexpr (OWN) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int r = r0 + t * 16 + col;
+            last[t] = r < sp.rows ? r / G : -1;
+            bits[t] = a.mask && r < sp.rows ? a.mask[(int64_t)s * a.M + r / G] : 0;
+        }
+    }
+    auto sees = [&](int64_t key, int t) __attribute__((always_inline)) {
+        const int64_t j = key - n;
+        return j < 0 || (a.mask ? j < a.M && (bits[t] >> (j & 63) & 1) != 0 : j <= last[t]);
     };
 
-    uint4 sk[NLD], sv[NLD];
-    auto fetch = [&](int64_t k0) {
+    // A tile's loads: a uniform base and 32-bit lane offsets; past the last key, the last key again (its scores are masked,
+    // and its values meet P = 0)
+    u4 sk[NLD], sv[NLD];
+    const uint32_t lane_at = (uint32_t)(tid / C) * (uint32_t)kstride + (uint32_t)(tid % C) * 8;
+    auto fetch = [&](int64_t k0) __attribute__((always_inline)) {
+        if (k0 + KB <= end) {
+            const T *kb = K + k0 * kstride, *vb = V + k0 * kstride;
 #pragma unroll
-        for (int i = 0; i < NLD; i++) {
-            const int idx = tid + i * NT, r = idx / C, ch = idx % C;
-            const bool in = k0 + r < end;
-            const int64_t at = (k0 + r) * kstride + ch * 8;
-            sk[i] = in ? *(const uint4 *)(K + at) : uint4{0, 0, 0, 0};
-            sv[i] = in ? *(const uint4 *)(V + at) : uint4{0, 0, 0, 0};
+            for (int i = 0; i < NLD; i++) {
+                sk[i] = *(const u4 *)(kb + lane_at);
+                sv[i] = *(const u4 *)(vb + lane_at);
+                kb += (NT / C) * kstride, vb += (NT / C) * kstride;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NLD; i++) {
+                const int64_t r = k0 + tid / C + i * (NT / C), at = (r < end ? r : end - 1) * kstride + (tid % C) * 8;
+                sk[i] = *(const u4 *)(K + at);
+                sv[i] = *(const u4 *)(V + at);
+            }
         }
     };
-    auto put = [&](int64_t k0, int buf) {
+    const int put_at = tile_at<D>(tid / C, tid % C);
+    static_assert((NT / C) % 8 == 0, "rows of a thread");
+    auto put = [&](int64_t k0, int buf) __attribute__((always_inline)) {
         char *tk = lds + buf * 2 * TILE, *tv = tk + TILE;
         if constexpr (OWN) {
             // non-finite values of new entries are taken out of the tile and added for the rows that see them
@@ -217,11 +240,12 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
                 bool any = false;
 #pragma unroll
                 for (int i = 0; i < NLD; i++) {
-                    uint32_t *w = (uint32_t *)&sv[i];
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        if ((w[j] & E) == E) w[j] &= 0xffff0000u, any = true;
-                        if ((w[j] & (E << 16)) == (E << 16)) w[j] &= 0xffffu, any = true;
+                        uint32_t w = sv[i][j];
+                        if ((w & E) == E) w &= 0xffff0000u, any = true;
+                        if ((w & (E << 16)) == (E << 16)) w &= 0xffffu, any = true;
+                        sv[i][j] = w;
                     }
                 }
                 if (any) bad[buf] = 1;
@@ -229,17 +253,28 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
         }
 #pragma unroll
         for (int i = 0; i < NLD; i++) {
-            const int idx = tid + i * NT, r = idx / C, ch = idx % C;
-            *(uint4 *)(tk + tile_at<D>(r, ch)) = sk[i];
-            *(uint4 *)(tv + tile_at<D>(r, ch)) = sv[i];
+            // (rows NT / C apart, a multiple of 8, permute their chunks alike)
+            *(u4 *)(tk + put_at + i * (NT / C) * (D * 2)) = sk[i];
+            *(u4 *)(tv + put_at + i * (NT / C) * (D * 2)) = sv[i];
         }
     };
 
-    auto compute = [&](int64_t k0, int buf) {
-        const char *tk = lds + buf * 2 * TILE, *tv = tk + TILE;
+    // LDS bytes of this lane's operands. The permutation of a row's chunks touches bits of (4 u + g) and (2 d + vc) that
+    // repeat every 16 chunks and is the same for rows 8 apart: a few addresses serve by constant offsets.
+    constexpr int KA = STEPS < 4 ? STEPS : 4, VA = DT < 8 ? DT : 8;
+    const int vr = (lane & 15) >> 2, vc = (lane & 3) >> 1, vb = (lane & 1) * 8;
+    int ka_at[KA], va_at[VA];
+#pragma unroll
+    for (int u = 0; u < KA; u++) ka_at[u] = tile_at<D>(col, 4 * u + g);
+#pragma unroll
+    for (int d = 0; d < VA; d++) va_at[d] = TILE + tile_at<D>(4 * g + vr, 2 * d + vc) + vb;
+
+    auto compute = [&](int64_t k0, int buf) __attribute__((always_inline)) {
+#pragma unroll 1
         for (int sub = wk; sub < KB / 32; sub += WK) {
             const int64_t key0 = k0 + sub * 32;
             if (key0 >= end) break;
+            const int base = buf * 2 * TILE + sub * 32 * (D * 2);
             f4 z[RT][2];
 #pragma unroll
             for (int t = 0; t < RT; t++) z[t][0] = z[t][1] = f4{0, 0, 0, 0};
@@ -247,7 +282,7 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
             for (int u = 0; u < STEPS; u++) {
                 v8 ka[2];
 #pragma unroll
-                for (int h = 0; h < 2; h++) ka[h] = *(const v8 *)(tk + tile_at<D>(sub * 32 + h * 16 + col, 4 * u + g));
+                for (int h = 0; h < 2; h++) ka[h] = *(const v8 *)(lds + base + ka_at[u % KA] + (u / KA) * 256 + h * 16 * (D * 2));
 #pragma unroll
                 for (int x = 0; x < X::LIMBS; x++)
 #pragma unroll
@@ -262,40 +297,37 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
             for (int t = 0; t < RT; t++) {
                 float x[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = z[t][i >> 2][i & 3] * c[t];
+                for (int i = 0; i < 8; i++) x[i] = z[t][i >> 2][i & 3];
                 if (partial) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int64_t key = key0 + (i >> 2) * 16 + 4 * g + (i & 3);
-                        const bool on = key < end && (!OWN || sees(key, r0 + t * 16 + col));
+                        const bool on = key < end && (!OWN || sees(key, t));
                         x[i] = on ? x[i] : -__builtin_inff();
                     }
                 }
-                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                const float top = c[t] * fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
                 // the reference point moves only when a row's maximum passes it by 2^7 (P then still fits its type)
                 if (__any(top > m[t] + 7.f)) {
-                    top = fmaxf(m[t], max_groups(top));
-                    const float keep = m[t] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[t] - top);
-                    m[t] = top;
+                    const float to = fmaxf(m[t], max_groups(top));
+                    const float keep = m[t] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[t] - to);
+                    m[t] = to;
                     l[t] *= keep;
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[t][d] *= keep;
                 }
-                const float off = m[t] == -__builtin_inff() ? 0.f : m[t] - X::BIAS;
+                const float off = m[t] == -__builtin_inff() ? 0.f : X::BIAS - m[t];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    pf[t][i] = __builtin_amdgcn_exp2f(x[i] - off);
-                    l[t] += pf[t][i];
-                }
+                for (int i = 0; i < 8; i++) pf[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c[t], off));
+                l[t] += ((pf[t][0] + pf[t][1]) + (pf[t][2] + pf[t][3])) + ((pf[t][4] + pf[t][5]) + (pf[t][6] + pf[t][7]));
                 limbs<TYPE>(pf[t], p[t]);
             }
             // transposing loads: 16 lanes read 4 keys x 16 values, lane i gets value i of the four
-            const int vr = (lane & 15) >> 2, vc = (lane & 3) >> 1, vb = (lane & 1) * 8;
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(tv + tile_at<D>(sub * 32 + 4 * g + vr, 2 * d + vc) + vb));
-                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(tv + tile_at<D>(sub * 32 + 16 + 4 * g + vr, 2 * d + vc) + vb));
-                typedef short s8 __attribute__((ext_vector_type(8)));
+                const char *at = lds + base + va_at[d % VA] + (d / VA) * 256;
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at);
+                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 16 * (D * 2)));
                 const v8 va = __builtin_bit_cast(v8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                 for (int x = 0; x < X::LIMBS; x++)
@@ -314,7 +346,7 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
                             for (int i = 0; i < 8; i++)
                                 if ((i >> 2) == (j >> 4) && (i & 3) == (j & 3)) mine = pf[t][i];
                             const float w = __shfl(mine, ((j >> 2) & 3) * 16 + col);
-                            const bool on = sees(key, r0 + t * 16 + col);
+                            const bool on = sees(key, t);
 #pragma unroll
                             for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -334,13 +366,13 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
         fetch(begin);
         __syncthreads();
         put(begin, 0);
-        if (begin + KB < end) fetch(begin + KB);
+        fetch(begin + KB < end ? begin + KB : begin);
         __syncthreads();
         int buf = 0;
         for (int64_t k0 = begin; k0 < end; k0 += KB) {
             if constexpr (NBUF == 2) {
                 if (k0 + KB < end) put(k0 + KB, buf ^ 1);
-                if (k0 + 2 * KB < end) fetch(k0 + 2 * KB);
+                fetch(k0 + 2 * KB < end ? k0 + 2 * KB : begin);
                 if (r0 < sp.rows) compute(k0, buf);
                 __syncthreads();
                 buf ^= 1;
@@ -349,7 +381,7 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
                 __syncthreads();
                 if (k0 + KB < end) {
                     put(k0 + KB, 0);
-                    if (k0 + 2 * KB < end) fetch(k0 + 2 * KB);
+                    fetch(k0 + 2 * KB < end ? k0 + 2 * KB : begin);
                     __syncthreads();
                 }
             }
@@ -404,43 +436,65 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
     }
 }
 
-// A wave a row: the parts' results, each times 2^(its maximum - the largest), over their sum.
-template <int D> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int parts, const float *__restrict__ opart,
-                                                                       const float2 *__restrict__ ml) {
-    __shared__ float weight[4][256];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t rows = (int64_t)a.n_seq * a.M * a.n_q, row = (int64_t)blockIdx.x * 4 + wave;
-    if (row >= rows) return;
+// The parts' results of a row, each times 2^(its maximum - the largest), over their sum: W waves a row (four where there
+// are many parts), each taking every W-th part, four loads in flight.
+template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int parts, const float *__restrict__ opart,
+                                                                              const float2 *__restrict__ ml) {
+    constexpr int E = D / 64, ROWS = 4 / W, LANES = W * 64;
+    __shared__ float weight[ROWS][256];
+    __shared__ float4 red[4][64];
+    __shared__ float tops[4], sums[4];
+    typedef float ve __attribute__((ext_vector_type(E)));
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, slot = wave / W, ws = wave % W;
+    const int64_t rows = (int64_t)a.n_seq * a.M * a.n_q;
+    int64_t row = (int64_t)blockIdx.x * ROWS + slot;
+    const bool real = row < rows;
+    if (!real) row = rows - 1;
     const int64_t tok = row / a.n_q;
     const int h = (int)(row - tok * a.n_q), n = a.len[tok / a.M];
-    if (n < 0) return;
-    constexpr int E = D / 64;
-    float *out = a.out + tok * a.ldo + (int64_t)h * D + lane * E;
-    typedef float ve __attribute__((ext_vector_type(E)));
-    ve acc = (ve)0.f;
-    float sum = 0.f;
-    if ((int64_t)n + a.M <= a.capacity) {
-        float top = -__builtin_inff();
-        for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[(int64_t)i * rows + row].x);
-        top = wave_max(top);
-        for (int i = lane; i < parts; i += 64) {
-            const float2 e = ml[(int64_t)i * rows + row];
-            const float keep = e.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(e.x - top);
-            weight[wave][i] = keep;
-            sum += keep * e.y;
-        }
-        sum = wave_sum(sum);
-        __builtin_amdgcn_wave_barrier();
-        for (int i = 0; i < parts; i++) {
-            const float keep = weight[wave][i];
-            if (keep == 0.f) continue;
-            acc += keep * *(const ve *)(opart + ((int64_t)i * rows + row) * D + lane * E);
-        }
-        acc = sum == 0.f ? (ve)0.f : acc / sum;
-    } else {
-        acc = (ve)__builtin_nanf("");
+    float top = -__builtin_inff(), sum = 0.f;
+    for (int i = ws * 64 + lane; i < parts; i += LANES) top = fmaxf(top, ml[(int64_t)i * rows + row].x);
+    top = wave_max(top);
+    if constexpr (W > 1) {
+        if (lane == 0) tops[wave] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     }
-    *(ve *)out = acc;
+    for (int i = ws * 64 + lane; i < parts; i += LANES) {
+        const float2 e = ml[(int64_t)i * rows + row];
+        const float keep = e.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(e.x - top);
+        weight[slot][i] = keep;
+        sum += keep * e.y;
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    if constexpr (W > 1) sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    ve acc = (ve)0.f;
+    const float *src = opart + row * D + lane * E;
+    for (int i = ws; i < parts; i += 4 * W) {
+        ve v[4];
+        float k[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int at = i + j * W < parts ? i + j * W : i;
+            v[j] = *(const ve *)(src + (int64_t)at * rows * D);
+            k[j] = i + j * W < parts ? weight[slot][at] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (i + j * W < parts) acc += k[j] * v[j];
+    }
+    if constexpr (W > 1) {
+        *(ve *)&red[wave][lane] = acc;
+        __syncthreads();
+        if (wave) return;
+        acc = (*(ve *)&red[0][lane] + *(ve *)&red[1][lane]) + (*(ve *)&red[2][lane] + *(ve *)&red[3][lane]);
+    }
+    if (!real || n < 0) return;
+    if ((int64_t)n + a.M > a.capacity) acc = (ve)__builtin_nanf("");  // (its parts were not written)
+    else acc = sum == 0.f ? (ve)0.f : acc / sum;
+    *(ve *)(a.out + tok * a.ldo + (int64_t)h * D + lane * E) = acc;
 }
 
 // ---- launch shapes ----
@@ -520,7 +574,8 @@ template <int TYPE, int D> hipError_t launch_all(const AttnArgs &a, const AttnPl
     if (a.P > 0) e = launch_parts<TYPE, D, false>(a, p.pre, p.pre_rows, opart, ml, st);
     if (e == hipSuccess) e = launch_parts<TYPE, D, true>(a, p.own, p.own_rows, opart, ml, st);
     if (e != hipSuccess) return e;
-    attn_join_kernel<D><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, p.parts, opart, ml);
+    if (p.parts > 8) attn_join_kernel<D, 4><<<(unsigned)rows, 256, 0, st>>>(a, p.parts, opart, ml);
+    else attn_join_kernel<D, 1><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, p.parts, opart, ml);
     return hipGetLastError();
 }
 

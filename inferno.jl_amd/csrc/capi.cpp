@@ -1006,6 +1006,7 @@ int check_rope(const char *name, const ihip_rope *r) {
 int check_kv(const char *name, const char *what, const ihip_kv *c) {
     if (!c || !c->k || !c->v) return fail(IHIP_EFAULT, "%s: NULL pointer in %s", name, what);
     if (c->type != IHIP_F16 && c->type != IHIP_BF16) return fail(IHIP_EINVAL, "%s: %s of type %d", name, what, c->type);
+    if (c->tok_stride > (1 << 24)) return fail(IHIP_EINVAL, "%s: %s tok_stride %lld above 2^24", name, what, (long long)c->tok_stride);
     if (c->n_seq < 1 || c->n_seq > 65535 || c->n_kv < 1 || c->n_kv > 4096 || c->head_dim < 8 || (c->head_dim & 7) ||
         c->head_dim > 65536 || c->capacity < 1 || c->capacity > 0x7fffffff)
         return fail(IHIP_EINVAL, "%s: %s of n_seq=%d n_kv=%d head_dim=%d capacity=%lld", name, what, c->n_seq, c->n_kv,
