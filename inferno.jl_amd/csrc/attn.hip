@@ -94,8 +94,8 @@ struct AttnSplit {
 };
 
 // WR x WK waves: wave (wr, wk) takes rows [16 RT wr, ..) of the block and every WK-th 32 keys of a tile of KB keys; the
-// tile is loaded to registers one round ahead and goes through NBUF buffers in LDS.
-template <int TYPE, int D, int RT, int WR, int WK, int KB, int NBUF, bool OWN>
+// next tile goes, part by part, through registers to the other buffer in LDS while one is worked on.
+template <int TYPE, int D, int RT, int WR, int WK, int KB, int ST, bool OWN>
 __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, AttnSplit sp, float *__restrict__ opart,
                                                               float2 *__restrict__ ml) {
     typedef Kv<TYPE> X;
@@ -104,8 +104,8 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
     constexpr int NT = WR * WK * 64, C = D / 8, STEPS = D / 32, DT = D / 16, ROWS = WR * RT * 16;
     constexpr int TILE = KB * D * 2, NLD = KB * C / NT;
     static_assert(KB % (32 * WK) == 0 && KB * C % NT == 0, "tile shape");
-    static_assert(WK == 1 || NBUF * 2 * TILE >= WR * WK * RT * 16 * D * 4, "the waves' results meet in the tile buffers");
-    __shared__ __align__(16) char lds[NBUF * 2 * TILE];  // NBUF x (K tile, V tile)
+    static_assert(WK == 1 || 4 * TILE >= WR * WK * RT * 16 * D * 4, "the waves' results meet in the tile buffers");
+    __shared__ __align__(16) char lds[4 * TILE];  // two of (K tile, V tile)
     __shared__ int bad[2];
     __shared__ float2 wml[WR * WK][RT * 16];
 
@@ -201,61 +201,63 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
             bits[t] = a.mask && r < sp.rows ? a.mask[(int64_t)s * a.M + r / G] : 0;
         }
     }
-    auto sees = [&](int64_t key, int t) __attribute__((always_inline)) {
-        const int64_t j = key - n;
-        return j < 0 || (a.mask ? j < a.M && (bits[t] >> (j & 63) & 1) != 0 : j <= last[t]);
+    // (no branches: of entry j behind n, below 0 one of the sequence's own)
+    const int tree = OWN && a.mask != nullptr;
+    auto sees = [&](int j, int t) __attribute__((always_inline)) {
+        const int in_tree = (int)(j < 0) | ((int)(j < a.M) & (int)(bits[t] >> (j & 63) & 1)), before = (int)(j <= last[t]);
+        return (tree & in_tree) | ((tree ^ 1) & before);
     };
 
-    // A tile's loads: a uniform base and 32-bit lane offsets; past the last key, the last key again (its scores are masked,
-    // and its values meet P = 0)
-    u4 sk[NLD], sv[NLD];
+    // A tile comes in ST parts through registers, a part ahead: a uniform base and 32-bit lane offsets; past the last key,
+    // the last key again (its scores are masked, and its values meet P = 0).
+    constexpr int RL = NT / C;  // rows a load of the workgroup covers, a multiple of 8: they permute alike
+    static_assert(RL % 8 == 0 && NLD % ST == 0, "rows of a load");
+    u4 sk[NLD / ST], sv[NLD / ST];
     const uint32_t lane_at = (uint32_t)(tid / C) * (uint32_t)kstride + (uint32_t)(tid % C) * 8;
-    auto fetch = [&](int64_t k0) __attribute__((always_inline)) {
-        if (k0 + KB <= end) {
+    const int put_at = tile_at<D>(tid / C, tid % C);
+    auto fetch = [&](int64_t k0, int part) __attribute__((always_inline)) {
+        k0 += part * (KB / ST);
+        if (k0 + KB / ST <= end) {
             const T *kb = K + k0 * kstride, *vb = V + k0 * kstride;
 #pragma unroll
-            for (int i = 0; i < NLD; i++) {
+            for (int i = 0; i < NLD / ST; i++) {
                 sk[i] = *(const u4 *)(kb + lane_at);
                 sv[i] = *(const u4 *)(vb + lane_at);
-                kb += (NT / C) * kstride, vb += (NT / C) * kstride;
+                kb += RL * kstride, vb += RL * kstride;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NLD; i++) {
-                const int64_t r = k0 + tid / C + i * (NT / C), at = (r < end ? r : end - 1) * kstride + (tid % C) * 8;
+            for (int i = 0; i < NLD / ST; i++) {
+                const int64_t r = k0 + tid / C + i * RL, at = (r < end ? r : end - 1) * kstride + (tid % C) * 8;
                 sk[i] = *(const u4 *)(K + at);
                 sv[i] = *(const u4 *)(V + at);
             }
         }
     };
-    const int put_at = tile_at<D>(tid / C, tid % C);
-    static_assert((NT / C) % 8 == 0, "rows of a thread");
-    auto put = [&](int64_t k0, int buf) __attribute__((always_inline)) {
-        char *tk = lds + buf * 2 * TILE, *tv = tk + TILE;
-        if constexpr (OWN) {
-            // non-finite values of new entries are taken out of the tile and added for the rows that see them
-            // (0 times infinity would reach the others)
-            if (k0 + KB > n) {
-                constexpr uint32_t E = TYPE == KV_F16 ? 0x7c00u : 0x7f80u;
-                bool any = false;
+    auto put = [&](int buf, int part) __attribute__((always_inline)) {
+        char *tk = lds + buf * 2 * TILE + part * (TILE / ST) + put_at;
 #pragma unroll
-                for (int i = 0; i < NLD; i++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t w = sv[i][j];
-                        if ((w & E) == E) w &= 0xffff0000u, any = true;
-                        if ((w & (E << 16)) == (E << 16)) w &= 0xffffu, any = true;
-                        sv[i][j] = w;
-                    }
-                }
-                if (any) bad[buf] = 1;
-            }
+        for (int i = 0; i < NLD / ST; i++) {
+            *(u4 *)(tk + i * RL * (D * 2)) = sk[i];
+            *(u4 *)(tk + TILE + i * RL * (D * 2)) = sv[i];
         }
-#pragma unroll
+    };
+    // Non-finite values of new entries are taken out of the tile and added for the rows that see them (0 times infinity
+    // would reach the others).
+    auto sift = [&](int buf) __attribute__((always_inline)) {
+        constexpr uint32_t E = TYPE == KV_F16 ? 0x7c00u : 0x7f80u;
         for (int i = 0; i < NLD; i++) {
-            // (rows NT / C apart, a multiple of 8, permute their chunks alike)
-            *(u4 *)(tk + put_at + i * (NT / C) * (D * 2)) = sk[i];
-            *(u4 *)(tv + put_at + i * (NT / C) * (D * 2)) = sv[i];
+            u4 *at = (u4 *)(lds + buf * 2 * TILE + TILE + (i * NT + tid) * 16);
+            u4 v = *at;
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t w = v[j];
+                if ((w & E) == E) w &= 0xffff0000u, any = true;
+                if ((w & (E << 16)) == (E << 16)) w &= 0xffffu, any = true;
+                v[j] = w;
+            }
+            if (any) *at = v, bad[buf] = 1;
         }
     };
 
@@ -269,9 +271,9 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
 #pragma unroll
     for (int d = 0; d < VA; d++) va_at[d] = TILE + tile_at<D>(4 * g + vr, 2 * d + vc) + vb;
 
-    auto compute = [&](int64_t k0, int buf) __attribute__((always_inline)) {
+    auto compute = [&](int64_t k0, int buf, int part) __attribute__((always_inline)) {
 #pragma unroll 1
-        for (int sub = wk; sub < KB / 32; sub += WK) {
+        for (int sub = part * (KB / 32 / ST) + wk; sub < (part + 1) * (KB / 32 / ST); sub += WK) {
             const int64_t key0 = k0 + sub * 32;
             if (key0 >= end) break;
             const int base = buf * 2 * TILE + sub * 32 * (D * 2);
@@ -290,35 +292,54 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
 #pragma unroll
                         for (int h = 0; h < 2; h++) z[t][h] = X::mfma(ka[h], q[t][u][x], z[t][h]);
             }
+            // (the operand loads two steps ahead of the products)
+            __builtin_amdgcn_sched_group_barrier(0x100, STEPS < 2 ? 2 : 4, 0);
+#pragma unroll
+            for (int u = 0; u + 2 < STEPS; u++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * RT * X::LIMBS, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4 * RT * X::LIMBS, 0);
             const bool partial = OWN ? key0 + 32 > n : key0 + 32 > end;
-            v8 p[RT][X::LIMBS];
-            float pf[RT][8];
+            if (partial) {
+                const int there = (int)(end - key0 < 32 ? end - key0 : 32), j0 = OWN ? (int)(key0 - n) : 0;
 #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = z[t][i >> 2][i & 3];
-                if (partial) {
+                for (int t = 0; t < RT; t++)
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int64_t key = key0 + (i >> 2) * 16 + 4 * g + (i & 3);
-                        const bool on = key < end && (!OWN || sees(key, t));
-                        x[i] = on ? x[i] : -__builtin_inff();
+                        const int at = (i >> 2) * 16 + 4 * g + (i & 3);
+                        int on = (int)(at < there);
+                        if constexpr (OWN) on &= sees(j0 + at, t);
+                        z[t][i >> 2][i & 3] = on ? z[t][i >> 2][i & 3] : -__builtin_inff();
                     }
-                }
-                const float top = c[t] * fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                // the reference point moves only when a row's maximum passes it by 2^7 (P then still fits its type)
-                if (__any(top > m[t] + 7.f)) {
-                    const float to = fmaxf(m[t], max_groups(top));
+            }
+            float top[RT];
+            bool past = false;
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const f4 x = z[t][0], y = z[t][1];
+                top[t] = c[t] * fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+                past |= top[t] > m[t] + 7.f;
+            }
+            // the reference point moves only when a row's maximum passes it by 2^7 (P then still fits its type)
+            if (__any(past)) {
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    const float to = fmaxf(m[t], max_groups(top[t]));
                     const float keep = m[t] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[t] - to);
                     m[t] = to;
                     l[t] *= keep;
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[t][d] *= keep;
                 }
+            }
+            v8 p[RT][X::LIMBS];
+            float pf[RT][8];
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
                 const float off = m[t] == -__builtin_inff() ? 0.f : X::BIAS - m[t];
 #pragma unroll
-                for (int i = 0; i < 8; i++) pf[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c[t], off));
+                for (int i = 0; i < 8; i++) pf[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i >> 2][i & 3], c[t], off));
                 l[t] += ((pf[t][0] + pf[t][1]) + (pf[t][2] + pf[t][3])) + ((pf[t][4] + pf[t][5]) + (pf[t][6] + pf[t][7]));
                 limbs<TYPE>(pf[t], p[t]);
             }
@@ -334,6 +355,13 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
 #pragma unroll
                     for (int t = 0; t < RT; t++) o[t][d] = X::mfma(va, p[t][x], o[t][d]);
             }
+            __builtin_amdgcn_sched_group_barrier(0x100, 6, 1);
+#pragma unroll
+            for (int d = 0; d + 3 < DT; d++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, RT * X::LIMBS, 1);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 3 * RT * X::LIMBS, 1);
             if constexpr (OWN) {
                 if (k0 + KB > n && bad[buf]) {
                     for (int j = 0; j < 32; j++) {
@@ -346,7 +374,7 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
                             for (int i = 0; i < 8; i++)
                                 if ((i >> 2) == (j >> 4) && (i & 3) == (j & 3)) mine = pf[t][i];
                             const float w = __shfl(mine, ((j >> 2) & 3) * 16 + col);
-                            const bool on = sees(key, t);
+                            const int on = sees((int)(key - n), t);
 #pragma unroll
                             for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -363,30 +391,30 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
 
     if (tid < 2) bad[tid] = 0;
     if (begin < end) {
-        fetch(begin);
+#pragma unroll
+        for (int part = 0; part < ST; part++) fetch(begin, part), put(0, part);
+        fetch(begin + KB < end ? begin + KB : begin, 0);
+    }
+    int buf = 0;
+    for (int64_t k0 = begin; k0 < end; k0 += KB, buf ^= 1) {
         __syncthreads();
-        put(begin, 0);
-        fetch(begin + KB < end ? begin + KB : begin);
-        __syncthreads();
-        int buf = 0;
-        for (int64_t k0 = begin; k0 < end; k0 += KB) {
-            if constexpr (NBUF == 2) {
-                if (k0 + KB < end) put(k0 + KB, buf ^ 1);
-                fetch(k0 + 2 * KB < end ? k0 + 2 * KB : begin);
-                if (r0 < sp.rows) compute(k0, buf);
+        if constexpr (OWN) {
+            if (k0 + KB > n) {
+                sift(buf);
                 __syncthreads();
-                buf ^= 1;
-            } else {
-                if (r0 < sp.rows) compute(k0, 0);
-                __syncthreads();
-                if (k0 + KB < end) {
-                    put(k0 + KB, 0);
-                    fetch(k0 + 2 * KB < end ? k0 + 2 * KB : begin);
-                    __syncthreads();
-                }
             }
         }
+        // (the last tiles' loads and stores of a tile that is not there repeat the first: no branch, no use)
+        const int64_t k1 = k0 + KB < end ? k0 + KB : begin, k2 = k0 + 2 * KB < end ? k0 + 2 * KB : begin;
+#pragma unroll
+        for (int part = 0; part < ST; part++) {
+            put(buf ^ 1, part);
+            if (part + 1 < ST) fetch(k1, part + 1);
+            else fetch(k2, 0);
+            if (r0 < sp.rows) compute(k0, buf, part);
+        }
     }
+    if constexpr (WK > 1) __syncthreads();
 #pragma unroll
     for (int t = 0; t < RT; t++) l[t] = sum_groups(l[t]);
 
@@ -503,7 +531,7 @@ constexpr int MOST_PARTS = 256;
 
 // Row-block rows of the variant that serves `rows` query rows of a key head.
 int block_rows(int D, int64_t rows) {
-    if (D == 256) return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    if (D == 256) return rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
 }
 
@@ -541,26 +569,25 @@ AttnPlan plan_of(const AttnArgs &a) {
     return p;
 }
 
-template <int TYPE, int D, int RT, int WR, int WK, int KB, int NBUF, bool OWN>
+template <int TYPE, int D, int RT, int WR, int WK, int KB, int ST, bool OWN>
 hipError_t launch_part(const AttnArgs &a, const AttnSplit &sp, float *opart, float2 *ml, hipStream_t st) {
     const int64_t units = (int64_t)sp.splits * a.n_kv;
     const int64_t grid = OWN ? units * sp.blocks * a.n_seq : (units + 7) / 8 * 8 * sp.blocks;
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    attn_part_kernel<TYPE, D, RT, WR, WK, KB, NBUF, OWN><<<(unsigned)grid, WR * WK * 64, 0, st>>>(a, sp, opart, ml);
+    attn_part_kernel<TYPE, D, RT, WR, WK, KB, ST, OWN><<<(unsigned)grid, WR * WK * 64, 0, st>>>(a, sp, opart, ml);
     return hipGetLastError();
 }
 
 template <int TYPE, int D, bool OWN>
 hipError_t launch_parts(const AttnArgs &a, const AttnSplit &sp, int rows, float *opart, float2 *ml, hipStream_t st) {
     if constexpr (D == 256) {
-        if (rows == 16) return launch_part<TYPE, D, 1, 1, 4, 128, 1, OWN>(a, sp, opart, ml, st);
-        if (rows == 32) return launch_part<TYPE, D, 1, 2, 2, 64, 2, OWN>(a, sp, opart, ml, st);
-        if (rows == 64) return launch_part<TYPE, D, 1, 4, 2, 64, 2, OWN>(a, sp, opart, ml, st);
+        if (rows == 32) return launch_part<TYPE, D, 1, 2, 2, 64, 1, OWN>(a, sp, opart, ml, st);
+        if (rows == 64) return launch_part<TYPE, D, 1, 4, 2, 64, 1, OWN>(a, sp, opart, ml, st);
         return launch_part<TYPE, D, 1, 8, 1, 64, 2, OWN>(a, sp, opart, ml, st);
     } else {
-        if (rows == 16) return launch_part<TYPE, D, 1, 1, 4, 128, 2, OWN>(a, sp, opart, ml, st);
-        if (rows == 32) return launch_part<TYPE, D, 2, 1, 4, 128, 2, OWN>(a, sp, opart, ml, st);
-        if (rows == 64) return launch_part<TYPE, D, 2, 2, 4, 128, 2, OWN>(a, sp, opart, ml, st);
+        if (rows == 16) return launch_part<TYPE, D, 1, 1, 4, 128, 1, OWN>(a, sp, opart, ml, st);
+        if (rows == 32) return launch_part<TYPE, D, 2, 1, 4, 128, 1, OWN>(a, sp, opart, ml, st);
+        if (rows == 64) return launch_part<TYPE, D, 2, 2, 4, 128, 1, OWN>(a, sp, opart, ml, st);
         if (rows == 128) return launch_part<TYPE, D, 2, 4, 2, 128, 2, OWN>(a, sp, opart, ml, st);
         return launch_part<TYPE, D, 2, 8, 1, 128, 2, OWN>(a, sp, opart, ml, st);
     }
