@@ -561,7 +561,7 @@ int ihip_attn_prefix(const float *q_dev, int64_t ldq, float *out_dev,
  * each sequence, clamped to T; o and snapshots past them are left as they
  * were, and with 0 or less state_out is state_in. All fp32. dk 64 or 128, dv
  * a multiple of 4 up to 512; pointers 16-byte aligned (g and beta: 4), ld's
- * multiples of 4 (ldg, ldb: any). o may not overlap the inputs. ws:
+ * multiples of 4 up to 2^24 (ldg, ldb: any). o may not overlap the inputs. ws:
  * ihip_delta_ws_bytes, 16-byte aligned, not shared by calls that overlap in
  * time. Few tokens (and every call with snapshots) go one by one; many go in
  * chunks of 64 on the matrix cores, where each chunk's tokens become one

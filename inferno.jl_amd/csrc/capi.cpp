@@ -1194,7 +1194,7 @@ int ihip_gated_delta_rule(const ihip_delta *d, void *ws, size_t ws_bytes, void *
     if (rc != IHIP_OK) return rc;
     const int64_t wk = (int64_t)d->n_k * d->dk, wv = (int64_t)d->n_v * d->dv;
     if (d->ldq < wk || d->ldk < wk || d->ldv < wv || d->ldo < wv || d->ldg < d->n_v || d->ldb < d->n_v ||
-        ((d->ldq | d->ldk | d->ldv | d->ldo) & 3))
+        ((d->ldq | d->ldk | d->ldv | d->ldo) & 3) || d->ldv > (1 << 24) || d->ldo > (1 << 24))
         return fail(IHIP_EINVAL, "ihip_gated_delta_rule: rows at ldq=%lld ldk=%lld ldv=%lld ldo=%lld ldg=%lld ldb=%lld",
                     (long long)d->ldq, (long long)d->ldk, (long long)d->ldv, (long long)d->ldo, (long long)d->ldg,
                     (long long)d->ldb);

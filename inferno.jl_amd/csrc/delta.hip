@@ -337,13 +337,15 @@ typedef __attribute__((address_space(3))) s4 lds_s4;
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 // NS pairs of waves, each pair 16 columns of the state. Wave A of a pair carries the state: R from K S, X = T R, the new
-// state; wave B forms the outputs from Q S and P X, and brings the next chunk's operands to LDS. The state's limbs and X's
-// go from A to B through LDS; two barriers a chunk.
+// state; wave B forms the outputs from Q S and P X, and brings the next chunk's operands to LDS, half a chunk ahead. The
+// state's limbs and X's go from A to B through LDS; two barriers a chunk.
 template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
     constexpr int IMG = img_bytes(DK), U = DK / 32, R = DK / 16, NB = NS * 64;
-    constexpr int NK = IMG / 16 / NB, NTP = TP_BYTES / 16 / NB;  // pieces of an image, of T or P, a thread of B brings
+    constexpr int NI = IMG / 16 / NB, NTP = TP_BYTES / 16 / NB;  // pieces of an image, of T or P, a thread of B brings
     static_assert(IMG % (16 * NB) == 0 && TP_BYTES % (16 * NB) == 0, "pieces");
-    __shared__ __align__(16) char kbuf[2][IMG], qbuf[IMG], tbuf[TP_BYTES], pbuf[TP_BYTES];
+    // kbuf 2 x IMG, qbuf IMG, T, P
+    constexpr int QB = 2 * IMG, TB = 3 * IMG, PB = TB + TP_BYTES;
+    __shared__ __align__(16) char lds[PB + TP_BYTES];
     __shared__ __align__(16) char sbuf[NS][U * 2048], xbuf[NS][4096];
     __shared__ __align__(16) float scal[2][SCAL];
     __shared__ float sdown[NS][64], xdown[NS][64];
@@ -351,31 +353,40 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % NS;
     const bool carries = wave < NS;
     const int hv = blockIdx.y, s = blockIdx.z, hk = hv / (a.n_v / a.n_k), n = tokens_of(a, s), chunks = (n + CH - 1) / CH;
-    const int c0 = (blockIdx.x * NS + pair) * 16 + col;
+    const int w0 = (blockIdx.x * NS + pair) * 16, c0 = w0 + col;
     const bool in = c0 < a.dv;
     const int64_t head = ((int64_t)s * a.n_v + hv) * DK * a.dv + c0;
+    const char *const lane16 = lds + lane * 16;
 
     const char *img = w.img + ((int64_t)s * a.n_k + hk) * w.chunks * (2 * IMG);
     const char *tp = w.tp + ((int64_t)s * a.n_v + hv) * w.chunks * (2 * TP_BYTES);
     const float *sc = w.scal + ((int64_t)s * a.n_v + hv) * w.chunks * SCAL;
 
-    // operand of 16 rows: values 32 u + 4 g + 0..3 and 32 u + 16 + 4 g + 0..3 of row 16 t + col - the order in which the
-    // accumulators of two 16-row tiles, side by side, are a B operand
-    auto rows = [&](const char *im, int t, int u) __attribute__((always_inline)) {
-        const int r = t * 16 + col;
-        typedef _Float16 q4 __attribute__((ext_vector_type(4)));
-        const q4 x = *(const q4 *)(im + img_at<DK>(r, 4 * u + (g >> 1)) + (g & 1) * 8);
-        const q4 y = *(const q4 *)(im + img_at<DK>(r, 4 * u + 2 + (g >> 1)) + (g & 1) * 8);
-        return (h8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    // Operand of 16 rows: values 32 u + 4 g + 0..3 and 32 u + 16 + 4 g + 0..3 of row 16 t + col - the order in which the
+    // accumulators of two 16-row tiles, side by side, are a B operand. (Rows 16 apart permute alike: the lanes' addresses
+    // are kept, tiles and limbs are constant offsets.)
+    int ra[U][2], ca[R];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) ra[u][h] = img_at<DK>(col, 4 * u + 2 * h + (g >> 1)) + (g & 1) * 8;
+    typedef _Float16 q4 __attribute__((ext_vector_type(4)));
+    auto rows = [&](int base, int t, int u) __attribute__((always_inline)) {
+        const char *im = lds + base + t * 16 * (DK * 2);
+        return (h8)__builtin_shufflevector(*(const q4 *)(im + ra[u][0]), *(const q4 *)(im + ra[u][1]), 0, 1, 2, 3, 4, 5, 6, 7);
     };
     // operand of 16 columns 16 r .. as rows, tokens 32 u ..: transposing loads of 4 tokens x 16 values
-    auto cols = [&](const char *im, int r, int u) __attribute__((always_inline)) {
-        const int tok = 32 * u + 4 * g + (col >> 2), ch = 2 * r + ((col & 3) >> 1), b = (col & 1) * 8;
-        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(im + img_at<DK>(tok, ch) + b));
-        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(im + img_at<DK>(tok + 16, ch) + b));
+#pragma unroll
+    for (int r = 0; r < R; r++) ca[r] = img_at<DK>(4 * g + (col >> 2), 2 * r + ((col & 3) >> 1)) + (col & 1) * 8;
+    auto cols = [&](int base, int r, int u) __attribute__((always_inline)) {
+        const char *im = lds + base + ca[r] + 32 * u * (DK * 2);
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)im);
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(im + 16 * (DK * 2)));
         return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto per_row = [&](int buf, int which, int t) __attribute__((always_inline)) { return *(const f4 *)(&scal[buf][which * CH + t * 16 + 4 * g]); };
+    auto per_row = [&](int buf, int which, int t) __attribute__((always_inline)) {
+        return *(const f4 *)(&scal[buf][which * CH + t * 16 + 4 * g]);
+    };
     // tiles v[0 .. 2 U2) of one column to limbs, its largest to [2^13, 2^14); returns what undoes the power of two
     auto limbs_of = [&](const auto &v, auto &l, auto count) __attribute__((always_inline)) {
         constexpr int U2 = decltype(count)::value;
@@ -397,33 +408,82 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
     };
     typedef Count<U> CU;
     typedef Count<2> C2;
-
-    u4 pk[NK], pq[NK], pt[NTP], pp[NTP];
-    const int bt = tid - NB;  // thread of the B waves
-    auto get = [&](auto &to, const char *from) __attribute__((always_inline)) {
-        constexpr int N = sizeof(to) / 16;
+    // x[t] += rows of an image times the limbs l (the four tiles' products in turn, so that none waits for its own last)
+    auto image_times = [&](int base, const auto &l, f4 (&x)[4]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < N; i++) to[i] = *(const u4 *)(from + (bt + i * NB) * 16);
+        for (int t = 0; t < 4; t++) x[t] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            h8 hi[4], lo[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) hi[t] = rows(base, t, u), lo[t] = rows(base + IMG / 2, t, u);
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[t] = mma(hi[t], l[u][0], x[t]);
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[t] = mma(hi[t], l[u][1], x[t]);
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[t] = mma(lo[t], l[u][0], x[t]);
+        }
     };
-    auto put = [&](char *to, const auto &from) __attribute__((always_inline)) {
-        constexpr int N = sizeof(from) / 16;
+    // x[t] += T or P times the limbs l
+    auto lower_times = [&](int base, const h8 (&l)[2][2], f4 (&x)[4]) __attribute__((always_inline)) {
+        const char *at = lane16 + base;
 #pragma unroll
-        for (int i = 0; i < N; i++) *(u4 *)(to + (bt + i * NB) * 16) = from[i];
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+#pragma unroll
+                for (int t = 2 * u; t < 4; t++)
+                    x[t] = mma(*(const h8 *)(at + tp_block(t, u) * 2048 + (p == 2 ? 1024 : 0)), l[u][p == 1], x[t]);
+    };
+
+    // B: a chunk's operands come in two sets, an image and T or P each: K with P of the chunk before, Q with T
+    u4 st[NI + NTP];
+    const uint32_t b16 = (uint32_t)(tid - NB) * 16;
+    auto get = [&](const char *image, const char *low) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) st[i] = *(const u4 *)(image + i * NB * 16 + b16);
+#pragma unroll
+        for (int i = 0; i < NTP; i++) st[NI + i] = *(const u4 *)(low + i * NB * 16 + b16);
+    };
+    auto put = [&](int image, int low) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) *(u4 *)(lds + image + i * NB * 16 + b16) = st[i];
+#pragma unroll
+        for (int i = 0; i < NTP; i++) *(u4 *)(lds + low + i * NB * 16 + b16) = st[NI + i];
     };
     auto put_scal = [&](int c) __attribute__((always_inline)) {
-        for (int i = bt; i < SCAL; i += NB) scal[c & 1][i] = sc[(int64_t)c * SCAL + i];
+        for (int i = tid - NB; i < SCAL; i += NB) scal[c & 1][i] = sc[(int64_t)c * SCAL + i];
     };
+    // (past the last chunk the last one again: loads without a branch, never used)
+    auto q_of = [&](int c) __attribute__((always_inline)) { return img + (int64_t)(c < chunks ? c : chunks - 1) * (2 * IMG); };
+    auto t_of = [&](int c) __attribute__((always_inline)) { return tp + (int64_t)(c < chunks ? c : chunks - 1) * (2 * TP_BYTES); };
 
+    // A lane's values of v and o: rows 4 g + i of a tile, column c0
+    const uint32_t v_at = (uint32_t)(4 * g) * (uint32_t)a.ldv + (uint32_t)(in ? c0 : 0);
+    const uint32_t o_at = (uint32_t)(4 * g) * (uint32_t)a.ldo + (uint32_t)c0;
+    const float *const vb = a.v + (int64_t)s * a.T * a.ldv + (int64_t)hv * a.dv;
+    float *const ob = a.o + (int64_t)s * a.T * a.ldo + (int64_t)hv * a.dv;
     f4 S[R], v[4];
     h8 Sl[U][2];
     auto load_v = [&](int c) __attribute__((always_inline)) {
+        if (c >= chunks) return;
+        const float *from = vb + (int64_t)c * CH * a.ldv;
+        if ((c + 1) * CH <= n) {
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int tok = c * CH + t * 16 + 4 * g + i;
-                v[t][i] = in && tok < n ? a.v[((int64_t)s * a.T + tok) * a.ldv + (int64_t)hv * a.dv + c0] : 0.f;
-            }
+                for (int i = 0; i < 4; i++) v[t][i] = (from + (int64_t)(t * 16 + i) * a.ldv)[v_at];
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int tok = c * CH + t * 16 + 4 * g + i;
+                    const float x = vb[(int64_t)(tok < n ? tok : n - 1) * a.ldv + (in ? c0 : 0)];
+                    v[t][i] = tok < n ? x : 0.f;
+                }
+        }
     };
     float Sdown = 1.f;
     auto publish = [&]() __attribute__((always_inline)) {
@@ -439,84 +499,79 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int i = 0; i < 4; i++) S[r][i] = in && a.state_in ? a.state_in[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] : 0.f;
-        if (chunks) {
-            load_v(0);
-            publish();
-        }
+        load_v(0);
+        publish();
     } else if (chunks) {
-        get(pk, img + IMG), get(pq, img), get(pt, tp), get(pp, tp + TP_BYTES);
-        put(kbuf[0], pk), put(qbuf, pq), put(tbuf, pt);
+        get(q_of(0) + IMG, t_of(0) + TP_BYTES);
+        put(0, PB);
+        get(q_of(0), t_of(0));
+        put(QB, TB);
         put_scal(0);
-        if (chunks > 1) get(pk, img + 3 * IMG), get(pq, img + 2 * IMG), get(pt, tp + 2 * TP_BYTES);
+        get(q_of(1) + IMG, t_of(0) + TP_BYTES);
     }
     __syncthreads();
     for (int c = 0; c < chunks; c++) {
-        const int buf = c & 1;
-        const char *K = kbuf[buf];
+        const int buf = c & 1, K = buf * IMG;
         f4 x[4];
         if (carries) {
-            h8 Rl[2][2], Xl[2][2];
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                x[t] = f4{0, 0, 0, 0};
-#pragma unroll
-                for (int u = 0; u < U; u++) x[t] = mma3(rows(K, t, u), rows(K + IMG / 2, t, u), Sl[u][0], Sl[u][1], x[t]);
-            }
+            h8 l[2][2];
+            image_times(K, Sl, x);
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] = per_row(buf, 0, t) * v[t] - (per_row(buf, 1, t) * Sdown) * x[t];
-            if (c + 1 < chunks) load_v(c + 1);
-            const float down = limbs_of(x, Rl, C2{});
+            load_v(c + 1);
+            const float down = limbs_of(x, l, C2{});
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                x[t] = f4{0, 0, 0, 0};
+            for (int t = 0; t < 4; t++) x[t] = f4{0, 0, 0, 0};
+            lower_times(TB, l, x);
 #pragma unroll
-                for (int u = 0; u <= t / 2; u++) {
-                    const char *T = tbuf + tp_block(t, u) * 2048 + lane * 16;
-                    x[t] = mma3(*(const h8 *)T, *(const h8 *)(T + 1024), Rl[u][0], Rl[u][1], x[t]);
-                }
-                x[t] *= down;
-            }
-            xdown[pair][lane] = limbs_of(x, Xl, C2{});
+            for (int t = 0; t < 4; t++) x[t] *= down;
+            xdown[pair][lane] = limbs_of(x, l, C2{});
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int y = 0; y < 2; y++) *(h8 *)(xbuf[pair] + (u * 2 + y) * 1024 + lane * 16) = Xl[u][y];
+                for (int y = 0; y < 2; y++) *(h8 *)(xbuf[pair] + (u * 2 + y) * 1024 + lane * 16) = l[u][y];
         } else {
-            if (c + 1 < chunks) put(kbuf[buf ^ 1], pk), put_scal(c + 1);
-            put(pbuf, pp);
-            if (c + 2 < chunks) get(pk, img + (int64_t)(2 * c + 5) * IMG);
-            if (c + 1 < chunks) get(pp, tp + (int64_t)(2 * c + 3) * TP_BYTES);
+            put(K ^ IMG, PB);
+            if (c + 1 < chunks) put_scal(c + 1);
+            get(q_of(c + 1), t_of(c + 1));
             h8 l[U][2];
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int y = 0; y < 2; y++) l[u][y] = *(const h8 *)(sbuf[pair] + (u * 2 + y) * 1024 + lane * 16);
             const float down = sdown[pair][lane];
+            image_times(QB, l, x);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                x[t] = f4{0, 0, 0, 0};
-#pragma unroll
-                for (int u = 0; u < U; u++) x[t] = mma3(rows(qbuf, t, u), rows(qbuf + IMG / 2, t, u), l[u][0], l[u][1], x[t]);
-                x[t] *= per_row(buf, 2, t) * down;
-            }
+            for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 2, t) * down;
         }
         __syncthreads();
         if (carries) {
-            h8 Xl[2][2];
+            h8 l[2][2];
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 4, t);
-            const float down = limbs_of(x, Xl, C2{}), grown = scal[buf][5 * CH];
+            const float down = limbs_of(x, l, C2{}), grown = scal[buf][5 * CH];
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                f4 y = {0, 0, 0, 0};
+            for (int r = 0; r < R; r += 2) {
+                f4 y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-                for (int u = 0; u < 2; u++) y = mma3(cols(K, r, u), cols(K + IMG / 2, r, u), Xl[u][0], Xl[u][1], y);
-                S[r] = grown * S[r] + down * y;
+                for (int u = 0; u < 2; u++) {
+                    h8 hi[2], lo[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) hi[j] = cols(K, r + j, u), lo[j] = cols(K + IMG / 2, r + j, u);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) y[j] = mma(hi[j], l[u][0], y[j]);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) y[j] = mma(hi[j], l[u][1], y[j]);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) y[j] = mma(lo[j], l[u][0], y[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) S[r + j] = grown * S[r + j] + down * y[j];
             }
             publish();
         } else {
-            if (c + 1 < chunks) put(qbuf, pq), put(tbuf, pt);
-            if (c + 2 < chunks) get(pq, img + (int64_t)(2 * c + 4) * IMG), get(pt, tp + (int64_t)(2 * c + 4) * TP_BYTES);
+            put(QB, TB);
+            get(q_of(c + 2) + IMG, t_of(c + 1) + TP_BYTES);
             h8 l[2][2];
 #pragma unroll
             for (int u = 0; u < 2; u++)
@@ -524,19 +579,22 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
                 for (int y = 0; y < 2; y++) l[u][y] = *(const h8 *)(xbuf[pair] + (u * 2 + y) * 1024 + lane * 16);
             const float down = xdown[pair][lane], up = 1.0f / down;
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                x[t] *= up;
+            for (int t = 0; t < 4; t++) x[t] *= up;
+            lower_times(PB, l, x);
+            float *to = ob + (int64_t)c * CH * a.ldo;
 #pragma unroll
-                for (int u = 0; u <= t / 2; u++) {
-                    const char *P = pbuf + tp_block(t, u) * 2048 + lane * 16;
-                    x[t] = mma3(*(const h8 *)P, *(const h8 *)(P + 1024), l[u][0], l[u][1], x[t]);
-                }
-                x[t] *= per_row(buf, 3, t) * down;
+            for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 3, t) * down;
+            if ((c + 1) * CH <= n && w0 + 16 <= a.dv) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int tok = c * CH + t * 16 + 4 * g + i;
-                    if (in && tok < n) a.o[((int64_t)s * a.T + tok) * a.ldo + (int64_t)hv * a.dv + c0] = x[t][i];
-                }
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (in && c * CH + t * 16 + 4 * g + i < n) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
             }
         }
         __syncthreads();
