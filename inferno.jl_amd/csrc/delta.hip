@@ -326,37 +326,34 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
     }
 }
 
-template <int N> struct Count {
-    static constexpr int value = N;
-};
-
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// NS pairs of waves, each pair 16 columns of the state. Wave A of a pair carries the state: R from K S, X = T R, the new
-// state; wave B forms the outputs from Q S and P X, and brings the next chunk's operands to LDS, half a chunk ahead. The
-// state's limbs and X's go from A to B through LDS; two barriers a chunk.
-template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
+// NS groups of three waves, each group 16 columns of the state. Wave A of a group carries the state: R from K S, X = T R,
+// the new state. Wave B forms the outputs from Q S and P X. Wave C brings the chunks' operands to LDS, loaded a chunk
+// ahead. The state's limbs and X go from A to B through LDS; two barriers a chunk: B works on Q S while A finds X, and on
+// P X while A forms the new state.
+template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
     constexpr int IMG = img_bytes(DK), U = DK / 32, R = DK / 16, NB = NS * 64;
-    constexpr int NI = IMG / 16 / NB, NTP = TP_BYTES / 16 / NB;  // pieces of an image, of T or P, a thread of B brings
+    constexpr int NI = IMG / 16 / NB, NTP = TP_BYTES / 16 / NB;  // 16-byte pieces of an image, of T or P, a thread of C brings
+    constexpr int NSC = (SCAL / 4 + NB - 1) / NB;
     static_assert(IMG % (16 * NB) == 0 && TP_BYTES % (16 * NB) == 0, "pieces");
     // kbuf 2 x IMG, qbuf IMG, T, P
     constexpr int QB = 2 * IMG, TB = 3 * IMG, PB = TB + TP_BYTES;
     __shared__ __align__(16) char lds[PB + TP_BYTES];
     __shared__ __align__(16) char sbuf[NS][U * 2048], xbuf[NS][4096];
     __shared__ __align__(16) float scal[2][SCAL];
-    __shared__ float sdown[NS][64], xdown[NS][64];
+    __shared__ float sdown[NS][64];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % NS;
-    const bool carries = wave < NS;
+    const bool carries = wave < NS, brings = wave >= 2 * NS;
     const int hv = blockIdx.y, s = blockIdx.z, hk = hv / (a.n_v / a.n_k), n = tokens_of(a, s), chunks = (n + CH - 1) / CH;
     const int w0 = (blockIdx.x * NS + pair) * 16, c0 = w0 + col;
     const bool in = c0 < a.dv;
     const int64_t head = ((int64_t)s * a.n_v + hv) * DK * a.dv + c0;
-    const char *const lane16 = lds + lane * 16;
 
     const char *img = w.img + ((int64_t)s * a.n_k + hk) * w.chunks * (2 * IMG);
     const char *tp = w.tp + ((int64_t)s * a.n_v + hv) * w.chunks * (2 * TP_BYTES);
@@ -369,7 +366,9 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) ra[u][h] = img_at<DK>(col, 4 * u + 2 * h + (g >> 1)) + (g & 1) * 8;
+        for (int h = 0; h < 2; h++) ra[u][h] = (carries ? 0 : QB) + img_at<DK>(col, 4 * u + 2 * h + (g >> 1)) + (g & 1) * 8;
+    int low_at = lane * 16 + (carries ? TB : PB);
+    asm("" : "+v"(low_at));  // (kept as one register: the blocks are constant offsets from it)
     typedef _Float16 q4 __attribute__((ext_vector_type(4)));
     auto rows = [&](int base, int t, int u) __attribute__((always_inline)) {
         const char *im = lds + base + t * 16 * (DK * 2);
@@ -387,18 +386,17 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
     auto per_row = [&](int buf, int which, int t) __attribute__((always_inline)) {
         return *(const f4 *)(&scal[buf][which * CH + t * 16 + 4 * g]);
     };
-    // tiles v[0 .. 2 U2) of one column to limbs, its largest to [2^13, 2^14); returns what undoes the power of two
-    auto limbs_of = [&](const auto &v, auto &l, auto count) __attribute__((always_inline)) {
-        constexpr int U2 = decltype(count)::value;
+    // the four tiles of one column to limbs, its largest to [2^13, 2^14); returns what undoes the power of two
+    auto limbs_of = [&](const f4 (&v)[4], h8 (&l)[2][2]) __attribute__((always_inline)) {
         float most = 0.f;
 #pragma unroll
-        for (int t = 0; t < 2 * U2; t++)
+        for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(v[t][i]));
         const int e = lift(groups_max(most), 13);
         const float up = pow2(e);
 #pragma unroll
-        for (int u = 0; u < U2; u++) {
+        for (int u = 0; u < 2; u++) {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = v[2 * u + (i >> 2)][i & 3];
@@ -406,54 +404,74 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
         }
         return pow2(-e);
     };
-    typedef Count<U> CU;
-    typedef Count<2> C2;
-    // x[t] += rows of an image times the limbs l (the four tiles' products in turn, so that none waits for its own last)
+    // x[t] = rows of an image (A: K at `base`, B: Q) times the limbs l: the four tiles' products in turn, so that none waits
+    // for its own last; the next operands are on their way meanwhile
     auto image_times = [&](int base, const auto &l, f4 (&x)[4]) __attribute__((always_inline)) {
+        h8 hi[2][4], lo[2][4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) x[t] = f4{0, 0, 0, 0};
+        for (int t = 0; t < 4; t++) {
+            x[t] = f4{0, 0, 0, 0};
+            hi[0][t] = rows(base, t, 0), lo[0][t] = rows(base + IMG / 2, t, 0);
+        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            h8 hi[4], lo[4];
+            if (u + 1 < U) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) hi[t] = rows(base, t, u), lo[t] = rows(base + IMG / 2, t, u);
+                for (int t = 0; t < 4; t++) hi[(u + 1) & 1][t] = rows(base, t, u + 1), lo[(u + 1) & 1][t] = rows(base + IMG / 2, t, u + 1);
+            }
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = mma(hi[t], l[u][0], x[t]);
+            for (int t = 0; t < 4; t++) x[t] = mma(hi[u & 1][t], l[u][0], x[t]);
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = mma(hi[t], l[u][1], x[t]);
+            for (int t = 0; t < 4; t++) x[t] = mma(hi[u & 1][t], l[u][1], x[t]);
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = mma(lo[t], l[u][0], x[t]);
+            for (int t = 0; t < 4; t++) x[t] = mma(lo[u & 1][t], l[u][0], x[t]);
         }
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+        for (int u = 0; u + 1 < U; u++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+            }
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 12, 0);
     };
-    // x[t] += T or P times the limbs l
-    auto lower_times = [&](int base, const h8 (&l)[2][2], f4 (&x)[4]) __attribute__((always_inline)) {
-        const char *at = lane16 + base;
+    // x[t] += T (A) or P (B) times the limbs l
+    auto lower_times = [&](const h8 (&l)[2][2], f4 (&x)[4]) __attribute__((always_inline)) {
+        h8 m[6][2];
+#pragma unroll
+        for (int i = 0; i < 6; i++)
+#pragma unroll
+            for (int y = 0; y < 2; y++) m[i][y] = *(const h8 *)(lds + low_at + i * 2048 + y * 1024);
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int p = 0; p < 3; p++)
 #pragma unroll
-                for (int t = 2 * u; t < 4; t++)
-                    x[t] = mma(*(const h8 *)(at + tp_block(t, u) * 2048 + (p == 2 ? 1024 : 0)), l[u][p == 1], x[t]);
+                for (int t = 2 * u; t < 4; t++) x[t] = mma(m[tp_block(t, u)][p == 2], l[u][p == 1], x[t]);
     };
 
-    // B: a chunk's operands come in two sets, an image and T or P each: K with P of the chunk before, Q with T
-    u4 st[NI + NTP];
-    const uint32_t b16 = (uint32_t)(tid - NB) * 16;
-    auto get = [&](const char *image, const char *low) __attribute__((always_inline)) {
+    // C: a chunk's operands come in two sets, K with P of the chunk before and the factors, Q with T
+    u4 ka[NI], pa[NTP], fa[NSC], qa[NI], ta[NTP];
+    const uint32_t ct = (uint32_t)(tid - 2 * NB), c16 = ct * 16;
+    auto get = [&](auto &to, const char *from) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < NI; i++) st[i] = *(const u4 *)(image + i * NB * 16 + b16);
-#pragma unroll
-        for (int i = 0; i < NTP; i++) st[NI + i] = *(const u4 *)(low + i * NB * 16 + b16);
+        for (int i = 0; i < (int)(sizeof(to) / 16); i++) to[i] = *(const u4 *)(from + i * NB * 16 + c16);
     };
-    auto put = [&](int image, int low) __attribute__((always_inline)) {
+    auto put = [&](int to, const auto &from) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < NI; i++) *(u4 *)(lds + image + i * NB * 16 + b16) = st[i];
-#pragma unroll
-        for (int i = 0; i < NTP; i++) *(u4 *)(lds + low + i * NB * 16 + b16) = st[NI + i];
+        for (int i = 0; i < (int)(sizeof(from) / 16); i++) *(u4 *)(lds + to + i * NB * 16 + c16) = from[i];
     };
-    auto put_scal = [&](int c) __attribute__((always_inline)) {
-        for (int i = tid - NB; i < SCAL; i += NB) scal[c & 1][i] = sc[(int64_t)c * SCAL + i];
+    auto get_fac = [&](int c) __attribute__((always_inline)) {
+        const float *from = sc + (int64_t)(c < chunks ? c : chunks - 1) * SCAL;
+#pragma unroll
+        for (int i = 0; i < NSC; i++) fa[i] = *(const u4 *)(from + (ct + i * NB < SCAL / 4 ? ct + i * NB : SCAL / 4 - 1) * 4);
+    };
+    auto put_fac = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NSC; i++)
+            if (ct + i * NB < SCAL / 4) *(u4 *)&scal[c & 1][(ct + i * NB) * 4] = fa[i];
     };
     // (past the last chunk the last one again: loads without a branch, never used)
     auto q_of = [&](int c) __attribute__((always_inline)) { return img + (int64_t)(c < chunks ? c : chunks - 1) * (2 * IMG); };
@@ -485,102 +503,152 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
                 }
         }
     };
-    float Sdown = 1.f;
+    // The state's limbs: one power of two a column, kept from chunk to chunk while the column's largest stays in
+    // [2^3, 2^15) of it (below 2^15 nothing overflows, and 22 bits remain down to 2^-2).
+    float Sup = 1.f;
+    auto split_tiles = [&](int u) __attribute__((always_inline)) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = S[2 * u + (i >> 2)][i & 3];
+        split8(x, Sup, Sl[u][0], Sl[u][1]);
+    };
     auto publish = [&]() __attribute__((always_inline)) {
-        Sdown = limbs_of(S, Sl, CU{});
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
             for (int x = 0; x < 2; x++) *(h8 *)(sbuf[pair] + (u * 2 + x) * 1024 + lane * 16) = Sl[u][x];
-        sdown[pair][lane] = Sdown;
+        sdown[pair][lane] = 1.0f / Sup;
     };
+    auto largest = [&]() __attribute__((always_inline)) {
+        float most = 0.f;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r][i]));
+        return groups_max(most);
+    };
+    auto scale_state = [&](float most) __attribute__((always_inline)) {
+        Sup = pow2(lift(most, 11));
+#pragma unroll
+        for (int u = 0; u < U; u++) split_tiles(u);
+    };
+    // (a loop each, with the same two barriers a turn: no role keeps another's registers)
     if (carries) {
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int i = 0; i < 4; i++) S[r][i] = in && a.state_in ? a.state_in[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] : 0.f;
         load_v(0);
+        scale_state(largest());
         publish();
-    } else if (chunks) {
-        get(q_of(0) + IMG, t_of(0) + TP_BYTES);
-        put(0, PB);
-        get(q_of(0), t_of(0));
-        put(QB, TB);
-        put_scal(0);
-        get(q_of(1) + IMG, t_of(0) + TP_BYTES);
-    }
-    __syncthreads();
-    for (int c = 0; c < chunks; c++) {
-        const int buf = c & 1, K = buf * IMG;
-        f4 x[4];
-        if (carries) {
+        __syncthreads();
+        for (int c = 0; c < chunks; c++) {
+            const int buf = c & 1, K = buf * IMG;
+            f4 x[4];
             h8 l[2][2];
             image_times(K, Sl, x);
+            const float Sdown = 1.0f / Sup;
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] = per_row(buf, 0, t) * v[t] - (per_row(buf, 1, t) * Sdown) * x[t];
             load_v(c + 1);
-            const float down = limbs_of(x, l, C2{});
+            const float Rdown = limbs_of(x, l);
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] = f4{0, 0, 0, 0};
-            lower_times(TB, l, x);
+            lower_times(l, x);
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] *= down;
-            xdown[pair][lane] = limbs_of(x, l, C2{});
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int y = 0; y < 2; y++) *(h8 *)(xbuf[pair] + (u * 2 + y) * 1024 + lane * 16) = l[u][y];
-        } else {
-            put(K ^ IMG, PB);
-            if (c + 1 < chunks) put_scal(c + 1);
-            get(q_of(c + 1), t_of(c + 1));
-            h8 l[U][2];
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int y = 0; y < 2; y++) l[u][y] = *(const h8 *)(sbuf[pair] + (u * 2 + y) * 1024 + lane * 16);
-            const float down = sdown[pair][lane];
-            image_times(QB, l, x);
-#pragma unroll
-            for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 2, t) * down;
-        }
-        __syncthreads();
-        if (carries) {
-            h8 l[2][2];
+            for (int t = 0; t < 4; t++) {
+                x[t] *= Rdown;
+                *(f4 *)(xbuf[pair] + t * 1024 + lane * 16) = x[t];
+            }
+            __syncthreads();
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 4, t);
-            const float down = limbs_of(x, l, C2{}), grown = scal[buf][5 * CH];
+            const float down = limbs_of(x, l), grown = scal[buf][5 * CH];
+            float most = 0.f;
+            h8 hi[2][2][2], lo[2][2][2];  // [set][tile of the pair][tokens]
+            auto bring = [&](int r, int set) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) hi[set][j][u] = cols(K, r + j, u), lo[set][j][u] = cols(K + IMG / 2, r + j, u);
+            };
+            bring(0, 0);
 #pragma unroll
             for (int r = 0; r < R; r += 2) {
-                f4 y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                const int set = (r >> 1) & 1;
+                if (r + 2 < R) bring(r + 2, set ^ 1);
+                f4 y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, z[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    h8 hi[2], lo[2];
+                for (int j = 0; j < 2; j++) y[j] = mma(hi[set][j][0], l[0][0], y[j]), z[j] = mma(hi[set][j][1], l[1][0], z[j]);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) hi[j] = cols(K, r + j, u), lo[j] = cols(K + IMG / 2, r + j, u);
+                for (int j = 0; j < 2; j++) y[j] = mma(hi[set][j][0], l[0][1], y[j]), z[j] = mma(hi[set][j][1], l[1][1], z[j]);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) y[j] = mma(hi[j], l[u][0], y[j]);
+                for (int j = 0; j < 2; j++) y[j] = mma(lo[set][j][0], l[0][0], y[j]), z[j] = mma(lo[set][j][1], l[1][0], z[j]);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) y[j] = mma(hi[j], l[u][1], y[j]);
+                for (int j = 0; j < 2; j++) {
+                    S[r + j] = grown * S[r + j] + down * (y[j] + z[j]);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) y[j] = mma(lo[j], l[u][0], y[j]);
+                    for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r + j][i]));
                 }
-#pragma unroll
-                for (int j = 0; j < 2; j++) S[r + j] = grown * S[r + j] + down * y[j];
+                split_tiles(r >> 1);
             }
+            most = groups_max(most);
+            const float big = most * Sup;
+            if (__any(!(big < 32768.f && (big >= 8.f || most == 0.f)))) scale_state(most);
             publish();
-        } else {
-            put(QB, TB);
-            get(q_of(c + 2) + IMG, t_of(c + 1) + TP_BYTES);
+            __syncthreads();
+        }
+        if (in && a.state_out) {
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) a.state_out[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] = S[r][i];
+        }
+    } else if (brings) {
+        if (chunks) {
+            get(ka, q_of(0) + IMG), get(qa, q_of(0)), get(ta, t_of(0));
+            get_fac(0);
+            put(0, ka), put(QB, qa), put(TB, ta);
+            put_fac(0);
+            get(ka, q_of(1) + IMG), get(pa, t_of(0) + TP_BYTES);
+            get_fac(1);
+            get(qa, q_of(1)), get(ta, t_of(1));
+        }
+        __syncthreads();
+        for (int c = 0; c < chunks; c++) {
+            put((c & 1 ? 0 : IMG), ka), put(PB, pa);
+            put_fac(c + 1);
+            get(ka, q_of(c + 2) + IMG), get(pa, t_of(c + 1) + TP_BYTES);
+            get_fac(c + 2);
+            __syncthreads();
+            put(QB, qa), put(TB, ta);
+            get(qa, q_of(c + 2)), get(ta, t_of(c + 2));
+            __syncthreads();
+        }
+    } else {
+        __syncthreads();
+        for (int c = 0; c < chunks; c++) {
+            const int buf = c & 1;
+            f4 x[4], y[4];
+            {
+                h8 l[U][2];
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) l[u][i] = *(const h8 *)(sbuf[pair] + (u * 2 + i) * 1024 + lane * 16);
+                const float down = sdown[pair][lane];
+                image_times(0, l, x);
+#pragma unroll
+                for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 2, t) * down;
+            }
+            __syncthreads();
             h8 l[2][2];
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int y = 0; y < 2; y++) l[u][y] = *(const h8 *)(xbuf[pair] + (u * 2 + y) * 1024 + lane * 16);
-            const float down = xdown[pair][lane], up = 1.0f / down;
+            for (int t = 0; t < 4; t++) y[t] = *(const f4 *)(xbuf[pair] + t * 1024 + lane * 16);
+            const float down = limbs_of(y, l), up = 1.0f / down;
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] *= up;
-            lower_times(PB, l, x);
+            lower_times(l, x);
             float *to = ob + (int64_t)c * CH * a.ldo;
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 3, t) * down;
@@ -596,14 +664,8 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 128) void delta_chun
                     for (int i = 0; i < 4; i++)
                         if (in && c * CH + t * 16 + 4 * g + i < n) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
             }
+            __syncthreads();
         }
-        __syncthreads();
-    }
-    if (carries && in && a.state_out) {
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) a.state_out[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] = S[r][i];
     }
 }
 
@@ -625,8 +687,12 @@ template <int DK> hipError_t launch_chunked(const DeltaArgs &a, void *ws, hipStr
     delta_prep_kernel<DK><<<dim3((unsigned)w.chunks, (unsigned)a.n_k, (unsigned)a.n_seq), 256, 0, st>>>(a, w);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    constexpr int NS = 2;
-    delta_chunk_kernel<DK, NS><<<dim3((unsigned)((a.dv + 16 * NS - 1) / (16 * NS)), (unsigned)a.n_v, (unsigned)a.n_seq), NS * 128, 0, st>>>(a, w);
+    // one group a workgroup where that leaves no CU with two of them to do; else two, which share the operands in LDS
+    const unsigned groups = (unsigned)((a.dv + 15) / 16);
+    if ((int64_t)groups * a.n_v * a.n_seq <= 256)
+        delta_chunk_kernel<DK, 1><<<dim3(groups, (unsigned)a.n_v, (unsigned)a.n_seq), 192, 0, st>>>(a, w);
+    else
+        delta_chunk_kernel<DK, 2><<<dim3((groups + 1) / 2, (unsigned)a.n_v, (unsigned)a.n_seq), 384, 0, st>>>(a, w);
     return hipGetLastError();
 }
 
