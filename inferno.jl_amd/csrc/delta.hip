@@ -92,10 +92,12 @@ constexpr int SCAL = 5 * CH + 16;   // floats: a, b, f, p, d per token, e^(G_63)
 
 __host__ __device__ constexpr int img_bytes(int dk) { return 2 * CH * dk * 2; }  // both limbs of 64 rows
 
-// byte of 16-byte chunk c of row r: chunks permuted so that 16 rows' loads of one chunk, and the transposing loads of 4
-// rows' two chunks, meet in no bank
+// An image holds a row's values in the order of the operand: 16-byte piece 4 u + q has values 32 u + 4 q .. + 3 and
+// 32 u + 16 + 4 q .. + 3, what lane group q takes of 32 values when the other operand is two accumulator tiles side by
+// side. Byte of piece c of row r: the pieces of a row are permuted so that neither 16 rows' loads of one piece nor the
+// transposing loads of 4 rows' halves of 4 pieces meet in a bank.
 template <int DK> __device__ __forceinline__ int img_at(int r, int c) {
-    const int x = DK == 64 ? ((r >> 1) & 3) * 2 + ((r >> 3) & 1) : (r & 7) * 2 + ((r >> 3) & 1);
+    const int x = DK == 64 ? ((r >> 1) & 1) * 4 + ((r >> 2) & 3) : (r & 3) * 4 + ((r >> 2) & 3);
     return r * (DK * 2) + ((c ^ x) << 4);
 }
 // 16 x 32 block (row tile t, columns 32 u ..) of T or P
@@ -166,9 +168,8 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
             float x[PER / 2][8], sum = 0.f, most = 0.f;
 #pragma unroll
             for (int i = 0; i < PER / 2; i++) {
-                const int ch = i * 4 + part;  // 8 values
-                *(f4 *)(x[i]) = in ? *(const f4 *)(src + ch * 8) : f4{0, 0, 0, 0};
-                *(f4 *)(x[i] + 4) = in ? *(const f4 *)(src + ch * 8 + 4) : f4{0, 0, 0, 0};
+                *(f4 *)(x[i]) = in ? *(const f4 *)(src + i * 32 + part * 4) : f4{0, 0, 0, 0};
+                *(f4 *)(x[i] + 4) = in ? *(const f4 *)(src + i * 32 + 16 + part * 4) : f4{0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < 8; j++) sum = __builtin_fmaf(x[i][j], x[i][j], sum), most = fmaxf(most, fabsf(x[i][j]));
             }
@@ -332,6 +333,9 @@ typedef __attribute__((address_space(3))) s4 lds_s4;
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
+// nothing is moved across: loads stay ahead of the products that do not need them
+#define STAGE() __builtin_amdgcn_sched_barrier(0)
+
 // NS groups of three waves, each group 16 columns of the state. Wave A of a group carries the state: R from K S, X = T R,
 // the new state. Wave B forms the outputs from Q S and P X. Wave C brings the chunks' operands to LDS, loaded a chunk
 // ahead. The state's limbs and X go from A to B through LDS; two barriers a chunk: B works on Q S while A finds X, and on
@@ -347,11 +351,18 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
     __shared__ __align__(16) char sbuf[NS][U * 2048], xbuf[NS][4096];
     __shared__ __align__(16) float scal[2][SCAL];
     __shared__ float sdown[NS][64];
+    constexpr int LV = 16 * NS + 4;  // floats between rows of v in LDS (a row's pad keeps rows 4 apart in other banks)
+    __shared__ __align__(16) float vbuf[CH * LV];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % NS;
     const bool carries = wave < NS, brings = wave >= 2 * NS;
-    const int hv = blockIdx.y, s = blockIdx.z, hk = hv / (a.n_v / a.n_k), n = tokens_of(a, s), chunks = (n + CH - 1) / CH;
-    const int w0 = (blockIdx.x * NS + pair) * 16, c0 = w0 + col;
+    // consecutive workgroups go to the eight XCDs in turn: a head's column groups, and the heads of a key head, are given
+    // to one XCD, whose L2 then fetches the operands once for all of them
+    const int groups = (a.dv + 16 * NS - 1) / (16 * NS), heads = a.n_v * a.n_seq, per = (heads + 7) / 8;
+    const int unit = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3) / groups, grp = (int)(blockIdx.x >> 3) % groups;
+    if (unit >= heads) return;
+    const int hv = unit % a.n_v, s = unit / a.n_v, hk = hv / (a.n_v / a.n_k), n = tokens_of(a, s), chunks = (n + CH - 1) / CH;
+    const int w0 = (grp * NS + pair) * 16, c0 = w0 + col;
     const bool in = c0 < a.dv;
     const int64_t head = ((int64_t)s * a.n_v + hv) * DK * a.dv + c0;
 
@@ -359,26 +370,20 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
     const char *tp = w.tp + ((int64_t)s * a.n_v + hv) * w.chunks * (2 * TP_BYTES);
     const float *sc = w.scal + ((int64_t)s * a.n_v + hv) * w.chunks * SCAL;
 
-    // Operand of 16 rows: values 32 u + 4 g + 0..3 and 32 u + 16 + 4 g + 0..3 of row 16 t + col - the order in which the
-    // accumulators of two 16-row tiles, side by side, are a B operand. (Rows 16 apart permute alike: the lanes' addresses
-    // are kept, tiles and limbs are constant offsets.)
-    int ra[U][2], ca[R];
+    // Operand of 16 rows, 32 values; of 16 columns as rows, 32 tokens (transposing loads of 4 tokens x 16 values). Rows 16
+    // apart permute alike: the lanes' addresses are kept, tiles and limbs are constant offsets.
+    int ra[U], ca[U], low_at = lane * 16 + (carries ? TB : PB);
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) ra[u][h] = (carries ? 0 : QB) + img_at<DK>(col, 4 * u + 2 * h + (g >> 1)) + (g & 1) * 8;
-    int low_at = lane * 16 + (carries ? TB : PB);
+    for (int u = 0; u < U; u++) {
+        ra[u] = (carries ? 0 : QB) + img_at<DK>(col, 4 * u + g);
+        ca[u] = img_at<DK>(4 * g + (col >> 2), 4 * u + (col & 3));
+    }
     asm("" : "+v"(low_at));  // (kept as one register: the blocks are constant offsets from it)
-    typedef _Float16 q4 __attribute__((ext_vector_type(4)));
     auto rows = [&](int base, int t, int u) __attribute__((always_inline)) {
-        const char *im = lds + base + t * 16 * (DK * 2);
-        return (h8)__builtin_shufflevector(*(const q4 *)(im + ra[u][0]), *(const q4 *)(im + ra[u][1]), 0, 1, 2, 3, 4, 5, 6, 7);
+        return *(const h8 *)(lds + base + ra[u] + t * 16 * (DK * 2));
     };
-    // operand of 16 columns 16 r .. as rows, tokens 32 u ..: transposing loads of 4 tokens x 16 values
-#pragma unroll
-    for (int r = 0; r < R; r++) ca[r] = img_at<DK>(4 * g + (col >> 2), 2 * r + ((col & 3) >> 1)) + (col & 1) * 8;
     auto cols = [&](int base, int r, int u) __attribute__((always_inline)) {
-        const char *im = lds + base + ca[r] + 32 * u * (DK * 2);
+        const char *im = lds + base + ca[r >> 1] + (r & 1) * 8 + 32 * u * (DK * 2);
         const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)im);
         const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(im + 16 * (DK * 2)));
         return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -409,33 +414,23 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
     auto image_times = [&](int base, const auto &l, f4 (&x)[4]) __attribute__((always_inline)) {
         h8 hi[2][4], lo[2][4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            x[t] = f4{0, 0, 0, 0};
-            hi[0][t] = rows(base, t, 0), lo[0][t] = rows(base + IMG / 2, t, 0);
-        }
+        for (int t = 0; t < 4; t++) hi[0][t] = rows(base, t, 0), lo[0][t] = rows(base + IMG / 2, t, 0);
+        STAGE();
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (u + 1 < U) {
 #pragma unroll
                 for (int t = 0; t < 4; t++) hi[(u + 1) & 1][t] = rows(base, t, u + 1), lo[(u + 1) & 1][t] = rows(base + IMG / 2, t, u + 1);
+                STAGE();
             }
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = mma(hi[u & 1][t], l[u][0], x[t]);
+            for (int t = 0; t < 4; t++) x[t] = mma(hi[u & 1][t], l[u][0], u ? x[t] : f4{0, 0, 0, 0});
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] = mma(hi[u & 1][t], l[u][1], x[t]);
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] = mma(lo[u & 1][t], l[u][0], x[t]);
+            STAGE();
         }
-        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-        for (int u = 0; u + 1 < U; u++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
-            }
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, 12, 0);
     };
     // x[t] += T (A) or P (B) times the limbs l
     auto lower_times = [&](const h8 (&l)[2][2], f4 (&x)[4]) __attribute__((always_inline)) {
@@ -477,32 +472,28 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
     auto q_of = [&](int c) __attribute__((always_inline)) { return img + (int64_t)(c < chunks ? c : chunks - 1) * (2 * IMG); };
     auto t_of = [&](int c) __attribute__((always_inline)) { return tp + (int64_t)(c < chunks ? c : chunks - 1) * (2 * TP_BYTES); };
 
-    // A lane's values of v and o: rows 4 g + i of a tile, column c0
-    const uint32_t v_at = (uint32_t)(4 * g) * (uint32_t)a.ldv + (uint32_t)(in ? c0 : 0);
-    const uint32_t o_at = (uint32_t)(4 * g) * (uint32_t)a.ldo + (uint32_t)c0;
-    const float *const vb = a.v + (int64_t)s * a.T * a.ldv + (int64_t)hv * a.dv;
-    float *const ob = a.o + (int64_t)s * a.T * a.ldo + (int64_t)hv * a.dv;
-    f4 S[R], v[4];
-    h8 Sl[U][2];
-    auto load_v = [&](int c) __attribute__((always_inline)) {
-        if (c >= chunks) return;
-        const float *from = vb + (int64_t)c * CH * a.ldv;
-        if ((c + 1) * CH <= n) {
+    // C: 4 values of 4 rows of v a thread; past the last row that row again (its factor is 0), past the last column the
+    // last four (their state is never stored)
+    u4 va[4];
+    const int vr = (int)ct / (4 * NS), vc = (int)ct % (4 * NS) * 4, vx = grp * NS * 16 + vc;
+    const float *const vb = a.v + (int64_t)s * a.T * a.ldv + (int64_t)hv * a.dv + (vx + 4 <= a.dv ? vx : a.dv - 4);
+    auto get_v = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[t][i] = (from + (int64_t)(t * 16 + i) * a.ldv)[v_at];
-        } else {
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int tok = c * CH + t * 16 + 4 * g + i;
-                    const float x = vb[(int64_t)(tok < n ? tok : n - 1) * a.ldv + (in ? c0 : 0)];
-                    v[t][i] = tok < n ? x : 0.f;
-                }
+        for (int i = 0; i < 4; i++) {
+            const int tok = c * CH + i * 16 + vr;
+            va[i] = *(const u4 *)(vb + (int64_t)(tok < n ? tok : n - 1) * a.ldv);
         }
     };
+    auto put_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) *(u4 *)(vbuf + (i * 16 + vr) * LV + vc) = va[i];
+    };
+
+    // a lane's values of o: rows 4 g + i of a tile, column c0
+    const uint32_t o_at = (uint32_t)(4 * g) * (uint32_t)a.ldo + (uint32_t)c0;
+    float *const ob = a.o + (int64_t)s * a.T * a.ldo + (int64_t)hv * a.dv;
+    f4 S[R];
+    h8 Sl[U][2];
     // The state's limbs: one power of two a column, kept from chunk to chunk while the column's largest stays in
     // [2^3, 2^15) of it (below 2^15 nothing overflows, and 22 bits remain down to 2^-2).
     float Sup = 1.f;
@@ -538,7 +529,6 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int i = 0; i < 4; i++) S[r][i] = in && a.state_in ? a.state_in[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] : 0.f;
-        load_v(0);
         scale_state(largest());
         publish();
         __syncthreads();
@@ -546,11 +536,17 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             const int buf = c & 1, K = buf * IMG;
             f4 x[4];
             h8 l[2][2];
-            image_times(K, Sl, x);
             const float Sdown = 1.0f / Sup;
+            f4 v[4], fb[4];
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = per_row(buf, 0, t) * v[t] - (per_row(buf, 1, t) * Sdown) * x[t];
-            load_v(c + 1);
+            for (int t = 0; t < 4; t++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[t][i] = vbuf[(t * 16 + 4 * g + i) * LV + pair * 16 + col];
+                v[t] *= per_row(buf, 0, t), fb[t] = per_row(buf, 1, t) * Sdown;
+            }
+            image_times(K, Sl, x);
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[t] = v[t] - fb[t] * x[t];
             const float Rdown = limbs_of(x, l);
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] = f4{0, 0, 0, 0};
@@ -573,25 +569,43 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
                     for (int u = 0; u < 2; u++) hi[set][j][u] = cols(K, r + j, u), lo[set][j][u] = cols(K + IMG / 2, r + j, u);
             };
             bring(0, 0);
-#pragma unroll
-            for (int r = 0; r < R; r += 2) {
-                const int set = (r >> 1) & 1;
-                if (r + 2 < R) bring(r + 2, set ^ 1);
-                f4 y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, z[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-                for (int j = 0; j < 2; j++) y[j] = mma(hi[set][j][0], l[0][0], y[j]), z[j] = mma(hi[set][j][1], l[1][0], z[j]);
-#pragma unroll
-                for (int j = 0; j < 2; j++) y[j] = mma(hi[set][j][0], l[0][1], y[j]), z[j] = mma(hi[set][j][1], l[1][1], z[j]);
-#pragma unroll
-                for (int j = 0; j < 2; j++) y[j] = mma(lo[set][j][0], l[0][0], y[j]), z[j] = mma(lo[set][j][1], l[1][0], z[j]);
+            STAGE();
+            // a pair of tiles' products while the pair before is added to the state and split
+            f4 y[2][2], z[2][2];
+            auto add = [&](int r, int set) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    S[r + j] = grown * S[r + j] + down * (y[j] + z[j]);
+                    S[r + j] = grown * S[r + j] + down * (y[set][j] + z[set][j]);
 #pragma unroll
                     for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r + j][i]));
                 }
                 split_tiles(r >> 1);
+            };
+#pragma unroll
+            for (int r = 0; r < R; r += 2) {
+                const int set = (r >> 1) & 1;
+                if (r + 2 < R) bring(r + 2, set ^ 1);
+                STAGE();
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    y[set][j] = mma(hi[set][j][0], l[0][0], f4{0, 0, 0, 0});
+                    z[set][j] = mma(hi[set][j][1], l[1][0], f4{0, 0, 0, 0});
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) y[set][j] = mma(hi[set][j][0], l[0][1], y[set][j]), z[set][j] = mma(hi[set][j][1], l[1][1], z[set][j]);
+#pragma unroll
+                for (int j = 0; j < 2; j++) y[set][j] = mma(lo[set][j][0], l[0][0], y[set][j]), z[set][j] = mma(lo[set][j][1], l[1][0], z[set][j]);
+                if (r) {
+                    add(r - 2, set ^ 1);
+#pragma unroll
+                    for (int i = 0; i < 12; i++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+                    }
+                }
+                STAGE();
             }
+            add(R - 2, (R / 2 - 1) & 1);
             most = groups_max(most);
             const float big = most * Sup;
             if (__any(!(big < 32768.f && (big >= 8.f || most == 0.f)))) scale_state(most);
@@ -608,11 +622,14 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
         if (chunks) {
             get(ka, q_of(0) + IMG), get(qa, q_of(0)), get(ta, t_of(0));
             get_fac(0);
+            get_v(0);
             put(0, ka), put(QB, qa), put(TB, ta);
             put_fac(0);
+            put_v();
             get(ka, q_of(1) + IMG), get(pa, t_of(0) + TP_BYTES);
             get_fac(1);
             get(qa, q_of(1)), get(ta, t_of(1));
+            get_v(1);
         }
         __syncthreads();
         for (int c = 0; c < chunks; c++) {
@@ -622,7 +639,9 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             get_fac(c + 2);
             __syncthreads();
             put(QB, qa), put(TB, ta);
+            put_v();
             get(qa, q_of(c + 2)), get(ta, t_of(c + 2));
+            get_v(c + 2);
             __syncthreads();
         }
     } else {
@@ -688,11 +707,12 @@ template <int DK> hipError_t launch_chunked(const DeltaArgs &a, void *ws, hipStr
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // one group a workgroup where that leaves no CU with two of them to do; else two, which share the operands in LDS
-    const unsigned groups = (unsigned)((a.dv + 15) / 16);
-    if ((int64_t)groups * a.n_v * a.n_seq <= 256)
-        delta_chunk_kernel<DK, 1><<<dim3(groups, (unsigned)a.n_v, (unsigned)a.n_seq), 192, 0, st>>>(a, w);
+    const int groups = (a.dv + 15) / 16, heads = a.n_v * a.n_seq;
+    const int64_t per = (heads + 7) / 8;
+    if ((int64_t)groups * heads <= 256)
+        delta_chunk_kernel<DK, 1><<<(unsigned)(8 * per * groups), 192, 0, st>>>(a, w);
     else
-        delta_chunk_kernel<DK, 2><<<dim3((groups + 1) / 2, (unsigned)a.n_v, (unsigned)a.n_seq), 384, 0, st>>>(a, w);
+        delta_chunk_kernel<DK, 2><<<(unsigned)(8 * per * ((groups + 1) / 2)), 384, 0, st>>>(a, w);
     return hipGetLastError();
 }
 
