@@ -94,20 +94,38 @@ struct AttnSplit {
 };
 
 // WR x WK waves: wave (wr, wk) takes rows [16 RT wr, ..) of the block and every WK-th 32 keys of a tile of KB keys; the
-// next tile goes, part by part, through registers to the other buffer in LDS while one is worked on.
-template <int TYPE, int D, int RT, int WR, int WK, int KB, int ST, bool OWN>
-__global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, AttnSplit sp, float *__restrict__ opart,
-                                                              float2 *__restrict__ ml) {
+// next tile goes, in ST parts, through registers to the other buffer in LDS while one is worked on.
+template <int RT_, int WR_, int WK_, int KB_, int ST_> struct Shape {
+    static constexpr int RT = RT_, WR = WR_, WK = WK_, KB = KB_, ST = ST_, ROWS = WR * RT * 16;
+    static_assert(WR * WK == 8, "eight waves");
+};
+// By the rows of a block: few rows split a tile's keys over the waves, many rows share it. (Two workgroups' worth of
+// registers a SIMD, 256 each, and 128 KiB of LDS: one workgroup a CU.)
+template <int D, int ID> struct ShapeOf;
+template <int D> struct ShapeOf<D, 0> : Shape<1, 2, 4, 128, 1> {};
+template <int D> struct ShapeOf<D, 1> : Shape<2, 2, 4, 128, 1> {};
+template <int D> struct ShapeOf<D, 2> : Shape<2, 8, 1, 128, 2> {};
+template <> struct ShapeOf<256, 1> : Shape<1, 4, 2, 64, 1> {};
+template <> struct ShapeOf<256, 2> : Shape<1, 8, 1, 64, 2> {};
+
+struct Shared {
+    int bad[2];
+    float2 ml[8][32];
+};
+
+template <int TYPE, int D, typename SH, bool OWN>
+__device__ __forceinline__ void attn_part(const AttnArgs &a, const AttnSplit &sp, int block, char *lds, Shared &sh,
+                                          float *__restrict__ opart, float2 *__restrict__ ml) {
     typedef Kv<TYPE> X;
     typedef typename X::t T;
     typedef typename X::v8 v8;
+    constexpr int RT = SH::RT, WR = SH::WR, WK = SH::WK, KB = SH::KB, ST = SH::ST;
     constexpr int NT = WR * WK * 64, C = D / 8, STEPS = D / 32, DT = D / 16, ROWS = WR * RT * 16;
     constexpr int TILE = KB * D * 2, NLD = KB * C / NT;
     static_assert(KB % (32 * WK) == 0 && KB * C % NT == 0, "tile shape");
     static_assert(WK == 1 || 4 * TILE >= WR * WK * RT * 16 * D * 4, "the waves' results meet in the tile buffers");
-    __shared__ __align__(16) char lds[4 * TILE];  // two of (K tile, V tile)
-    __shared__ int bad[2];
-    __shared__ float2 wml[WR * WK][RT * 16];
+    int *const bad = sh.bad;
+    float2(*const wml)[32] = sh.ml;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave / WK, wk = wave % WK, g = lane >> 4, col = lane & 15;
@@ -119,7 +137,7 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
     const T *K, *V;
     int64_t kstride;
     if constexpr (OWN) {
-        int id = blockIdx.x;
+        int id = block;
         split = id % sp.splits, id /= sp.splits;
         rb = id % sp.blocks, id /= sp.blocks;
         hk = id % a.n_kv, s = id / a.n_kv;
@@ -134,7 +152,7 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
     } else {
         // row blocks of one range of keys go to one XCD (consecutive workgroups to the eight in turn), whose L2 then
         // holds the range for all of them
-        const int id = blockIdx.x, x = id & 7, y = id >> 3;
+        const int id = block, x = id & 7, y = id >> 3;
         rb = y % sp.blocks;
         const int pair = (y / sp.blocks) * 8 + x;
         if (pair >= sp.splits * a.n_kv) return;
@@ -146,6 +164,42 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
         V = (const T *)a.pv + hk * a.p_head_stride;
     }
     const int r0 = rb * ROWS + wr * RT * 16;
+
+    // A tile comes in ST parts through registers, a part ahead: a uniform base and 32-bit lane offsets; past the last key,
+    // the last key again (its scores are masked, and its values meet P = 0).
+    constexpr int RL = NT / C;  // rows a load of the workgroup covers, a multiple of 8: they permute alike
+    static_assert(RL % 8 == 0 && NLD % ST == 0, "rows of a load");
+    u4 sk[NLD / ST], sv[NLD / ST];
+    const uint32_t lane_at = (uint32_t)(tid / C) * (uint32_t)kstride + (uint32_t)(tid % C) * 8;
+    const int put_at = tile_at<D>(tid / C, tid % C);
+    auto fetch = [&](int64_t k0, int part) __attribute__((always_inline)) {
+        k0 += part * (KB / ST);
+        if (k0 + KB / ST <= end) {
+            const T *kb = K + k0 * kstride, *vb = V + k0 * kstride;
+#pragma unroll
+            for (int i = 0; i < NLD / ST; i++) {
+                sk[i] = *(const u4 *)(kb + lane_at);
+                sv[i] = *(const u4 *)(vb + lane_at);
+                kb += RL * kstride, vb += RL * kstride;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NLD / ST; i++) {
+                const int64_t r = k0 + tid / C + i * RL, at = (r < end ? r : end - 1) * kstride + (tid % C) * 8;
+                sk[i] = *(const u4 *)(K + at);
+                sv[i] = *(const u4 *)(V + at);
+            }
+        }
+    };
+    auto put = [&](int buf, int part) __attribute__((always_inline)) {
+        char *tk = lds + buf * 2 * TILE + part * (TILE / ST) + put_at;
+#pragma unroll
+        for (int i = 0; i < NLD / ST; i++) {
+            *(u4 *)(tk + i * RL * (D * 2)) = sk[i];
+            *(u4 *)(tk + TILE + i * RL * (D * 2)) = sv[i];
+        }
+    };
+    if (begin < end) fetch(begin, 0);  // (on its way while the queries are split)
 
     // this lane's query rows (one a row tile): the token row, its place in the sequence, its head
     auto token = [&](int r) { return (int64_t)s * a.M + r / G; };
@@ -208,40 +262,6 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
         return (tree & in_tree) | ((tree ^ 1) & before);
     };
 
-    // A tile comes in ST parts through registers, a part ahead: a uniform base and 32-bit lane offsets; past the last key,
-    // the last key again (its scores are masked, and its values meet P = 0).
-    constexpr int RL = NT / C;  // rows a load of the workgroup covers, a multiple of 8: they permute alike
-    static_assert(RL % 8 == 0 && NLD % ST == 0, "rows of a load");
-    u4 sk[NLD / ST], sv[NLD / ST];
-    const uint32_t lane_at = (uint32_t)(tid / C) * (uint32_t)kstride + (uint32_t)(tid % C) * 8;
-    const int put_at = tile_at<D>(tid / C, tid % C);
-    auto fetch = [&](int64_t k0, int part) __attribute__((always_inline)) {
-        k0 += part * (KB / ST);
-        if (k0 + KB / ST <= end) {
-            const T *kb = K + k0 * kstride, *vb = V + k0 * kstride;
-#pragma unroll
-            for (int i = 0; i < NLD / ST; i++) {
-                sk[i] = *(const u4 *)(kb + lane_at);
-                sv[i] = *(const u4 *)(vb + lane_at);
-                kb += RL * kstride, vb += RL * kstride;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NLD / ST; i++) {
-                const int64_t r = k0 + tid / C + i * RL, at = (r < end ? r : end - 1) * kstride + (tid % C) * 8;
-                sk[i] = *(const u4 *)(K + at);
-                sv[i] = *(const u4 *)(V + at);
-            }
-        }
-    };
-    auto put = [&](int buf, int part) __attribute__((always_inline)) {
-        char *tk = lds + buf * 2 * TILE + part * (TILE / ST) + put_at;
-#pragma unroll
-        for (int i = 0; i < NLD / ST; i++) {
-            *(u4 *)(tk + i * RL * (D * 2)) = sk[i];
-            *(u4 *)(tk + TILE + i * RL * (D * 2)) = sv[i];
-        }
-    };
     // Non-finite values of new entries are taken out of the tile and added for the rows that see them (0 times infinity
     // would reach the others).
     auto sift = [&](int buf) __attribute__((always_inline)) {
@@ -392,7 +412,10 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
     if (tid < 2) bad[tid] = 0;
     if (begin < end) {
 #pragma unroll
-        for (int part = 0; part < ST; part++) fetch(begin, part), put(0, part);
+        for (int part = 0; part < ST; part++) {
+            if (part) fetch(begin, part);
+            put(0, part);
+        }
         fetch(begin + KB < end ? begin + KB : begin, 0);
     }
     int buf = 0;
@@ -464,6 +487,19 @@ __global__ __launch_bounds__(WR *WK * 64) void attn_part_kernel(AttnArgs a, Attn
     }
 }
 
+// The prefix's blocks, then the sequences' own: one launch, so that the short ones fill the gaps of the long.
+template <int TYPE, int D, int PRE, int SELF>
+__global__ __launch_bounds__(512) void attn_part_kernel(AttnArgs a, AttnSplit pre, AttnSplit own, int n_pre,
+                                                      float *__restrict__ opart, float2 *__restrict__ ml) {
+    typedef ShapeOf<D, PRE> P;
+    typedef ShapeOf<D, SELF> S;
+    constexpr int KB = P::KB > S::KB ? P::KB : S::KB;
+    __shared__ __align__(16) char lds[4 * KB * D * 2];  // two of (K tile, V tile)
+    __shared__ Shared sh;
+    if ((int)blockIdx.x < n_pre) attn_part<TYPE, D, P, false>(a, pre, (int)blockIdx.x, lds, sh, opart, ml);
+    else attn_part<TYPE, D, S, true>(a, own, (int)blockIdx.x - n_pre, lds, sh, opart, ml);
+}
+
 // The parts' results of a row, each times 2^(its maximum - the largest), over their sum: W waves a row (four where there
 // are many parts), each taking every W-th part, four loads in flight.
 template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int parts, const float *__restrict__ opart,
@@ -480,6 +516,13 @@ template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(
     if (!real) row = rows - 1;
     const int64_t tok = row / a.n_q;
     const int h = (int)(row - tok * a.n_q), n = a.len[tok / a.M];
+    const float *src = opart + row * D + lane * E;
+    ve v[4];
+    auto four = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = *(const ve *)(src + (int64_t)(i + j * W < parts ? i + j * W : parts - 1) * rows * D);
+    };
+    four(ws);  // (on their way while the weights are found)
     float top = -__builtin_inff(), sum = 0.f;
     for (int i = ws * 64 + lane; i < parts; i += LANES) top = fmaxf(top, ml[(int64_t)i * rows + row].x);
     top = wave_max(top);
@@ -499,19 +542,11 @@ template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(
     __syncthreads();
     if constexpr (W > 1) sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     ve acc = (ve)0.f;
-    const float *src = opart + row * D + lane * E;
     for (int i = ws; i < parts; i += 4 * W) {
-        ve v[4];
-        float k[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int at = i + j * W < parts ? i + j * W : i;
-            v[j] = *(const ve *)(src + (int64_t)at * rows * D);
-            k[j] = i + j * W < parts ? weight[slot][at] : 0.f;
-        }
+        if (i != ws) four(i);
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (i + j * W < parts) acc += k[j] * v[j];
+            if (i + j * W < parts) acc += weight[slot][i + j * W] * v[j];
     }
     if constexpr (W > 1) {
         *(ve *)&red[wave][lane] = acc;
@@ -529,77 +564,72 @@ template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(
 
 constexpr int MOST_PARTS = 256;
 
-// Row-block rows of the variant that serves `rows` query rows of a key head.
-int block_rows(int D, int64_t rows) {
-    if (D == 256) return rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-}
+// The shape that serves `rows` query rows of a key head, and its rows a block.
+int shape_for(int D, int64_t rows) { return rows <= 32 && D < 256 ? 0 : rows <= 64 ? 1 : 2; }
+int shape_rows(int D, int id) { return id == 0 ? 32 : id == 1 ? 64 : D == 256 ? 128 : 256; }
 
 struct AttnPlan {
     AttnSplit pre, own;
-    int parts, pre_rows, own_rows;
+    int parts, pre_shape, own_shape;
 };
 
+// One workgroup fills a CU. The sequences' own entries: ranges of 128 keys or more, up to 512 workgroups; the prefix: as
+// many ranges (of 64 keys or more) as fill the chip beside them, or once over where they are many.
 AttnPlan plan_of(const AttnArgs &a) {
     AttnPlan p{};
-    const int64_t G = a.n_q / a.n_kv;
-    // one workgroup fills a CU: ranges of keys are added until there are about 256, none shorter than 64 keys
-    if (a.P > 0) {
-        const int64_t rows = (int64_t)a.n_seq * a.M * G;
-        p.pre_rows = block_rows(a.head_dim, rows);
-        p.pre.rows = (int)rows;
-        p.pre.blocks = (int)((rows + p.pre_rows - 1) / p.pre_rows);
-        int64_t splits = 256 / ((int64_t)p.pre.blocks * a.n_kv);
-        splits = splits < 1 ? 1 : splits > 128 ? 128 : splits;
-        const int64_t most = (a.P + 63) / 64;
-        splits = splits < most ? splits : most;
-        p.pre.per = ((a.P + splits - 1) / splits + 31) / 32 * 32;
-        p.pre.splits = (int)((a.P + p.pre.per - 1) / p.pre.per);
-    }
-    const int64_t rows = (int64_t)a.M * G;
-    p.own_rows = block_rows(a.head_dim, rows);
-    p.own.rows = (int)rows;
-    p.own.blocks = (int)((rows + p.own_rows - 1) / p.own_rows);
-    int64_t splits = 512 / ((int64_t)p.own.blocks * a.n_kv * a.n_seq);
+    const int64_t G = a.n_q / a.n_kv, own_rows = a.M * G;
+    p.own_shape = shape_for(a.head_dim, own_rows);
+    const int own_block = shape_rows(a.head_dim, p.own_shape);
+    p.own.rows = (int)own_rows;
+    p.own.blocks = (int)((own_rows + own_block - 1) / own_block);
+    const int64_t units = (int64_t)p.own.blocks * a.n_kv * a.n_seq;
+    int64_t splits = 512 / units;
     splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
     const int64_t most = (a.capacity + 127) / 128;
     p.own.splits = (int)(splits < most ? splits : most);
+    p.pre_shape = p.own_shape;
+    if (a.P > 0) {
+        const int64_t rows = (int64_t)a.n_seq * own_rows;
+        p.pre_shape = shape_for(a.head_dim, rows);
+        const int block = shape_rows(a.head_dim, p.pre_shape);
+        p.pre.rows = (int)rows;
+        p.pre.blocks = (int)((rows + block - 1) / block);
+        const int64_t beside = units * p.own.splits, room = beside <= 128 ? 256 - beside : 256;
+        int64_t n = room / ((int64_t)p.pre.blocks * a.n_kv);
+        n = n < 1 ? 1 : n > 128 ? 128 : n;
+        const int64_t top = (a.P + 63) / 64;
+        n = n < top ? n : top;
+        p.pre.per = ((a.P + n - 1) / n + 31) / 32 * 32;
+        p.pre.splits = (int)((a.P + p.pre.per - 1) / p.pre.per);
+    }
     p.own.first = p.pre.splits;
     p.parts = p.pre.splits + p.own.splits;
     return p;
 }
 
-template <int TYPE, int D, int RT, int WR, int WK, int KB, int ST, bool OWN>
-hipError_t launch_part(const AttnArgs &a, const AttnSplit &sp, float *opart, float2 *ml, hipStream_t st) {
-    const int64_t units = (int64_t)sp.splits * a.n_kv;
-    const int64_t grid = OWN ? units * sp.blocks * a.n_seq : (units + 7) / 8 * 8 * sp.blocks;
+template <int TYPE, int D, int PRE, int SELF>
+hipError_t launch_part(const AttnArgs &a, const AttnPlan &p, float *opart, float2 *ml, hipStream_t st) {
+    const int64_t n_pre = a.P > 0 ? ((int64_t)p.pre.splits * a.n_kv + 7) / 8 * 8 * p.pre.blocks : 0;
+    const int64_t grid = n_pre + (int64_t)p.own.splits * p.own.blocks * a.n_kv * a.n_seq;
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    attn_part_kernel<TYPE, D, RT, WR, WK, KB, ST, OWN><<<(unsigned)grid, WR * WK * 64, 0, st>>>(a, sp, opart, ml);
+    attn_part_kernel<TYPE, D, PRE, SELF><<<(unsigned)grid, 512, 0, st>>>(a, p.pre, p.own, (int)n_pre, opart, ml);
     return hipGetLastError();
-}
-
-template <int TYPE, int D, bool OWN>
-hipError_t launch_parts(const AttnArgs &a, const AttnSplit &sp, int rows, float *opart, float2 *ml, hipStream_t st) {
-    if constexpr (D == 256) {
-        if (rows == 32) return launch_part<TYPE, D, 1, 2, 2, 64, 1, OWN>(a, sp, opart, ml, st);
-        if (rows == 64) return launch_part<TYPE, D, 1, 4, 2, 64, 1, OWN>(a, sp, opart, ml, st);
-        return launch_part<TYPE, D, 1, 8, 1, 64, 2, OWN>(a, sp, opart, ml, st);
-    } else {
-        if (rows == 16) return launch_part<TYPE, D, 1, 1, 4, 128, 1, OWN>(a, sp, opart, ml, st);
-        if (rows == 32) return launch_part<TYPE, D, 2, 1, 4, 128, 1, OWN>(a, sp, opart, ml, st);
-        if (rows == 64) return launch_part<TYPE, D, 2, 2, 4, 128, 1, OWN>(a, sp, opart, ml, st);
-        if (rows == 128) return launch_part<TYPE, D, 2, 4, 2, 128, 2, OWN>(a, sp, opart, ml, st);
-        return launch_part<TYPE, D, 2, 8, 1, 128, 2, OWN>(a, sp, opart, ml, st);
-    }
 }
 
 template <int TYPE, int D> hipError_t launch_all(const AttnArgs &a, const AttnPlan &p, void *ws, hipStream_t st) {
     const int64_t rows = (int64_t)a.n_seq * a.M * a.n_q;
     float2 *ml = (float2 *)ws;
     float *opart = (float *)((char *)ws + ((size_t)p.parts * rows * sizeof(float2) + 255) / 256 * 256);
-    hipError_t e = hipSuccess;
-    if (a.P > 0) e = launch_parts<TYPE, D, false>(a, p.pre, p.pre_rows, opart, ml, st);
-    if (e == hipSuccess) e = launch_parts<TYPE, D, true>(a, p.own, p.own_rows, opart, ml, st);
+    hipError_t e = hipErrorInvalidValue;
+    const int shapes = p.pre_shape * 3 + p.own_shape;  // (own_shape <= pre_shape)
+    if constexpr (D < 256) {
+        if (shapes == 0) e = launch_part<TYPE, D, 0, 0>(a, p, opart, ml, st);
+        if (shapes == 3) e = launch_part<TYPE, D, 1, 0>(a, p, opart, ml, st);
+        if (shapes == 6) e = launch_part<TYPE, D, 2, 0>(a, p, opart, ml, st);
+    }
+    if (shapes == 4) e = launch_part<TYPE, D, 1, 1>(a, p, opart, ml, st);
+    if (shapes == 7) e = launch_part<TYPE, D, 2, 1>(a, p, opart, ml, st);
+    if (shapes == 8) e = launch_part<TYPE, D, 2, 2>(a, p, opart, ml, st);
     if (e != hipSuccess) return e;
     if (p.parts > 8) attn_join_kernel<D, 4><<<(unsigned)rows, 256, 0, st>>>(a, p.parts, opart, ml);
     else attn_join_kernel<D, 1><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, p.parts, opart, ml);

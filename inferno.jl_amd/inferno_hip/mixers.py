@@ -22,24 +22,65 @@ DELTA_L2NORM = 1
 _SCALINGS = {"none": ROPE_PLAIN, "linear": ROPE_LINEAR, "by_parts": ROPE_BY_PARTS}
 
 
-def _here(*tensors):
-    """The tensors are on the current device, whose stream the call takes."""
-    import torch
-    at = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != at:
-            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{at}")
+# The per-call checks are kept to a few attribute reads a tensor (a call's host time is most of a one-token call's); what
+# they refuse goes to _refuse for the message.
+_f32 = _i32 = _i64 = _u8 = _current_device = _Tensor = None
 
 
-def _rows(t, name: str, width: int, rows: int | None = None):
-    """t as fp32 [rows, >= width] with unit column stride; its row stride."""
+def _torch():
+    """torch's names, looked up once (the package itself does not import it)."""
+    global _f32, _i32, _i64, _u8, _current_device, _Tensor
     import torch
-    check_tensor(t, name, torch.float32, contiguous=False)
-    if t.dim() != 2 or t.shape[1] < width or (rows is not None and t.shape[0] != rows) or t.shape[0] < 1 \
-            or (t.stride(1) != 1 and t.shape[1] > 1):
+    _f32, _i32, _i64, _u8, _Tensor = torch.float32, torch.int32, torch.int64, torch.uint8, torch.Tensor
+    _current_device = torch.cuda.current_device
+
+
+def _refuse(t, name: str, dtype, shape=None, contiguous: bool = True, dev: int | None = None):
+    """The ValueError for a tensor that is not as it should be."""
+    check_tensor(t, name, dtype, shape, contiguous)
+    if dev is not None and t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{dev}")
+    raise ValueError(f"{name}: strides {t.stride()} of {tuple(t.shape)}")
+
+
+def _device_of(t, name: str) -> int:
+    """The device of a GPU tensor, which is the current one."""
+    dev = t.get_device() if isinstance(t, _Tensor) else -1
+    if dev < 0:
+        check_tensor(t, name)
+    if dev != _current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
+    return dev
+
+
+def _call(name: str):
+    """A bound function of the library."""
+    return getattr(_lib._lib or _lib.load(), name)
+
+
+def _whole(t, name: str, dtype, shape, dev: int):
+    """A contiguous tensor of exactly this type and shape on device dev; its address."""
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        _refuse(t, name, dtype, shape, True, dev)
+    return t.data_ptr()
+
+
+def _workspace(ws, dev: int):
+    if not isinstance(ws, _Tensor) or ws.dtype is not _u8 or ws.get_device() != dev or not ws.is_contiguous():
+        _refuse(ws, "ws", _u8, None, True, dev)
+    return ws.data_ptr(), ws.numel()
+
+
+def _rows(t, name: str, width: int, rows: int | None, dev: int):
+    """t as fp32 [rows, >= width] with unit column stride on device dev; its address, rows and row stride."""
+    if not isinstance(t, _Tensor) or t.dtype is not _f32 or t.get_device() != dev:
+        _refuse(t, name, _f32, None, False, dev)
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] < width or shape[0] < 1 or (rows is not None and shape[0] != rows) \
+            or (stride[1] != 1 and shape[1] > 1):
         raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, >= {width}] float32 with unit column "
-                         f"stride, got {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+                         f"stride, got {tuple(shape)} of strides {stride}")
+    return t.data_ptr(), shape[0], stride[0] if shape[0] > 1 else max(stride[0], shape[1])
 
 
 class RopeParams:
@@ -67,6 +108,11 @@ class RopeParams:
                                               None if freq_factors is None else _ptr(freq_factors)))
         self._ref = C.byref(self._c)
 
+    def _on(self, dev: int):
+        if self.freq_factors is not None and self.freq_factors.get_device() != dev:
+            raise ValueError(f"freq_factors are on {self.freq_factors.device}, the current device is cuda:{dev}")
+        return self._ref
+
 
 class KVCache:
     """ihip_kv over two float16 or bfloat16 GPU tensors k and v of shape
@@ -88,24 +134,27 @@ class KVCache:
         self.n_seq, self.capacity, self.n_kv, self.head_dim = k.shape
         self._c = _lib.Kv(F16 if k.dtype == torch.float16 else BF16, self.n_seq, self.n_kv, self.head_dim,
                           self.capacity, _ptr(k), _ptr(v), k.stride(0), k.stride(1), k.stride(2))
-        self._ref = C.byref(self._c)
+        self._ref, self._dev = C.byref(self._c), k.get_device()
+
+    def _on(self, dev: int):
+        if self._dev != dev:
+            raise ValueError(f"the cache is on cuda:{self._dev}, the current device is cuda:{dev}")
+        return self._ref
 
 
 def rope(x, positions, n_heads: int, params: RopeParams, out=None, stream=None):
     """x [tokens, n_heads * head_dim] float32 (unit column stride) with each
     head rotated to its row's position (int32 [tokens]); out may be x."""
-    import torch
+    if _f32 is None:
+        _torch()
+    dev = _device_of(x, "x")
     width = n_heads * params.head_dim
-    ldx = _rows(x, "x", width)
-    if x.shape[1] != width:
-        x = x[:, :width]
-    check_tensor(positions, "positions", torch.int32, (x.shape[0],))
+    xp, rows, ldx = _rows(x, "x", width, None, dev)
+    pp = _whole(positions, "positions", _i32, (rows,), dev)
     if out is None:
-        out = torch.empty((x.shape[0], width), dtype=torch.float32, device=x.device)
-    ldo = _rows(out, "out", width, x.shape[0])
-    _here(x, positions, out, params.freq_factors)
-    _lib.check(_lib.load().ihip_rope_apply(params._ref, _ptr(x), ldx, _ptr(out), ldo, n_heads, _ptr(positions),
-                                           x.shape[0], _stream(stream)))
+        out = x.new_empty((rows, width))
+    yp, _, ldy = _rows(out, "out", width, rows, dev)
+    _lib.check(_call("ihip_rope_apply")(params._on(dev), xp, ldx, yp, ldy, n_heads, pp, rows, _stream(stream)))
     return out
 
 
@@ -117,22 +166,20 @@ def rope_append(qkv, n_q: int, cache: KVCache, lengths, params: RopeParams, posi
     cache's entries lengths[s] + m. positions int32 [sequences * M], or pos0 +
     lengths[s] + m. lengths int32 [sequences]: below 0 an idle sequence (left
     as it was); where M entries do not fit, NaN rows and the cache as it was."""
-    import torch
-    d = params.head_dim
-    ld = _rows(qkv, "qkv", (n_q + 2 * cache.n_kv) * d)
-    rows = qkv.shape[0]
-    if rows % cache.n_seq:
-        raise ValueError(f"{rows} rows for {cache.n_seq} sequences")
-    check_tensor(lengths, "lengths", torch.int32, (cache.n_seq,))
-    if positions is not None:
-        check_tensor(positions, "positions", torch.int32, (rows,))
+    if _f32 is None:
+        _torch()
+    dev = _device_of(qkv, "qkv")
+    d, s = params.head_dim, cache.n_seq
+    xp, rows, ld = _rows(qkv, "qkv", (n_q + 2 * cache.n_kv) * d, None, dev)
+    if rows % s:
+        raise ValueError(f"{rows} rows for {s} sequences")
+    lp = _whole(lengths, "lengths", _i32, (s,), dev)
+    pp = None if positions is None else _whole(positions, "positions", _i32, (rows,), dev)
     if out is None:
-        out = torch.empty((rows, n_q * d), dtype=torch.float32, device=qkv.device)
-    ldq = _rows(out, "out", n_q * d, rows)
-    _here(qkv, cache.k, lengths, positions, out, params.freq_factors)
-    _lib.check(_lib.load().ihip_rope_append(params._ref, _ptr(qkv), ld, _ptr(out), ldq, n_q, cache._ref, _ptr(lengths),
-                                            None if positions is None else _ptr(positions), pos0, rows // cache.n_seq,
-                                            _stream(stream)))
+        out = qkv.new_empty((rows, n_q * d))
+    yp, _, ldq = _rows(out, "out", n_q * d, rows, dev)
+    _lib.check(_call("ihip_rope_append")(params._on(dev), xp, ld, yp, ldq, n_q, cache._on(dev), lp, pp, pos0, rows // s,
+                                         _stream(stream)))
     return out
 
 
@@ -152,28 +199,25 @@ def attn_prefix(q, n_q: int, cache: KVCache, lengths, prefix: KVCache | None = N
     tree_mask (int64 [sequences, M], M <= 64) for new entry j. scale: default
     head_dim ** -0.5. A row that sees nothing is zero; lengths below 0 leave a
     sequence's rows as they were, and one past its capacity gets NaN rows."""
-    import torch
-    d = cache.head_dim
-    ldq = _rows(q, "q", n_q * d)
-    rows = q.shape[0]
-    if rows % cache.n_seq:
-        raise ValueError(f"{rows} rows for {cache.n_seq} sequences")
-    m = rows // cache.n_seq
-    check_tensor(lengths, "lengths", torch.int32, (cache.n_seq,))
-    if tree_mask is not None:
-        check_tensor(tree_mask, "tree_mask", torch.int64, (cache.n_seq, m))
+    if _f32 is None:
+        _torch()
+    dev = _device_of(q, "q")
+    d, n = cache.head_dim, cache.n_seq
+    qp, rows, ldq = _rows(q, "q", n_q * d, None, dev)
+    if rows % n:
+        raise ValueError(f"{rows} rows for {n} sequences")
+    m = rows // n
+    lp = _whole(lengths, "lengths", _i32, (n,), dev)
+    mp = None if tree_mask is None else _whole(tree_mask, "tree_mask", _i64, (n, m), dev)
     if out is None:
-        out = torch.empty((rows, n_q * d), dtype=torch.float32, device=q.device)
-    ldo = _rows(out, "out", n_q * d, rows)
+        out = q.new_empty((rows, n_q * d))
+    op, _, ldo = _rows(out, "out", n_q * d, rows, dev)
     if ws is None:
-        ws = torch.empty(attn_prefix_ws_bytes(n_q, m, cache, prefix), dtype=torch.uint8, device=q.device)
-    check_tensor(ws, "ws", torch.uint8)
-    _here(q, cache.k, None if prefix is None else prefix.k, lengths, tree_mask, out, ws)
-    _lib.check(_lib.load().ihip_attn_prefix(_ptr(q), ldq, _ptr(out), ldo, n_q, m, cache._ref, _ptr(lengths),
-                                            None if prefix is None else prefix._ref,
-                                            None if tree_mask is None else _ptr(tree_mask),
-                                            d ** -0.5 if scale is None else scale, _ptr(ws), ws.numel(),
-                                            _stream(stream)))
+        ws = q.new_empty(attn_prefix_ws_bytes(n_q, m, cache, prefix), dtype=_u8)
+    wp, wn = _workspace(ws, dev)
+    _lib.check(_call("ihip_attn_prefix")(qp, ldq, op, ldo, n_q, m, cache._on(dev), lp,
+                                         None if prefix is None else prefix._on(dev), mp,
+                                         d ** -0.5 if scale is None else scale, wp, wn, _stream(stream)))
     return out
 
 
@@ -189,18 +233,19 @@ def gated_delta_rule_ws_bytes(n_seq: int, t: int, n_k: int, n_v: int, dk: int, d
     return _delta_ws_bytes(n_seq, t, n_k, n_v, dk, dv, int(bool(snapshots)))
 
 
-def _heads(t, name: str, shape):
-    """t as fp32 [sequences, tokens, heads, values], each token's heads side by side, the tokens' rows evenly spaced
-    over all sequences; the row stride."""
-    import torch
-    check_tensor(t, name, torch.float32, shape, contiguous=False)
-    s, n, h, d = t.shape
+def _heads(t, name: str, s: int, n: int, h: int, d: int, dev: int):
+    """t as fp32 [sequences, tokens, heads, values] (values 0: [sequences, tokens, heads]) on device dev, each token's heads
+    side by side, the tokens' rows evenly spaced over all sequences; its address and the row stride."""
+    shape = (s, n, h, d) if d else (s, n, h)
+    if not isinstance(t, _Tensor) or t.dtype is not _f32 or t.shape != shape or t.get_device() != dev:
+        _refuse(t, name, _f32, shape, False, dev)
     st = t.stride()
-    ld = st[1] if n > 1 else st[0] if s > 1 else h * d
-    if (d > 1 and st[3] != 1) or (h > 1 and st[2] != d) or (s > 1 and n > 1 and st[0] != n * ld) or ld < h * d:
-        raise ValueError(f"{name} {tuple(t.shape)} of strides {st}: the heads of a token must be contiguous and the "
-                         "rows of all tokens evenly spaced")
-    return ld
+    w = h * d if d else h
+    ld = st[1] if n > 1 else st[0] if s > 1 else w
+    if (st[-1] != 1 and shape[-1] > 1) or (d and h > 1 and st[2] != d) or (s > 1 and n > 1 and st[0] != n * ld) or ld < w:
+        raise ValueError(f"{name} {shape} of strides {st}: the heads of a token must be contiguous and the rows of all "
+                         "tokens evenly spaced")
+    return t.data_ptr(), ld
 
 
 def gated_delta_rule(q, k, v, g, beta, state, new_state=None, snapshots=None, lengths=None, l2norm: bool = False,
@@ -215,36 +260,36 @@ def gated_delta_rule(q, k, v, g, beta, state, new_state=None, snapshots=None, le
     every token (T <= 64; commit_state_ picks from them). lengths int32
     [sequences]: tokens of each, rows past them left as they were. Returns
     out [sequences, T, n_v, dv]."""
-    import torch
-    check_tensor(k, "k", torch.float32, (None, None, None, None), contiguous=False)
-    check_tensor(v, "v", torch.float32, (None, None, None, None), contiguous=False)
+    if _f32 is None:
+        _torch()
+    dev = _device_of(q, "q")
+    for x, name in ((k, "k"), (v, "v")):
+        if not isinstance(x, _Tensor) or x.dim() != 4 or x.numel() == 0:
+            raise ValueError(f"{name} must be a float32 GPU tensor [sequences, tokens, heads, values] with something in it")
     s, t, n_k, dk = k.shape
     n_v, dv = v.shape[2], v.shape[3]
-    if 0 in k.shape or 0 in v.shape:
-        raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)}: nothing to do")
-    ldq, ldk = _heads(q, "q", (s, t, n_k, dk)), _heads(k, "k", (s, t, n_k, dk))
-    ldv = _heads(v, "v", (s, t, n_v, dv))
-    for x, name in ((g, "g"), (beta, "beta")):
-        check_tensor(x, name, torch.float32, (s, t, n_v), contiguous=False)
-    ldg, ldb = (_heads(x.unsqueeze(3), name, (s, t, n_v, 1)) for x, name in ((g, "g"), (beta, "beta")))
+    a = _lib.Delta()
+    a.q, a.ldq = _heads(q, "q", s, t, n_k, dk, dev)
+    a.k, a.ldk = _heads(k, "k", s, t, n_k, dk, dev)
+    a.v, a.ldv = _heads(v, "v", s, t, n_v, dv, dev)
+    a.g, a.ldg = _heads(g, "g", s, t, n_v, 0, dev)
+    a.beta, a.ldb = _heads(beta, "beta", s, t, n_v, 0, dev)
     if out is None:
-        out = torch.empty((s, t, n_v, dv), dtype=torch.float32, device=v.device)
-    ldo = _heads(out, "out", (s, t, n_v, dv))
-    for x, name in ((state, "state"), (new_state, "new_state")):
-        if x is not None:
-            check_tensor(x, name, torch.float32, (s, n_v, dk, dv))
+        out = v.new_empty((s, t, n_v, dv))
+    a.o, a.ldo = _heads(out, "out", s, t, n_v, dv, dev)
+    if state is not None:
+        a.state_in = _whole(state, "state", _f32, (s, n_v, dk, dv), dev)
+    if new_state is not None:
+        a.state_out = _whole(new_state, "new_state", _f32, (s, n_v, dk, dv), dev)
     if snapshots is not None:
-        check_tensor(snapshots, "snapshots", torch.float32, (s, t, n_v, dk, dv))
+        a.snap_out = _whole(snapshots, "snapshots", _f32, (s, t, n_v, dk, dv), dev)
     if lengths is not None:
-        check_tensor(lengths, "lengths", torch.int32, (s,))
+        a.len = _whole(lengths, "lengths", _i32, (s,), dev)
     if ws is None:
-        ws = torch.empty(gated_delta_rule_ws_bytes(s, t, n_k, n_v, dk, dv, snapshots is not None), dtype=torch.uint8,
-                         device=v.device)
-    check_tensor(ws, "ws", torch.uint8)
-    _here(q, k, v, g, beta, state, new_state, snapshots, lengths, out, ws)
-    p = lambda x: None if x is None else _ptr(x)  # noqa: E731
-    a = _lib.Delta(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), ldq, ldk, ldv, ldg, ldb, _ptr(out), ldo, p(state),
-                   p(new_state), p(snapshots), p(lengths), s, t, n_k, n_v, dk, dv,
-                   dk ** -0.5 if scale is None else scale, DELTA_L2NORM if l2norm else 0)
-    _lib.check(_lib.load().ihip_gated_delta_rule(C.byref(a), _ptr(ws), ws.numel(), _stream(stream)))
+        ws = v.new_empty(gated_delta_rule_ws_bytes(s, t, n_k, n_v, dk, dv, snapshots is not None), dtype=_u8)
+    wp, wn = _workspace(ws, dev)
+    a.n_seq, a.T, a.n_k, a.n_v, a.dk, a.dv = s, t, n_k, n_v, dk, dv
+    a.scale = dk ** -0.5 if scale is None else scale
+    a.flags = DELTA_L2NORM if l2norm else 0
+    _lib.check(_call("ihip_gated_delta_rule")(C.byref(a), wp, wn, _stream(stream)))
     return out
