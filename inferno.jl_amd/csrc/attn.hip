@@ -47,17 +47,28 @@ template <> struct Kv<KV_BF16> {
 // x = l[0] + l[1] (+ l[2]), each limb the rest rounded to its type
 template <int TYPE> __device__ __forceinline__ void limbs(const float *x, typename Kv<TYPE>::v8 *l) {
     typedef typename Kv<TYPE>::t t;
-    float r[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) r[i] = x[i];
-#pragma unroll
-    for (int n = 0; n < Kv<TYPE>::LIMBS; n++)
+    if constexpr (TYPE == KV_F16) {
+        float one = 1.f;
+        asm("" : "+v"(one));  // (x - hi as a mixed fma that rounds to f16 itself: one instruction a value)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const t h = (t)r[i];
-            l[n][i] = h;
-            r[i] -= (float)h;
+            const t h = (t)x[i];
+            l[0][i] = h;
+            l[1][i] = (t)__builtin_fmaf(-(float)h, one, x[i]);
         }
+    } else {
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = x[i];
+#pragma unroll
+        for (int n = 0; n < Kv<TYPE>::LIMBS; n++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const t h = (t)r[i];
+                l[n][i] = h;
+                r[i] -= (float)h;
+            }
+    }
 }
 
 __device__ __forceinline__ float max_groups(float v) {  // over the four lane groups of a row
