@@ -156,23 +156,46 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
     if (t0 >= n) return;
     const int rep = a.n_v / a.n_k;
 
+    // running sums of two heads' g, a wave each, in fp64: a difference of two sums of the chunk keeps its digits however far
+    // both have fallen
+    auto decays = [&](int h0) __attribute__((always_inline)) {
+        if (wave < 2 && h0 + wave < rep) {
+            const int hv = hk * rep + h0 + wave;
+            const bool in = t0 + lane < n;
+            const int64_t row = (int64_t)s * a.T + t0 + lane;
+            double v = in ? (double)a.g[row * a.ldg + hv] : 0.0;
+            beta[wave][lane] = in ? a.beta[row * a.ldb + hv] : 0.f;
+            for (int o = 1; o < 64; o <<= 1) {
+                const double up = __shfl_up(v, o);
+                if (lane >= o) v += up;
+            }
+            G[wave][lane] = v;
+        }
+    };
     // rows of q (image 0) and k (image 1) to limbs: 4 threads a row
     {
         const int r = tid >> 2, part = tid & 3;
         const bool in = t0 + r < n;
         const int64_t row = (int64_t)s * a.T + t0 + r;
         char *out = w.img + (((int64_t)s * a.n_k + hk) * w.chunks + c) * (2 * IMG);
+        float x[2][PER / 2][8];
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             const float *src = (m ? a.k + row * a.ldk : a.q + row * a.ldq) + (int64_t)hk * DK;
-            float x[PER / 2][8], sum = 0.f, most = 0.f;
 #pragma unroll
             for (int i = 0; i < PER / 2; i++) {
-                *(f4 *)(x[i]) = in ? *(const f4 *)(src + i * 32 + part * 4) : f4{0, 0, 0, 0};
-                *(f4 *)(x[i] + 4) = in ? *(const f4 *)(src + i * 32 + 16 + part * 4) : f4{0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < 8; j++) sum = __builtin_fmaf(x[i][j], x[i][j], sum), most = fmaxf(most, fabsf(x[i][j]));
+                *(f4 *)(x[m][i]) = in ? *(const f4 *)(src + i * 32 + part * 4) : f4{0, 0, 0, 0};
+                *(f4 *)(x[m][i] + 4) = in ? *(const f4 *)(src + i * 32 + 16 + part * 4) : f4{0, 0, 0, 0};
             }
+        }
+        decays(0);
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            float sum = 0.f, most = 0.f;
+#pragma unroll
+            for (int i = 0; i < PER / 2; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) sum = __builtin_fmaf(x[m][i][j], x[m][i][j], sum), most = fmaxf(most, fabsf(x[m][i][j]));
             sum += __shfl_xor(sum, 1);
             most = fmaxf(most, __shfl_xor(most, 1));
             sum += __shfl_xor(sum, 2);
@@ -183,7 +206,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
 #pragma unroll
             for (int i = 0; i < PER / 2; i++) {
                 h8 hi, lo;
-                split8(x[i], up, hi, lo);
+                split8(x[m][i], up, hi, lo);
                 const int at = m * IMG + img_at<DK>(r, i * 4 + part);
                 *(h8 *)(lds + at) = hi;
                 *(h8 *)(lds + at + IMG / 2) = lo;
@@ -215,19 +238,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
     float *const M = (float *)lds;  // A of two heads, then P of two: [64][LD]
     for (int h0 = 0; h0 < rep; h0 += 2) {
         __syncthreads();  // (the images, or the pair before, are done with)
-        if (wave < 2 && h0 + wave < rep) {
-            const int hv = hk * rep + h0 + wave;
-            const bool in = t0 + lane < n;
-            const int64_t row = (int64_t)s * a.T + t0 + lane;
-            // fp64: a difference of two sums of the chunk keeps its digits however far both have fallen
-            double v = in ? (double)a.g[row * a.ldg + hv] : 0.0;
-            for (int o = 1; o < 64; o <<= 1) {
-                const double up = __shfl_up(v, o);
-                if (lane >= o) v += up;
-            }
-            G[wave][lane] = v;
-            beta[wave][lane] = in ? a.beta[row * a.ldb + hv] : 0.f;
-        }
+        if (h0) decays(h0);
         __syncthreads();
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -246,13 +257,14 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
             }
         }
         __syncthreads();
+        // T by blocks of 16. On the diagonal, a wave a head: lane 16 b + c has column c of block b, x_i = [i = c] - sum_j
+        // A_ij x_j (rows of A read by 16 lanes at once).
         if (wave < 2 && h0 + wave < rep) {
-            // column `lane` of T: x_i = [i = lane] - sum_j A_ij x_j
-            float *const A = M + wave * CH * LD;
-            float x[CH], most = 1.f;
+            float *const A = M + wave * CH * LD + (lane >> 4) * (16 * LD + 16);
+            float x[16];
 #pragma unroll
-            for (int i = 0; i < CH; i++) {
-                float v0 = lane == i ? 1.f : 0.f, v1 = 0.f;
+            for (int i = 0; i < 16; i++) {
+                float v0 = col == i ? 1.f : 0.f, v1 = 0.f;
 #pragma unroll
                 for (int j = 0; j < i; j += 4) {
                     const f4 m = *(const f4 *)(A + i * LD + j);
@@ -262,11 +274,62 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
                     if (j + 3 < i) v1 = __builtin_fmaf(-m[3], x[j + 3], v1);
                 }
                 x[i] = v0 + v1;
-                most = fmaxf(most, fabsf(x[i]));
             }
-            colup[wave][lane] = pow2(lift(most, 13));
 #pragma unroll
-            for (int i = 0; i < CH; i++) A[i * LD + lane] = x[i];
+            for (int i = 0; i < 16; i++) A[i * LD + col] = x[i];
+        }
+        __syncthreads();
+        // Below it, block column by block column: T_rc = -T_rr sum_{c<=k<r} A_rk T_kc in fp32 MFMAs, whose accumulators are
+        // the B operand of the next product (16 columns, rows 4 g + i by instruction i). Two waves a head: column 0, and
+        // columns 1 and 2.
+        {
+            const int h = wave >> 1, first = wave & 1;
+            float *const A = M + h * CH * LD;
+            f4 t[3];  // T_10 T_20 T_30 or T_21 T_31 T_32
+            if (h0 + h < rep) {
+                auto block = [&](int r, int k) __attribute__((always_inline)) { return *(const f4 *)(A + (16 * r + col) * LD + 16 * k + 4 * g); };
+                auto times = [&](const f4 &m, const f4 &x, f4 y) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(m[i], x[i], y, 0, 0, 0);
+                    return y;
+                };
+                auto corner = [&](int k) __attribute__((always_inline)) {  // T_kk as accumulators
+                    f4 x;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = A[(16 * k + 4 * g + i) * LD + 16 * k + col];
+                    return x;
+                };
+                const f4 zero = {0, 0, 0, 0};
+                if (first == 0) {
+                    const f4 x0 = corner(0);
+                    t[0] = -times(block(1, 1), times(block(1, 0), x0, zero), zero);
+                    t[1] = -times(block(2, 2), times(block(2, 1), t[0], times(block(2, 0), x0, zero)), zero);
+                    t[2] = -times(block(3, 3), times(block(3, 2), t[1], times(block(3, 1), t[0], times(block(3, 0), x0, zero))), zero);
+                } else {
+                    const f4 x1 = corner(1), x2 = corner(2);
+                    t[0] = -times(block(2, 2), times(block(2, 1), x1, zero), zero);
+                    t[1] = -times(block(3, 3), times(block(3, 2), t[0], times(block(3, 1), x1, zero)), zero);
+                    t[2] = -times(block(3, 3), times(block(3, 2), x2, zero), zero);
+                }
+            }
+            __syncthreads();  // (A is done with: T takes its place)
+            if (h0 + h < rep) {
+#pragma unroll
+                for (int b = 0; b < 3; b++) {
+                    const int r = first == 0 ? b + 1 : b == 0 ? 2 : 3, k = first == 0 ? 0 : b == 2 ? 2 : 1;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) A[(16 * r + 4 * g + i) * LD + 16 * k + col] = t[b][i];
+                }
+            }
+        }
+        __syncthreads();
+        // a power of two for each column of T (its largest is at least 1, on the diagonal)
+        if (wave < 2 && h0 + wave < rep) {
+            const float *const A = M + wave * CH * LD;
+            float most = 1.f;
+#pragma unroll
+            for (int i = 0; i < CH; i++) most = fmaxf(most, i >= (lane & ~15) ? fabsf(A[i * LD + lane]) : 0.f);
+            colup[wave][lane] = pow2(lift(most, 13));
         }
         __syncthreads();
         // operands: wave t takes row tile t of T and P of both heads
