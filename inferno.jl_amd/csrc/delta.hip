@@ -413,7 +413,7 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
     __shared__ __align__(16) char lds[PB + TP_BYTES];
     __shared__ __align__(16) char sbuf[NS][U * 2048], xbuf[NS][4096];
     __shared__ __align__(16) float scal[2][SCAL];
-    __shared__ float sdown[NS][64];
+    __shared__ float sdown[NS][64], xdown[NS][64];
     constexpr int LV = 16 * NS + 4;  // floats between rows of v in LDS (a row's pad keeps rows 4 apart in other banks)
     __shared__ __align__(16) float vbuf[CH * LV];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
@@ -615,15 +615,11 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             for (int t = 0; t < 4; t++) x[t] = f4{0, 0, 0, 0};
             lower_times(l, x);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                x[t] *= Rdown;
-                *(f4 *)(xbuf[pair] + t * 1024 + lane * 16) = x[t];
-            }
+            for (int t = 0; t < 4; t++) *(f4 *)(xbuf[pair] + t * 1024 + lane * 16) = x[t];  // (in units of R's limbs)
+            xdown[pair][lane] = Rdown;
             __syncthreads();
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 4, t);
-            const float down = limbs_of(x, l), grown = scal[buf][5 * CH];
-            float most = 0.f;
             h8 hi[2][2][2], lo[2][2][2];  // [set][tile of the pair][tokens]
             auto bring = [&](int r, int set) __attribute__((always_inline)) {
 #pragma unroll
@@ -633,12 +629,14 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             };
             bring(0, 0);
             STAGE();
+            const float down = limbs_of(x, l) * Rdown, grown = scal[buf][5 * CH];
+            float most = 0.f;
             // a pair of tiles' products while the pair before is added to the state and split
-            f4 y[2][2], z[2][2];
+            f4 z[2][2];
             auto add = [&](int r, int set) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    S[r + j] = grown * S[r + j] + down * (y[set][j] + z[set][j]);
+                    S[r + j] = grown * S[r + j] + down * z[set][j];
 #pragma unroll
                     for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r + j][i]));
                 }
@@ -650,14 +648,12 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
                 if (r + 2 < R) bring(r + 2, set ^ 1);
                 STAGE();
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    y[set][j] = mma(hi[set][j][0], l[0][0], f4{0, 0, 0, 0});
-                    z[set][j] = mma(hi[set][j][1], l[1][0], f4{0, 0, 0, 0});
-                }
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) y[set][j] = mma(hi[set][j][0], l[0][1], y[set][j]), z[set][j] = mma(hi[set][j][1], l[1][1], z[set][j]);
+                    for (int p = 0; p < 3; p++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) y[set][j] = mma(lo[set][j][0], l[0][0], y[set][j]), z[set][j] = mma(lo[set][j][1], l[1][0], z[set][j]);
+                        for (int j = 0; j < 2; j++)
+                            z[set][j] = mma((p == 2 ? lo : hi)[set][j][u], l[u][p == 1], u || p ? z[set][j] : f4{0, 0, 0, 0});
                 if (r) {
                     add(r - 2, set ^ 1);
 #pragma unroll
@@ -727,7 +723,7 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             h8 l[2][2];
 #pragma unroll
             for (int t = 0; t < 4; t++) y[t] = *(const f4 *)(xbuf[pair] + t * 1024 + lane * 16);
-            const float down = limbs_of(y, l), up = 1.0f / down;
+            const float down = limbs_of(y, l) * xdown[pair][lane], up = 1.0f / down;
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] *= up;
             lower_times(l, x);
