@@ -393,6 +393,21 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(1))) const char g_char;
+template <int N> struct Count {
+    static constexpr int value = N;
+};
+// all but the last N of this wave's vector memory operations have completed (they complete in order)
+template <int N> __device__ __forceinline__ void wait_vmem() { __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14); }
+// __syncthreads without its wait for every load under way: this wave's LDS stores have completed, and what it loaded to LDS
+// is the caller's to wait for
+__device__ __forceinline__ void bare_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -510,17 +525,31 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
                 for (int t = 2 * u; t < 4; t++) x[t] = mma(m[tp_block(t, u)][p == 2], l[u][p == 1], x[t]);
     };
 
-    // C: a chunk's operands come in two sets, K with P of the chunk before and the factors, Q with T
-    u4 ka[NI], pa[NTP], fa[NSC], qa[NI], ta[NTP];
+    // C: a chunk's operands go straight from memory to LDS, 16 bytes a lane, in two sets: K with P of the chunk before, Q
+    // with T. The lines of the next chunk's set are touched meanwhile (a word of each 128 bytes), so that they are in L2
+    // when their turn comes.
     const uint32_t ct = (uint32_t)(tid - 2 * NB), c16 = ct * 16;
-    auto get = [&](auto &to, const char *from) __attribute__((always_inline)) {
+    const int cw = (wave - 2 * NS) * 1024;
+    auto get = [&](int to, const char *from, auto count) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(to) / 16); i++) to[i] = *(const u4 *)(from + i * NB * 16 + c16);
+        for (int i = 0; i < decltype(count)::value; i++)
+            __builtin_amdgcn_global_load_lds((g_char *)(from + i * NB * 16 + c16), (lds_char *)(lds + to + i * NB * 16 + cw), 16, 0, 0);
     };
-    auto put = [&](int to, const auto &from) __attribute__((always_inline)) {
+    typedef Count<NI> Image;
+    typedef Count<NTP> Low;
+    constexpr int TI = NI / 8, TL = (NTP + 7) / 8;  // touches of an image, of T or P
+    uint32_t touched[TI + TL];
+    auto touch = [&](const char *image, const char *low) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(from) / 16); i++) *(u4 *)(lds + to + i * NB * 16 + c16) = from[i];
+        for (int i = 0; i < TI; i++) touched[i] = *(const uint32_t *)(image + (i * NB + ct) * 128);
+#pragma unroll
+        for (int i = 0; i < TL; i++) touched[TI + i] = *(const uint32_t *)(low + ((i * NB + ct) * 128 < TP_BYTES ? (i * NB + ct) * 128 : 0));
     };
+    auto touch_done = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < TI + TL; i++) asm volatile("" ::"v"(touched[i]));
+    };
+    u4 fa[NSC];
     auto get_fac = [&](int c) __attribute__((always_inline)) {
         const float *from = sc + (int64_t)(c < chunks ? c : chunks - 1) * SCAL;
 #pragma unroll
@@ -679,29 +708,37 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
         }
     } else if (brings) {
         if (chunks) {
-            get(ka, q_of(0) + IMG), get(qa, q_of(0)), get(ta, t_of(0));
+            get(0, q_of(0) + IMG, Image{}), get(QB, q_of(0), Image{}), get(TB, t_of(0), Low{});
             get_fac(0);
             get_v(0);
-            put(0, ka), put(QB, qa), put(TB, ta);
             put_fac(0);
             put_v();
-            get(ka, q_of(1) + IMG), get(pa, t_of(0) + TP_BYTES);
             get_fac(1);
-            get(qa, q_of(1)), get(ta, t_of(1));
-            get_v(1);
+            wait_stores_done();
         }
         __syncthreads();
+        // (LDS is written from registers before the loads to LDS are asked for: the compiler lets no store pass them)
         for (int c = 0; c < chunks; c++) {
-            put((c & 1 ? 0 : IMG), ka), put(PB, pa);
+            if (c) touch_done();
             put_fac(c + 1);
-            get(ka, q_of(c + 2) + IMG), get(pa, t_of(c + 1) + TP_BYTES);
-            get_fac(c + 2);
-            __syncthreads();
-            put(QB, qa), put(TB, ta);
+            STAGE();
+            get(PB, t_of(c) + TP_BYTES, Low{}), get(c & 1 ? 0 : IMG, q_of(c + 1) + IMG, Image{});
+            STAGE();
+            get_v(c + 1);
+            touch(q_of(c + 1), t_of(c + 1));
+            STAGE();
+            wait_vmem<4 + TI + TL>();
+            bare_barrier();
+            touch_done();
             put_v();
-            get(qa, q_of(c + 2)), get(ta, t_of(c + 2));
-            get_v(c + 2);
-            __syncthreads();
+            STAGE();
+            get(QB, q_of(c + 1), Image{}), get(TB, t_of(c + 1), Low{});
+            STAGE();
+            get_fac(c + 2);
+            touch(q_of(c + 2) + IMG, t_of(c + 1) + TP_BYTES);
+            STAGE();
+            wait_vmem<NSC + TI + TL>();
+            bare_barrier();
         }
     } else {
         __syncthreads();
