@@ -112,6 +112,9 @@ __device__ __forceinline__ int lift(float most, int top) {
     const int e = top - (b - 127);
     return e < -80 ? -80 : e > 80 ? 80 : e;
 }
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < __builtin_inff(); }
+// the larger of two; not a number if either is not
+__device__ __forceinline__ float max_or_nan(float x, float y) { return __builtin_elementwise_maximum(x, y); }
 __device__ __forceinline__ float groups_max(float v) {
     const uint32_t x = __float_as_uint(v);
     const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
@@ -151,20 +154,24 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
     __shared__ __align__(16) char lds[2 * IMG > 4 * CH * LD * 4 ? 2 * IMG : 4 * CH * LD * 4];
     __shared__ float ck[CH], cq[CH], beta[2][CH], colup[2][CH];
     __shared__ double G[2][CH];
+    __shared__ int bad[2][CH];  // rows of A with a value that is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
     const int c = blockIdx.x, hk = blockIdx.y, s = blockIdx.z, t0 = c * CH, n = tokens_of(a, s);
     if (t0 >= n) return;
     const int rep = a.n_v / a.n_k;
 
     // running sums of two heads' g, a wave each, in fp64: a difference of two sums of the chunk keeps its digits however far
-    // both have fallen
+    // both have fallen. e^-4096 is 0 in fp32 as is e^g of any g below, -inf among them: such a g counts as -4096, and the
+    // sums behind it stay finite and keep their digits.
     auto decays = [&](int h0) __attribute__((always_inline)) {
         if (wave < 2 && h0 + wave < rep) {
             const int hv = hk * rep + h0 + wave;
             const bool in = t0 + lane < n;
             const int64_t row = (int64_t)s * a.T + t0 + lane;
-            double v = in ? (double)a.g[row * a.ldg + hv] : 0.0;
+            const float gv = in ? a.g[row * a.ldg + hv] : 0.f;
+            double v = gv < -4096.f ? -4096.0 : (double)gv;
             beta[wave][lane] = in ? a.beta[row * a.ldb + hv] : 0.f;
+            bad[wave][lane] = 0;
             for (int o = 1; o < 64; o <<= 1) {
                 const double up = __shfl_up(v, o);
                 if (lane >= o) v += up;
@@ -243,6 +250,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             if (h0 + h >= rep) break;
+            f4 most = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (j > wave) continue;
@@ -251,9 +259,21 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
                 for (int i = 0; i < 4; i++) {
                     const int r = wave * 16 + 4 * g + i;
                     const float e = cj <= r ? expf((float)(G[h][r] - G[h][cj])) * ck[cj] : 0.f;
-                    M[h * CH * LD + r * LD + cj] = cj < r ? beta[h][r] * e * (kk[j][i] * ck[r]) : 0.f;
-                    M[(2 + h) * CH * LD + r * LD + cj] = e * (qk[j][i] * (cq[r] * a.scale));
+                    const float x = cj < r ? beta[h][r] * e * (kk[j][i] * ck[r]) : 0.f;
+                    most[i] = max_or_nan(most[i], fabsf(x));
+                    M[h * CH * LD + r * LD + cj] = x;
+                    M[(2 + h) * CH * LD + r * LD + cj] = cj <= r ? e * (qk[j][i] * (cq[r] * a.scale)) : 0.f;
                 }
+            }
+            // A row of A that is not finite must not reach the rows of T above it (0 times it is not 0): it is taken out here,
+            // and the token's own factor then makes its row of R, and with it every later one, not a number.
+            if (__any(!is_finite(most[0]) | !is_finite(most[1]) | !is_finite(most[2]) | !is_finite(most[3]))) {
+                for (int j = 0; j <= wave; j++)
+                    for (int i = 0; i < 4; i++) {
+                        const int r = wave * 16 + 4 * g + i;
+                        float *x = M + h * CH * LD + r * LD + j * 16 + col;
+                        if (!is_finite(*x)) *x = 0.f, bad[h][r] = 1;
+                    }
             }
         }
         __syncthreads();
@@ -379,9 +399,9 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
                 float *sc = w.scal + unit * SCAL;
                 const float grown = expf((float)G[h][r]), left = expf((float)(G[h][CH - 1] - G[h][r]));
                 const float down = beta[h][r] / colup[h][r];
-                sc[r] = down;
+                sc[r] = bad[h][r] ? __builtin_nanf("") : down;
                 sc[CH + r] = down * grown * ck[r];
-                sc[2 * CH + r] = a.scale * grown * cq[r] * pow2(e);
+                sc[2 * CH + r] = a.scale * grown * cq[r];
                 sc[3 * CH + r] = pow2(-e);
                 sc[4 * CH + r] = left * ck[r];
                 if (r == CH - 1) sc[5 * CH] = grown;
@@ -470,12 +490,15 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
         return *(const f4 *)(&scal[buf][which * CH + t * 16 + 4 * g]);
     };
     // the four tiles of one column to limbs, its largest to [2^13, 2^14); returns what undoes the power of two
-    auto limbs_of = [&](const f4 (&v)[4], h8 (&l)[2][2]) __attribute__((always_inline)) {
+    auto largest_of = [&](const f4 (&v)[4]) __attribute__((always_inline)) {
         float most = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(v[t][i]));
+            for (int i = 0; i < 4; i++) most = max_or_nan(most, fabsf(v[t][i]));
+        return most;
+    };
+    auto limbs_of = [&](const f4 (&v)[4], float most, h8 (&l)[2][2]) __attribute__((always_inline)) {
         const int e = lift(groups_max(most), 13);
         const float up = pow2(e);
 #pragma unroll
@@ -486,6 +509,37 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             split8(x, up, l[u][0], l[u][1]);
         }
         return pow2(-e);
+    };
+    // A token whose row is not finite must not reach the tokens before it (its 0 in T or P times it is not 0): from the
+    // column's first such row on, rows count as 0 in the product, and `spoil` makes them not a number after it. Returns that
+    // row, 64 if there is none.
+    auto sound = [&](f4 (&v)[4], float &most) __attribute__((always_inline)) {
+        int first = CH;
+        if (__any(!is_finite(most))) {
+#pragma unroll
+            for (int t = 3; t >= 0; t--)
+#pragma unroll
+                for (int i = 3; i >= 0; i--) first = is_finite(v[t][i]) ? first : t * 16 + 4 * g + i;
+            first = min(first, __shfl_xor(first, 16));
+            first = min(first, __shfl_xor(first, 32));
+            most = 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v[t][i] = t * 16 + 4 * g + i < first ? v[t][i] : 0.f;
+                    most = fmaxf(most, fabsf(v[t][i]));
+                }
+        }
+        return first;
+    };
+    auto spoil = [&](f4 (&v)[4], int first) __attribute__((always_inline)) {
+        if (__any(first < CH)) {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[t][i] = t * 16 + 4 * g + i < first ? v[t][i] : __builtin_nanf("");
+        }
     };
     // x[t] = rows of an image (A: K at `base`, B: Q) times the limbs l: the four tiles' products in turn, so that none waits
     // for its own last; the next operands are on their way meanwhile
@@ -639,10 +693,13 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             image_times(K, Sl, x);
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] = v[t] - fb[t] * x[t];
-            const float Rdown = limbs_of(x, l);
+            float mostR = largest_of(x);
+            const int first = sound(x, mostR);
+            const float Rdown = limbs_of(x, mostR, l);
 #pragma unroll
             for (int t = 0; t < 4; t++) x[t] = f4{0, 0, 0, 0};
             lower_times(l, x);
+            spoil(x, first);
 #pragma unroll
             for (int t = 0; t < 4; t++) *(f4 *)(xbuf[pair] + t * 1024 + lane * 16) = x[t];  // (in units of R's limbs)
             xdown[pair][lane] = Rdown;
@@ -658,7 +715,7 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             };
             bring(0, 0);
             STAGE();
-            const float down = limbs_of(x, l) * Rdown, grown = scal[buf][5 * CH];
+            const float down = limbs_of(x, largest_of(x), l) * Rdown, grown = scal[buf][5 * CH];
             float most = 0.f;
             // a pair of tiles' products while the pair before is added to the state and split
             f4 z[2][2];
@@ -760,13 +817,16 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
             h8 l[2][2];
 #pragma unroll
             for (int t = 0; t < 4; t++) y[t] = *(const f4 *)(xbuf[pair] + t * 1024 + lane * 16);
-            const float down = limbs_of(y, l) * xdown[pair][lane], up = 1.0f / down;
+            float most = largest_of(y);
+            const int first = sound(y, most);
+            const float down = limbs_of(y, most, l) * xdown[pair][lane];
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] *= up;
-            lower_times(l, x);
+            for (int t = 0; t < 4; t++) y[t] = f4{0, 0, 0, 0};
+            lower_times(l, y);
             float *to = ob + (int64_t)c * CH * a.ldo;
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 3, t) * down;
+            for (int t = 0; t < 4; t++) x[t] += y[t] * (per_row(buf, 3, t) * down);
+            spoil(x, first);
             if ((c + 1) * CH <= n && w0 + 16 <= a.dv) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)

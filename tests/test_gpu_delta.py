@@ -218,3 +218,51 @@ def test_repeats_streams_and_graph(ih, t):
         torch.cuda.synchronize()
         assert torch.equal(out, eager[i]) and torch.equal(st, states[i]), i
         ih.gated_delta_rule(*o2[:5], o2[5])
+
+
+@pytest.mark.parametrize("t", [5, 200])
+@pytest.mark.parametrize("far", [float("-inf"), -3e38, -1e6, -150.0])
+def test_a_decay_that_clears_the_state(ih, t, far):
+    """A token whose decay leaves nothing of the state (where documents are packed one behind the other): the tokens behind
+    it are those of a fresh state, with all their digits."""
+    import torch
+    at = t // 2
+    q, k, v, g, b, st = make(2, t, 2, 4, 64, 64, seed=17)
+    g[0, at] = far
+    g[1, 1], g[1, t - 2] = far, far
+    o, _, last = R.delta(q, k, v, g, b, st)
+    new = torch.empty_like(st)
+    check(ih.gated_delta_rule(q, k, v, g, b, st, new_state=new), o, "o")
+    check(new, last, "state")
+    fresh, _, alone = R.delta(*(x[:1, at:] for x in (q, k, v, g, b)), torch.zeros_like(st[:1]))
+    check(new[:1], alone, "state after the cleared one")
+
+
+@pytest.mark.parametrize("t,at", [(5, 2), (100, 0), (100, 17), (100, 50), (100, 63), (100, 64), (100, 99), (300, 150)])
+@pytest.mark.parametrize("what", ["q", "k", "v", "g", "beta"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_bad_token_spoils_no_earlier_one(ih, t, at, what, value):
+    """One token's q, k, v, g or beta is not finite: the tokens before it, the heads that do not share it, and for v the
+    other columns, are as without it; what it reaches is not finite (q: its own row; else every later row, and the state)."""
+    import torch
+    if what == "g" and value > 0:
+        value = float("nan")  # (e^inf times a state is infinite or not a number, which of them is not fixed)
+    q, k, v, g, b, st = make(2, t, 2, 4, 128, 64, seed=19)
+    o, _, last = R.delta(q, k, v, g, b, st)
+    {"q": q, "k": k, "v": v, "g": g, "beta": b}[what][(1, at, 1) + ((5,) if what in ("q", "k", "v") else ())] = value
+    new = torch.empty_like(st)
+    out = ih.gated_delta_rule(q, k, v, g, b, st, new_state=new)
+    bad = torch.zeros(out.shape, dtype=torch.bool)
+    gone = torch.zeros(new.shape, dtype=torch.bool)
+    if what == "q":
+        bad[1, at, 2:] = True
+    elif what == "k":
+        bad[1, at:, 2:], gone[1, 2:] = True, True
+    elif what == "v":
+        bad[1, at:, 1, 5], gone[1, 1, :, 5] = True, True
+    else:
+        bad[1, at:, 1], gone[1, 1] = True, True
+    out, new = out.cpu(), new.cpu()
+    assert not bool(torch.isfinite(out[bad]).any()) and not bool(torch.isfinite(new[gone]).any())
+    check(torch.where(bad, 0.0, out), torch.where(bad, 0.0, o.cpu().double()), "o")
+    check(torch.where(gone, 0.0, new), torch.where(gone, 0.0, last.cpu().double()), "state")
