@@ -152,7 +152,7 @@ __device__ __forceinline__ int tokens_of(const DeltaArgs &a, int s) {
 template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, DeltaWs w) {
     constexpr int IMG = img_bytes(DK), LD = 68, U = DK / 32, PER = DK / 16;  // PER: 16-byte pieces of a row a thread takes
     __shared__ __align__(16) char lds[2 * IMG > 4 * CH * LD * 4 ? 2 * IMG : 4 * CH * LD * 4];
-    __shared__ float ck[CH], cq[CH], beta[2][CH], colup[2][CH];
+    __shared__ __align__(16) float ck[CH], cq[CH], beta[2][CH], colup[2][CH];
     __shared__ double G[2][CH];
     __shared__ int bad[2][CH];  // rows of A with a value that is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
@@ -230,16 +230,29 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
             return *(const h8 *)(lds + m * IMG + limb * (IMG / 2) + img_at<DK>(tile * 16 + col, 4 * u + g));
         };
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            kk[j] = qk[j] = f4{0, 0, 0, 0};
-            if (j <= wave) {
+        for (int j = 0; j < 4; j++) kk[j] = qk[j] = f4{0, 0, 0, 0};
+        h8 own[2][2][2], all[2][4][2];  // [set][image][limb], [set][tile][limb]: the next 32 values come in during a product
+        auto bring = [&](int u, int set) __attribute__((always_inline)) {
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const h8 bh = rows(1, 0, j, u), bl = rows(1, 1, j, u);
-                    kk[j] = mma3(rows(1, 0, wave, u), rows(1, 1, wave, u), bh, bl, kk[j]);
-                    qk[j] = mma3(rows(0, 0, wave, u), rows(0, 1, wave, u), bh, bl, qk[j]);
-                }
+            for (int y = 0; y < 2; y++) {
+#pragma unroll
+                for (int m = 0; m < 2; m++) own[set][m][y] = rows(m, y, wave, u);
+#pragma unroll
+                for (int j = 0; j < 4; j++) all[set][j][y] = rows(1, y, j, u);
             }
+        };
+        bring(0, 0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (u + 1 < U) bring(u + 1, (u + 1) & 1);
+            const auto &o = own[u & 1];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (j <= wave) {
+                    const auto &b = all[u & 1][j];
+                    kk[j] = mma3(o[1][0], o[1][1], b[0], b[1], kk[j]);
+                    qk[j] = mma3(o[0][0], o[0][1], b[0], b[1], qk[j]);
+                }
         }
     }
     float *const M = (float *)lds;  // A of two heads, then P of two: [64][LD]
@@ -250,19 +263,31 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             if (h0 + h >= rep) break;
-            f4 most = {0, 0, 0, 0};
+            // e^(G_r - G_c): left of the diagonal tile by way of the row tile's first token, a factor a row and one a column
+            const int r0 = wave * 16 + 4 * g;
+            const double mid = G[h][wave * 16];
+            double gr[4], gc[4];
+            float kc[4], ec[4];
+            const f4 kr = *(const f4 *)(ck + r0), b = *(const f4 *)(beta[h] + r0), qr = *(const f4 *)(cq + r0);
+            f4 most = {0, 0, 0, 0}, er;
+#pragma unroll
+            for (int i = 0; i < 4; i++) gr[i] = G[h][r0 + i], gc[i] = G[h][i * 16 + col], kc[i] = ck[i * 16 + col];
+#pragma unroll
+            for (int i = 0; i < 4; i++) er[i] = expf((float)(gr[i] - mid));
+#pragma unroll
+            for (int j = 0; j < 4; j++) ec[j] = j < wave ? expf((float)(mid - gc[j])) * kc[j] : 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (j > wave) continue;
                 const int cj = j * 16 + col;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int r = wave * 16 + 4 * g + i;
-                    const float e = cj <= r ? expf((float)(G[h][r] - G[h][cj])) * ck[cj] : 0.f;
-                    const float x = cj < r ? beta[h][r] * e * (kk[j][i] * ck[r]) : 0.f;
+                    const int r = r0 + i;
+                    const float e = j < wave ? er[i] * ec[j] : expf((float)(gr[i] - gc[j])) * kc[j];
+                    const float x = cj < r ? b[i] * e * (kk[j][i] * kr[i]) : 0.f;
                     most[i] = max_or_nan(most[i], fabsf(x));
                     M[h * CH * LD + r * LD + cj] = x;
-                    M[(2 + h) * CH * LD + r * LD + cj] = cj <= r ? e * (qk[j][i] * (cq[r] * a.scale)) : 0.f;
+                    M[(2 + h) * CH * LD + r * LD + cj] = cj <= r ? e * (qk[j][i] * (qr[i] * a.scale)) : 0.f;
                 }
             }
             // A row of A that is not finite must not reach the rows of T above it (0 times it is not 0): it is taken out here,
@@ -346,9 +371,11 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
         // a power of two for each column of T (its largest is at least 1, on the diagonal)
         if (wave < 2 && h0 + wave < rep) {
             const float *const A = M + wave * CH * LD;
-            float most = 1.f;
+            float most = 1.f, t[CH];
 #pragma unroll
-            for (int i = 0; i < CH; i++) most = fmaxf(most, i >= (lane & ~15) ? fabsf(A[i * LD + lane]) : 0.f);
+            for (int i = 0; i < CH; i++) t[i] = A[i * LD + lane];
+#pragma unroll
+            for (int i = 0; i < CH; i++) most = fmaxf(most, i >= (lane & ~15) ? fabsf(t[i]) : 0.f);
             colup[wave][lane] = pow2(lift(most, 13));
         }
         __syncthreads();
@@ -360,40 +387,42 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
             char *const out = w.tp + unit * (2 * TP_BYTES) + lane * 16;
             const int r = wave * 16 + col;
             const int us = wave < 2 ? 1 : 2;
-            float p[2][8], most = 0.f;
+            f4 t[2][2], p[2][2], cu[2][2];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                if (u >= us) continue;
-                float t[8];
-                const float *src = M + h * CH * LD + r * LD + 32 * u + 4 * g;
-                *(f4 *)t = *(const f4 *)src, *(f4 *)(t + 4) = *(const f4 *)(src + 16);
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int cj = 32 * u + 4 * g + (i & 3) + (i >> 2) * 16;
-                    // (past the row's tile nothing was written)
-                    t[i] = cj < (wave + 1) * 16 ? t[i] * colup[h][cj] : 0.f;
+                for (int y = 0; y < 2; y++) {
+                    const float *src = M + h * CH * LD + r * LD + 32 * u + 16 * y + 4 * g;
+                    t[u][y] = *(const f4 *)src;
+                    p[u][y] = *(const f4 *)(src + 2 * CH * LD);
+                    cu[u][y] = *(const f4 *)(colup[h] + 32 * u + 16 * y + 4 * g);
                 }
-                h8 hi, lo;
-                split8(t, 1.f, hi, lo);
-                char *to = out + tp_block(wave, u) * 2048;
-                *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
-                src += 2 * CH * LD;
-                *(f4 *)p[u] = *(const f4 *)src, *(f4 *)(p[u] + 4) = *(const f4 *)(src + 16);
+            float most = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int cj = 32 * u + 4 * g + (i & 3) + (i >> 2) * 16;
-                    if (cj >= (wave + 1) * 16) p[u][i] = 0.f;
-                    most = fmaxf(most, fabsf(p[u][i]));
-                }
-            }
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // (past the row's tile nothing was written)
+                        const bool there = 2 * u + y <= wave;
+                        t[u][y][i] = there ? t[u][y][i] * cu[u][y][i] : 0.f;
+                        p[u][y][i] = there ? p[u][y][i] : 0.f;
+                        most = fmaxf(most, fabsf(p[u][y][i]));
+                    }
             const int e = lift(groups_max(most), 13);
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 if (u >= us) continue;
+                float x[8];
                 h8 hi, lo;
-                split8(p[u], pow2(e), hi, lo);
-                char *to = out + TP_BYTES + tp_block(wave, u) * 2048;
+                char *to = out + tp_block(wave, u) * 2048;
+                *(f4 *)x = t[u][0], *(f4 *)(x + 4) = t[u][1];
+                split8(x, 1.f, hi, lo);
                 *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
+                *(f4 *)x = p[u][0], *(f4 *)(x + 4) = p[u][1];
+                split8(x, pow2(e), hi, lo);
+                *(h8 *)(to + TP_BYTES) = hi, *(h8 *)(to + TP_BYTES + 1024) = lo;
             }
             if (g == 0) {
                 float *sc = w.scal + unit * SCAL;
