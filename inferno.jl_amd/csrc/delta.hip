@@ -105,6 +105,8 @@ __device__ __forceinline__ int tp_block(int t, int u) { return t < 2 ? t : t * 2
 
 // 2^e as a float, e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// 2^x by the one instruction (its argument rounded to fp32 costs |x| 2^-25, as expf's own would)
+__device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
 // exponent of the power of two that brings a largest absolute value to [2^top, 2^(top + 1)); 0 for 0 and non-finite
 __device__ __forceinline__ int lift(float most, int top) {
     const int b = (int)((__float_as_uint(most) >> 23) & 255);
@@ -155,22 +157,23 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
     __shared__ __align__(16) float ck[CH], cq[CH], beta[2][CH], colup[2][CH];
     __shared__ double G[2][CH];
     __shared__ int bad[2][CH];  // rows of A with a value that is not finite
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
-    const int c = blockIdx.x, hk = blockIdx.y, s = blockIdx.z, t0 = c * CH, n = tokens_of(a, s);
-    if (t0 >= n) return;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = blockIdx.x, hk = blockIdx.y, s = blockIdx.z, t0 = c * CH;
     const int rep = a.n_v / a.n_k;
 
-    // running sums of two heads' g, a wave each, in fp64: a difference of two sums of the chunk keeps its digits however far
+    // running sums of two heads' g log2(e), a wave each, in fp64: a difference of two sums of the chunk keeps its digits however far
     // both have fallen. e^-4096 is 0 in fp32 as is e^g of any g below, -inf among them: such a g counts as -4096, and the
     // sums behind it stay finite and keep their digits.
     auto decays = [&](int h0) __attribute__((always_inline)) {
         if (wave < 2 && h0 + wave < rep) {
             const int hv = hk * rep + h0 + wave;
-            const bool in = t0 + lane < n;
+            const bool at = t0 + lane < a.T;
             const int64_t row = (int64_t)s * a.T + t0 + lane;
-            const float gv = in ? a.g[row * a.ldg + hv] : 0.f;
-            double v = gv < -4096.f ? -4096.0 : (double)gv;
-            beta[wave][lane] = in ? a.beta[row * a.ldb + hv] : 0.f;
+            const float gv = at ? a.g[row * a.ldg + hv] : 0.f, bv = at ? a.beta[row * a.ldb + hv] : 0.f;
+            const bool in = t0 + lane < tokens_of(a, s);
+            double v = !in ? 0.0 : (gv < -4096.f ? -4096.0 : (double)gv) * 1.4426950408889634;
+            beta[wave][lane] = in ? bv : 0.f;
             bad[wave][lane] = 0;
             for (int o = 1; o < 64; o <<= 1) {
                 const double up = __shfl_up(v, o);
@@ -179,10 +182,11 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
             G[wave][lane] = v;
         }
     };
-    // rows of q (image 0) and k (image 1) to limbs: 4 threads a row
+    // rows of q (image 0) and k (image 1) to limbs: 4 threads a row (loaded before it is known how many tokens there are,
+    // then taken for zeros past them)
     {
         const int r = tid >> 2, part = tid & 3;
-        const bool in = t0 + r < n;
+        const bool at = t0 + r < a.T;
         const int64_t row = (int64_t)s * a.T + t0 + r;
         char *out = w.img + (((int64_t)s * a.n_k + hk) * w.chunks + c) * (2 * IMG);
         float x[2][PER / 2][8];
@@ -191,13 +195,20 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
             const float *src = (m ? a.k + row * a.ldk : a.q + row * a.ldq) + (int64_t)hk * DK;
 #pragma unroll
             for (int i = 0; i < PER / 2; i++) {
-                *(f4 *)(x[m][i]) = in ? *(const f4 *)(src + i * 32 + part * 4) : f4{0, 0, 0, 0};
-                *(f4 *)(x[m][i] + 4) = in ? *(const f4 *)(src + i * 32 + 16 + part * 4) : f4{0, 0, 0, 0};
+                *(f4 *)(x[m][i]) = at ? *(const f4 *)(src + i * 32 + part * 4) : f4{0, 0, 0, 0};
+                *(f4 *)(x[m][i] + 4) = at ? *(const f4 *)(src + i * 32 + 16 + part * 4) : f4{0, 0, 0, 0};
             }
         }
         decays(0);
+        const int n = tokens_of(a, s);
+        if (t0 >= n) return;
+        const bool in = t0 + r < n;
 #pragma unroll
         for (int m = 0; m < 2; m++) {
+#pragma unroll
+            for (int i = 0; i < PER / 2; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[m][i][j] = in ? x[m][i][j] : 0.f;
             float sum = 0.f, most = 0.f;
 #pragma unroll
             for (int i = 0; i < PER / 2; i++)
@@ -226,8 +237,11 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
     // wave t: row tile t of K K^T and Q K^T, columns up to its own tile
     f4 kk[4], qk[4];
     {
-        auto rows = [&](int m, int limb, int tile, int u) {
-            return *(const h8 *)(lds + m * IMG + limb * (IMG / 2) + img_at<DK>(tile * 16 + col, 4 * u + g));
+        int ra[U];  // (rows 16 apart permute alike)
+#pragma unroll
+        for (int u = 0; u < U; u++) ra[u] = img_at<DK>(col, 4 * u + g);
+        auto rows = [&](int m, int limb, int tile, int u) __attribute__((always_inline)) {
+            return *(const h8 *)(lds + m * IMG + limb * (IMG / 2) + ra[u] + tile * 16 * (DK * 2));
         };
 #pragma unroll
         for (int j = 0; j < 4; j++) kk[j] = qk[j] = f4{0, 0, 0, 0};
@@ -260,7 +274,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
         __syncthreads();  // (the images, or the pair before, are done with)
         if (h0) decays(h0);
         __syncthreads();
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < 2; h++) {
             if (h0 + h >= rep) break;
             // e^(G_r - G_c): left of the diagonal tile by way of the row tile's first token, a factor a row and one a column
@@ -273,9 +287,9 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
 #pragma unroll
             for (int i = 0; i < 4; i++) gr[i] = G[h][r0 + i], gc[i] = G[h][i * 16 + col], kc[i] = ck[i * 16 + col];
 #pragma unroll
-            for (int i = 0; i < 4; i++) er[i] = expf((float)(gr[i] - mid));
+            for (int i = 0; i < 4; i++) er[i] = exp2_of(gr[i] - mid);
 #pragma unroll
-            for (int j = 0; j < 4; j++) ec[j] = j < wave ? expf((float)(mid - gc[j])) * kc[j] : 0.f;
+            for (int j = 0; j < 4; j++) ec[j] = j < wave ? exp2_of(mid - gc[j]) * kc[j] : 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (j > wave) continue;
@@ -283,7 +297,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int r = r0 + i;
-                    const float e = j < wave ? er[i] * ec[j] : expf((float)(gr[i] - gc[j])) * kc[j];
+                    const float e = j < wave ? er[i] * ec[j] : exp2_of(gr[i] - gc[j]) * kc[j];
                     const float x = cj < r ? b[i] * e * (kk[j][i] * kr[i]) : 0.f;
                     most[i] = max_or_nan(most[i], fabsf(x));
                     M[h * CH * LD + r * LD + cj] = x;
@@ -380,7 +394,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
         }
         __syncthreads();
         // operands: wave t takes row tile t of T and P of both heads
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < 2; h++) {
             if (h0 + h >= rep) break;
             const int64_t unit = ((int64_t)s * a.n_v + hk * rep + h0 + h) * w.chunks + c;
@@ -426,7 +440,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
             }
             if (g == 0) {
                 float *sc = w.scal + unit * SCAL;
-                const float grown = expf((float)G[h][r]), left = expf((float)(G[h][CH - 1] - G[h][r]));
+                const float grown = exp2_of(G[h][r]), left = exp2_of(G[h][CH - 1] - G[h][r]);
                 const float down = beta[h][r] / colup[h][r];
                 sc[r] = bad[h][r] ? __builtin_nanf("") : down;
                 sc[CH + r] = down * grown * ck[r];
