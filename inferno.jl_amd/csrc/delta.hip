@@ -74,34 +74,40 @@ template <int DK> __global__ __launch_bounds__(64) void delta_token_kernel(Delta
 // With G the running sum of g inside a chunk and S the state before it, the
 // chunk's writes X (row i: beta_i (v_i - S_i^T k_i), S_i the state token i
 // meets) solve (I + A) X = R, A_ij = beta_i e^(G_i - G_j) k_i.k_j below the
-// diagonal, R_i = beta_i (v_i - e^(G_i) S^T k_i); then
+// diagonal, R_i = beta_i (v_i - e^(G_i) S^T k_i). With T = (I + A)^-1, X = T R:
 //   o_i = scale (e^(G_i) S^T q_i + sum_{j<=i} e^(G_i - G_j) (q_i.k_j) x_j)
-//   S'  = e^(G_63) S + sum_j e^(G_63 - G_j) k_j x_j^T
+//       = scale e^(G_i) S^T q_i + sum_j (P T)_ij r_j
+//   S'  = e^(G_63) S + sum_i e^(G_63 - G_i) k_i x_i^T = e^(G_63) S + W R,
+//   W   = sum_i e^(G_63 - G_i) k_i T_i.
 // Every exponent is <= 0 for g <= 0. What does not need the state is prepared
-// for all chunks at once (delta_prep_kernel): T = (I + A)^-1 by forward
-// substitution (the powers of A that a product form would need can be huge where
-// keys repeat), P_ij = e^(G_i - G_j) q_i.k_j, and q, k, T, P as fp16 operands.
-// Chunk after chunk (delta_chunk_kernel), a wave carries 16 columns of S in its
+// for all chunks at once (delta_prep_kernel): T by forward substitution (the
+// powers of A that a product form would need can be huge where keys repeat),
+// then q, k, W and P T as fp16 operands. What is left to do chunk after chunk
+// (delta_chunk_kernel) is two products on the state's way, K S and W R, and two
+// beside it, Q S and (P T) R; a wave carries 16 columns of S in its
 // accumulators. The products run on 16x16x32 f16 MFMAs; an fp32 factor is two f16
-// limbs (22 bits) times a power of two - a row's for q, k and P, a column's for T
-// and for the state, R and X - and a product is hi hi + hi lo + lo hi.
+// limbs (22 bits) times a power of two - a row's for q, k and P T, a column's for
+// W, P T, the state and R - and a product is hi hi + hi lo + lo hi.
 
 constexpr int CH = 64;
-constexpr int TP_BYTES = 6 * 2048;  // T or P: the six 16 x 32 blocks at or below the diagonal, two limbs
-constexpr int SCAL = 5 * CH + 16;   // floats: a, b, f, p, d per token, e^(G_63)
+constexpr int PT_BYTES = 6 * 2048;   // P T: the six 16 x 32 blocks at or below the diagonal, two limbs
+constexpr int SCAL = 6 * CH + 16;    // floats: b, f, w, p, a, d per token (below), e^(G_63)
+// R = b v - f (K S);  state += W (w R);  o = a (Q S) + d ((P T) (p R))
+enum { ROW_B, ROW_F, ROW_W, ROW_P, ROW_A, ROW_D };
 
-__host__ __device__ constexpr int img_bytes(int dk) { return 2 * CH * dk * 2; }  // both limbs of 64 rows
+__host__ __device__ constexpr int img_bytes(int dk) { return 2 * CH * dk * 2; }  // both limbs of 64 rows; W has as many
 
-// An image holds a row's values in the order of the operand: 16-byte piece 4 u + q has values 32 u + 4 q .. + 3 and
-// 32 u + 16 + 4 q .. + 3, what lane group q takes of 32 values when the other operand is two accumulator tiles side by
-// side. Byte of piece c of row r: the pieces of a row are permuted so that neither 16 rows' loads of one piece nor the
-// transposing loads of 4 rows' halves of 4 pieces meet in a bank.
+// An operand in memory: 1 KB blocks of 16 rows and 32 values, limb after limb, 16 bytes a lane in the lanes' order: lane
+// 16 q + c has of row c the values 32 u + 4 q .. + 3 and 32 u + 16 + 4 q .. + 3, what lane group q takes of 32 values when
+// the other operand is two accumulator tiles side by side. Blocks go row tile, u, limb.
+// In the preparation's LDS a row's pieces stay together. Byte of piece 4 u + q of row r: the pieces of a row are permuted so
+// that neither 16 rows' loads of one piece nor the transposing loads of 4 rows' halves of 4 pieces meet in a bank.
 template <int DK> __device__ __forceinline__ int img_at(int r, int c) {
     const int x = DK == 64 ? ((r >> 1) & 1) * 4 + ((r >> 2) & 3) : (r & 3) * 4 + ((r >> 2) & 3);
     return r * (DK * 2) + ((c ^ x) << 4);
 }
-// 16 x 32 block (row tile t, columns 32 u ..) of T or P
-__device__ __forceinline__ int tp_block(int t, int u) { return t < 2 ? t : t * 2 - 2 + u; }
+// 16 x 32 block (row tile t, columns 32 u ..) of P or P T
+__device__ __forceinline__ int pt_block(int t, int u) { return t < 2 ? t : t * 2 - 2 + u; }
 
 // 2^e as a float, e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -110,9 +116,8 @@ __device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp
 // exponent of the power of two that brings a largest absolute value to [2^top, 2^(top + 1)); 0 for 0 and non-finite
 __device__ __forceinline__ int lift(float most, int top) {
     const int b = (int)((__float_as_uint(most) >> 23) & 255);
-    if (b == 0 || b == 255) return 0;
     const int e = top - (b - 127);
-    return e < -80 ? -80 : e > 80 ? 80 : e;
+    return (e < -80 ? -80 : e > 80 ? 80 : e) & -(int)((uint32_t)(b - 1) < 254u);
 }
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < __builtin_inff(); }
 // the larger of two; not a number if either is not
@@ -125,21 +130,33 @@ __device__ __forceinline__ float groups_max(float v) {
     const auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+// (the first limbs are made opaque where they stand packed: else each is rounded a second time on its own for the second)
 __device__ __forceinline__ void split8(const float *x, float up, h8 &hi, h8 &lo) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float v = x[i] * up;
-        const _Float16 h = (_Float16)v;
-        hi[i] = h;
-        lo[i] = (_Float16)(v - (float)h);
-    }
+    for (int i = 0; i < 8; i++) hi[i] = (_Float16)(x[i] * up);
+    asm("" : "+v"(hi));
+#pragma unroll
+    for (int i = 0; i < 8; i++) lo[i] = (_Float16)__builtin_fmaf(x[i], up, -(float)hi[i]);
 }
 __device__ __forceinline__ f4 mma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4 mma3(h8 ah, h8 al, h8 bh, h8 bl, f4 c) { return mma(al, bh, mma(ah, bl, mma(ah, bh, c))); }
 
+__device__ __forceinline__ void split4(const f4 &x, float up, h4 &hi, h4 &lo) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) hi[i] = (_Float16)(x[i] * up);
+    asm("" : "+v"(hi));
+#pragma unroll
+    for (int i = 0; i < 4; i++) lo[i] = (_Float16)__builtin_fmaf(x[i], up, -(float)hi[i]);
+}
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
 struct DeltaWs {
-    char *img;    // [seq][key head][chunk]: q image, k image
-    char *tp;     // [seq][value head][chunk]: T, P
+    char *img;    // [seq][key head][chunk]: q, k
+    char *wpt;    // [seq][value head][chunk]: W, P T
     float *scal;  // [seq][value head][chunk][SCAL]
     int chunks;
 };
@@ -150,98 +167,102 @@ __device__ __forceinline__ int tokens_of(const DeltaArgs &a, int s) {
     return w < 0 ? 0 : w < a.T ? w : a.T;
 }
 
-// One workgroup a chunk of a key head; its value heads two at a time.
-template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, DeltaWs w) {
-    constexpr int IMG = img_bytes(DK), LD = 68, U = DK / 32, PER = DK / 16;  // PER: 16-byte pieces of a row a thread takes
-    __shared__ __align__(16) char lds[2 * IMG > 4 * CH * LD * 4 ? 2 * IMG : 4 * CH * LD * 4];
-    __shared__ __align__(16) float ck[CH], cq[CH], beta[2][CH], colup[2][CH];
-    __shared__ double G[2][CH];
-    __shared__ int bad[2][CH];  // rows of A with a value that is not finite
+// One workgroup a chunk of a key head and `each` of its value heads, one after the other (a wave: row tile, or column tile,
+// `tile`).
+template <int DK> __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaArgs a, DeltaWs w, int each) {
+    constexpr int IMG = img_bytes(DK), LD = 68, U = DK / 32;
+    // k; q, whose place A (then T), P and P's limbs take
+    constexpr int AAT = IMG, PAT = AAT + CH * LD * 4, LAT = PAT + CH * LD * 4, END = LAT + PT_BYTES;
+    static_assert(END >= 2 * IMG, "q");
+    __shared__ __align__(16) char lds[END];
+    __shared__ __align__(16) float ck[CH], cq[CH], beta[CH], left[CH];
+    __shared__ double G[CH];
+    __shared__ int bad[CH];  // rows of A with a value that is not finite
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = blockIdx.x, hk = blockIdx.y, s = blockIdx.z, t0 = c * CH;
-    const int rep = a.n_v / a.n_k;
+    const int tile = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rep = a.n_v / a.n_k, parts = (rep + each - 1) / each;
+    const int c = blockIdx.x, hk = blockIdx.y / parts, part0 = (blockIdx.y - hk * parts) * each, s = blockIdx.z, t0 = c * CH;
 
-    // running sums of two heads' g log2(e), a wave each, in fp64: a difference of two sums of the chunk keeps its digits however far
+    // running sums of a head's g log2(e), in fp64: a difference of two sums of the chunk keeps its digits however far
     // both have fallen. e^-4096 is 0 in fp32 as is e^g of any g below, -inf among them: such a g counts as -4096, and the
     // sums behind it stay finite and keep their digits.
-    auto decays = [&](int h0) __attribute__((always_inline)) {
-        if (wave < 2 && h0 + wave < rep) {
-            const int hv = hk * rep + h0 + wave;
+    auto decays = [&](int hv) __attribute__((always_inline)) {
+        if (tile == 0) {
             const bool at = t0 + lane < a.T;
             const int64_t row = (int64_t)s * a.T + t0 + lane;
             const float gv = at ? a.g[row * a.ldg + hv] : 0.f, bv = at ? a.beta[row * a.ldb + hv] : 0.f;
             const bool in = t0 + lane < tokens_of(a, s);
             double v = !in ? 0.0 : (gv < -4096.f ? -4096.0 : (double)gv) * 1.4426950408889634;
-            beta[wave][lane] = in ? bv : 0.f;
-            bad[wave][lane] = 0;
+            beta[lane] = in ? bv : 0.f;
+            bad[lane] = 0;
             for (int o = 1; o < 64; o <<= 1) {
                 const double up = __shfl_up(v, o);
                 if (lane >= o) v += up;
             }
-            G[wave][lane] = v;
+            G[lane] = v;
         }
     };
-    // rows of q (image 0) and k (image 1) to limbs: 4 threads a row (loaded before it is known how many tokens there are,
-    // then taken for zeros past them)
+    // rows of q and k to limbs: 4 threads a row (loaded before it is known how many tokens there are, then taken for zeros
+    // past them)
     {
         const int r = tid >> 2, part = tid & 3;
         const bool at = t0 + r < a.T;
         const int64_t row = (int64_t)s * a.T + t0 + r;
         char *out = w.img + (((int64_t)s * a.n_k + hk) * w.chunks + c) * (2 * IMG);
-        float x[2][PER / 2][8];
+        float x[2][U][8];
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             const float *src = (m ? a.k + row * a.ldk : a.q + row * a.ldq) + (int64_t)hk * DK;
 #pragma unroll
-            for (int i = 0; i < PER / 2; i++) {
+            for (int i = 0; i < U; i++) {
                 *(f4 *)(x[m][i]) = at ? *(const f4 *)(src + i * 32 + part * 4) : f4{0, 0, 0, 0};
                 *(f4 *)(x[m][i] + 4) = at ? *(const f4 *)(src + i * 32 + 16 + part * 4) : f4{0, 0, 0, 0};
             }
         }
-        decays(0);
+        decays(hk * rep + part0);
         const int n = tokens_of(a, s);
         if (t0 >= n) return;
         const bool in = t0 + r < n;
 #pragma unroll
         for (int m = 0; m < 2; m++) {
 #pragma unroll
-            for (int i = 0; i < PER / 2; i++)
+            for (int i = 0; i < U; i++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[m][i][j] = in ? x[m][i][j] : 0.f;
             float sum = 0.f, most = 0.f;
 #pragma unroll
-            for (int i = 0; i < PER / 2; i++)
+            for (int i = 0; i < U; i++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) sum = __builtin_fmaf(x[m][i][j], x[m][i][j], sum), most = fmaxf(most, fabsf(x[m][i][j]));
-            sum += __shfl_xor(sum, 1);
-            most = fmaxf(most, __shfl_xor(most, 1));
-            sum += __shfl_xor(sum, 2);
-            most = fmaxf(most, __shfl_xor(most, 2));
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                sum += __shfl_xor(sum, o);
+                most = fmaxf(most, __shfl_xor(most, o));
+            }
             const int e = lift(most, 13);
             const float up = pow2(e);
             if (part == 0) (m ? ck : cq)[r] = pow2(-e) * (a.l2norm ? 1.0f / sqrtf(sum + 1e-6f) : 1.0f);
 #pragma unroll
-            for (int i = 0; i < PER / 2; i++) {
+            for (int i = 0; i < U; i++) {
                 h8 hi, lo;
                 split8(x[m][i], up, hi, lo);
-                const int at = m * IMG + img_at<DK>(r, i * 4 + part);
-                *(h8 *)(lds + at) = hi;
-                *(h8 *)(lds + at + IMG / 2) = lo;
-                *(h8 *)(out + at) = hi;
-                *(h8 *)(out + at + IMG / 2) = lo;
+                char *in_lds = lds + (m ? 0 : IMG) + img_at<DK>(r, i * 4 + part);
+                *(h8 *)in_lds = hi;
+                *(h8 *)(in_lds + IMG / 2) = lo;
+                char *to = out + m * IMG + ((r >> 4) * U + i) * 2048 + (part * 16 + (r & 15)) * 16;
+                if (part0 == 0) *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
             }
         }
     }
     __syncthreads();
-    // wave t: row tile t of K K^T and Q K^T, columns up to its own tile
+    // the wave's row tile of K K^T and Q K^T, columns up to its own tile
     f4 kk[4], qk[4];
     {
         int ra[U];  // (rows 16 apart permute alike)
 #pragma unroll
         for (int u = 0; u < U; u++) ra[u] = img_at<DK>(col, 4 * u + g);
-        auto rows = [&](int m, int limb, int tile, int u) __attribute__((always_inline)) {
-            return *(const h8 *)(lds + m * IMG + limb * (IMG / 2) + ra[u] + tile * 16 * (DK * 2));
+        auto rows = [&](int m, int limb, int t, int u) __attribute__((always_inline)) {
+            return *(const h8 *)(lds + (m ? 0 : IMG) + limb * (IMG / 2) + ra[u] + t * 16 * (DK * 2));
         };
 #pragma unroll
         for (int j = 0; j < 4; j++) kk[j] = qk[j] = f4{0, 0, 0, 0};
@@ -250,7 +271,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
 #pragma unroll
             for (int y = 0; y < 2; y++) {
 #pragma unroll
-                for (int m = 0; m < 2; m++) own[set][m][y] = rows(m, y, wave, u);
+                for (int m = 0; m < 2; m++) own[set][m][y] = rows(m, y, tile, u);
 #pragma unroll
                 for (int j = 0; j < 4; j++) all[set][j][y] = rows(1, y, j, u);
             }
@@ -262,71 +283,74 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
             const auto &o = own[u & 1];
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (j <= wave) {
+                if (j <= tile) {
                     const auto &b = all[u & 1][j];
                     kk[j] = mma3(o[1][0], o[1][1], b[0], b[1], kk[j]);
                     qk[j] = mma3(o[0][0], o[0][1], b[0], b[1], qk[j]);
                 }
         }
     }
-    float *const M = (float *)lds;  // A of two heads, then P of two: [64][LD]
-    for (int h0 = 0; h0 < rep; h0 += 2) {
-        __syncthreads();  // (the images, or the pair before, are done with)
-        if (h0) decays(h0);
-        __syncthreads();
-#pragma unroll 1
-        for (int h = 0; h < 2; h++) {
-            if (h0 + h >= rep) break;
+    float *const A = (float *)(lds + AAT), *const P = (float *)(lds + PAT);  // [64][LD]
+    char *const pl = lds + LAT + lane * 16;
+    for (int h = part0; h < min(part0 + each, rep); h++) {
+        const int64_t unit = ((int64_t)s * a.n_v + hk * rep + h) * w.chunks + c;
+        float *const sc = w.scal + unit * SCAL;
+        __syncthreads();  // (q's limbs, or the head before, are done with)
+        if (h > part0) {
+            decays(hk * rep + h);
+            __syncthreads();
+        }
+        {
             // e^(G_r - G_c): left of the diagonal tile by way of the row tile's first token, a factor a row and one a column
-            const int r0 = wave * 16 + 4 * g;
-            const double mid = G[h][wave * 16];
+            const int r0 = tile * 16 + 4 * g;
+            const double mid = G[tile * 16];
             double gr[4], gc[4];
             float kc[4], ec[4];
-            const f4 kr = *(const f4 *)(ck + r0), b = *(const f4 *)(beta[h] + r0), qr = *(const f4 *)(cq + r0);
+            const f4 kr = *(const f4 *)(ck + r0), b = *(const f4 *)(beta + r0), qr = *(const f4 *)(cq + r0);
             f4 most = {0, 0, 0, 0}, er;
 #pragma unroll
-            for (int i = 0; i < 4; i++) gr[i] = G[h][r0 + i], gc[i] = G[h][i * 16 + col], kc[i] = ck[i * 16 + col];
+            for (int i = 0; i < 4; i++) gr[i] = G[r0 + i], gc[i] = G[i * 16 + col], kc[i] = ck[i * 16 + col];
 #pragma unroll
             for (int i = 0; i < 4; i++) er[i] = exp2_of(gr[i] - mid);
 #pragma unroll
-            for (int j = 0; j < 4; j++) ec[j] = j < wave ? exp2_of(mid - gc[j]) * kc[j] : 0.f;
+            for (int j = 0; j < 4; j++) ec[j] = j < tile ? exp2_of(mid - gc[j]) * kc[j] : 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if (j > wave) continue;
+                if (j > tile) continue;
                 const int cj = j * 16 + col;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int r = r0 + i;
-                    const float e = j < wave ? er[i] * ec[j] : exp2_of(gr[i] - gc[j]) * kc[j];
+                    const float e = j < tile ? er[i] * ec[j] : exp2_of(gr[i] - gc[j]) * kc[j];
                     const float x = cj < r ? b[i] * e * (kk[j][i] * kr[i]) : 0.f;
                     most[i] = max_or_nan(most[i], fabsf(x));
-                    M[h * CH * LD + r * LD + cj] = x;
-                    M[(2 + h) * CH * LD + r * LD + cj] = cj <= r ? e * (qk[j][i] * (qr[i] * a.scale)) : 0.f;
+                    A[r * LD + cj] = x;
+                    P[r * LD + cj] = cj <= r ? e * (qk[j][i] * (qr[i] * a.scale)) : 0.f;
                 }
             }
             // A row of A that is not finite must not reach the rows of T above it (0 times it is not 0): it is taken out here,
             // and the token's own factor then makes its row of R, and with it every later one, not a number.
             if (__any(!is_finite(most[0]) | !is_finite(most[1]) | !is_finite(most[2]) | !is_finite(most[3]))) {
-                for (int j = 0; j <= wave; j++)
+                for (int j = 0; j <= tile; j++)
                     for (int i = 0; i < 4; i++) {
-                        const int r = wave * 16 + 4 * g + i;
-                        float *x = M + h * CH * LD + r * LD + j * 16 + col;
-                        if (!is_finite(*x)) *x = 0.f, bad[h][r] = 1;
+                        const int r = tile * 16 + 4 * g + i;
+                        float *x = A + r * LD + j * 16 + col;
+                        if (!is_finite(*x)) *x = 0.f, bad[r] = 1;
                     }
             }
         }
         __syncthreads();
-        // T by blocks of 16. On the diagonal, a wave a head: lane 16 b + c has column c of block b, x_i = [i = c] - sum_j
-        // A_ij x_j (rows of A read by 16 lanes at once).
-        if (wave < 2 && h0 + wave < rep) {
-            float *const A = M + wave * CH * LD + (lane >> 4) * (16 * LD + 16);
+        // T by blocks of 16. On the diagonal, the first wave: lane 16 b + c has column c of block b, x_i = [i = c] -
+        // sum_j A_ij x_j (rows of A read by 16 lanes at once).
+        if (tile == 0) {
+            float *const D = A + (lane >> 4) * (16 * LD + 16);
             float x[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 float v0 = col == i ? 1.f : 0.f, v1 = 0.f;
 #pragma unroll
                 for (int j = 0; j < i; j += 4) {
-                    const f4 m = *(const f4 *)(A + i * LD + j);
+                    const f4 m = *(const f4 *)(D + i * LD + j);
                     v0 = __builtin_fmaf(-m[0], x[j], v0);
                     if (j + 1 < i) v1 = __builtin_fmaf(-m[1], x[j + 1], v1);
                     if (j + 2 < i) v0 = __builtin_fmaf(-m[2], x[j + 2], v0);
@@ -335,17 +359,56 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
                 x[i] = v0 + v1;
             }
 #pragma unroll
-            for (int i = 0; i < 16; i++) A[i * LD + col] = x[i];
+            for (int i = 0; i < 16; i++) D[i * LD + col] = x[i];
+        }
+        // The others: P's limbs (row tiles 0 and 1, 2, 3), the factors that need no T.
+        if (tile) {
+            for (int t = tile == 1 ? 0 : tile; t <= tile; t++) {
+                const int us = t < 2 ? 1 : 2, r = t * 16 + col;
+                f4 p[2][2];
+                float most = 0.f;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++) p[u][y] = *(const f4 *)(P + r * LD + 32 * u + 16 * y + 4 * g);
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            p[u][y][i] = 2 * u + y <= t ? p[u][y][i] : 0.f;  // (past the row's tile nothing was written)
+                            most = fmaxf(most, fabsf(p[u][y][i]));
+                        }
+                const int e = lift(groups_max(most), 13);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    if (u >= us) continue;
+                    float x[8];
+                    h8 hi, lo;
+                    *(f4 *)x = p[u][0], *(f4 *)(x + 4) = p[u][1];
+                    split8(x, pow2(e), hi, lo);
+                    char *to = pl + pt_block(t, u) * 2048;
+                    *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
+                }
+                if (g == 0) sc[ROW_D * CH + r] = pow2(-e);
+            }
+        }
+        if (tile == 2) {
+            const float grown = exp2_of(G[lane]), b = beta[lane];
+            left[lane] = exp2_of(G[CH - 1] - G[lane]) * ck[lane];
+            sc[ROW_B * CH + lane] = bad[lane] ? __builtin_nanf("") : b;
+            sc[ROW_F * CH + lane] = b * grown * ck[lane];
+            sc[ROW_A * CH + lane] = a.scale * grown * cq[lane];
+            if (lane == CH - 1) sc[6 * CH] = grown;
         }
         __syncthreads();
         // Below it, block column by block column: T_rc = -T_rr sum_{c<=k<r} A_rk T_kc in fp32 MFMAs, whose accumulators are
-        // the B operand of the next product (16 columns, rows 4 g + i by instruction i). Two waves a head: column 0, and
-        // columns 1 and 2.
+        // the B operand of the next product (16 columns, rows 4 g + i by instruction i). Two waves: column 0, and columns 1
+        // and 2.
         {
-            const int h = wave >> 1, first = wave & 1;
-            float *const A = M + h * CH * LD;
             f4 t[3];  // T_10 T_20 T_30 or T_21 T_31 T_32
-            if (h0 + h < rep) {
+            if (tile < 2) {
                 auto block = [&](int r, int k) __attribute__((always_inline)) { return *(const f4 *)(A + (16 * r + col) * LD + 16 * k + 4 * g); };
                 auto times = [&](const f4 &m, const f4 &x, f4 y) __attribute__((always_inline)) {
 #pragma unroll
@@ -359,7 +422,7 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
                     return x;
                 };
                 const f4 zero = {0, 0, 0, 0};
-                if (first == 0) {
+                if (tile == 0) {
                     const f4 x0 = corner(0);
                     t[0] = -times(block(1, 1), times(block(1, 0), x0, zero), zero);
                     t[1] = -times(block(2, 2), times(block(2, 1), t[0], times(block(2, 0), x0, zero)), zero);
@@ -372,99 +435,101 @@ template <int DK> __global__ __launch_bounds__(256) void delta_prep_kernel(Delta
                 }
             }
             __syncthreads();  // (A is done with: T takes its place)
-            if (h0 + h < rep) {
+            if (tile < 2) {
 #pragma unroll
                 for (int b = 0; b < 3; b++) {
-                    const int r = first == 0 ? b + 1 : b == 0 ? 2 : 3, k = first == 0 ? 0 : b == 2 ? 2 : 1;
+                    const int r = tile == 0 ? b + 1 : b == 0 ? 2 : 3, k = tile == 0 ? 0 : b == 2 ? 2 : 1;
 #pragma unroll
                     for (int i = 0; i < 4; i++) A[(16 * r + 4 * g + i) * LD + 16 * k + col] = t[b][i];
                 }
             }
         }
         __syncthreads();
-        // a power of two for each column of T (its largest is at least 1, on the diagonal)
-        if (wave < 2 && h0 + wave < rep) {
-            const float *const A = M + wave * CH * LD;
-            float most = 1.f, t[CH];
-#pragma unroll
-            for (int i = 0; i < CH; i++) t[i] = A[i * LD + lane];
-#pragma unroll
-            for (int i = 0; i < CH; i++) most = fmaxf(most, i >= (lane & ~15) ? fabsf(t[i]) : 0.f);
-            colup[wave][lane] = pow2(lift(most, 13));
-        }
-        __syncthreads();
-        // operands: wave t takes row tile t of T and P of both heads
-#pragma unroll 1
-        for (int h = 0; h < 2; h++) {
-            if (h0 + h >= rep) break;
-            const int64_t unit = ((int64_t)s * a.n_v + hk * rep + h0 + h) * w.chunks + c;
-            char *const out = w.tp + unit * (2 * TP_BYTES) + lane * 16;
-            const int r = wave * 16 + col;
-            const int us = wave < 2 ? 1 : 2;
-            f4 t[2][2], p[2][2], cu[2][2];
+        // The wave's column tile of T, transposed, as the operand of two products: with the tokens' e^(G_63 - G_l) for W^T (times
+        // K), and for (P T)^T (times P^T). A power of two for each column; the products' accumulators, 2^-19 of them (64 terms
+        // below 2^28), are 4 of the 8 values of an operand's lane each.
+        {
+            f4 t[2][2], tw[2][2];
+            float most = 0.f, mostw = 0.f;
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
-                    const float *src = M + h * CH * LD + r * LD + 32 * u + 16 * y + 4 * g;
-                    t[u][y] = *(const f4 *)src;
-                    p[u][y] = *(const f4 *)(src + 2 * CH * LD);
-                    cu[u][y] = *(const f4 *)(colup[h] + 32 * u + 16 * y + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) t[u][y][i] = A[(32 * u + 16 * y + 4 * g + i) * LD + tile * 16 + col];
+                    tw[u][y] = *(const f4 *)(left + 32 * u + 16 * y + 4 * g);
                 }
-            float most = 0.f;
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int y = 0; y < 2; y++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        // (past the row's tile nothing was written)
-                        const bool there = 2 * u + y <= wave;
-                        t[u][y][i] = there ? t[u][y][i] * cu[u][y][i] : 0.f;
-                        p[u][y][i] = there ? p[u][y][i] : 0.f;
-                        most = fmaxf(most, fabsf(p[u][y][i]));
+                        t[u][y][i] = 2 * u + y >= tile ? t[u][y][i] : 0.f;  // (above the diagonal tile nothing was written)
+                        tw[u][y][i] *= t[u][y][i];
+                        most = fmaxf(most, fabsf(t[u][y][i]));
+                        mostw = fmaxf(mostw, fabsf(tw[u][y][i]));
                     }
-            const int e = lift(groups_max(most), 13);
+            mostw = groups_max(mostw);
+            const int e = lift(groups_max(most), 13), ew = lift(mostw, 13);
+            constexpr float DOWN = 1.0f / (1 << 19);
+            if (g == 0) {
+                // (nothing of a token whose column is gone, whatever its R: it must not set the scale of the others)
+                sc[ROW_W * CH + tile * 16 + col] = mostw < 0x1p-126f ? 0.f : pow2(19 - ew);
+                sc[ROW_P * CH + tile * 16 + col] = pow2(19 - e);
+            }
+            h8 l[2][2], lw[2][2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                if (u >= us) continue;
                 float x[8];
-                h8 hi, lo;
-                char *to = out + tp_block(wave, u) * 2048;
                 *(f4 *)x = t[u][0], *(f4 *)(x + 4) = t[u][1];
-                split8(x, 1.f, hi, lo);
-                *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
-                *(f4 *)x = p[u][0], *(f4 *)(x + 4) = p[u][1];
-                split8(x, pow2(e), hi, lo);
-                *(h8 *)(to + TP_BYTES) = hi, *(h8 *)(to + TP_BYTES + 1024) = lo;
+                split8(x, pow2(e), l[u][0], l[u][1]);
+                *(f4 *)x = tw[u][0], *(f4 *)(x + 4) = tw[u][1];
+                split8(x, pow2(ew), lw[u][0], lw[u][1]);
             }
-            if (g == 0) {
-                float *sc = w.scal + unit * SCAL;
-                const float grown = exp2_of(G[h][r]), left = exp2_of(G[h][CH - 1] - G[h][r]);
-                const float down = beta[h][r] / colup[h][r];
-                sc[r] = bad[h][r] ? __builtin_nanf("") : down;
-                sc[CH + r] = down * grown * ck[r];
-                sc[2 * CH + r] = a.scale * grown * cq[r];
-                sc[3 * CH + r] = pow2(-e);
-                sc[4 * CH + r] = left * ck[r];
-                if (r == CH - 1) sc[5 * CH] = grown;
+            const int u0 = tile >> 1;  // (columns 32 .. have no rows 0 .. 31)
+            char *const wo = w.wpt + unit * (IMG + PT_BYTES) + lane * 16 + (tile & 1) * 8;
+            auto cols = [&](int limb, int r, int u) __attribute__((always_inline)) {  // 16 columns of k as rows, 32 tokens
+                const char *im = lds + limb * (IMG / 2) + img_at<DK>(4 * g + (col >> 2), 4 * (r >> 1) + (col & 3)) + (r & 1) * 8 + 32 * u * (DK * 2);
+                const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)im);
+                const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(im + 16 * (DK * 2)));
+                return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+#pragma unroll
+            for (int r = 0; r < DK / 16; r++) {
+                f4 z = {0, 0, 0, 0};
+                if (u0 == 0) z = mma3(lw[0][0], lw[0][1], cols(0, r, 0), cols(1, r, 0), z);
+                z = mma3(lw[1][0], lw[1][1], cols(0, r, 1), cols(1, r, 1), z);
+                h4 hi, lo;
+                split4(z, DOWN, hi, lo);
+                char *to = wo + (r * 2 + u0) * 2048;
+                *(h4 *)to = hi, *(h4 *)(to + 1024) = lo;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {  // row tile r of P T
+                if (r + (tile & 1) < tile) continue;
+                f4 z = {0, 0, 0, 0};
+                if (r >= tile) {
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        if (u < u0 || 2 * u > r) continue;
+                        const char *from = pl + pt_block(r, u) * 2048;
+                        z = mma3(l[u][0], l[u][1], *(const h8 *)from, *(const h8 *)(from + 1024), z);
+                    }
+                }
+                h4 hi, lo;
+                split4(z, DOWN, hi, lo);
+                char *to = wo + IMG + pt_block(r, u0) * 2048;
+                *(h4 *)to = hi, *(h4 *)(to + 1024) = lo;
             }
         }
     }
 }
 
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef short s8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) s4 lds_s4;
-typedef __attribute__((address_space(3))) char lds_char;
-typedef __attribute__((address_space(1))) const char g_char;
 template <int N> struct Count {
     static constexpr int value = N;
 };
-// all but the last N of this wave's vector memory operations have completed (they complete in order)
-template <int N> __device__ __forceinline__ void wait_vmem() { __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14); }
-// __syncthreads without its wait for every load under way: this wave's LDS stores have completed, and what it loaded to LDS
-// is the caller's to wait for
+// __syncthreads without its wait for every load under way: only this wave's LDS accesses have completed
 __device__ __forceinline__ void bare_barrier() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xC07F);
@@ -472,65 +537,41 @@ __device__ __forceinline__ void bare_barrier() {
     asm volatile("" ::: "memory");
 }
 
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-
 // nothing is moved across: loads stay ahead of the products that do not need them
 #define STAGE() __builtin_amdgcn_sched_barrier(0)
 
-// NS groups of three waves, each group 16 columns of the state. Wave A of a group carries the state: R from K S, X = T R,
-// the new state. Wave B forms the outputs from Q S and P X. Wave C brings the chunks' operands to LDS, loaded a chunk
-// ahead. The state's limbs and X go from A to B through LDS; two barriers a chunk: B works on Q S while A finds X, and on
-// P X while A forms the new state.
-template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
-    constexpr int IMG = img_bytes(DK), U = DK / 32, R = DK / 16, NB = NS * 64;
-    constexpr int NI = IMG / 16 / NB, NTP = TP_BYTES / 16 / NB;  // 16-byte pieces of an image, of T or P, a thread of C brings
-    constexpr int NSC = (SCAL / 4 + NB - 1) / NB;
-    static_assert(IMG % (16 * NB) == 0 && TP_BYTES % (16 * NB) == 0, "pieces");
-    // kbuf 2 x IMG, qbuf IMG, T, P
-    constexpr int QB = 2 * IMG, TB = 3 * IMG, PB = TB + TP_BYTES;
-    __shared__ __align__(16) char lds[PB + TP_BYTES];
-    __shared__ __align__(16) char sbuf[NS][U * 2048], xbuf[NS][4096];
-    __shared__ __align__(16) float scal[2][SCAL];
-    __shared__ float sdown[NS][64], xdown[NS][64];
-    constexpr int LV = 16 * NS + 4;  // floats between rows of v in LDS (a row's pad keeps rows 4 apart in other banks)
-    __shared__ __align__(16) float vbuf[CH * LV];
+// Four waves carry 16 columns of a head's state through its chunks. Waves A0 and A1 have the state, half of its rows each: R
+// from K S for 32 of the tokens each, then the new state's rows from W R. Waves B0 and B1, a chunk behind, form the outputs of 32
+// tokens each from Q S and (P T) R, and bring v and the factors to LDS. Each has its operands of the next chunk on their way in
+// registers while it works on this one's. The state's limbs (each half's with a power of two of its own) and R go through LDS;
+// two barriers a chunk.
+template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
+    constexpr int IMG = img_bytes(DK), U = DK / 32, H = DK / 32, HU = U / 2;  // H, HU: a half's tiles of 16 rows, of 32
+    constexpr int LV = 20;  // floats between rows of v in LDS (a row's pad keeps rows 4 apart in other banks)
+    __shared__ __align__(16) char sbuf[4][U * 2048], xbuf[2][4096];
+    __shared__ __align__(16) float scal[4][SCAL], vbuf[2][CH * LV];
+    __shared__ float sdown[4][2][64];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % NS;
-    const bool carries = wave < NS, brings = wave >= 2 * NS;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave & 1;
+    const uint32_t l16 = lane * 16;
     // consecutive workgroups go to the eight XCDs in turn: a head's column groups, and the heads of a key head, are given
     // to one XCD, whose L2 then fetches the operands once for all of them
-    const int groups = (a.dv + 16 * NS - 1) / (16 * NS), heads = a.n_v * a.n_seq, per = (heads + 7) / 8;
+    const int groups = (a.dv + 15) / 16, heads = a.n_v * a.n_seq, per = (heads + 7) / 8;
     const int unit = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3) / groups, grp = (int)(blockIdx.x >> 3) % groups;
     if (unit >= heads) return;
     const int hv = unit % a.n_v, s = unit / a.n_v, hk = hv / (a.n_v / a.n_k), n = tokens_of(a, s), chunks = (n + CH - 1) / CH;
-    const int w0 = (grp * NS + pair) * 16, c0 = w0 + col;
+    const int c0 = grp * 16 + col;
     const bool in = c0 < a.dv;
-    const int64_t head = ((int64_t)s * a.n_v + hv) * DK * a.dv + c0;
 
     const char *img = w.img + ((int64_t)s * a.n_k + hk) * w.chunks * (2 * IMG);
-    const char *tp = w.tp + ((int64_t)s * a.n_v + hv) * w.chunks * (2 * TP_BYTES);
+    const char *wpt = w.wpt + ((int64_t)s * a.n_v + hv) * w.chunks * (IMG + PT_BYTES);
     const float *sc = w.scal + ((int64_t)s * a.n_v + hv) * w.chunks * SCAL;
+    // (past the last chunk the last one again: loads without a branch, never used)
+    auto q_of = [&](int c) __attribute__((always_inline)) { return img + (int64_t)(c < chunks ? c : chunks - 1) * (2 * IMG); };
+    auto w_of = [&](int c) __attribute__((always_inline)) { return wpt + (int64_t)(c < chunks ? c : chunks - 1) * (IMG + PT_BYTES); };
 
-    // Operand of 16 rows, 32 values; of 16 columns as rows, 32 tokens (transposing loads of 4 tokens x 16 values). Rows 16
-    // apart permute alike: the lanes' addresses are kept, tiles and limbs are constant offsets.
-    int ra[U], ca[U], low_at = lane * 16 + (carries ? TB : PB);
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        ra[u] = (carries ? 0 : QB) + img_at<DK>(col, 4 * u + g);
-        ca[u] = img_at<DK>(4 * g + (col >> 2), 4 * u + (col & 3));
-    }
-    asm("" : "+v"(low_at));  // (kept as one register: the blocks are constant offsets from it)
-    auto rows = [&](int base, int t, int u) __attribute__((always_inline)) {
-        return *(const h8 *)(lds + base + ra[u] + t * 16 * (DK * 2));
-    };
-    auto cols = [&](int base, int r, int u) __attribute__((always_inline)) {
-        const char *im = lds + base + ca[r >> 1] + (r & 1) * 8 + 32 * u * (DK * 2);
-        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)im);
-        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(im + 16 * (DK * 2)));
-        return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
-    auto per_row = [&](int buf, int which, int t) __attribute__((always_inline)) {
-        return *(const f4 *)(&scal[buf][which * CH + t * 16 + 4 * g]);
+    auto per_row = [&](int c, int which, int t) __attribute__((always_inline)) {
+        return *(const f4 *)(&scal[c & 3][which * CH + t * 16 + 4 * g]);
     };
     // the four tiles of one column to limbs, its largest to [2^13, 2^14); returns what undoes the power of two
     auto largest_of = [&](const f4 (&v)[4]) __attribute__((always_inline)) {
@@ -553,8 +594,8 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
         }
         return pow2(-e);
     };
-    // A token whose row is not finite must not reach the tokens before it (its 0 in T or P times it is not 0): from the
-    // column's first such row on, rows count as 0 in the product, and `spoil` makes them not a number after it. Returns that
+    // A token whose row is not finite must not reach the tokens before it (its 0 in P T times it is not 0): from the
+    // column's first such row on, rows count as 0 in the product, and are made not a number after it. Returns that
     // row, 64 if there is none.
     auto sound = [&](f4 (&v)[4], float &most) __attribute__((always_inline)) {
         int first = CH;
@@ -576,315 +617,246 @@ template <int DK, int NS> __global__ __launch_bounds__(NS * 192) void delta_chun
         }
         return first;
     };
-    auto spoil = [&](f4 (&v)[4], int first) __attribute__((always_inline)) {
-        if (__any(first < CH)) {
+    // 32 rows of an image (K or Q), and x[y] = the image times the limbs of the state's half y; the next chunk's values take
+    // the place of what is done with
+    h8 M[U][2][2];
+    auto get_rows = [&](const char *from, int u) __attribute__((always_inline)) {
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[t][i] = t * 16 + 4 * g + i < first ? v[t][i] : __builtin_nanf("");
-        }
+            for (int y = 0; y < 2; y++) M[u][t][y] = *(const h8 *)(from + half * (U * 4096) + ((t * U + u) * 2 + y) * 1024 + l16);
     };
-    // x[t] = rows of an image (A: K at `base`, B: Q) times the limbs l: the four tiles' products in turn, so that none waits
-    // for its own last; the next operands are on their way meanwhile
-    auto image_times = [&](int base, const auto &l, f4 (&x)[4]) __attribute__((always_inline)) {
-        h8 hi[2][4], lo[2][4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) hi[0][t] = rows(base, t, 0), lo[0][t] = rows(base + IMG / 2, t, 0);
-        STAGE();
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (u + 1 < U) {
-#pragma unroll
-                for (int t = 0; t < 4; t++) hi[(u + 1) & 1][t] = rows(base, t, u + 1), lo[(u + 1) & 1][t] = rows(base + IMG / 2, t, u + 1);
-                STAGE();
-            }
-#pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = mma(hi[u & 1][t], l[u][0], u ? x[t] : f4{0, 0, 0, 0});
-#pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = mma(hi[u & 1][t], l[u][1], x[t]);
-#pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = mma(lo[u & 1][t], l[u][0], x[t]);
-            STAGE();
-        }
-    };
-    // x[t] += T (A) or P (B) times the limbs l
-    auto lower_times = [&](const h8 (&l)[2][2], f4 (&x)[4]) __attribute__((always_inline)) {
-        h8 m[6][2];
-#pragma unroll
-        for (int i = 0; i < 6; i++)
-#pragma unroll
-            for (int y = 0; y < 2; y++) m[i][y] = *(const h8 *)(lds + low_at + i * 2048 + y * 1024);
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int p = 0; p < 3; p++)
-#pragma unroll
-                for (int t = 2 * u; t < 4; t++) x[t] = mma(m[tp_block(t, u)][p == 2], l[u][p == 1], x[t]);
-    };
-
-    // C: a chunk's operands go straight from memory to LDS, 16 bytes a lane, in two sets: K with P of the chunk before, Q
-    // with T. The lines of the next chunk's set are touched meanwhile (a word of each 128 bytes), so that they are in L2
-    // when their turn comes.
-    const uint32_t ct = (uint32_t)(tid - 2 * NB), c16 = ct * 16;
-    const int cw = (wave - 2 * NS) * 1024;
-    auto get = [&](int to, const char *from, auto count) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < decltype(count)::value; i++)
-            __builtin_amdgcn_global_load_lds((g_char *)(from + i * NB * 16 + c16), (lds_char *)(lds + to + i * NB * 16 + cw), 16, 0, 0);
-    };
-    typedef Count<NI> Image;
-    typedef Count<NTP> Low;
-    constexpr int TI = NI / 8, TL = (NTP + 7) / 8;  // touches of an image, of T or P
-    uint32_t touched[TI + TL];
-    auto touch = [&](const char *image, const char *low) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < TI; i++) touched[i] = *(const uint32_t *)(image + (i * NB + ct) * 128);
-#pragma unroll
-        for (int i = 0; i < TL; i++) touched[TI + i] = *(const uint32_t *)(low + ((i * NB + ct) * 128 < TP_BYTES ? (i * NB + ct) * 128 : 0));
-    };
-    auto touch_done = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < TI + TL; i++) asm volatile("" ::"v"(touched[i]));
-    };
-    u4 fa[NSC];
-    auto get_fac = [&](int c) __attribute__((always_inline)) {
-        const float *from = sc + (int64_t)(c < chunks ? c : chunks - 1) * SCAL;
-#pragma unroll
-        for (int i = 0; i < NSC; i++) fa[i] = *(const u4 *)(from + (ct + i * NB < SCAL / 4 ? ct + i * NB : SCAL / 4 - 1) * 4);
-    };
-    auto put_fac = [&](int c) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NSC; i++)
-            if (ct + i * NB < SCAL / 4) *(u4 *)&scal[c & 1][(ct + i * NB) * 4] = fa[i];
-    };
-    // (past the last chunk the last one again: loads without a branch, never used)
-    auto q_of = [&](int c) __attribute__((always_inline)) { return img + (int64_t)(c < chunks ? c : chunks - 1) * (2 * IMG); };
-    auto t_of = [&](int c) __attribute__((always_inline)) { return tp + (int64_t)(c < chunks ? c : chunks - 1) * (2 * TP_BYTES); };
-
-    // C: 4 values of 4 rows of v a thread; past the last row that row again (its factor is 0), past the last column the
-    // last four (their state is never stored)
-    u4 va[4];
-    const int vr = (int)ct / (4 * NS), vc = (int)ct % (4 * NS) * 4, vx = grp * NS * 16 + vc;
-    const float *const vb = a.v + (int64_t)s * a.T * a.ldv + (int64_t)hv * a.dv + (vx + 4 <= a.dv ? vx : a.dv - 4);
-    auto get_v = [&](int c) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int tok = c * CH + i * 16 + vr;
-            va[i] = *(const u4 *)(vb + (int64_t)(tok < n ? tok : n - 1) * a.ldv);
-        }
-    };
-    auto put_v = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) *(u4 *)(vbuf + (i * 16 + vr) * LV + vc) = va[i];
-    };
-
-    // a lane's values of o: rows 4 g + i of a tile, column c0
-    const uint32_t o_at = (uint32_t)(4 * g) * (uint32_t)a.ldo + (uint32_t)c0;
-    float *const ob = a.o + (int64_t)s * a.T * a.ldo + (int64_t)hv * a.dv;
-    f4 S[R];
-    h8 Sl[U][2];
-    // The state's limbs: one power of two a column, kept from chunk to chunk while the column's largest stays in
-    // [2^3, 2^15) of it (below 2^15 nothing overflows, and 22 bits remain down to 2^-2).
-    float Sup = 1.f;
-    auto split_tiles = [&](int u) __attribute__((always_inline)) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = S[2 * u + (i >> 2)][i & 3];
-        split8(x, Sup, Sl[u][0], Sl[u][1]);
-    };
-    auto publish = [&]() __attribute__((always_inline)) {
+    auto image_times = [&](int c, const char *next, f4 (&x)[2][2]) __attribute__((always_inline)) {
+        h8 l[U][2];
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int x = 0; x < 2; x++) *(h8 *)(sbuf[pair] + (u * 2 + x) * 1024 + lane * 16) = Sl[u][x];
-        sdown[pair][lane] = 1.0f / Sup;
-    };
-    auto largest = [&]() __attribute__((always_inline)) {
-        float most = 0.f;
+            for (int i = 0; i < 2; i++) l[u][i] = *(const h8 *)(sbuf[c & 3] + (u * 2 + i) * 1024 + l16);
 #pragma unroll
-        for (int r = 0; r < R; r++)
+        for (int u = 0; u < HU; u++) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r][i]));
-        return groups_max(most);
-    };
-    auto scale_state = [&](float most) __attribute__((always_inline)) {
-        Sup = pow2(lift(most, 11));
+            for (int p = 0; p < 3; p++)
 #pragma unroll
-        for (int u = 0; u < U; u++) split_tiles(u);
+                for (int y = 0; y < 2; y++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+                        x[y][t] = mma(M[y * HU + u][t][p == 2], l[y * HU + u][p == 1], u || p ? x[y][t] : f4{0, 0, 0, 0});
+            STAGE();
+            get_rows(next, u), get_rows(next, HU + u);
+            STAGE();
+        }
     };
     // (a loop each, with the same two barriers a turn: no role keeps another's registers)
-    if (carries) {
+    if (wave < 2) {
+        // The half is held times a power of two, one a column, kept from chunk to chunk while the column's largest value stays
+        // in [2^3, 2^15) (below 2^15 its limbs do not overflow, and 22 bits remain down to 2^-2).
+        f4 S[H];
+        float Sup = 1.f, Sdown = 1.f;
+        const int64_t head = (((int64_t)s * a.n_v + hv) * DK + half * (DK / 2)) * a.dv + c0;
+        auto publish = [&](int c, int u) __attribute__((always_inline)) {
+            float x[8];
 #pragma unroll
-        for (int r = 0; r < R; r++)
+            for (int i = 0; i < 8; i++) x[i] = S[2 * u + (i >> 2)][i & 3];
+            h8 hi, lo;
+            split8(x, 1.f, hi, lo);
+            char *to = sbuf[c & 3] + (half * HU + u) * 2048 + l16;
+            *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
+        };
+        auto largest = [&]() __attribute__((always_inline)) {
+            float most = 0.f;
+#pragma unroll
+            for (int r = 0; r < H; r++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r][i]));
+            return groups_max(most);
+        };
+        auto scale_state = [&](int c, float most) __attribute__((always_inline)) {
+            const int have = (int)(__float_as_uint(Sup) >> 23) - 127, want = have + lift(most, 11);  // (from -80 to 80 in all)
+            const int e = (want < -80 ? -80 : want > 80 ? 80 : want) - have;
+            Sup *= pow2(e), Sdown *= pow2(-e);
+#pragma unroll
+            for (int r = 0; r < H; r++) S[r] *= pow2(e);
+#pragma unroll
+            for (int u = 0; u < HU; u++) publish(c, u);
+        };
+#pragma unroll
+        for (int r = 0; r < H; r++)
 #pragma unroll
             for (int i = 0; i < 4; i++) S[r][i] = in && a.state_in ? a.state_in[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] : 0.f;
-        scale_state(largest());
-        publish();
-        __syncthreads();
+        scale_state(0, largest());
+        sdown[0][half][lane] = Sdown;
+        h8 W[H][2][2];
+        auto get_w = [&](const char *from, int r) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) W[r][u][y] = *(const h8 *)(from + half * (IMG / 2) + ((r * 2 + u) * 2 + y) * 1024 + l16);
+        };
+        if (chunks) {
+#pragma unroll
+            for (int u = 0; u < U; u++) get_rows(q_of(0) + IMG, u);
+#pragma unroll
+            for (int r = 0; r < H; r++) get_w(w_of(0), r);
+        }
+        bare_barrier();
         for (int c = 0; c < chunks; c++) {
-            const int buf = c & 1, K = buf * IMG;
-            f4 x[4];
-            h8 l[2][2];
-            const float Sdown = 1.0f / Sup;
-            f4 v[4], fb[4];
+            f4 z[2][2], x[4];
+            {
+                f4 v[2], fb[2];
+                const float d0 = sdown[c & 3][0][lane], d1 = sdown[c & 3][1][lane];
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
+                for (int t = 0; t < 2; t++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[t][i] = vbuf[(t * 16 + 4 * g + i) * LV + pair * 16 + col];
-                v[t] *= per_row(buf, 0, t), fb[t] = per_row(buf, 1, t) * Sdown;
-            }
-            image_times(K, Sl, x);
-#pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = v[t] - fb[t] * x[t];
-            float mostR = largest_of(x);
-            const int first = sound(x, mostR);
-            const float Rdown = limbs_of(x, mostR, l);
-#pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = f4{0, 0, 0, 0};
-            lower_times(l, x);
-            spoil(x, first);
-#pragma unroll
-            for (int t = 0; t < 4; t++) *(f4 *)(xbuf[pair] + t * 1024 + lane * 16) = x[t];  // (in units of R's limbs)
-            xdown[pair][lane] = Rdown;
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 4, t);
-            h8 hi[2][2][2], lo[2][2][2];  // [set][tile of the pair][tokens]
-            auto bring = [&](int r, int set) __attribute__((always_inline)) {
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++) hi[set][j][u] = cols(K, r + j, u), lo[set][j][u] = cols(K + IMG / 2, r + j, u);
-            };
-            bring(0, 0);
-            STAGE();
-            const float down = limbs_of(x, largest_of(x), l) * Rdown, grown = scal[buf][5 * CH];
-            float most = 0.f;
-            // a pair of tiles' products while the pair before is added to the state and split
-            f4 z[2][2];
-            auto add = [&](int r, int set) __attribute__((always_inline)) {
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    S[r + j] = grown * S[r + j] + down * z[set][j];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r + j][i]));
+                    for (int i = 0; i < 4; i++) v[t][i] = vbuf[c & 1][((2 * half + t) * 16 + 4 * g + i) * LV + col];
+                    v[t] *= per_row(c, ROW_B, 2 * half + t), fb[t] = per_row(c, ROW_F, 2 * half + t);
                 }
-                split_tiles(r >> 1);
-            };
+                image_times(c, q_of(c + 1) + IMG, z);
 #pragma unroll
-            for (int r = 0; r < R; r += 2) {
-                const int set = (r >> 1) & 1;
-                if (r + 2 < R) bring(r + 2, set ^ 1);
-                STAGE();
+                for (int t = 0; t < 2; t++)
+                    *(f4 *)(xbuf[c & 1] + (2 * half + t) * 1024 + l16) = v[t] - fb[t] * (z[0][t] * d0 + z[1][t] * d1);
+            }
+            bare_barrier();
+            h8 l[2][2];
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[t] = *(const f4 *)(xbuf[c & 1] + t * 1024 + l16) * per_row(c, ROW_W, t);
+            const float down = limbs_of(x, largest_of(x), l) * Sup, grown = scal[c & 3][6 * CH];
+            const char *const next = w_of(c + 1);
+#pragma unroll
+            for (int q = 0; q < H; q += 2) {
+                f4 y[2];
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int p = 0; p < 3; p++)
 #pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            z[set][j] = mma((p == 2 ? lo : hi)[set][j][u], l[u][p == 1], u || p ? z[set][j] : f4{0, 0, 0, 0});
-                if (r) {
-                    add(r - 2, set ^ 1);
+                        for (int r = 0; r < 2; r++) y[r] = mma(W[q + r][u][p == 2], l[u][p == 1], u || p ? y[r] : f4{0, 0, 0, 0});
+                STAGE();
+                get_w(next, q), get_w(next, q + 1);
 #pragma unroll
-                    for (int i = 0; i < 12; i++) {
-                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-                    }
-                }
+                for (int r = 0; r < 2; r++) S[q + r] = grown * S[q + r] + down * y[r];
+                publish(c + 1, q / 2);
                 STAGE();
             }
-            add(R - 2, (R / 2 - 1) & 1);
-            most = groups_max(most);
-            const float big = most * Sup;
-            if (__any(!(big < 32768.f && (big >= 8.f || most == 0.f)))) scale_state(most);
-            publish();
-            __syncthreads();
+            const float most = largest();
+            if (__any(!(most < 32768.f && (most >= 8.f || most == 0.f)))) scale_state(c + 1, most);
+            sdown[(c + 1) & 3][half][lane] = Sdown;
+            bare_barrier();
         }
         if (in && a.state_out) {
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int r = 0; r < H; r++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) a.state_out[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] = S[r][i];
+                for (int i = 0; i < 4; i++) a.state_out[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] = S[r][i] * Sdown;
         }
-    } else if (brings) {
+        return;
+    }
+
+    const int ct = tid - 128;
+    u4 fa, va[2];
+    auto get_fac = [&](int c) __attribute__((always_inline)) {
+        const float *from = sc + (int64_t)(c < chunks ? c : chunks - 1) * SCAL;
+        fa = *(const u4 *)(from + (ct < SCAL / 4 ? ct : SCAL / 4 - 1) * 4);
+    };
+    auto put_fac = [&](int c) __attribute__((always_inline)) {
+        if (ct < SCAL / 4) *(u4 *)&scal[c & 3][ct * 4] = fa;
+    };
+    // 4 values of 2 rows of v a lane; past the last row that row again (its factor is 0), past the last column the last
+    // four (their state is never stored)
+    const int vr = ct >> 2, vc = (ct & 3) * 4, vx = grp * 16 + vc;
+    const float *const vb = a.v + (int64_t)s * a.T * a.ldv + (int64_t)hv * a.dv + (vx + 4 <= a.dv ? vx : a.dv - 4);
+    auto get_v = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int tok = c * CH + i * 32 + vr;
+            va[i] = *(const u4 *)(vb + (int64_t)(tok < n ? tok : n - 1) * a.ldv);
+        }
+    };
+    auto put_v = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) *(u4 *)(&vbuf[c & 1][(i * 32 + vr) * LV + vc]) = va[i];
+    };
+    // a lane's values of o: rows 4 g + i of a tile, column c0
+    const uint32_t o_at = (uint32_t)(4 * g) * (uint32_t)a.ldo + (uint32_t)c0;
+    float *const ob = a.o + ((int64_t)s * a.T + half * 32) * a.ldo + (int64_t)hv * a.dv;
+    auto outputs = [&](auto which) __attribute__((always_inline)) {
+        constexpr int HALF = decltype(which)::value;
+        h8 PT[2][HALF + 1][2];
+        auto get_pt = [&](int c) __attribute__((always_inline)) {
+            const char *from = w_of(c) + IMG;
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int u = 0; u <= HALF; u++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++) PT[t][u][y] = *(const h8 *)(from + pt_block(2 * HALF + t, u) * 2048 + y * 1024 + l16);
+        };
         if (chunks) {
-            get(0, q_of(0) + IMG, Image{}), get(QB, q_of(0), Image{}), get(TB, t_of(0), Low{});
-            get_fac(0);
-            get_v(0);
-            put_fac(0);
-            put_v();
-            get_fac(1);
-            wait_stores_done();
+            get_fac(0), get_v(0);
+            put_fac(0), put_v(0);
+            get_fac(1), get_v(1);
+#pragma unroll
+            for (int u = 0; u < U; u++) get_rows(q_of(0), u);
+            get_pt(0);
         }
-        __syncthreads();
-        // (LDS is written from registers before the loads to LDS are asked for: the compiler lets no store pass them)
-        for (int c = 0; c < chunks; c++) {
-            if (c) touch_done();
-            put_fac(c + 1);
-            STAGE();
-            get(PB, t_of(c) + TP_BYTES, Low{}), get(c & 1 ? 0 : IMG, q_of(c + 1) + IMG, Image{});
-            STAGE();
-            get_v(c + 1);
-            touch(q_of(c + 1), t_of(c + 1));
-            STAGE();
-            wait_vmem<4 + TI + TL>();
+        bare_barrier();
+        if (chunks) {
+            put_fac(1), put_v(1);
+            get_fac(2), get_v(2);
             bare_barrier();
-            touch_done();
-            put_v();
-            STAGE();
-            get(QB, q_of(c + 1), Image{}), get(TB, t_of(c + 1), Low{});
-            STAGE();
-            get_fac(c + 2);
-            touch(q_of(c + 2) + IMG, t_of(c + 1) + TP_BYTES);
-            STAGE();
-            wait_vmem<NSC + TI + TL>();
             bare_barrier();
         }
-    } else {
-        __syncthreads();
-        for (int c = 0; c < chunks; c++) {
-            const int buf = c & 1;
-            f4 x[4], y[4];
-            {
-                h8 l[U][2];
+        for (int c = 0; c < chunks; c++) {  // (A works on chunk c + 1)
+            put_fac(c + 2), put_v(c + 2);
+            STAGE();
+            get_fac(c + 3), get_v(c + 3);
+            STAGE();
+            f4 z[2][2], x[2], y[4], o[2];
+            const float d0 = sdown[c & 3][0][lane], d1 = sdown[c & 3][1][lane];
+            image_times(c, q_of(c + 1), z);
 #pragma unroll
-                for (int u = 0; u < U; u++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) l[u][i] = *(const h8 *)(sbuf[pair] + (u * 2 + i) * 1024 + lane * 16);
-                const float down = sdown[pair][lane];
-                image_times(0, l, x);
-#pragma unroll
-                for (int t = 0; t < 4; t++) x[t] *= per_row(buf, 2, t) * down;
-            }
-            __syncthreads();
+            for (int t = 0; t < 2; t++) x[t] = per_row(c, ROW_A, 2 * HALF + t) * (z[0][t] * d0 + z[1][t] * d1);
+            if (c + 1 < chunks) bare_barrier();
             h8 l[2][2];
 #pragma unroll
-            for (int t = 0; t < 4; t++) y[t] = *(const f4 *)(xbuf[pair] + t * 1024 + lane * 16);
+            for (int t = 0; t < 4; t++) y[t] = *(const f4 *)(xbuf[c & 1] + t * 1024 + l16) * per_row(c, ROW_P, t);
             float most = largest_of(y);
             const int first = sound(y, most);
-            const float down = limbs_of(y, most, l) * xdown[pair][lane];
+            const float down = limbs_of(y, most, l);
 #pragma unroll
-            for (int t = 0; t < 4; t++) y[t] = f4{0, 0, 0, 0};
-            lower_times(l, y);
+            for (int u = 0; u <= HALF; u++)
+#pragma unroll
+                for (int p = 0; p < 3; p++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) o[t] = mma(PT[t][u][p == 2], l[u][p == 1], u || p ? o[t] : f4{0, 0, 0, 0});
+            STAGE();
+            get_pt(c + 1);
+            STAGE();
+#pragma unroll
+            for (int t = 0; t < 2; t++) x[t] += o[t] * (per_row(c, ROW_D, 2 * HALF + t) * down);
+            if (__any(first < CH)) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[t][i] = (2 * HALF + t) * 16 + 4 * g + i < first ? x[t][i] : __builtin_nanf("");
+            }
             float *to = ob + (int64_t)c * CH * a.ldo;
+            if ((c + 1) * CH <= n && grp * 16 + 16 <= a.dv) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] += y[t] * (per_row(buf, 3, t) * down);
-            spoil(x, first);
-            if ((c + 1) * CH <= n && w0 + 16 <= a.dv) {
-#pragma unroll
-                for (int t = 0; t < 4; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
             } else {
 #pragma unroll
-                for (int t = 0; t < 4; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        if (in && c * CH + t * 16 + 4 * g + i < n) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
+                        if (in && c * CH + (2 * HALF + t) * 16 + 4 * g + i < n) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
             }
-            __syncthreads();
+            if (c + 1 < chunks) bare_barrier();
         }
-    }
+    };
+    if (half) outputs(Count<1>{});
+    else outputs(Count<0>{});
 }
 
 // Chunks from 32 tokens on, where no snapshots are asked for.
@@ -893,25 +865,22 @@ bool chunked(const DeltaArgs &a, bool snapshots) { return !snapshots && a.T >= 3
 void ws_of(const DeltaArgs &a, char *ws, DeltaWs &w, size_t &bytes) {
     w.chunks = (a.T + CH - 1) / CH;
     const size_t img = (size_t)a.n_seq * a.n_k * w.chunks * 2 * img_bytes(a.dk);
-    const size_t tp = (size_t)a.n_seq * a.n_v * w.chunks * 2 * TP_BYTES;
-    w.img = ws, w.tp = ws + img, w.scal = (float *)(ws + img + tp);
-    bytes = img + tp + (size_t)a.n_seq * a.n_v * w.chunks * SCAL * sizeof(float);
+    const size_t wpt = (size_t)a.n_seq * a.n_v * w.chunks * (img_bytes(a.dk) + PT_BYTES);
+    w.img = ws, w.wpt = ws + img, w.scal = (float *)(ws + img + wpt);
+    bytes = img + wpt + (size_t)a.n_seq * a.n_v * w.chunks * SCAL * sizeof(float);
 }
 
 template <int DK> hipError_t launch_chunked(const DeltaArgs &a, void *ws, hipStream_t st) {
     DeltaWs w;
     size_t bytes;
     ws_of(a, (char *)ws, w, bytes);
-    delta_prep_kernel<DK><<<dim3((unsigned)w.chunks, (unsigned)a.n_k, (unsigned)a.n_seq), 256, 0, st>>>(a, w);
+    const int rep = a.n_v / a.n_k;
+    const int each = (int64_t)w.chunks * a.n_k * a.n_seq < 512 ? 1 : rep;
+    delta_prep_kernel<DK><<<dim3((unsigned)w.chunks, (unsigned)(a.n_k * ((rep + each - 1) / each)), (unsigned)a.n_seq), 256, 0, st>>>(a, w, each);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // one group a workgroup where that leaves no CU with two of them to do; else two, which share the operands in LDS
-    const int groups = (a.dv + 15) / 16, heads = a.n_v * a.n_seq;
-    const int64_t per = (heads + 7) / 8;
-    if ((int64_t)groups * heads <= 256)
-        delta_chunk_kernel<DK, 1><<<(unsigned)(8 * per * groups), 192, 0, st>>>(a, w);
-    else
-        delta_chunk_kernel<DK, 2><<<(unsigned)(8 * per * ((groups + 1) / 2)), 384, 0, st>>>(a, w);
+    const int64_t groups = (a.dv + 15) / 16, heads = (int64_t)a.n_v * a.n_seq;
+    delta_chunk_kernel<DK><<<(unsigned)(8 * ((heads + 7) / 8) * groups), 256, 0, st>>>(a, w);
     return hipGetLastError();
 }
 
