@@ -130,13 +130,20 @@ __device__ __forceinline__ float groups_max(float v) {
     const auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-// (the first limbs are made opaque where they stand packed: else each is rounded a second time on its own for the second)
+// (Opaque where they stand: the first limbs packed, else each is rounded a second time on its own for the second; the
+// differences in fp32, since the mixed fma to half a register takes half as long again as one to fp32 and the packed rounding.)
 __device__ __forceinline__ void split8(const float *x, float up, h8 &hi, h8 &lo) {
+    float d[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) hi[i] = (_Float16)(x[i] * up);
     asm("" : "+v"(hi));
 #pragma unroll
-    for (int i = 0; i < 8; i++) lo[i] = (_Float16)__builtin_fmaf(x[i], up, -(float)hi[i]);
+    for (int i = 0; i < 8; i++) {
+        d[i] = __builtin_fmaf(x[i], up, -(float)hi[i]);
+        asm("" : "+v"(d[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) lo[i] = (_Float16)d[i];
 }
 __device__ __forceinline__ f4 mma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4 mma3(h8 ah, h8 al, h8 bh, h8 bl, f4 c) { return mma(al, bh, mma(ah, bl, mma(ah, bh, c))); }
@@ -549,8 +556,10 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
     constexpr int IMG = img_bytes(DK), U = DK / 32, H = DK / 32, HU = U / 2;  // H, HU: a half's tiles of 16 rows, of 32
     constexpr int LV = 20;  // floats between rows of v in LDS (a row's pad keeps rows 4 apart in other banks)
     __shared__ __align__(16) char sbuf[4][U * 2048], xbuf[2][4096];
-    __shared__ __align__(16) float scal[4][SCAL], vbuf[2][CH * LV];
+    __shared__ __align__(16) float scal[4][SCAL], vbuf[4][CH * LV];
+    __shared__ __align__(16) char lbuf[2][4096];
     __shared__ float sdown[4][2][64];
+    __shared__ uint32_t off[2][2];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave & 1;
     const uint32_t l16 = lane * 16;
@@ -698,28 +707,67 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
 #pragma unroll
             for (int r = 0; r < H; r++) get_w(w_of(0), r);
         }
+        // of the half's 32 tokens: b v, f, w
+        f4 v[2], fb[2], fw[2];
+        auto get_tokens = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[t][i] = vbuf[c & 3][((2 * half + t) * 16 + 4 * g + i) * LV + col];
+                v[t] *= per_row(c, ROW_B, 2 * half + t), fb[t] = per_row(c, ROW_F, 2 * half + t), fw[t] = per_row(c, ROW_W, 2 * half + t);
+            }
+        };
+        // R's limbs too are times a power of two, one a column, kept while the column's largest stays in [2^3, 2^15): each wave
+        // makes those of its own tokens without waiting to know it. Where a column left it both waves take all of R again.
+        float Rup = 1.f, Rdown = 1.f;
         bare_barrier();
+        if (chunks) get_tokens(0);
         for (int c = 0; c < chunks; c++) {
-            f4 z[2][2], x[4];
+            f4 z[2][2];
             {
-                f4 v[2], fb[2];
                 const float d0 = sdown[c & 3][0][lane], d1 = sdown[c & 3][1][lane];
+                image_times(c, q_of(c + 1) + IMG, z);
+                float x[8], most = 0.f;
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
+                    const f4 r = v[t] - fb[t] * (z[0][t] * d0 + z[1][t] * d1);
+                    *(f4 *)(xbuf[c & 1] + (2 * half + t) * 1024 + l16) = r;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) v[t][i] = vbuf[c & 1][((2 * half + t) * 16 + 4 * g + i) * LV + col];
-                    v[t] *= per_row(c, ROW_B, 2 * half + t), fb[t] = per_row(c, ROW_F, 2 * half + t);
+                    for (int i = 0; i < 4; i++) x[4 * t + i] = r[i] * fw[t][i], most = max_or_nan(most, fabsf(x[4 * t + i]));
                 }
-                image_times(c, q_of(c + 1) + IMG, z);
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-                    *(f4 *)(xbuf[c & 1] + (2 * half + t) * 1024 + l16) = v[t] - fb[t] * (z[0][t] * d0 + z[1][t] * d1);
+                most *= Rup;
+                h8 hi, lo;
+                split8(x, Rup, hi, lo);
+                char *to = lbuf[c & 1] + half * 2048 + l16;
+                *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
+                const uint64_t over = __ballot(!(most < 32768.f));
+                uint64_t there = __ballot(most >= 8.f);
+                there |= there >> 32;
+                off[c & 1][half] = over ? ~0u : ~(uint32_t)(there | there >> 16) & 0xffff;
             }
             bare_barrier();
             h8 l[2][2];
 #pragma unroll
-            for (int t = 0; t < 4; t++) x[t] = *(const f4 *)(xbuf[c & 1] + t * 1024 + l16) * per_row(c, ROW_W, t);
-            const float down = limbs_of(x, largest_of(x), l) * Sup, grown = scal[c & 3][6 * CH];
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) l[u][y] = *(const h8 *)(lbuf[c & 1] + (u * 2 + y) * 1024 + l16);
+            const uint32_t o0 = off[c & 1][0], o1 = off[c & 1][1];
+            if (__builtin_amdgcn_readfirstlane(((o0 | o1) >> 16) | (o0 & o1))) {
+                f4 x[4];
+#pragma unroll
+                for (int t = 0; t < 4; t++) x[t] = *(const f4 *)(xbuf[c & 1] + t * 1024 + l16) * per_row(c, ROW_W, t);
+                const int e = lift(groups_max(largest_of(x)), 11);
+                Rup = pow2(e), Rdown = pow2(-e);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    float y[8];
+                    *(f4 *)y = x[2 * u], *(f4 *)(y + 4) = x[2 * u + 1];
+                    split8(y, Rup, l[u][0], l[u][1]);
+                }
+            }
+            const float down = Rdown * Sup, grown = scal[c & 3][6 * CH];
+            get_tokens(c + 1);
+            STAGE();
             const char *const next = w_of(c + 1);
 #pragma unroll
             for (int q = 0; q < H; q += 2) {
@@ -773,7 +821,7 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
     };
     auto put_v = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) *(u4 *)(&vbuf[c & 1][(i * 32 + vr) * LV + vc]) = va[i];
+        for (int i = 0; i < 2; i++) *(u4 *)(&vbuf[c & 3][(i * 32 + vr) * LV + vc]) = va[i];
     };
     // a lane's values of o: rows 4 g + i of a tile, column c0
     const uint32_t o_at = (uint32_t)(4 * g) * (uint32_t)a.ldo + (uint32_t)c0;
@@ -791,31 +839,32 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
                     for (int y = 0; y < 2; y++) PT[t][u][y] = *(const h8 *)(from + pt_block(2 * HALF + t, u) * 2048 + y * 1024 + l16);
         };
         if (chunks) {
-            get_fac(0), get_v(0);
-            put_fac(0), put_v(0);
-            get_fac(1), get_v(1);
+            u4 f3[3], v3[3][2];
+#pragma unroll
+            for (int i = 0; i < 3; i++) get_fac(i), get_v(i), f3[i] = fa, v3[i][0] = va[0], v3[i][1] = va[1];
+#pragma unroll
+            for (int i = 0; i < 3; i++) fa = f3[i], va[0] = v3[i][0], va[1] = v3[i][1], put_fac(i), put_v(i);
+            get_fac(3), get_v(3);
 #pragma unroll
             for (int u = 0; u < U; u++) get_rows(q_of(0), u);
             get_pt(0);
         }
         bare_barrier();
         if (chunks) {
-            put_fac(1), put_v(1);
-            get_fac(2), get_v(2);
             bare_barrier();
             bare_barrier();
         }
         for (int c = 0; c < chunks; c++) {  // (A works on chunk c + 1)
-            put_fac(c + 2), put_v(c + 2);
-            STAGE();
-            get_fac(c + 3), get_v(c + 3);
-            STAGE();
             f4 z[2][2], x[2], y[4], o[2];
             const float d0 = sdown[c & 3][0][lane], d1 = sdown[c & 3][1][lane];
             image_times(c, q_of(c + 1), z);
 #pragma unroll
             for (int t = 0; t < 2; t++) x[t] = per_row(c, ROW_A, 2 * HALF + t) * (z[0][t] * d0 + z[1][t] * d1);
             if (c + 1 < chunks) bare_barrier();
+            put_fac(c + 3), put_v(c + 3);  // (4 chunks' places: c to c + 3)
+            STAGE();
+            get_fac(c + 4), get_v(c + 4);
+            STAGE();
             h8 l[2][2];
 #pragma unroll
             for (int t = 0; t < 4; t++) y[t] = *(const f4 *)(xbuf[c & 1] + t * 1024 + l16) * per_row(c, ROW_P, t);
