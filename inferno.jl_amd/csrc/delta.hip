@@ -533,9 +533,6 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_prep_kernel(De
     }
 }
 
-template <int N> struct Count {
-    static constexpr int value = N;
-};
 // __syncthreads without its wait for every load under way: only this wave's LDS accesses have completed
 __device__ __forceinline__ void bare_barrier() {
     asm volatile("" ::: "memory");
@@ -547,21 +544,22 @@ __device__ __forceinline__ void bare_barrier() {
 // nothing is moved across: loads stay ahead of the products that do not need them
 #define STAGE() __builtin_amdgcn_sched_barrier(0)
 
-// Four waves carry 16 columns of a head's state through its chunks. Waves A0 and A1 have the state, half of its rows each: R
-// from K S for 32 of the tokens each, then the new state's rows from W R. Waves B0 and B1, a chunk behind, form the outputs of 32
-// tokens each from Q S and (P T) R, and bring v and the factors to LDS. Each has its operands of the next chunk on their way in
-// registers while it works on this one's. The state's limbs (each half's with a power of two of its own) and R go through LDS;
-// two barriers a chunk.
-template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
-    constexpr int IMG = img_bytes(DK), U = DK / 32, H = DK / 32, HU = U / 2;  // H, HU: a half's tiles of 16 rows, of 32
+// DK / 32 pairs of waves carry 16 columns of a head's state through its chunks. Waves A have the state, 32 of its rows each: R
+// from K S for TT of the four tiles of 16 tokens each, then the new state's rows from W R. Waves B, a chunk behind, form the
+// outputs of as many tokens each from Q S and (P T) R, and bring v and the factors to LDS. Each has its operands of the next
+// chunk on their way in registers while it works on this one's. The state's limbs (a power of two of its own for each wave's
+// part) and R go through LDS; two barriers a chunk. (One wave issues a vector instruction in 8 clocks, two on a SIMD one in 4
+// to 5: the work between the products, more than the products, is why a head is cut this fine.)
+template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
+    constexpr int IMG = img_bytes(DK), U = DK / 32, TT = 4 / U;
     constexpr int LV = 20;  // floats between rows of v in LDS (a row's pad keeps rows 4 apart in other banks)
     __shared__ __align__(16) char sbuf[4][U * 2048], xbuf[2][4096];
     __shared__ __align__(16) float scal[4][SCAL], vbuf[4][CH * LV];
     __shared__ __align__(16) char lbuf[2][4096];
-    __shared__ float sdown[4][2][64];
-    __shared__ uint32_t off[2][2];
+    __shared__ float sdown[4][U][64];
+    __shared__ uint32_t off[2][U];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave & 1;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % U;
     const uint32_t l16 = lane * 16;
     // consecutive workgroups go to the eight XCDs in turn: a head's column groups, and the heads of a key head, are given
     // to one XCD, whose L2 then fetches the operands once for all of them
@@ -626,55 +624,61 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
         }
         return first;
     };
-    // 32 rows of an image (K or Q), and x[y] = the image times the limbs of the state's half y; the next chunk's values take
-    // the place of what is done with
-    h8 M[U][2][2];
-    auto get_rows = [&](const char *from, int u) __attribute__((always_inline)) {
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int y = 0; y < 2; y++) M[u][t][y] = *(const h8 *)(from + half * (U * 4096) + ((t * U + u) * 2 + y) * 1024 + l16);
-    };
-    auto image_times = [&](int c, const char *next, f4 (&x)[2][2]) __attribute__((always_inline)) {
-        h8 l[U][2];
+    // the wave's rows of an image (K or Q), and the image times the state: each part's limbs have a power of two of their own
+    h8 M[U][TT][2];
+    auto get_rows = [&](const char *from) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
+            for (int t = 0; t < TT; t++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) M[u][t][y] = *(const h8 *)(from + part * (TT * U * 2048) + ((t * U + u) * 2 + y) * 1024 + l16);
+    };
+    auto image_times = [&](int c, const char *next, f4 (&x)[TT]) __attribute__((always_inline)) {
+        h8 l[U][2];
+        f4 z[U][TT];
+        float down[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
             for (int i = 0; i < 2; i++) l[u][i] = *(const h8 *)(sbuf[c & 3] + (u * 2 + i) * 1024 + l16);
+            down[u] = sdown[c & 3][u][lane];
+        }
 #pragma unroll
-        for (int u = 0; u < HU; u++) {
+        for (int p = 0; p < 3; p++)
 #pragma unroll
-            for (int p = 0; p < 3; p++)
+            for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int y = 0; y < 2; y++)
+                for (int t = 0; t < TT; t++) z[u][t] = mma(M[u][t][p == 2], l[u][p == 1], p ? z[u][t] : f4{0, 0, 0, 0});
+        STAGE();
+        get_rows(next);
+        STAGE();
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
-                        x[y][t] = mma(M[y * HU + u][t][p == 2], l[y * HU + u][p == 1], u || p ? x[y][t] : f4{0, 0, 0, 0});
-            STAGE();
-            get_rows(next, u), get_rows(next, HU + u);
-            STAGE();
+        for (int t = 0; t < TT; t++) {
+            x[t] = z[0][t] * down[0];
+#pragma unroll
+            for (int u = 1; u < U; u++) x[t] += z[u][t] * down[u];
         }
     };
     // (a loop each, with the same two barriers a turn: no role keeps another's registers)
-    if (wave < 2) {
-        // The half is held times a power of two, one a column, kept from chunk to chunk while the column's largest value stays
+    if (wave < U) {
+        // The part is held times a power of two, one a column, kept from chunk to chunk while the column's largest value stays
         // in [2^3, 2^15) (below 2^15 its limbs do not overflow, and 22 bits remain down to 2^-2).
-        f4 S[H];
+        f4 S[2];
         float Sup = 1.f, Sdown = 1.f;
-        const int64_t head = (((int64_t)s * a.n_v + hv) * DK + half * (DK / 2)) * a.dv + c0;
-        auto publish = [&](int c, int u) __attribute__((always_inline)) {
+        const int64_t head = (((int64_t)s * a.n_v + hv) * DK + part * 32) * a.dv + c0;
+        auto publish = [&](int c) __attribute__((always_inline)) {
             float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = S[2 * u + (i >> 2)][i & 3];
             h8 hi, lo;
+            *(f4 *)x = S[0], *(f4 *)(x + 4) = S[1];
             split8(x, 1.f, hi, lo);
-            char *to = sbuf[c & 3] + (half * HU + u) * 2048 + l16;
+            char *to = sbuf[c & 3] + part * 2048 + l16;
             *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
         };
         auto largest = [&]() __attribute__((always_inline)) {
             float most = 0.f;
 #pragma unroll
-            for (int r = 0; r < H; r++)
+            for (int r = 0; r < 2; r++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r][i]));
             return groups_max(most);
@@ -683,67 +687,71 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
             const int have = (int)(__float_as_uint(Sup) >> 23) - 127, want = have + lift(most, 11);  // (from -80 to 80 in all)
             const int e = (want < -80 ? -80 : want > 80 ? 80 : want) - have;
             Sup *= pow2(e), Sdown *= pow2(-e);
-#pragma unroll
-            for (int r = 0; r < H; r++) S[r] *= pow2(e);
-#pragma unroll
-            for (int u = 0; u < HU; u++) publish(c, u);
+            S[0] *= pow2(e), S[1] *= pow2(e);
+            publish(c);
         };
 #pragma unroll
-        for (int r = 0; r < H; r++)
+        for (int r = 0; r < 2; r++)
 #pragma unroll
             for (int i = 0; i < 4; i++) S[r][i] = in && a.state_in ? a.state_in[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] : 0.f;
         scale_state(0, largest());
-        sdown[0][half][lane] = Sdown;
-        h8 W[H][2][2];
-        auto get_w = [&](const char *from, int r) __attribute__((always_inline)) {
+        sdown[0][part][lane] = Sdown;
+        h8 W[2][2][2];
+        auto get_w = [&](const char *from) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+            for (int r = 0; r < 2; r++)
 #pragma unroll
-                for (int y = 0; y < 2; y++) W[r][u][y] = *(const h8 *)(from + half * (IMG / 2) + ((r * 2 + u) * 2 + y) * 1024 + l16);
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++) W[r][u][y] = *(const h8 *)(from + part * 8192 + ((r * 2 + u) * 2 + y) * 1024 + l16);
         };
-        if (chunks) {
-#pragma unroll
-            for (int u = 0; u < U; u++) get_rows(q_of(0) + IMG, u);
-#pragma unroll
-            for (int r = 0; r < H; r++) get_w(w_of(0), r);
-        }
-        // of the half's 32 tokens: b v, f, w
-        f4 v[2], fb[2], fw[2];
+        if (chunks) get_rows(q_of(0) + IMG), get_w(w_of(0));
+        // of the wave's tokens: b v, f, w
+        f4 v[TT], fb[TT], fw[TT];
         auto get_tokens = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+            for (int t = 0; t < TT; t++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[t][i] = vbuf[c & 3][((2 * half + t) * 16 + 4 * g + i) * LV + col];
-                v[t] *= per_row(c, ROW_B, 2 * half + t), fb[t] = per_row(c, ROW_F, 2 * half + t), fw[t] = per_row(c, ROW_W, 2 * half + t);
+                for (int i = 0; i < 4; i++) v[t][i] = vbuf[c & 3][((TT * part + t) * 16 + 4 * g + i) * LV + col];
+                v[t] *= per_row(c, ROW_B, TT * part + t), fb[t] = per_row(c, ROW_F, TT * part + t), fw[t] = per_row(c, ROW_W, TT * part + t);
             }
         };
         // R's limbs too are times a power of two, one a column, kept while the column's largest stays in [2^3, 2^15): each wave
-        // makes those of its own tokens without waiting to know it. Where a column left it both waves take all of R again.
+        // makes those of its own tokens without waiting to know it. Where a column left it all waves take all of R again.
         float Rup = 1.f, Rdown = 1.f;
         bare_barrier();
         if (chunks) get_tokens(0);
         for (int c = 0; c < chunks; c++) {
-            f4 z[2][2];
             {
-                const float d0 = sdown[c & 3][0][lane], d1 = sdown[c & 3][1][lane];
-                image_times(c, q_of(c + 1) + IMG, z);
-                float x[8], most = 0.f;
+                f4 x[TT];
+                image_times(c, q_of(c + 1) + IMG, x);
+                float most = 0.f;
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const f4 r = v[t] - fb[t] * (z[0][t] * d0 + z[1][t] * d1);
-                    *(f4 *)(xbuf[c & 1] + (2 * half + t) * 1024 + l16) = r;
+                for (int t = 0; t < TT; t++) {
+                    x[t] = v[t] - fb[t] * x[t];
+                    *(f4 *)(xbuf[c & 1] + (TT * part + t) * 1024 + l16) = x[t];
+                    x[t] *= fw[t];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[4 * t + i] = r[i] * fw[t][i], most = max_or_nan(most, fabsf(x[4 * t + i]));
+                    for (int i = 0; i < 4; i++) most = max_or_nan(most, fabsf(x[t][i]));
                 }
                 most *= Rup;
-                h8 hi, lo;
-                split8(x, Rup, hi, lo);
-                char *to = lbuf[c & 1] + half * 2048 + l16;
-                *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
+                if constexpr (TT == 2) {
+                    float y[8];
+                    h8 hi, lo;
+                    *(f4 *)y = x[0], *(f4 *)(y + 4) = x[1];
+                    split8(y, Rup, hi, lo);
+                    char *to = lbuf[c & 1] + part * 2048 + l16;
+                    *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
+                } else {
+                    h4 hi, lo;
+                    split4(x[0], Rup, hi, lo);
+                    char *to = lbuf[c & 1] + (part >> 1) * 2048 + l16 + (part & 1) * 8;
+                    *(h4 *)to = hi, *(h4 *)(to + 1024) = lo;
+                }
                 const uint64_t over = __ballot(!(most < 32768.f));
                 uint64_t there = __ballot(most >= 8.f);
                 there |= there >> 32;
-                off[c & 1][half] = over ? ~0u : ~(uint32_t)(there | there >> 16) & 0xffff;
+                off[c & 1][part] = over ? ~0u : ~(uint32_t)(there | there >> 16) & 0xffff;
             }
             bare_barrier();
             h8 l[2][2];
@@ -751,8 +759,10 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int y = 0; y < 2; y++) l[u][y] = *(const h8 *)(lbuf[c & 1] + (u * 2 + y) * 1024 + l16);
-            const uint32_t o0 = off[c & 1][0], o1 = off[c & 1][1];
-            if (__builtin_amdgcn_readfirstlane(((o0 | o1) >> 16) | (o0 & o1))) {
+            uint32_t any = off[c & 1][0], all = any;
+#pragma unroll
+            for (int u = 1; u < U; u++) any |= off[c & 1][u], all &= off[c & 1][u];
+            if (__builtin_amdgcn_readfirstlane(any >> 16 | all)) {
                 f4 x[4];
 #pragma unroll
                 for (int t = 0; t < 4; t++) x[t] = *(const f4 *)(xbuf[c & 1] + t * 1024 + l16) * per_row(c, ROW_W, t);
@@ -766,41 +776,37 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
                 }
             }
             const float down = Rdown * Sup, grown = scal[c & 3][6 * CH];
-            get_tokens(c + 1);
+            f4 y[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int p = 0; p < 3; p++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) y[r] = mma(W[r][u][p == 2], l[u][p == 1], u || p ? y[r] : f4{0, 0, 0, 0});
             STAGE();
-            const char *const next = w_of(c + 1);
+            get_w(w_of(c + 1));
+            STAGE();
 #pragma unroll
-            for (int q = 0; q < H; q += 2) {
-                f4 y[2];
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int p = 0; p < 3; p++)
-#pragma unroll
-                        for (int r = 0; r < 2; r++) y[r] = mma(W[q + r][u][p == 2], l[u][p == 1], u || p ? y[r] : f4{0, 0, 0, 0});
-                STAGE();
-                get_w(next, q), get_w(next, q + 1);
-#pragma unroll
-                for (int r = 0; r < 2; r++) S[q + r] = grown * S[q + r] + down * y[r];
-                publish(c + 1, q / 2);
-                STAGE();
-            }
+            for (int r = 0; r < 2; r++) S[r] = grown * S[r] + down * y[r];
+            publish(c + 1);
             const float most = largest();
             if (__any(!(most < 32768.f && (most >= 8.f || most == 0.f)))) scale_state(c + 1, most);
-            sdown[(c + 1) & 3][half][lane] = Sdown;
+            sdown[(c + 1) & 3][part][lane] = Sdown;
+            get_tokens(c + 1);
             bare_barrier();
         }
         if (in && a.state_out) {
 #pragma unroll
-            for (int r = 0; r < H; r++)
+            for (int r = 0; r < 2; r++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) a.state_out[head + (int64_t)(r * 16 + 4 * g + i) * a.dv] = S[r][i] * Sdown;
         }
         return;
     }
 
-    const int ct = tid - 128;
-    u4 fa, va[2];
+    constexpr int NB = U * 64, VR = NB / 4;  // threads of B; rows of v they bring at once
+    const int ct = tid - NB;
+    u4 fa, va[CH / VR];
     auto get_fac = [&](int c) __attribute__((always_inline)) {
         const float *from = sc + (int64_t)(c < chunks ? c : chunks - 1) * SCAL;
         fa = *(const u4 *)(from + (ct < SCAL / 4 ? ct : SCAL / 4 - 1) * 4);
@@ -808,104 +814,112 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(D
     auto put_fac = [&](int c) __attribute__((always_inline)) {
         if (ct < SCAL / 4) *(u4 *)&scal[c & 3][ct * 4] = fa;
     };
-    // 4 values of 2 rows of v a lane; past the last row that row again (its factor is 0), past the last column the last
+    // 4 values of 1 or 2 rows of v a thread; past the last row that row again (its factor is 0), past the last column the last
     // four (their state is never stored)
     const int vr = ct >> 2, vc = (ct & 3) * 4, vx = grp * 16 + vc;
     const float *const vb = a.v + (int64_t)s * a.T * a.ldv + (int64_t)hv * a.dv + (vx + 4 <= a.dv ? vx : a.dv - 4);
     auto get_v = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int tok = c * CH + i * 32 + vr;
+        for (int i = 0; i < CH / VR; i++) {
+            const int tok = c * CH + i * VR + vr;
             va[i] = *(const u4 *)(vb + (int64_t)(tok < n ? tok : n - 1) * a.ldv);
         }
     };
     auto put_v = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) *(u4 *)(&vbuf[c & 3][(i * 32 + vr) * LV + vc]) = va[i];
+        for (int i = 0; i < CH / VR; i++) *(u4 *)(&vbuf[c & 3][(i * VR + vr) * LV + vc]) = va[i];
     };
     // a lane's values of o: rows 4 g + i of a tile, column c0
     const uint32_t o_at = (uint32_t)(4 * g) * (uint32_t)a.ldo + (uint32_t)c0;
-    float *const ob = a.o + ((int64_t)s * a.T + half * 32) * a.ldo + (int64_t)hv * a.dv;
-    auto outputs = [&](auto which) __attribute__((always_inline)) {
-        constexpr int HALF = decltype(which)::value;
-        h8 PT[2][HALF + 1][2];
-        auto get_pt = [&](int c) __attribute__((always_inline)) {
-            const char *from = w_of(c) + IMG;
+    float *const ob = a.o + ((int64_t)s * a.T + part * TT * 16) * a.ldo + (int64_t)hv * a.dv;
+    // P T's blocks of the wave's row tiles: of 32 .. 63's columns too where the rows are (the same again, unused, elsewhere)
+    const bool low = (part + 1) * TT > 2;
+    h8 PT[TT][2][2];
+    auto get_pt = [&](int c) __attribute__((always_inline)) {
+        const char *from = w_of(c) + IMG;
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+        for (int t = 0; t < TT; t++)
 #pragma unroll
-                for (int u = 0; u <= HALF; u++)
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int y = 0; y < 2; y++) PT[t][u][y] = *(const h8 *)(from + pt_block(2 * HALF + t, u) * 2048 + y * 1024 + l16);
-        };
-        if (chunks) {
-            u4 f3[3], v3[3][2];
-#pragma unroll
-            for (int i = 0; i < 3; i++) get_fac(i), get_v(i), f3[i] = fa, v3[i][0] = va[0], v3[i][1] = va[1];
-#pragma unroll
-            for (int i = 0; i < 3; i++) fa = f3[i], va[0] = v3[i][0], va[1] = v3[i][1], put_fac(i), put_v(i);
-            get_fac(3), get_v(3);
-#pragma unroll
-            for (int u = 0; u < U; u++) get_rows(q_of(0), u);
-            get_pt(0);
-        }
-        bare_barrier();
-        if (chunks) {
-            bare_barrier();
-            bare_barrier();
-        }
-        for (int c = 0; c < chunks; c++) {  // (A works on chunk c + 1)
-            f4 z[2][2], x[2], y[4], o[2];
-            const float d0 = sdown[c & 3][0][lane], d1 = sdown[c & 3][1][lane];
-            image_times(c, q_of(c + 1), z);
-#pragma unroll
-            for (int t = 0; t < 2; t++) x[t] = per_row(c, ROW_A, 2 * HALF + t) * (z[0][t] * d0 + z[1][t] * d1);
-            if (c + 1 < chunks) bare_barrier();
-            put_fac(c + 3), put_v(c + 3);  // (4 chunks' places: c to c + 3)
-            STAGE();
-            get_fac(c + 4), get_v(c + 4);
-            STAGE();
-            h8 l[2][2];
-#pragma unroll
-            for (int t = 0; t < 4; t++) y[t] = *(const f4 *)(xbuf[c & 1] + t * 1024 + l16) * per_row(c, ROW_P, t);
-            float most = largest_of(y);
-            const int first = sound(y, most);
-            const float down = limbs_of(y, most, l);
-#pragma unroll
-            for (int u = 0; u <= HALF; u++)
-#pragma unroll
-                for (int p = 0; p < 3; p++)
-#pragma unroll
-                    for (int t = 0; t < 2; t++) o[t] = mma(PT[t][u][p == 2], l[u][p == 1], u || p ? o[t] : f4{0, 0, 0, 0});
-            STAGE();
-            get_pt(c + 1);
-            STAGE();
-#pragma unroll
-            for (int t = 0; t < 2; t++) x[t] += o[t] * (per_row(c, ROW_D, 2 * HALF + t) * down);
-            if (__any(first < CH)) {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[t][i] = (2 * HALF + t) * 16 + 4 * g + i < first ? x[t][i] : __builtin_nanf("");
-            }
-            float *to = ob + (int64_t)c * CH * a.ldo;
-            if ((c + 1) * CH <= n && grp * 16 + 16 <= a.dv) {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
-            } else {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (in && c * CH + (2 * HALF + t) * 16 + 4 * g + i < n) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
-            }
-            if (c + 1 < chunks) bare_barrier();
-        }
+                for (int y = 0; y < 2; y++) PT[t][u][y] = *(const h8 *)(from + pt_block(TT * part + t, low ? u : 0) * 2048 + y * 1024 + l16);
     };
-    if (half) outputs(Count<1>{});
-    else outputs(Count<0>{});
+    if (chunks) {
+        u4 f3[3], v3[3][CH / VR];
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            get_fac(i), get_v(i);
+            f3[i] = fa;
+#pragma unroll
+            for (int j = 0; j < CH / VR; j++) v3[i][j] = va[j];
+        }
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            fa = f3[i];
+#pragma unroll
+            for (int j = 0; j < CH / VR; j++) va[j] = v3[i][j];
+            put_fac(i), put_v(i);
+        }
+        get_fac(3), get_v(3);
+        get_rows(q_of(0)), get_pt(0);
+    }
+    bare_barrier();
+    if (chunks) {
+        bare_barrier();
+        bare_barrier();
+    }
+    for (int c = 0; c < chunks; c++) {  // (A works on chunk c + 1)
+        f4 x[TT], y[4], o[TT];
+        image_times(c, q_of(c + 1), x);
+#pragma unroll
+        for (int t = 0; t < TT; t++) x[t] *= per_row(c, ROW_A, TT * part + t);
+        if (c + 1 < chunks) bare_barrier();
+        put_fac(c + 3), put_v(c + 3);  // (4 chunks' places: c to c + 3)
+        STAGE();
+        get_fac(c + 4), get_v(c + 4);
+        STAGE();
+        h8 l[2][2];
+#pragma unroll
+        for (int t = 0; t < 4; t++) y[t] = *(const f4 *)(xbuf[c & 1] + t * 1024 + l16) * per_row(c, ROW_P, t);
+        float most = largest_of(y);
+        const int first = sound(y, most);
+        const float down = limbs_of(y, most, l);
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+#pragma unroll
+            for (int t = 0; t < TT; t++) o[t] = mma(PT[t][0][p == 2], l[0][p == 1], p ? o[t] : f4{0, 0, 0, 0});
+        if (low) {
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+#pragma unroll
+                for (int t = 0; t < TT; t++) o[t] = mma(PT[t][1][p == 2], l[1][p == 1], o[t]);
+        }
+        STAGE();
+        get_pt(c + 1);
+        STAGE();
+#pragma unroll
+        for (int t = 0; t < TT; t++) x[t] += o[t] * (per_row(c, ROW_D, TT * part + t) * down);
+        if (__any(first < CH)) {
+#pragma unroll
+            for (int t = 0; t < TT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[t][i] = (TT * part + t) * 16 + 4 * g + i < first ? x[t][i] : __builtin_nanf("");
+        }
+        float *to = ob + (int64_t)c * CH * a.ldo;
+        if ((c + 1) * CH <= n && grp * 16 + 16 <= a.dv) {
+#pragma unroll
+            for (int t = 0; t < TT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
+        } else {
+#pragma unroll
+            for (int t = 0; t < TT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (in && c * CH + (TT * part + t) * 16 + 4 * g + i < n) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
+        }
+        if (c + 1 < chunks) bare_barrier();
+    }
 }
 
 // Chunks from 32 tokens on, where no snapshots are asked for.
@@ -929,7 +943,7 @@ template <int DK> hipError_t launch_chunked(const DeltaArgs &a, void *ws, hipStr
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t groups = (a.dv + 15) / 16, heads = (int64_t)a.n_v * a.n_seq;
-    delta_chunk_kernel<DK><<<(unsigned)(8 * ((heads + 7) / 8) * groups), 256, 0, st>>>(a, w);
+    delta_chunk_kernel<DK><<<(unsigned)(8 * ((heads + 7) / 8) * groups), DK * 4, 0, st>>>(a, w);
     return hipGetLastError();
 }
 
