@@ -554,7 +554,7 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
     constexpr int IMG = img_bytes(DK), U = DK / 32, TT = 4 / U;
     constexpr int LV = 20;  // floats between rows of v in LDS (a row's pad keeps rows 4 apart in other banks)
     __shared__ __align__(16) char sbuf[4][U * 2048], xbuf[2][4096];
-    __shared__ __align__(16) float scal[4][SCAL], vbuf[4][CH * LV];
+    __shared__ __align__(16) float scal[4][SCAL], vbuf[4][CH * LV], obuf[U][16 * LV];
     __shared__ __align__(16) char lbuf[2][4096];
     __shared__ float sdown[4][U][64];
     __shared__ uint32_t off[2][U];
@@ -829,9 +829,7 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
 #pragma unroll
         for (int i = 0; i < CH / VR; i++) *(u4 *)(&vbuf[c & 3][(i * VR + vr) * LV + vc]) = va[i];
     };
-    // a lane's values of o: rows 4 g + i of a tile, column c0
-    const uint32_t o_at = (uint32_t)(4 * g) * (uint32_t)a.ldo + (uint32_t)c0;
-    float *const ob = a.o + ((int64_t)s * a.T + part * TT * 16) * a.ldo + (int64_t)hv * a.dv;
+    float *const ob = a.o + (int64_t)s * a.T * a.ldo + (int64_t)hv * a.dv + vx;
     // P T's blocks of the wave's row tiles: of 32 .. 63's columns too where the rows are (the same again, unused, elsewhere)
     const bool low = (part + 1) * TT > 2;
     h8 PT[TT][2][2];
@@ -905,18 +903,14 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[t][i] = (TT * part + t) * 16 + 4 * g + i < first ? x[t][i] : __builtin_nanf("");
         }
-        float *to = ob + (int64_t)c * CH * a.ldo;
-        if ((c + 1) * CH <= n && grp * 16 + 16 <= a.dv) {
+        // by way of LDS to 4 values of a row a lane: one store a tile, not four
 #pragma unroll
-            for (int t = 0; t < TT; t++)
+        for (int t = 0; t < TT; t++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
-        } else {
-#pragma unroll
-            for (int t = 0; t < TT; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (in && c * CH + (TT * part + t) * 16 + 4 * g + i < n) (to + (int64_t)(t * 16 + i) * a.ldo)[o_at] = x[t][i];
+            for (int i = 0; i < 4; i++) obuf[part][(4 * g + i) * LV + col] = x[t][i];
+            const int tok = c * CH + (TT * part + t) * 16 + (lane >> 2);
+            const f4 y = *(const f4 *)&obuf[part][(lane >> 2) * LV + (lane & 3) * 4];
+            if (tok < n && vx < a.dv) *(f4 *)(ob + (int64_t)tok * a.ldo) = y;
         }
         if (c + 1 < chunks) bare_barrier();
     }
