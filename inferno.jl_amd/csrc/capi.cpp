@@ -1055,6 +1055,8 @@ int check_delta_shape(const char *name, int n_seq, int T, int n_k, int n_v, int 
     if (n_k < 1 || n_v < 1 || n_v % n_k || n_v > 4096) return fail(IHIP_EINVAL, "%s: n_k=%d n_v=%d", name, n_k, n_v);
     if ((dk != 64 && dk != 128) || dv < 4 || (dv & 3) || dv > 512)
         return fail(IHIP_EINVAL, "%s: dk=%d (64 or 128) dv=%d (a multiple of 4 up to 512)", name, dk, dv);
+    if ((int64_t)n_seq * n_v * ((dv + 15) / 16) > (1 << 22))  // (a launch holds 2^32 threads, 512 of them 16 columns)
+        return fail(IHIP_EINVAL, "%s: %d sequences of %d heads of %d columns", name, n_seq, n_v, dv);
     return IHIP_OK;
 }
 

@@ -548,15 +548,15 @@ __device__ __forceinline__ void bare_barrier() {
 // from K S for TT of the four tiles of 16 tokens each, then the new state's rows from W R. Waves B, a chunk behind, form the
 // outputs of as many tokens each from Q S and (P T) R, and bring v and the factors to LDS. Each has its operands of the next
 // chunk on their way in registers while it works on this one's. The state's limbs (a power of two of its own for each wave's
-// part) and R go through LDS; two barriers a chunk. (One wave issues a vector instruction in 8 clocks, two on a SIMD one in 4
+// part) and R go through LDS; two barriers a chunk, the first behind B's last look at the limbs whose place the next take. (One wave issues a vector instruction in 8 clocks, two on a SIMD one in 4
 // to 5: the work between the products, more than the products, is why a head is cut this fine.)
 template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kernel(DeltaArgs a, DeltaWs w) {
     constexpr int IMG = img_bytes(DK), U = DK / 32, TT = 4 / U;
     constexpr int LV = 20;  // floats between rows of v in LDS (a row's pad keeps rows 4 apart in other banks)
-    __shared__ __align__(16) char sbuf[4][U * 2048], xbuf[2][4096];
+    __shared__ __align__(16) char sbuf[2][U * 2048], xbuf[2][4096];
     __shared__ __align__(16) float scal[4][SCAL], vbuf[4][CH * LV], obuf[U][16 * LV];
     __shared__ __align__(16) char lbuf[2][4096];
-    __shared__ float sdown[4][U][64];
+    __shared__ float sdown[2][U][64];
     __shared__ uint32_t off[2][U];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % U;
@@ -641,8 +641,8 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
 #pragma unroll
         for (int u = 0; u < U; u++) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) l[u][i] = *(const h8 *)(sbuf[c & 3] + (u * 2 + i) * 1024 + l16);
-            down[u] = sdown[c & 3][u][lane];
+            for (int i = 0; i < 2; i++) l[u][i] = *(const h8 *)(sbuf[c & 1] + (u * 2 + i) * 1024 + l16);
+            down[u] = sdown[c & 1][u][lane];
         }
 #pragma unroll
         for (int p = 0; p < 3; p++)
@@ -672,7 +672,7 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
             h8 hi, lo;
             *(f4 *)x = S[0], *(f4 *)(x + 4) = S[1];
             split8(x, 1.f, hi, lo);
-            char *to = sbuf[c & 3] + part * 2048 + l16;
+            char *to = sbuf[c & 1] + part * 2048 + l16;
             *(h8 *)to = hi, *(h8 *)(to + 1024) = lo;
         };
         auto largest = [&]() __attribute__((always_inline)) {
@@ -791,7 +791,7 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
             publish(c + 1);
             const float most = largest();
             if (__any(!(most < 32768.f && (most >= 8.f || most == 0.f)))) scale_state(c + 1, most);
-            sdown[(c + 1) & 3][part][lane] = Sdown;
+            sdown[(c + 1) & 1][part][lane] = Sdown;
             get_tokens(c + 1);
             bare_barrier();
         }
@@ -916,8 +916,15 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
     }
 }
 
-// Chunks from 32 tokens on, where no snapshots are asked for.
-bool chunked(const DeltaArgs &a, bool snapshots) { return !snapshots && a.T >= 32; }
+// Chunks where no snapshots are asked for and there are tokens enough: a chunk costs as much with one token as with 64, the
+// recurrence as many times more as there are tokens. Where the two meet, by the number of 16-column groups there are to carry,
+// in microseconds (recurrence, chunks) at dk = dv = 128, 32 heads: 1 sequence (256 groups) 16 tokens 22.9, 19.3; 4 (1024)
+// 20 tokens 31.6, 34.9 and 24 tokens 37.0, 35; 16 (4096) 40 tokens 78, 87 and 64 tokens 118, 89. dk = dv = 64, 16 heads: 1
+// sequence (64) 16 tokens 17.4, 15.6; 16 (1024) 20 tokens 23.7, 27.2 and 28 tokens 31.5, 27.2.
+bool chunked(const DeltaArgs &a, bool snapshots) {
+    const int64_t groups = (int64_t)a.n_seq * a.n_v * ((a.dv + 15) / 16);
+    return !snapshots && a.T >= 14 + (groups < 4096 ? groups / 128 : 32);
+}
 
 void ws_of(const DeltaArgs &a, char *ws, DeltaWs &w, size_t &bytes) {
     w.chunks = (a.T + CH - 1) / CH;
@@ -931,6 +938,10 @@ template <int DK> hipError_t launch_chunked(const DeltaArgs &a, void *ws, hipStr
     DeltaWs w;
     size_t bytes;
     ws_of(a, (char *)ws, w, bytes);
+    // A workgroup a value head where that still leaves no CU more than the two that fit at once to do, else one for all value
+    // heads of a key head, which then prepares q and k once: in all, 37.2 us against 43.2 at 512 tokens of 16 key and 32 value
+    // heads (128 chunks), 84.6 against 93.2 at 2048 (512 chunks, both ways alike); 139 against 128 for 16 sequences of 128
+    // tokens (512 chunks, twice as many workgroups as fit).
     const int rep = a.n_v / a.n_k;
     const int each = (int64_t)w.chunks * a.n_k * a.n_seq < 512 ? 1 : rep;
     delta_prep_kernel<DK><<<dim3((unsigned)w.chunks, (unsigned)(a.n_k * ((rep + each - 1) / each)), (unsigned)a.n_seq), 256, 0, st>>>(a, w, each);

@@ -266,3 +266,69 @@ def test_a_bad_token_spoils_no_earlier_one(ih, t, at, what, value):
     assert not bool(torch.isfinite(out[bad]).any()) and not bool(torch.isfinite(new[gone]).any())
     check(torch.where(bad, 0.0, out), torch.where(bad, 0.0, o.cpu().double()), "o")
     check(torch.where(gone, 0.0, new), torch.where(gone, 0.0, last.cpu().double()), "state")
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 32), (128, 128)])
+@pytest.mark.parametrize("t", [13, 14, 15, 16, 17, 31, 32, 33, 47])
+def test_few_tokens(ih, t, dk, dv):
+    """Around the lengths where the recurrence gives way to a chunk, which is then mostly empty."""
+    import torch
+    q, k, v, g, b, st = make(2, t, 2, 4, dk, dv, seed=23)
+    o, _, last = R.delta(q, k, v, g, b, st, l2norm=True)
+    new = torch.empty_like(st)
+    check(ih.gated_delta_rule(q, k, v, g, b, st, new_state=new, l2norm=True), o, "o")
+    check(new, last, "state")
+
+
+@pytest.mark.parametrize("shape", [(64, 65, 4, 12, 64, 8), (64, 65, 4, 8, 128, 16), (1, 4200, 8, 16, 64, 16), (64, 50, 8, 8, 128, 128)])
+def test_many_chunks(ih, shape):
+    """So many chunks that a key head's value heads (two, three, one) are prepared one after the other, and more columns than
+    the GPU carries at once."""
+    import torch
+    q, k, v, g, b, st = make(*shape, seed=29)
+    o, _, last = R.delta(q, k, v, g, b, st, l2norm=True)
+    new = torch.empty_like(st)
+    check(ih.gated_delta_rule(q, k, v, g, b, st, new_state=new, l2norm=True), o, "o")
+    check(new, last, "state")
+
+
+@pytest.mark.parametrize("t", [100])
+@pytest.mark.parametrize("size", [1e-12, 1e-6, 1e6, 1e12])
+@pytest.mark.parametrize("what", ["v", "state", "q", "k"])
+def test_sizes_far_from_one(ih, t, size, what):
+    """Values, states, queries of another size than the rest, and keys of one that the rule's own norm undoes: each has a
+    scale of its own."""
+    import torch
+    q, k, v, g, b, st = make(1, t, 1, 2, 128, 64, seed=31)
+    l2 = what == "k"
+    if what != "k" or size > 1:  # (the square of a small key would meet the norm's own 1e-6)
+        {"v": v, "state": st, "q": q, "k": k}[what].mul_(size)
+    o, _, last = R.delta(q, k, v, g, b, st, l2norm=l2)
+    new = torch.empty_like(st)
+    check(ih.gated_delta_rule(q, k, v, g, b, st, new_state=new, l2norm=l2), o, "o")
+    check(new, last, "state")
+
+
+def test_writes_stop_while_the_state_fades(ih):
+    """The last tokens of a chunk decay and write nothing: what is left of the state is small beside what the chunk wrote, and
+    as exact. Their outputs, sum_j (P T)_rj R_j with R_j = 0 from there on, shrink under the row's other entries, so they are
+    allowed what the operand's limbs leave of those: P's row and T's column are brought to below 2^14 (at least 2^13), their
+    product is kept times 2^-19 as an fp16 pair, whose last place is 2^-24, so (P T)_rj is off by up to
+    2^-25 2^19 2^-13 2^-13 max|P_r| max|T_j| = 2^-32 max|P_r| max|T_j| besides its 22 bits; for unit keys, queries and beta in
+    [0, 1] max|P_r| <= 128^-1/2, max|T_j| <= 1 and |R_j| <= |v_j| + |S| of the column."""
+    import torch
+    q, k, v, g, b, st = make(2, 128, 2, 2, 128, 64, seed=37)
+    g.fill_(-1.0)
+    b[:, 40:64] = 0.0
+    b[:, 100:] = 0.0
+    o, kept, last = R.delta(q, k, v, g, b, st)
+    new = torch.empty_like(st)
+    out = ih.gated_delta_rule(q, k, v, g, b, st, new_state=new)
+    check(new, last, "state")
+    for i in range(0, 128, 8):
+        first = i // 64 * 64
+        before = st.double().cpu() if first == 0 else kept[:, first - 1]
+        size = v[:, first:first + 64].double().cpu().abs().sum(1) + 64 * before.norm(dim=2)
+        allowed = TOL * float(o[:, i:i + 8].norm()) + 2.0 ** -32 * 128 ** -0.5 * 8 ** 0.5 * float(size.norm())
+        diff = float((out[:, i:i + 8].double().cpu() - o[:, i:i + 8]).norm())
+        assert diff <= allowed, (i, diff, allowed)

@@ -97,7 +97,7 @@ def test_attn_refusals(lib):
 def test_delta_refusals(lib):
     nb = C.c_size_t()
     for bad in ((0, 1, 1, 1, 64, 64), (1, 0, 1, 1, 64, 64), (1, 1, 2, 3, 64, 64), (1, 1, 0, 1, 64, 64), (1, 1, 1, 1, 96, 64),
-                (1, 1, 1, 1, 64, 30), (1, 1, 1, 1, 64, 516), (65536, 1, 1, 1, 64, 64)):
+                (1, 1, 1, 1, 64, 30), (1, 1, 1, 1, 64, 516), (65536, 1, 1, 1, 64, 64), (60000, 1, 1, 128, 64, 64)):
         assert lib.ihip_delta_ws_bytes(*bad, 0, C.byref(nb)) == -22, bad
     assert lib.ihip_delta_ws_bytes(1, 1, 1, 1, 64, 64, 0, None) == -14
     assert lib.ihip_delta_ws_bytes(2, 9, 1, 2, 64, 64, 0, C.byref(nb)) == 0 and nb.value > 0
