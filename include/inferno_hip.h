@@ -508,8 +508,8 @@ int ihip_rope_apply(const ihip_rope *rope, const float *x_dev, int64_t ldx,
  * A sequence with len_dev[s] < 0 is idle: its rows and cache stay as they
  * were. One whose M entries do not fit its capacity gets NaN rows of q_out,
  * and its cache stays as it was (the lengths are read on the device, so that
- * a captured step can follow ihip_spec_advance_len). Counts of rows x heads
- * and pointers as in ihip_kv; the KV write of src/ModelCPU.jl:245-258. */
+ * a captured step can follow ihip_spec_advance_len). Up to 2^23 rows (of
+ * ihip_rope_apply too); the KV write of src/ModelCPU.jl:245-258. */
 int ihip_rope_append(const ihip_rope *rope, const float *qkv_dev, int64_t ld,
                      float *q_out_dev, int64_t ldq, int n_q,
                      const ihip_kv *cache, const int32_t *len_dev,
@@ -531,8 +531,9 @@ int ihip_rope_append(const ihip_rope *rope, const float *qkv_dev, int64_t ld,
  * effect on it, NaN and infinities included; a row that sees a non-finite
  * score or value gets a non-finite result there. A sequence with len_dev[s]
  * < 0 is idle (its rows of out stay as they were); one with len_dev[s] + M >
- * capacity gets NaN rows. head_dim 64, 128 or 256. q and out 16-byte aligned,
- * ldq and ldo multiples of 4. Results do not depend on what runs beside the
+ * capacity gets NaN rows. Sums of p v are divided by the sum of p at the end:
+ * |v| below 2^100. head_dim 64, 128 or 256; up to 2^22 query rows (n_seq M
+ * n_q). q and out 16-byte aligned, ldq and ldo multiples of 4. Results do not depend on what runs beside the
  * call (no atomics). ws: ihip_attn_prefix_ws_bytes, 16-byte aligned, not
  * shared by calls that overlap in time. Replaces the cached attention of
  * src/ModelCPU.jl:730-856 for the tokens of a verify step. */
@@ -559,12 +560,15 @@ int ihip_attn_prefix(const float *q_dev, int64_t ldq, float *out_dev,
  * [T][n_v][dk][dv] (the state after every token, what ihip_spec_commit_state
  * picks from; NULL: not kept; T <= 64). len_dev (NULL: T for all): tokens of
  * each sequence, clamped to T; o and snapshots past them are left as they
- * were, and with 0 or less state_out is state_in. All fp32. dk 64 or 128, dv
+ * were, and with 0 or less state_out is state_in. A g of -inf clears the state
+ * before its token. A token with a value that is not finite spoils its own row
+ * of o and, unless the value is q's, the later ones and the state of that head
+ * (v's: of that column), no earlier row. All fp32; n_seq n_v dv / 16 up to 2^22. dk 64 or 128, dv
  * a multiple of 4 up to 512; pointers 16-byte aligned (g and beta: 4), ld's
  * multiples of 4 up to 2^24 (ldg, ldb: any). o may not overlap the inputs. ws:
  * ihip_delta_ws_bytes, 16-byte aligned, not shared by calls that overlap in
- * time. Few tokens (and every call with snapshots) go one by one; many go in
- * chunks of 64 on the matrix cores, where each chunk's tokens become one
+ * time. Few tokens (up to some dozens, by the number of states; and every call
+ * with snapshots) go one by one; many go in chunks of 64 on the matrix cores, where each chunk's tokens become one
  * triangular system (fp32 accuracy both ways). */
 #define IHIP_DELTA_L2NORM 1
 typedef struct ihip_delta {

@@ -1031,8 +1031,10 @@ int fill_attn(const char *name, AttnArgs &a, int n_q, int M, const ihip_kv *cach
     if (rc != IHIP_OK) return rc;
     if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256)
         return fail(IHIP_EINVAL, "%s: head_dim=%d (64, 128 or 256)", name, cache->head_dim);
-    if (n_q < 1 || n_q % cache->n_kv || n_q > 65535 || M < 1 || (int64_t)M * cache->n_seq * n_q > 0x7fffffff)
-        return fail(IHIP_EINVAL, "%s: n_q=%d over n_kv=%d, M=%d", name, n_q, cache->n_kv, M);
+    // (a launch holds 2^32 threads: up to 512 a query row)
+    if (n_q < 1 || n_q % cache->n_kv || n_q > 65535 || M < 1 || (int64_t)M * cache->n_seq * n_q > (1 << 22))
+        return fail(IHIP_EINVAL, "%s: n_q=%d over n_kv=%d, M=%d of n_seq=%d (up to 2^22 query rows)", name, n_q, cache->n_kv, M,
+                    cache->n_seq);
     a = AttnArgs{};
     a.n_q = n_q, a.M = M, a.n_seq = cache->n_seq, a.n_kv = cache->n_kv, a.head_dim = cache->head_dim;
     a.type = cache->type, a.k = cache->k, a.v = cache->v, a.capacity = cache->capacity;
@@ -1100,6 +1102,8 @@ static void rope_args(RopeArgs &a, RopeTable &tab, const ihip_rope *r) {
     memcpy(tab.turns, r->turns, sizeof tab.turns);
 }
 
+constexpr int64_t MOST_ROPE_TOKENS = 1 << 23;  // (a launch holds 2^32 threads, 256 of them a token)
+
 // 16-byte accesses: whole vectors in every part of a head, aligned rows
 static bool rope_vec(const RopeArgs &a) {
     return a.head_dim % 4 == 0 && a.rot_dim % (a.interleaved ? 4 : 8) == 0 && a.ldx % 4 == 0 && a.ldy % 4 == 0 &&
@@ -1112,7 +1116,7 @@ int ihip_rope_apply(const ihip_rope *rope, const float *x_dev, int64_t ldx, floa
     const int rc = check_rope("ihip_rope_apply", rope);
     if (rc != IHIP_OK) return rc;
     const int64_t width = (int64_t)heads * rope->head_dim;
-    if (heads < 1 || heads > 65536 || width > (1 << 24) || tokens < 1 || ldx < width || ldy < width)
+    if (heads < 1 || heads > 65536 || width > (1 << 24) || tokens < 1 || tokens > MOST_ROPE_TOKENS || ldx < width || ldy < width)
         return fail(IHIP_EINVAL, "ihip_rope_apply: heads=%d tokens=%d ldx=%lld ldy=%lld", heads, tokens, (long long)ldx,
                     (long long)ldy);
     if (x_dev == y_dev && ldx != ldy) return fail(IHIP_EINVAL, "ihip_rope_apply: in place needs ldy = ldx");
@@ -1134,7 +1138,7 @@ int ihip_rope_append(const ihip_rope *rope, const float *qkv_dev, int64_t ld, fl
     if (rope->head_dim != cache->head_dim)
         return fail(IHIP_EINVAL, "ihip_rope_append: head_dim %d and the cache's %d", rope->head_dim, cache->head_dim);
     const int64_t D = cache->head_dim, width = ((int64_t)n_q + 2 * cache->n_kv) * D;
-    if (n_q < 1 || n_q > 65536 || width > (1 << 24) || M < 1 || (int64_t)M * cache->n_seq > 0x7fffffff || ld < width ||
+    if (n_q < 1 || n_q > 65536 || width > (1 << 24) || M < 1 || (int64_t)M * cache->n_seq > MOST_ROPE_TOKENS || ld < width ||
         ldq < n_q * D)
         return fail(IHIP_EINVAL, "ihip_rope_append: n_q=%d M=%d ld=%lld ldq=%lld", n_q, M, (long long)ld, (long long)ldq);
     if (qkv_dev == q_out_dev && ld != ldq) return fail(IHIP_EINVAL, "ihip_rope_append: in place needs ldq = ld");

@@ -68,6 +68,7 @@ def test_append_refusals(lib):
     assert call(kv(), ld=1023) == -22 and call(kv(), ldq=511) == -22 and call(kv(), M=0) == -22 and call(kv(), n_q=0) == -22
     assert call(kv(), q=P) == -22  # in place, other row stride
     assert call(kv(d=64)) == -22 and b"head_dim" in lib.ihip_last_error()
+    assert call(kv(), M=1 << 23) == -22  # more tokens than a launch holds
     for bad in (kv(type=0), kv(n_seq=0), kv(n_kv=0), kv(cap=0), kv(k=P + 8), kv(strides=(4096, 256, 132)),
                 kv(strides=(4095 * 8, 128, 128)), kv(strides=(2048, 256, 128)), kv(strides=(-4096, 256, 128)),
                 kv(strides=(1 << 62, 1 << 61, 1 << 60), cap=1 << 30)):
@@ -81,6 +82,7 @@ def test_attn_refusals(lib):
     one = kv(n_seq=1, cap=100)
     assert ws(kv()) == 0 and nb.value > 0 and ws(kv(), pre=one) == 0
     assert lib.ihip_attn_prefix_ws_bytes(4, 1, C.byref(kv()), None, None) == -14
+    assert ws(kv(), M=1 << 20) == -22 and b"query rows" in lib.ihip_last_error()  # more than a launch holds
     assert ws(kv(d=96)) == -22 and ws(kv(), n_q=3) == -22 and ws(kv(), n_q=0) == -22 and ws(kv(), M=0) == -22
     for bad in (kv(n_seq=2), kv(n_seq=1, type=30), kv(n_seq=1, n_kv=1), kv(n_seq=1, d=64)):
         assert ws(kv(), pre=bad) == -22
