@@ -511,8 +511,10 @@ __global__ __launch_bounds__(512) void attn_part_kernel(AttnArgs a, AttnSplit pr
     else attn_part<TYPE, D, S, true>(a, own, (int)blockIdx.x - n_pre, lds, sh, opart, ml);
 }
 
-// The parts' results of a row, each times 2^(its maximum - the largest), over their sum: W waves a row (four where there
-// are many parts), each taking every W-th part, four loads in flight.
+// The parts' results of a row, each times 2^(its maximum - the largest), over their sum: W waves a row, each taking every W-th
+// part, four loads in flight. Bound by reading the parts (256 rows of a tree, 256 wide, 64 parts: 67 MB). With W = 4 and 1
+// (us, the whole call, 8 heads of D = 128): 16 query heads and 4 parts 10.4, 10.2, 16 parts 11.1, 12.8; 1024 and 4 25.3, 24.1,
+// 16 31.7, 32.2: four from 9 parts on.
 template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int parts, const float *__restrict__ opart,
                                                                               const float2 *__restrict__ ml) {
     constexpr int E = D / 64, ROWS = 4 / W, LANES = W * 64;
@@ -575,8 +577,21 @@ template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(
 
 constexpr int MOST_PARTS = 256;
 
-// The shape that serves `rows` query rows of a key head, and its rows a block.
-int shape_for(int D, int64_t rows) { return rows <= 32 && D < 256 ? 0 : rows <= 64 ? 1 : 2; }
+// The shape for `rows` query rows that meet `keys` keys in each of `units` heads (of sequences), and its rows a block. Blocks
+// of 32 rows are the quickest to finish, and where they are many take the fewest ranges of keys, whose results cost a pass of
+// their own; blocks of 64 and 256 (D = 256: 64 and 128) read less LDS for a product. Measured over a prefix in 2 or 8 heads
+// (us: blocks of 32, 64, 256; f16, D = 128): 256 rows, 4000 keys, 2 heads (2^21) 16.2, 19.6, 25.6; 512 rows, 4000, 8 (2^24)
+// 58.5, 57.5, 61.2; 1024, 4000, 8 (2^25) 105.5, 97.5, 99.3; 2048, 16000, 8 (2^28) 455, 361, 327; 2048, 1000, 2 (2^22) 51.6,
+// 44.2, 52.0. Of sequences' own entries (D = 64, bf16): 16 heads of 256 rows, 2064 keys 19.7, -, 28.9; 128 of 48 rows, 2012
+// keys 32.3, 25.9. D = 256 (blocks of 64, 128): 256 rows, 4000 keys, 2 heads (2^21) 25.6, 29.7; 16 heads of 256 rows, 2064 keys
+// (2^23) 59.6, 50.2. bf16 at D = 128 spills registers in blocks of 64: 1024 rows, 4000, 8 113, 117, 111.
+int shape_for(const AttnArgs &a, int64_t rows, int64_t units, int64_t keys) {
+    const double work = (double)rows * (double)units * (double)keys;
+    if (a.head_dim == 256) return rows <= 64 || work <= 1 << 22 ? 1 : 2;
+    const bool spills = a.head_dim == 128 && a.type == KV_BF16;
+    if (rows <= (spills ? 64 : 32) || (rows <= 1024 && work <= 1 << 24 && (rows + 31) / 32 * units < 256)) return 0;
+    return !spills && (rows <= 64 || work <= 1 << 26) ? 1 : 2;
+}
 int shape_rows(int D, int id) { return id == 0 ? 32 : id == 1 ? 64 : D == 256 ? 128 : 256; }
 
 struct AttnPlan {
@@ -584,24 +599,28 @@ struct AttnPlan {
     int parts, pre_shape, own_shape;
 };
 
-// One workgroup fills a CU. The sequences' own entries: ranges of 128 keys or more, up to 512 workgroups; the prefix: as
-// many ranges (of 64 keys or more) as fill the chip beside them, or once over where they are many.
+// One workgroup fills a CU. The sequences' own entries: ranges of 128 keys or more, up to 256 workgroups (5 tokens, 4 heads of 4
+// rows each, D = 128: 16 sequences of 4000 entries 29.5 us, 56.9 unsplit, 38.0 with up to 512; 4 of 200 12.7, 13.1, 21.3).
+// The prefix: as many ranges (of 64 keys or more) as fill the chip beside them, or once over where they are many: with 4
+// sequences of 500 entries beside 8000 shared 22.4 us, 28.9 where the prefix takes no account of them; with 16 sequences
+// 48.6 us once over, 375 with what little room they leave.
 AttnPlan plan_of(const AttnArgs &a) {
     AttnPlan p{};
     const int64_t G = a.n_q / a.n_kv, own_rows = a.M * G;
-    p.own_shape = shape_for(a.head_dim, own_rows);
+    p.own_shape = shape_for(a, own_rows, (int64_t)a.n_kv * a.n_seq, a.capacity);
     const int own_block = shape_rows(a.head_dim, p.own_shape);
     p.own.rows = (int)own_rows;
     p.own.blocks = (int)((own_rows + own_block - 1) / own_block);
     const int64_t units = (int64_t)p.own.blocks * a.n_kv * a.n_seq;
-    int64_t splits = 512 / units;
+    int64_t splits = 256 / units;
     splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
     const int64_t most = (a.capacity + 127) / 128;
     p.own.splits = (int)(splits < most ? splits : most);
     p.pre_shape = p.own_shape;
     if (a.P > 0) {
         const int64_t rows = (int64_t)a.n_seq * own_rows;
-        p.pre_shape = shape_for(a.head_dim, rows);
+        const int shape = shape_for(a, rows, a.n_kv, a.P);
+        p.pre_shape = shape > p.own_shape ? shape : p.own_shape;
         const int block = shape_rows(a.head_dim, p.pre_shape);
         p.pre.rows = (int)rows;
         p.pre.blocks = (int)((rows + block - 1) / block);
@@ -635,11 +654,14 @@ template <int TYPE, int D> hipError_t launch_all(const AttnArgs &a, const AttnPl
     const int shapes = p.pre_shape * 3 + p.own_shape;  // (own_shape <= pre_shape)
     if constexpr (D < 256) {
         if (shapes == 0) e = launch_part<TYPE, D, 0, 0>(a, p, opart, ml, st);
-        if (shapes == 3) e = launch_part<TYPE, D, 1, 0>(a, p, opart, ml, st);
+        if constexpr (!(D == 128 && TYPE == KV_BF16))
+            if (shapes == 3) e = launch_part<TYPE, D, 1, 0>(a, p, opart, ml, st);
         if (shapes == 6) e = launch_part<TYPE, D, 2, 0>(a, p, opart, ml, st);
     }
-    if (shapes == 4) e = launch_part<TYPE, D, 1, 1>(a, p, opart, ml, st);
-    if (shapes == 7) e = launch_part<TYPE, D, 2, 1>(a, p, opart, ml, st);
+    if constexpr (!(D == 128 && TYPE == KV_BF16)) {
+        if (shapes == 4) e = launch_part<TYPE, D, 1, 1>(a, p, opart, ml, st);
+        if (shapes == 7) e = launch_part<TYPE, D, 2, 1>(a, p, opart, ml, st);
+    }
     if (shapes == 8) e = launch_part<TYPE, D, 2, 2>(a, p, opart, ml, st);
     if (e != hipSuccess) return e;
     if (p.parts > 8) attn_join_kernel<D, 4><<<(unsigned)rows, 256, 0, st>>>(a, p.parts, opart, ml);
