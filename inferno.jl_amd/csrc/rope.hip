@@ -9,6 +9,13 @@
 // One workgroup takes one token (or a part of its heads where tokens are few):
 // the pairs' sines and cosines are formed once in LDS and serve every head, so
 // beyond that a value is read once, turned and written once, 16 bytes a lane.
+// Bound by those bytes where tokens are many, by one pass of loads and stores
+// where they are few:
+//   8190 rows of 16 q, 4 k and 4 v heads of 256 into fp32 rows and a bf16 cache
+//     (369 MB) 75.7 us, 4.9 TB/s; a copy of 1 GiB reaches 5.2. 4 bytes a lane
+//     instead of 16: 35.2 us for 29.8 (4096 rows of 48 heads of 128);
+//   one row of 32 q, 8 k and 8 v heads of 128: 3.2 us;
+//   64 rows of 32 heads of 128: 3.9 us.
 #include "common.h"
 #include "mixer.h"
 
@@ -119,7 +126,8 @@ template <int VEC> __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a
 hipError_t launch_rope(const RopeArgs &a, const RopeTable &tab, int64_t rows, bool vec, hipStream_t st) {
     const int per = vec ? 4 : 1;
     const int64_t units = (int64_t)(a.n_q + a.n_k + a.n_v) * (a.head_dim / per);
-    // a token's heads over up to 8 workgroups where tokens alone would not fill the chip
+    // a token's heads over up to 8 workgroups where tokens alone would not fill the chip (us, split and not: 1 row of 80 heads
+    // 3.2, 5.3; 512 rows 8.3, 9.6; 16384 rows 246, 239)
     int64_t split = rows >= 1024 ? 1 : (1024 + rows - 1) / rows;
     const int64_t most = (units + 511) / 512;
     split = split < most ? split : most;
