@@ -207,12 +207,16 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_prep_kernel(De
     // running sums of a head's g log2(e), in fp64: a difference of two sums of the chunk keeps its digits however far
     // both have fallen. e^-4096 is 0 in fp32 as is e^g of any g below, -inf among them: such a g counts as -4096, and the
     // sums behind it stay finite and keep their digits.
-    auto decays = [&](int hv) __attribute__((always_inline)) {
-        if (tile == 0) {
-            const bool at = t0 + lane < a.T;
+    float gv = 0.f, bv = 0.f;
+    auto get_decays = [&](int hv) __attribute__((always_inline)) {
+        if (tile == 0 && t0 + lane < a.T) {
             const int64_t row = (int64_t)s * a.T + t0 + lane;
-            const float gv = at ? a.g[row * a.ldg + hv] : 0.f, bv = at ? a.beta[row * a.ldb + hv] : 0.f;
-            const bool in = t0 + lane < tokens_of(a, s);
+            gv = a.g[row * a.ldg + hv], bv = a.beta[row * a.ldb + hv];
+        }
+    };
+    auto sum_decays = [&](int n) __attribute__((always_inline)) {
+        if (tile == 0) {
+            const bool in = t0 + lane < n;
             double v = !in ? 0.0 : (gv < -4096.f ? -4096.0 : (double)gv) * 1.4426950408889634;
             beta[lane] = in ? bv : 0.f;
             bad[lane] = 0;
@@ -225,6 +229,7 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_prep_kernel(De
     };
     // rows of q and k to limbs: 4 threads a row (loaded before it is known how many tokens there are, then taken for zeros
     // past them)
+    int n;
     {
         const int r = tid >> 2, part = tid & 3;
         const bool at = t0 + r < a.T;
@@ -240,8 +245,8 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_prep_kernel(De
                 *(f4 *)(x[m][i] + 4) = at ? *(const f4 *)(src + i * 32 + 16 + part * 4) : f4{0, 0, 0, 0};
             }
         }
-        decays(hk * rep + part0);
-        const int n = tokens_of(a, s);
+        get_decays(hk * rep + part0);
+        n = tokens_of(a, s);
         if (t0 >= n) return;
         const bool in = t0 + r < n;
 #pragma unroll
@@ -311,6 +316,7 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_prep_kernel(De
                 }
         }
     }
+    sum_decays(n);  // (by the wave with the fewest products)
     float *const A = (float *)(lds + AAT), *const P = (float *)(lds + PAT);  // [64][LD]
     char *const pl = lds + LAT + lane * 16;
     for (int h = part0; h < min(part0 + each, rep); h++) {
@@ -318,7 +324,8 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_prep_kernel(De
         float *const sc = w.scal + unit * SCAL;
         __syncthreads();  // (q's limbs, or the head before, are done with)
         if (h > part0) {
-            decays(hk * rep + h);
+            get_decays(hk * rep + h);
+            sum_decays(n);
             __syncthreads();
         }
         {

@@ -14,7 +14,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
-from .quantized_kernels import _ptr, _stream, check_tensor
+from .quantized_kernels import _ptr, _raw_stream, check_tensor
 
 F16, BF16 = 1, 30
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BY_PARTS = 0, 1, 2
@@ -24,15 +24,16 @@ _SCALINGS = {"none": ROPE_PLAIN, "linear": ROPE_LINEAR, "by_parts": ROPE_BY_PART
 
 # The per-call checks are kept to a few attribute reads a tensor (a call's host time is most of a one-token call's); what
 # they refuse goes to _refuse for the message.
-_f32 = _i32 = _i64 = _u8 = _current_device = _Tensor = None
+_f32 = _i32 = _i64 = _u8 = _current_device = _stream_of = _Tensor = None
 
 
 def _torch():
     """torch's names, looked up once (the package itself does not import it)."""
-    global _f32, _i32, _i64, _u8, _current_device, _Tensor
+    global _f32, _i32, _i64, _u8, _current_device, _stream_of, _Tensor
     import torch
-    _f32, _i32, _i64, _u8, _Tensor = torch.float32, torch.int32, torch.int64, torch.uint8, torch.Tensor
-    _current_device = torch.cuda.current_device
+    _current_device, _stream_of = torch.cuda.current_device, _raw_stream()
+    _i32, _i64, _u8, _Tensor = torch.int32, torch.int64, torch.uint8, torch.Tensor
+    _f32 = torch.float32  # (last: what the calls look at)
 
 
 def _refuse(t, name: str, dtype, shape=None, contiguous: bool = True, dev: int | None = None):
@@ -51,6 +52,11 @@ def _device_of(t, name: str) -> int:
     if dev != _current_device():
         raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
     return dev
+
+
+def _on(stream, dev: int) -> int:
+    """The stream's handle; without one that of torch's current stream."""
+    return _stream_of(dev) if stream is None else getattr(stream, "cuda_stream", stream)
 
 
 def _call(name: str):
@@ -154,7 +160,7 @@ def rope(x, positions, n_heads: int, params: RopeParams, out=None, stream=None):
     if out is None:
         out = x.new_empty((rows, width))
     yp, _, ldy = _rows(out, "out", width, rows, dev)
-    _lib.check(_call("ihip_rope_apply")(params._on(dev), xp, ldx, yp, ldy, n_heads, pp, rows, _stream(stream)))
+    _lib.check(_call("ihip_rope_apply")(params._on(dev), xp, ldx, yp, ldy, n_heads, pp, rows, _on(stream, dev)))
     return out
 
 
@@ -179,7 +185,7 @@ def rope_append(qkv, n_q: int, cache: KVCache, lengths, params: RopeParams, posi
         out = qkv.new_empty((rows, n_q * d))
     yp, _, ldq = _rows(out, "out", n_q * d, rows, dev)
     _lib.check(_call("ihip_rope_append")(params._on(dev), xp, ld, yp, ldq, n_q, cache._on(dev), lp, pp, pos0, rows // s,
-                                         _stream(stream)))
+                                         _on(stream, dev)))
     return out
 
 
@@ -217,7 +223,7 @@ def attn_prefix(q, n_q: int, cache: KVCache, lengths, prefix: KVCache | None = N
     wp, wn = _workspace(ws, dev)
     _lib.check(_call("ihip_attn_prefix")(qp, ldq, op, ldo, n_q, m, cache._on(dev), lp,
                                          None if prefix is None else prefix._on(dev), mp,
-                                         d ** -0.5 if scale is None else scale, wp, wn, _stream(stream)))
+                                         d ** -0.5 if scale is None else scale, wp, wn, _on(stream, dev)))
     return out
 
 
@@ -291,5 +297,5 @@ def gated_delta_rule(q, k, v, g, beta, state, new_state=None, snapshots=None, le
     a.n_seq, a.T, a.n_k, a.n_v, a.dk, a.dv = s, t, n_k, n_v, dk, dv
     a.scale = dk ** -0.5 if scale is None else scale
     a.flags = DELTA_L2NORM if l2norm else 0
-    _lib.check(_call("ihip_gated_delta_rule")(C.byref(a), wp, wn, _stream(stream)))
+    _lib.check(_call("ihip_gated_delta_rule")(C.byref(a), wp, wn, _on(stream, dev)))
     return out
