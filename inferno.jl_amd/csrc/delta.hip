@@ -95,13 +95,14 @@ template <int DK> __global__ __launch_bounds__(64) void delta_token_kernel(Delta
 //
 // What bounds it: the preparation by its bytes and, in a chunk, by steps that few
 // waves can share (T's diagonal blocks, its columns); the chunks by the way of the
-// state through them. 4096 tokens, 16 key and 32 value heads of 128: 68 us (230
-// MB, 3.4 TB/s) and 132 us, 2.05 us a chunk, in which a CU brings 108 KB of
-// operands for its 16 columns (13 TB/s over the chip, from L2; without these loads
-// the chunks take 88 us) between two barriers. 6 sequences of 333 tokens, 8 heads
-// of 64 x 96: 20 and 17 us, the first mostly one chunk's latency, the second 2.7
-// us a chunk. (Before the state's way was cut to two products - X formed for the
-// state too, operands by way of LDS - the chunks took 190 us.)
+// state through them. 4096 tokens, 16 key and 32 value heads of 128: 63 us (230
+// MB, 3.6 TB/s) and 127 us, 2 us a chunk, in which a CU brings 108 KB of operands
+// for its 16 columns (14 TB/s over the chip, from L2, which gives 27 to loads
+// alone; without these loads the chunks take 88 us) between two barriers; 178 us
+// together. 6 sequences of 333 tokens, 8 heads of 64 x 96: 19 and 17 us, the first
+// mostly one chunk's latency, the second 2.7 us a chunk. (Before the state's way
+// was cut to two products - X formed for the state too, operands by way of LDS -
+// the chunks took 190 us.)
 
 constexpr int CH = 64;
 constexpr int PT_BYTES = 6 * 2048;   // P T: the six 16 x 32 blocks at or below the diagonal, two limbs
@@ -863,6 +864,16 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
 #pragma unroll
                 for (int y = 0; y < 2; y++) PT[t][u][y] = *(const h8 *)(from + pt_block(TT * part + t, low ? u : 0) * 2048 + y * 1024 + l16);
     };
+    // The lines of a chunk some steps ahead are touched (a word of each 128 bytes, a head's column groups and their waves sharing
+    // them), so that they are in L2 when their loads come (4096 tokens: 131 -> 127 us; 115 with all
+    // operands there).
+    constexpr int LQ = 2 * IMG / 128, LINES = LQ + (IMG + PT_BYTES) / 128;
+    const int line = (lane * groups + grp) * U + part;
+    uint32_t touched = 0;
+    auto touch = [&](int c) __attribute__((always_inline)) {
+        asm volatile("" ::"v"(touched));
+        if (line < LINES) touched = *(const uint32_t *)(line < LQ ? q_of(c) + line * 128 : w_of(c) + (line - LQ) * 128);
+    };
     if (chunks) {
         u4 f3[3], v3[3][CH / VR];
 #pragma unroll
@@ -895,7 +906,7 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
         if (c + 1 < chunks) bare_barrier();
         put_fac(c + 3), put_v(c + 3);  // (4 chunks' places: c to c + 3)
         STAGE();
-        get_fac(c + 4), get_v(c + 4);
+        get_fac(c + 4), get_v(c + 4), touch(c + 6);
         STAGE();
         h8 l[2][2];
 #pragma unroll
