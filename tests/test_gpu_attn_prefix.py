@@ -241,3 +241,62 @@ def test_repeats_streams_and_graph(ih):
         torch.cuda.synchronize()
         want = ih.attn_prefix(c.q, 16, cache, first + 3 * i, prefix=prefix)
         assert torch.equal(out, want), i
+
+
+BIG = [  # s, m, hq, hkv, d, p, lens: what takes each pair of block shapes (the prefix's, the sequences' own)
+    (5, 55, 8, 2, 64, 300, [0, 3, 20, 70, 1]),           # 1100 rows share, 220 a sequence
+    (5, 55, 8, 2, 128, 300, [0, 3, 20, 70, 1]),
+    (1, 300, 8, 2, 64, 100, [40]),                       # 1200 rows of one
+    (1, 300, 8, 2, 128, 100, [40]),
+    (1, 300, 8, 2, 64, 28000, [0]),                      # and a long prefix
+    (64, 4, 32, 8, 64, 8300, [i % 5 for i in range(64)]),
+    (1, 1100, 32, 8, 64, 0, [900]),
+    (9, 4, 16, 4, 256, 7500, [7] * 9),
+    (1, 100, 16, 4, 256, 50, [2600]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("shape", BIG)
+def test_large(ih, shape, dtype):
+    """(The definition in 64 bits on the GPU, a sequence and key head at a time: these are too many for the other.)"""
+    import torch
+    c = Case(*shape, dtype=dtype, seed=41)
+    got = c.run(ih).double().view(c.s, c.m, c.hkv, -1, c.d)
+    q = c.q.double().view(got.shape)
+    diff = norm = 0.0
+    for i in range(c.s):
+        n = int(c.lens[i])
+        last = c.p + n + torch.arange(c.m, device="cuda")[:, None, None]
+        hides = torch.arange(c.p + n + c.m, device="cuda") > last  # [m, 1, keys]
+        for g in range(c.hkv):
+            k, v = (torch.cat([x[0, :c.p, g], y[i, :n + c.m, g]]).double() for x, y in ((c.pk, c.k), (c.pv, c.v)))
+            z = (q[i, :, g] @ k.T * c.scale).masked_fill(hides, float("-inf"))
+            w = torch.softmax(z, -1)
+            out, size = w @ v, w @ v.abs()
+            reach = (q[i, :, g].abs() @ k.abs().T * c.scale).masked_fill(hides, 0.0).amax(-1, keepdim=True)
+            err = (got[i, :, g] - out).abs()
+            bound = R.attention_bound(c.d, size, reach, (last + 1).double())
+            assert bool((err <= bound).all()), (i, g, float((err - bound).max()))
+            diff, norm = diff + float(err.square().sum()), norm + float(out.square().sum())
+    assert diff <= 1e-10 * norm, (diff, norm)  # rel-L2 1e-5
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "float16"), (128, "float16"), (128, "bfloat16"), (256, "bfloat16")])
+def test_tree_of_many_heads(ih, d, dtype):
+    """So many query heads over a key head that a sequence's own entries are met in tall blocks."""
+    c = Case(2, 64, 34, 2, d, 70, [30, 2050 if d == 256 else 5], dtype=dtype, tree=trees(2, 64, 3), seed=43)
+    c.check(c.run(ih))
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "float16"), (64, "bfloat16"), (128, "bfloat16"), (256, "float16")])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_large_unseen_values(ih, d, dtype, value):
+    """Tall blocks: an entry whose k and v are not finite reaches the rows that see it alone."""
+    import torch
+    m, n = 300, 1100 if d == 256 else 40
+    c = Case(1, m, 8, 2, d, 100, [n], dtype=dtype, seed=47)
+    good = c.run(ih)
+    c.k[0, n + 200:n + m], c.v[0, n + 200:n + m] = value, value
+    got = c.run(ih)
+    assert torch.equal(got[:200], good[:200]) and not bool(torch.isfinite(got[200:]).any())
