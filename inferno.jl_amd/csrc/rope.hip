@@ -12,7 +12,7 @@
 // Bound by those bytes where tokens are many, by one pass of loads and stores
 // where they are few:
 //   8190 rows of 16 q, 4 k and 4 v heads of 256 into fp32 rows and a bf16 cache
-//     (369 MB) 75.7 us, 4.9 TB/s; a copy of 1 GiB reaches 5.2. 4 bytes a lane
+//     (369 MB) 73.5 us, 5.0 TB/s; a copy of 1 GiB reaches 5.2. 4 bytes a lane
 //     instead of 16: 35.2 us for 29.8 (4096 rows of 48 heads of 128);
 //   one row of 32 q, 8 k and 8 v heads of 128: 3.2 us;
 //   64 rows of 32 heads of 128: 3.9 us.
@@ -38,7 +38,8 @@ template <int VEC> __device__ __forceinline__ void put_kv(void *base, int64_t at
     }
 }
 
-template <int VEC> __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, RopeTable tab) {
+// STREAM: rows of fp32 too many for the caches pass them by.
+template <int VEC, bool STREAM> __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, RopeTable tab) {
     __shared__ float2 cs[128];
     typedef typename Vec<VEC>::t vec;
     const int64_t row = blockIdx.x;
@@ -67,6 +68,14 @@ template <int VEC> __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a
     const int ru = a.rot_dim / (VEC == 4 && a.interleaved ? 4 : 2 * VEC);
     const int ut = ru + (D - a.rot_dim) / VEC, uv = D / VEC;
     const int n_turn = (a.n_q + a.n_k) * ut, total = n_turn + a.n_v * uv;
+    auto get = [&](int64_t at) __attribute__((always_inline)) {
+        if constexpr (STREAM) return __builtin_nontemporal_load((const vec *)(x + at));
+        else return *(const vec *)(x + at);
+    };
+    auto put = [&](int64_t at, const float *v) __attribute__((always_inline)) {
+        if constexpr (STREAM) __builtin_nontemporal_store(*(const vec *)v, (vec *)(y + at));
+        else *(vec *)(y + at) = *(const vec *)v;
+    };
     const int64_t slot = (int64_t)s * a.seq_stride + ((int64_t)n + m) * a.tok_stride;
     for (int i = blockIdx.y * 256 + tid; i < total; i += gridDim.y * 256) {
         const bool turn = i < n_turn;
@@ -83,7 +92,7 @@ template <int VEC> __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a
         }
         const int64_t src = (int64_t)head * D;
         float v0[VEC], v1[VEC];
-        *(vec *)v0 = *(const vec *)(x + src + d0);
+        *(vec *)v0 = get(src + d0);
         if (turn && u < ru) {
             if (VEC == 4 && a.interleaved) {
 #pragma unroll
@@ -94,7 +103,7 @@ template <int VEC> __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a
                     v0[c + 1] = p1 * e.x + p0 * e.y;
                 }
             } else {
-                *(vec *)v1 = *(const vec *)(x + src + d1);
+                *(vec *)v1 = get(src + d1);
 #pragma unroll
                 for (int c = 0; c < VEC; c++) {
                     const float2 e = cs[VEC * u + c];
@@ -109,8 +118,8 @@ template <int VEC> __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a
 #pragma unroll
                 for (int c = 0; c < VEC; c++) v0[c] = v1[c] = __builtin_nanf("");
             }
-            *(vec *)(y + src + d0) = *(vec *)v0;
-            if (d1 >= 0) *(vec *)(y + src + d1) = *(vec *)v1;
+            put(src + d0, v0);
+            if (d1 >= 0) put(src + d1, v1);
         } else if (fits) {
             const int kv = turn ? head - a.n_q : hd;
             void *base = turn ? a.k : a.v;
@@ -133,7 +142,11 @@ hipError_t launch_rope(const RopeArgs &a, const RopeTable &tab, int64_t rows, bo
     split = split < most ? split : most;
     if (split > 8) split = 8;
     const dim3 grid((unsigned)rows, (unsigned)(split < 1 ? 1 : split));
-    if (vec) rope_kernel<4><<<grid, 256, 0, st>>>(a, tab);
-    else rope_kernel<1><<<grid, 256, 0, st>>>(a, tab);
+    // past the caches from 32 MB of rows on, what the eight L2s hold: 8190 rows of 201 MB 73.5 us, 77.5 through them (fewer are
+    // read again by what comes next)
+    const bool stream = rows * units * per * 4 >= (int64_t)32 << 20;
+    if (vec && stream) rope_kernel<4, true><<<grid, 256, 0, st>>>(a, tab);
+    else if (vec) rope_kernel<4, false><<<grid, 256, 0, st>>>(a, tab);
+    else rope_kernel<1, false><<<grid, 256, 0, st>>>(a, tab);
     return hipGetLastError();
 }

@@ -138,3 +138,27 @@ def test_append_far_sequences(ih):
     k2, v2 = torch.zeros(s, cap, hkv, d, dtype=torch.float16, device="cuda"), torch.zeros(s, cap, hkv, d, dtype=torch.float16, device="cuda")
     q2 = ih.rope_append(qkv, 2, ih.KVCache(k2, v2), lens, ih.RopeParams(d))
     assert torch.equal(q, q2) and torch.equal(k, k2) and torch.equal(v, v2) and bool((k2[1, 5] != 0).any())
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rot", [(256, 64), (128, 128)])
+def test_many_rows_are_as_few(ih, d, rot, interleaved):
+    """More rows than the caches hold (their loads and stores pass them by): the same bits as a few at a time."""
+    import torch
+    n, hq, hkv = 2300, 16, 4
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(n, (hq + 2 * hkv) * d + 8, generator=g, device="cuda")[:, :(hq + 2 * hkv) * d]
+    rp = ih.RopeParams(d, rot, interleaved=interleaved, base=1e6)
+    def caches():
+        return [torch.full((1, n + 3, hkv, d), 7.0, device="cuda", dtype=torch.bfloat16) for _ in "kv"]
+    k, v = caches()
+    q = ih.rope_append(x, hq, ih.KVCache(k, v), torch.tensor([2], dtype=torch.int32, device="cuda"), rp, pos0=11)
+    k1, v1 = caches()
+    c1 = ih.KVCache(k1, v1)
+    for at in range(0, n, 500):
+        m = min(500, n - at)
+        part = ih.rope_append(x[at:at + m], hq, c1, torch.tensor([2 + at], dtype=torch.int32, device="cuda"), rp, pos0=11)
+        assert torch.equal(part, q[at:at + m]), at
+    assert torch.equal(k, k1) and torch.equal(v, v1)
+    pos = 13 + torch.arange(n, dtype=torch.int32, device="cuda")
+    assert torch.equal(ih.rope(x, pos, hq + 2 * hkv, rp)[:, :hq * d], q)
