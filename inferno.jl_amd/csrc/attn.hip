@@ -613,10 +613,12 @@ struct AttnPlan {
 };
 
 // One workgroup fills a CU. The sequences' own entries: ranges of 128 keys or more, up to 256 workgroups (5 tokens, 4 heads of 4
-// rows each, D = 128: 16 sequences of 4000 entries 29.5 us, 56.9 unsplit, 38.0 with up to 512; 4 of 200 12.7, 13.1, 21.3).
-// The prefix: as many ranges (of 64 keys or more) as fill the chip beside them, or once over where they are many: with 4
-// sequences of 500 entries beside 8000 shared 22.4 us, 28.9 where the prefix takes no account of them; with 16 sequences
-// 48.6 us once over, 375 with what little room they leave.
+// rows each, D = 128: 16 sequences of 4000 entries 29.5 us, 56.9 unsplit, 38.0 with up to 512; 4 of 200 12.7, 13.1, 21.3), half
+// that beside a prefix. The prefix: as many ranges (of 128 keys or more) as fill the chip beside them, or once over where they
+// are many. Half and all of the chip for the own entries (us, 8 heads of D = 128, 4 rows a token, 1024 to 4096 entries of
+// capacity): 4 sequences of 5 tokens, 777 shared entries 14.4, 21.0; 8, 1500 17.7, 23.6; 9, 4099 25.7, 29.8; 16 of one token,
+// 8000 23.5, 27.8; 16 of 5, 8000 55, 49. Ranges of 128 and of 64: one row a head over 777 entries 10.6, 11.1, at D = 256 over
+// 3000 14.8, 17.0.
 AttnPlan plan_of(const AttnArgs &a) {
     AttnPlan p{};
     const int64_t G = a.n_q / a.n_kv, own_rows = a.M * G;
@@ -625,7 +627,7 @@ AttnPlan plan_of(const AttnArgs &a) {
     p.own.rows = (int)own_rows;
     p.own.blocks = (int)((own_rows + own_block - 1) / own_block);
     const int64_t units = (int64_t)p.own.blocks * a.n_kv * a.n_seq;
-    int64_t splits = 256 / units;
+    int64_t splits = (a.P > 0 ? 128 : 256) / units;
     splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
     const int64_t most = (a.capacity + 127) / 128;
     p.own.splits = (int)(splits < most ? splits : most);
@@ -640,7 +642,7 @@ AttnPlan plan_of(const AttnArgs &a) {
         const int64_t beside = units * p.own.splits, room = beside <= 128 ? 256 - beside : 256;
         int64_t n = room / ((int64_t)p.pre.blocks * a.n_kv);
         n = n < 1 ? 1 : n > 128 ? 128 : n;
-        const int64_t top = (a.P + 63) / 64;
+        const int64_t top = (a.P + 127) / 128;
         n = n < top ? n : top;
         p.pre.per = ((a.P + n - 1) / n + 31) / 32 * 32;
         p.pre.splits = (int)((a.P + p.pre.per - 1) / p.pre.per);
