@@ -453,8 +453,8 @@ int ihip_spec_advance_len(int32_t *len_dev, const int32_t *n_accepted_dev,
  * tok_stride t + head_stride h values behind k (and behind v); an entry's
  * values are contiguous. k and v are 16-byte aligned, the strides multiples
  * of 8 values; they may be of either order ([S, cap, heads, D] or [S, heads,
- * cap, D]), tok_stride up to 2^24, the others past 32 bits. The reference keeps an fp32 cache per layer
- * (src/ModelCPU.jl:234-258). */
+ * cap, D]), tok_stride up to 2^24, the others past 32 bits. The reference keeps
+ * an fp32 cache per layer (src/ModelCPU.jl:234-258). */
 typedef struct ihip_kv {
     int type;            /* IHIP_F16 / IHIP_BF16 */
     int n_seq, n_kv, head_dim;
@@ -563,12 +563,13 @@ int ihip_attn_prefix(const float *q_dev, int64_t ldq, float *out_dev,
  * were, and with 0 or less state_out is state_in. A g of -inf clears the state
  * before its token. A token with a value that is not finite spoils its own row
  * of o and, unless the value is q's, the later ones and the state of that head
- * (v's: of that column), no earlier row. All fp32; n_seq n_v dv / 16 up to 2^22. dk 64 or 128, dv
- * a multiple of 4 up to 512; pointers 16-byte aligned (g and beta: 4), ld's
- * multiples of 4 up to 2^24 (ldg, ldb: any). o may not overlap the inputs. ws:
- * ihip_delta_ws_bytes, 16-byte aligned, not shared by calls that overlap in
- * time. Few tokens (up to some dozens, by the number of states; and every call
- * with snapshots) go one by one; many go in chunks of 64 on the matrix cores, where each chunk's tokens become one
+ * (v's: of that column), no earlier row. All fp32, below 2^90 in size; n_seq
+ * n_v dv / 16 up to 2^22. dk 64 or 128, dv a multiple of 4 up to 512; pointers
+ * 16-byte aligned (g and beta: 4), ld's multiples of 4 up to 2^24 (ldg, ldb:
+ * any). o may not overlap the inputs. ws: ihip_delta_ws_bytes, 16-byte aligned,
+ * not shared by calls that overlap in time. Few tokens (up to some dozens, by
+ * the number of states; and every call with snapshots) go one by one; many go in
+ * chunks of 64 on the matrix cores, where each chunk's tokens become one
  * triangular system (fp32 accuracy both ways). */
 #define IHIP_DELTA_L2NORM 1
 typedef struct ihip_delta {

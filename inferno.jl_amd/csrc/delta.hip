@@ -88,7 +88,7 @@ template <int DK> __global__ __launch_bounds__(64) void delta_token_kernel(Delta
 // powers of A that a product form would need can be huge where keys repeat),
 // then q, k, W and P T as fp16 operands. What is left to do chunk after chunk
 // (delta_chunk_kernel) is two products on the state's way, K S and W R, and two
-// beside it, Q S and (P T) R; a wave carries 16 columns of S in its
+// beside it, Q S and (P T) R; a workgroup carries 16 columns of S in its
 // accumulators. The products run on 16x16x32 f16 MFMAs; an fp32 factor is two f16
 // limbs (22 bits) times a power of two - a row's for q, k and P T, a column's for
 // W, P T, the state and R - and a product is hi hi + hi lo + lo hi.

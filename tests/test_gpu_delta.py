@@ -332,3 +332,32 @@ def test_writes_stop_while_the_state_fades(ih):
         allowed = TOL * float(o[:, i:i + 8].norm()) + 2.0 ** -32 * 128 ** -0.5 * 8 ** 0.5 * float(size.norm())
         diff = float((out[:, i:i + 8].double().cpu() - o[:, i:i + 8]).norm())
         assert diff <= allowed, (i, diff, allowed)
+
+
+def test_two_calls_in_two_graphs(ih):
+    """A chunked call and one token by token, each captured with a workspace of its own, replayed beside each other."""
+    import torch
+    cases, graphs = [], []
+    for seed, t in ((53, 300), (59, 7)):
+        q, k, v, g, b, st = make(2, t, 2, 4, 128, 64, seed=seed)
+        o, _, last = R.delta(q, k, v, g, b, st)
+        ws = torch.empty(ih.gated_delta_rule_ws_bytes(2, t, 2, 4, 128, 64), dtype=torch.uint8, device="cuda")
+        out, new = torch.empty_like(v), torch.empty_like(st)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            ih.gated_delta_rule(q, k, v, g, b, st, new_state=new, out=out, ws=ws, stream=stream)
+        cases.append((o, last, out, new, (q, k, v, g, b, st, ws)))
+        graphs.append((graph, stream))
+    for turn in range(4):
+        for _, _, out, new, _ in cases:
+            out.fill_(3.0)
+            new.fill_(3.0)
+        torch.cuda.synchronize()
+        for graph, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, last, out, new, _ in cases:
+            check(out, o, ("o", turn))
+            check(new, last, ("state", turn))
