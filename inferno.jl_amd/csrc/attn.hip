@@ -597,13 +597,15 @@ constexpr int MOST_PARTS = 256;
 // 58.5, 57.5, 61.2; 1024, 4000, 8 (2^25) 105.5, 97.5, 99.3; 2048, 16000, 8 (2^28) 455, 361, 327; 2048, 1000, 2 (2^22) 51.6,
 // 44.2, 52.0. Of sequences' own entries (D = 64, bf16): 16 heads of 256 rows, 2064 keys 19.7, -, 28.9; 128 of 48 rows, 2012
 // keys 32.3, 25.9. D = 256 (blocks of 64, 128): 256 rows, 4000 keys, 2 heads (2^21) 25.6, 29.7; 16 heads of 256 rows, 2064 keys
-// (2^23) 59.6, 50.2. bf16 at D = 128 spills registers in blocks of 64: 1024 rows, 4000, 8 113, 117, 111.
+// (2^23) 59.6, 50.2. With what 256 rows leave empty counted (f16, D = 128, 32000 keys, 8 heads; blocks of 64, 256): 256 rows
+// 135, 112, 320 rows 174, 202, 640 rows 190, 172. bf16 at D = 128 spills registers in blocks of 64: 1024 rows, 4000, 8 113, 117, 111.
 int shape_for(const AttnArgs &a, int64_t rows, int64_t units, int64_t keys) {
     const double work = (double)rows * (double)units * (double)keys;
     if (a.head_dim == 256) return rows <= 64 || work <= 1 << 22 ? 1 : 2;
     const bool spills = a.head_dim == 128 && a.type == KV_BF16;
     if (rows <= (spills ? 64 : 32) || (rows <= 1024 && work <= 1 << 24 && (rows + 31) / 32 * units < 256)) return 0;
-    return !spills && (rows <= 64 || work <= 1 << 26) ? 1 : 2;
+    const bool padded = (rows + 255) / 256 * 256 * 3 > rows * 4;
+    return !spills && (rows <= 64 || work <= 3 << 24 || padded) ? 1 : 2;
 }
 int shape_rows(int D, int id) { return id == 0 ? 32 : id == 1 ? 64 : D == 256 ? 128 : 256; }
 
