@@ -126,6 +126,7 @@ __device__ __forceinline__ int pt_block(int t, int u) { return t < 2 ? t : t * 2
 
 // 2^e as a float, e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ int exponent(float p) { return (int)(__float_as_uint(p) >> 23) - 127; }  // of a power of two
 // 2^x by the one instruction (its argument rounded to fp32 costs |x| 2^-25, as expf's own would)
 __device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
 // exponent of the power of two that brings a largest absolute value to [2^top, 2^(top + 1)); 0 for 0 and non-finite
@@ -705,11 +706,21 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
                 for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[r][i]));
             return groups_max(most);
         };
+        auto scale_by = [&](int e) __attribute__((always_inline)) {  // (|e| up to 160: in two steps)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int x = h ? e - e / 2 : e / 2;
+                Sup *= pow2(x), Sdown *= pow2(-x);
+                S[0] *= pow2(x), S[1] *= pow2(x);
+            }
+        };
+        // (the power wanted is found whole and then kept to 2^-80 .. 2^80: a column may come from one end to the other)
         auto scale_state = [&](int c, float most) __attribute__((always_inline)) {
-            const int have = (int)(__float_as_uint(Sup) >> 23) - 127, want = have + lift(most, 11);  // (from -80 to 80 in all)
-            const int e = (want < -80 ? -80 : want > 80 ? 80 : want) - have;
-            Sup *= pow2(e), Sdown *= pow2(-e);
-            S[0] *= pow2(e), S[1] *= pow2(e);
+            const int b = (int)((__float_as_uint(most) >> 23) & 255);
+            if ((uint32_t)(b - 1) < 254u) {
+                const int have = exponent(Sup), want = have + 11 - (b - 127);
+                scale_by((want < -80 ? -80 : want > 80 ? 80 : want) - have);
+            }
             publish(c);
         };
 #pragma unroll
@@ -796,6 +807,12 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
                     *(f4 *)y = x[2 * u], *(f4 *)(y + 4) = x[2 * u + 1];
                     split8(y, Rup, l[u][0], l[u][1]);
                 }
+            }
+            // A column of a tiny state (a power up to 2^80) may meet a large write (times up to 2^80 again): its power is brought
+            // down first, so that down is at most 2^40 and the sum, with y below 2^37, far from fp32's end.
+            if (__any(!(Rdown * Sup <= 0x1p40f))) {
+                const int over = exponent(Rdown) + exponent(Sup) - 40;
+                scale_by(over > 0 ? -over : 0);
             }
             const float down = Rdown * Sup, grown = scal[c & 3][6 * CH];
             f4 y[2];
