@@ -563,14 +563,23 @@ int ihip_attn_prefix(const float *q_dev, int64_t ldq, float *out_dev,
  * were, and with 0 or less state_out is state_in. A g of -inf clears the state
  * before its token. A token with a value that is not finite spoils its own row
  * of o and, unless the value is q's, the later ones and the state of that head
- * (v's: of that column), no earlier row. All fp32, below 2^90 in size; n_seq
- * n_v dv / 16 up to 2^22. dk 64 or 128, dv a multiple of 4 up to 512; pointers
+ * (v's: of that column), no earlier row. All fp32. Sizes: v, the states and the
+ * terms of the sums above below 2^80; q and k below 2^40, with IHIP_DELTA_L2NORM
+ * below 2^90; beta k.k up to 2 (a write that overshoots by no more than what it
+ * corrects; beyond, the state grows with every token). n_seq n_v dv / 16 up to
+ * 2^22. dk 64 or 128, dv a multiple of 4 up to 512; pointers
  * 16-byte aligned (g and beta: 4), ld's multiples of 4 up to 2^24 (ldg, ldb:
  * any). o may not overlap the inputs. ws: ihip_delta_ws_bytes, 16-byte aligned,
  * not shared by calls that overlap in time. Few tokens (up to some dozens, by
  * the number of states; and every call with snapshots) go one by one; many go in
  * chunks of 64 on the matrix cores, where each chunk's tokens become one
- * triangular system (fp32 accuracy both ways). */
+ * triangular system. The first are fp32 throughout. In a chunk the factors are
+ * pairs of fp16 (22 bits) whose scale the largest of a token's row or of a
+ * column sets: o is off by about 2^-22 of its own terms and besides by about
+ * 2^-31 of the largest |q.k| |beta (v - S^T k)| that its chunk has in its
+ * column, that of a later token included; parts of the state below 2^-60 have
+ * fewer digits, and what decays by more than e^-80 inside a chunk may count as
+ * gone. */
 #define IHIP_DELTA_L2NORM 1
 typedef struct ihip_delta {
     const float *q, *k, *v, *g, *beta;

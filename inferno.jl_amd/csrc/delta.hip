@@ -5,6 +5,10 @@
 
 namespace {
 
+// What values whose squares leave fp32's range are multiplied by before they are squared, and l2norm's 1e-6 then: values up to
+// 2^90 come to 2^58, and what falls below fp32's range, squares of less than 2^-126, is nothing beside 2^-84.
+constexpr float UNDER = 0x1p-32f, UNDER_EPS = 1e-6f * 0x1p-64f;
+
 // Token by token: a wave holds 32 columns of one head's state, lane c + 8 g the
 // 4 columns 4c .. of rows [g DK / 8, (g + 1) DK / 8). With S the state before
 // the token, a = e^g and k, q of unit length where asked for:
@@ -39,23 +43,47 @@ template <int DK> __global__ __launch_bounds__(64) void delta_token_kernel(Delta
         for (int i = 0; i < R / 4; i++) *(f4 *)(k + 4 * i) = kp[i], *(f4 *)(q + 4 * i) = qp[i];
         const f4 v = in ? *(const f4 *)(a.v + row * a.ldv + (int64_t)hv * a.dv + c0) : f4{0, 0, 0, 0};
         const float decay = expf(a.g[row * a.ldg + hv]), beta = a.beta[row * a.ldb + hv];
-        f4 p = {0, 0, 0, 0}, r = {0, 0, 0, 0};
-        float kq = 0.f, kk = 0.f, qq = 0.f;
+        f4 p, r;
+        float kq, kk, qq;
+        auto sums = [&]() __attribute__((always_inline)) {
+            p = r = f4{0, 0, 0, 0};
+            kq = kk = qq = 0.f;
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            p += S[i] * k[i];
-            r += S[i] * q[i];
-            kq += k[i] * q[i];
-            kk += k[i] * k[i];
-            qq += q[i] * q[i];
+            for (int i = 0; i < R; i++) {
+                p += S[i] * k[i];
+                r += S[i] * q[i];
+                kq += k[i] * q[i];
+                kk += k[i] * k[i];
+                qq += q[i] * q[i];
+            }
+            for (int o = 8; o < 64; o <<= 1) {
+                for (int c = 0; c < 4; c++) p[c] += __shfl_xor(p[c], o), r[c] += __shfl_xor(r[c], o);
+                kq += __shfl_xor(kq, o);
+                kk += __shfl_xor(kk, o);
+                qq += __shfl_xor(qq, o);
+            }
+        };
+        sums();
+        float nk = 1.0f, nq = 1.0f;
+        if (a.l2norm) {
+            nk = 1.0f / sqrtf(kk + 1e-6f), nq = 1.0f / sqrtf(qq + 1e-6f);
+            if (__any(!(kk + qq <= 0x1p40f))) {
+                // so large that their squares or products may leave fp32's range: brought to unit length first, and taken again
+                float k2 = 0.f, q2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    k[i] *= UNDER, q[i] *= UNDER;
+                    k2 += k[i] * k[i];
+                    q2 += q[i] * q[i];
+                }
+                for (int o = 8; o < 64; o <<= 1) k2 += __shfl_xor(k2, o), q2 += __shfl_xor(q2, o);
+                nk = 1.0f / sqrtf(k2 + UNDER_EPS), nq = 1.0f / sqrtf(q2 + UNDER_EPS);
+#pragma unroll
+                for (int i = 0; i < R; i++) k[i] *= nk, q[i] *= nq;
+                sums();
+                nk = nq = 1.0f;
+            }
         }
-        for (int o = 8; o < 64; o <<= 1) {
-            for (int c = 0; c < 4; c++) p[c] += __shfl_xor(p[c], o), r[c] += __shfl_xor(r[c], o);
-            kq += __shfl_xor(kq, o);
-            kk += __shfl_xor(kk, o);
-            qq += __shfl_xor(qq, o);
-        }
-        const float nk = a.l2norm ? 1.0f / sqrtf(kk + 1e-6f) : 1.0f, nq = a.l2norm ? 1.0f / sqrtf(qq + 1e-6f) : 1.0f;
         const f4 u = beta * (v - (decay * nk) * p);
 #pragma unroll
         for (int i = 0; i < R; i++) S[i] = decay * S[i] + (k[i] * nk) * u;
@@ -269,7 +297,21 @@ template <int DK> __global__ __launch_bounds__(256, 2) void delta_prep_kernel(De
             }
             const int e = lift(most, 13);
             const float up = pow2(e);
-            if (part == 0) (m ? ck : cq)[r] = pow2(-e) * (a.l2norm ? 1.0f / sqrtf(sum + 1e-6f) : 1.0f);
+            float norm = a.l2norm ? 1.0f / sqrtf(sum + 1e-6f) : 1.0f;
+            if (a.l2norm && !is_finite(sum)) {  // (the row's four threads alike)
+                sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < U; i++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float y = x[m][i][j] * UNDER;
+                        sum = __builtin_fmaf(y, y, sum);
+                    }
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor(sum, o);
+                norm = UNDER / sqrtf(sum + UNDER_EPS);
+            }
+            if (part == 0) (m ? ck : cq)[r] = pow2(-e) * norm;
 #pragma unroll
             for (int i = 0; i < U; i++) {
                 h8 hi, lo;

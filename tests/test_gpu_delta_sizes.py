@@ -70,3 +70,50 @@ def test_a_large_state_is_cleared_for_small_writes(ih, dk):  # noqa: F811
     # (the first chunk's outputs are of the large state but for its last token's, which is not judged beside them)
     check_chunks(out[:, 64:], o[:, 64:], "o")
     check(new, last, "state")
+
+
+@pytest.mark.parametrize("t", [1, 5, 100])
+@pytest.mark.parametrize("keys,queries", [(2.0 ** 60, 1.0), (2.0 ** 64, 2.0 ** 64), (2.0 ** 70, 1.0), (1.0, 2.0 ** 75),
+                                          (2.0 ** 86, 2.0 ** 86), (2.0 ** 21, 2.0 ** -70)])
+@pytest.mark.parametrize("dk,state", [(64, 1.0), (128, 2.0 ** 40)])
+def test_norms_of_large_keys_and_queries(ih, t, keys, queries, dk, state):  # noqa: F811
+    """l2norm takes keys and queries whose squares, and products with each other and the state, leave fp32's range: what comes
+    of them is of ordinary size. (Random normal values below 16: 2^86 times them stay below 2^90.)"""
+    import torch
+    q, k, v, g, b, st = make(2, t, 2, 4, dk, 64, seed=73, unit=False, rate=0.05)
+    q.mul_(queries), k.mul_(keys), st.mul_(state)
+    o, _, last = R.delta(q, k, v, g, b, st, l2norm=True)
+    new = torch.empty_like(st)
+    check_chunks(ih.gated_delta_rule(q, k, v, g, b, st, new_state=new, l2norm=True), o, "o")
+    check(new, last, "state")
+
+
+@pytest.mark.parametrize("t", [5, 100])
+def test_one_large_key_among_ordinary_ones(ih, t):  # noqa: F811
+    """A single token's key and query past the range, tokens and heads beside them as without."""
+    import torch
+    q, k, v, g, b, st = make(2, t, 2, 4, 128, 64, seed=79, unit=False, rate=0.05)
+    plain = ih.gated_delta_rule(q, k, v, g, b, st, l2norm=True)
+    k[1, t // 2, 1] *= 2.0 ** 80
+    q[1, t // 2, 1] *= 2.0 ** 80
+    o, _, last = R.delta(q, k, v, g, b, st, l2norm=True)
+    new = torch.empty_like(st)
+    got = ih.gated_delta_rule(q, k, v, g, b, st, new_state=new, l2norm=True)
+    check(got, o, "o")
+    check(new, last, "state")
+    assert torch.equal(got[0], plain[0]) and torch.equal(got[1, :, :2], plain[1, :, :2])
+
+
+@pytest.mark.parametrize("t", [5, 100, 250])
+@pytest.mark.parametrize("values,states,keys,queries", [(75, 75, 0, 0), (75, -40, 0, 0), (-40, 75, 0, 0), (30, 30, 36, 36)])
+def test_sizes_up_to_the_limits(ih, t, values, states, keys, queries):  # noqa: F811
+    """v, state, keys and queries times these powers of two (beta such that beta k.k stays): all at their ends at once. Chunk 0 of
+    a small state beside large values and the other way round is a sum of both, judged by its norm. (Values of 2^75 with keys of
+    2^-40 and such a beta are beyond them: beta v is 2^155 and k (beta v) 2^115, the first of which no fp32 number holds.)"""
+    import torch
+    q, k, v, g, b, st = make(2, t, 2, 4, 128, 64, seed=83, rate=0.05)
+    v.mul_(2.0 ** values), st.mul_(2.0 ** states), k.mul_(2.0 ** keys), q.mul_(2.0 ** queries), b.mul_(2.0 ** (-2 * keys))
+    o, _, last = R.delta(q, k, v, g, b, st)
+    new = torch.empty_like(st)
+    check_chunks(ih.gated_delta_rule(q, k, v, g, b, st, new_state=new), o, "o")
+    check(new, last, "state")
