@@ -3,7 +3,7 @@
 //
 // For a key head, the rows of its query heads (all sequences' for the prefix,
 // one sequence's for its own entries) meet a range of keys in one workgroup:
-//   S^T = K Q^T, P^T = 2^(S^T c - m), O^T += V^T P^T
+//   S^T = K Q^T, P^T = 2^(S^T c - r), O^T += V^T P^T
 // on 16x16x32 MFMAs, 32 keys at a time. Transposed, a lane's accumulators of
 // S^T belong to one query row (lane & 15), so the running maximum and sum are a
 // number a lane, and they are already the B operand of the second product (its
@@ -46,7 +46,7 @@ template <> struct Kv<KV_F16> {
     typedef _Float16 t;
     typedef h8 v8;
     static constexpr int LIMBS = 2;
-    static constexpr float BIAS = 8.f;  // P is 2^BIAS too large: its second limb then reaches 2^-33 of a row's largest
+    static constexpr float BIAS = 8.f;  // the largest P is 2^BIAS: its second limb then reaches 2^-33 of a row's largest
     static __device__ __forceinline__ f4 mfma(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Kv<KV_BF16> {
@@ -260,11 +260,17 @@ __device__ __forceinline__ void attn_part(const AttnArgs &a, const AttnSplit &sp
         }
     }
 
+    // P is 2^(score - ref): ref is 2^BIAS below the row's largest score when it last moved. It is an fp32 number, used as it is
+    // by every P, by l and by the join, so that its rounding (8 below a score of 2^27 may be no fp32 number) has no effect.
     f4 o[RT][DT];
-    float m[RT], l[RT];
+    float ref[RT], l[RT];
+    auto ref_for = [](float top) __attribute__((always_inline)) {
+        const float r = top - X::BIAS;
+        return top - r > X::BIAS + 7.f ? top : r;  // (where it was rounded down by 8 or more P would not fit its type)
+    };
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-        m[t] = -__builtin_inff(), l[t] = 0.f;
+        ref[t] = -__builtin_inff(), l[t] = 0.f;
 #pragma unroll
         for (int d = 0; d < DT; d++) o[t][d] = f4{0, 0, 0, 0};
     }
@@ -363,15 +369,15 @@ __device__ __forceinline__ void attn_part(const AttnArgs &a, const AttnSplit &sp
             for (int t = 0; t < RT; t++) {
                 const f4 x = z[t][0], y = z[t][1];
                 top[t] = c[t] * fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
-                past |= top[t] > m[t] + 7.f;
+                past |= top[t] - ref[t] > X::BIAS + 7.f;  // (a difference of near numbers is exact, a sum with 7 is not)
             }
-            // the reference point moves only when a row's maximum passes it by 2^7 (P then still fits its type)
+            // the reference point moves only when a row's maximum passes it by 2^7 more (P then still fits its type)
             if (__any(past)) {
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    const float to = fmaxf(m[t], max_groups(top[t]));
-                    const float keep = m[t] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[t] - to);
-                    m[t] = to;
+                    const float to = fmaxf(ref[t], ref_for(max_groups(top[t])));
+                    const float keep = ref[t] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref[t] - to);
+                    ref[t] = to;
                     l[t] *= keep;
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[t][d] *= keep;
@@ -381,7 +387,7 @@ __device__ __forceinline__ void attn_part(const AttnArgs &a, const AttnSplit &sp
             float pf[RT][8];
 #pragma unroll
             for (int t = 0; t < RT; t++) {
-                const float off = m[t] == -__builtin_inff() ? 0.f : X::BIAS - m[t];
+                const float off = ref[t] == -__builtin_inff() ? 0.f : -ref[t];
 #pragma unroll
                 for (int i = 0; i < 8; i++) pf[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][i >> 2][i & 3], c[t], off));
                 l[t] += ((pf[t][0] + pf[t][1]) + (pf[t][2] + pf[t][3])) + ((pf[t][4] + pf[t][5]) + (pf[t][6] + pf[t][7]));
@@ -473,7 +479,7 @@ __device__ __forceinline__ void attn_part(const AttnArgs &a, const AttnSplit &sp
             const int r = r0 + t * 16 + col;
             if (r < sp.rows) {
                 const int64_t at = place(r);
-                if (g == 0) ml[at] = float2{m[t], l[t]};
+                if (g == 0) ml[at] = float2{ref[t], l[t]};
 #pragma unroll
                 for (int d = 0; d < DT; d++) *(f4 *)(opart + at * D + d * 16 + 4 * g) = o[t][d];
             }
@@ -485,7 +491,7 @@ __device__ __forceinline__ void attn_part(const AttnArgs &a, const AttnSplit &sp
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             const int r = t * 16 + col;
-            if (g == 0) wml[wave][r] = float2{m[t], l[t]};
+            if (g == 0) wml[wave][r] = float2{ref[t], l[t]};
 #pragma unroll
             for (int d = 0; d < DT; d++) meet[(wave * RT * 16 + r) * Q + ((d * 4 + g) ^ (r & 7))] = o[t][d];
         }
@@ -524,7 +530,7 @@ __global__ __launch_bounds__(512) void attn_part_kernel(AttnArgs a, AttnSplit pr
     else attn_part<TYPE, D, S, true>(a, own, (int)blockIdx.x - n_pre, lds, sh, opart, ml);
 }
 
-// The parts' results of a row, each times 2^(its maximum - the largest), over their sum: W waves a row, each taking every W-th
+// The parts' results of a row, each times 2^(its reference - the largest), over their sum: W waves a row, each taking every W-th
 // part, four loads in flight. Bound by reading the parts (256 rows of a tree, 256 wide, 64 parts: 67 MB). With W = 4 and 1
 // (us, the whole call, 8 heads of D = 128): 16 query heads and 4 parts 10.4, 10.2, 16 parts 11.1, 12.8; 1024 and 4 25.3, 24.1,
 // 16 31.7, 32.2: four from 9 parts on.
