@@ -528,13 +528,15 @@ int ihip_rope_append(const ihip_rope *rope, const float *qkv_dev, int64_t ld,
  * fp32 accuracy: the queries and probabilities meet the 16-bit cache as two
  * (f16) or three (bf16) limbs on the matrix cores, statistics and sums are
  * fp32. A row that sees nothing is zero. Entries a row does not see have no
- * effect on it, NaN and infinities included; a row that sees a non-finite
- * score or value gets a non-finite result there. A sequence with len_dev[s]
- * < 0 is idle (its rows of out stay as they were); one with len_dev[s] + M >
- * capacity gets NaN rows. Sums of p v are divided by the sum of p at the end:
- * |v| below 2^100. head_dim 64, 128 or 256; up to 2^22 query rows (n_seq M
- * n_q). q and out 16-byte aligned, ldq and ldo multiples of 4. Results do not depend on what runs beside the
- * call (no atomics). ws: ihip_attn_prefix_ws_bytes, 16-byte aligned, not
+ * effect on it, NaN and infinities included. A row that sees a value that is
+ * not finite, or a score of NaN or +inf, gets results that are not finite there;
+ * a key that is not finite gives NaN, or an infinite score of which -inf has no
+ * weight. Scores may be as large as fp32 holds (|scale q| below 2^127), |v| up to
+ * 2^100: sums of p v are divided by the sum of p at the end. A sequence with
+ * len_dev[s] < 0 is idle (its rows of out stay as they were); one with len_dev[s]
+ * + M > capacity gets NaN rows. head_dim 64, 128 or 256; up to 2^22 query rows
+ * (n_seq M n_q). q and out 16-byte aligned, ldq and ldo multiples of 4. Results
+ * do not depend on what runs beside the call (no atomics). ws: ihip_attn_prefix_ws_bytes, 16-byte aligned, not
  * shared by calls that overlap in time. Replaces the cached attention of
  * src/ModelCPU.jl:730-856 for the tokens of a verify step. */
 int ihip_attn_prefix_ws_bytes(int n_q, int M, const ihip_kv *cache,

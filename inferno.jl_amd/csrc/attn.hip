@@ -248,7 +248,7 @@ __device__ __forceinline__ void attn_part(const AttnArgs &a, const AttnSplit &sp
         if constexpr (TYPE == KV_F16) {  // the row's largest to [2^13, 2^14)
             top = max_groups(top);
             int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-            e = e < -100 ? -100 : e > 110 ? 110 : e;
+            e = e < -100 ? -100 : e > 127 ? 127 : e;  // (128: a row that is not finite)
             up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
             c[t] = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
         }

@@ -70,3 +70,14 @@ def test_scores_where_numbers_are_16_apart(ih, period, d, dtype, own):  # noqa: 
     check(*attend(ih, low, a, b, period, 65536, d, dtype, own, hide=True), wb=2.0 ** -16)
     if not own:  # (the new entry's score of 0 is then far above all others)
         assert bool((attend(ih, low, a, b, period, 65536, d, dtype, own)[0] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("exponent", [-120, -104, 100, 112, 118, 122])
+def test_queries_of_any_size(ih, exponent, dtype):  # noqa: F811
+    """Queries of 2^exponent over small keys: scores that fp32 holds, of which the larger takes everything (or, where they are
+    tiny, an equal share)."""
+    q, a, b = [2.0 ** exponent], [2.0 ** -9], [2.0 ** -10]
+    got, sa, sb, na, nb, size = attend(ih, q, a, b, 128, 8192, 64, dtype, False, hide=True)
+    check(got, sa, sb, na, nb, size, wb=0.0 if exponent > 0 else 1.0)
+    check(*attend(ih, q, [0.0], [0.0], 128, 8192, 64, dtype, False, hide=True), wb=1.0)
