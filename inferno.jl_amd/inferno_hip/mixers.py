@@ -8,13 +8,18 @@ They take the fp32 rows the matmuls of quantized_kernels leave and give fp32
 rows to the next matmul; lengths and states are read and written on the
 device, so that a step of them can be captured in a HIP graph between
 speculative.advance_len_ and speculative.commit_state_.
+
+Kernels run on `stream` (default: torch's current one). What a call allocates
+itself (out, ws) is made for that stream; its inputs have to be ready there,
+and other streams wait for it before they read its outputs. A workspace that is
+given serves one call at a time.
 """
 from __future__ import annotations
 
 import ctypes as C
 
 from . import _lib
-from .quantized_kernels import _ptr, _raw_stream, check_tensor
+from .quantized_kernels import _ptr, _raw_stream, check_tensor, made_for
 
 F16, BF16 = 1, 30
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BY_PARTS = 0, 1, 2
@@ -158,7 +163,7 @@ def rope(x, positions, n_heads: int, params: RopeParams, out=None, stream=None):
     xp, rows, ldx = _rows(x, "x", width, None, dev)
     pp = _whole(positions, "positions", _i32, (rows,), dev)
     if out is None:
-        out = x.new_empty((rows, width))
+        out = made_for(stream, x.new_empty, (rows, width))
     yp, _, ldy = _rows(out, "out", width, rows, dev)
     _lib.check(_call("ihip_rope_apply")(params._on(dev), xp, ldx, yp, ldy, n_heads, pp, rows, _on(stream, dev)))
     return out
@@ -182,7 +187,7 @@ def rope_append(qkv, n_q: int, cache: KVCache, lengths, params: RopeParams, posi
     lp = _whole(lengths, "lengths", _i32, (s,), dev)
     pp = None if positions is None else _whole(positions, "positions", _i32, (rows,), dev)
     if out is None:
-        out = qkv.new_empty((rows, n_q * d))
+        out = made_for(stream, qkv.new_empty, (rows, n_q * d))
     yp, _, ldq = _rows(out, "out", n_q * d, rows, dev)
     _lib.check(_call("ihip_rope_append")(params._on(dev), xp, ld, yp, ldq, n_q, cache._on(dev), lp, pp, pos0, rows // s,
                                          _on(stream, dev)))
@@ -216,10 +221,10 @@ def attn_prefix(q, n_q: int, cache: KVCache, lengths, prefix: KVCache | None = N
     lp = _whole(lengths, "lengths", _i32, (n,), dev)
     mp = None if tree_mask is None else _whole(tree_mask, "tree_mask", _i64, (n, m), dev)
     if out is None:
-        out = q.new_empty((rows, n_q * d))
+        out = made_for(stream, q.new_empty, (rows, n_q * d))
     op, _, ldo = _rows(out, "out", n_q * d, rows, dev)
     if ws is None:
-        ws = q.new_empty(attn_prefix_ws_bytes(n_q, m, cache, prefix), dtype=_u8)
+        ws = made_for(stream, q.new_empty, attn_prefix_ws_bytes(n_q, m, cache, prefix), dtype=_u8, returned=False)
     wp, wn = _workspace(ws, dev)
     _lib.check(_call("ihip_attn_prefix")(qp, ldq, op, ldo, n_q, m, cache._on(dev), lp,
                                          None if prefix is None else prefix._on(dev), mp,
@@ -281,7 +286,7 @@ def gated_delta_rule(q, k, v, g, beta, state, new_state=None, snapshots=None, le
     a.g, a.ldg = _heads(g, "g", s, t, n_v, 0, dev)
     a.beta, a.ldb = _heads(beta, "beta", s, t, n_v, 0, dev)
     if out is None:
-        out = v.new_empty((s, t, n_v, dv))
+        out = made_for(stream, v.new_empty, (s, t, n_v, dv))
     a.o, a.ldo = _heads(out, "out", s, t, n_v, dv, dev)
     if state is not None:
         a.state_in = _whole(state, "state", _f32, (s, n_v, dk, dv), dev)
@@ -292,7 +297,8 @@ def gated_delta_rule(q, k, v, g, beta, state, new_state=None, snapshots=None, le
     if lengths is not None:
         a.len = _whole(lengths, "lengths", _i32, (s,), dev)
     if ws is None:
-        ws = v.new_empty(gated_delta_rule_ws_bytes(s, t, n_k, n_v, dk, dv, snapshots is not None), dtype=_u8)
+        ws = made_for(stream, v.new_empty, gated_delta_rule_ws_bytes(s, t, n_k, n_v, dk, dv, snapshots is not None),
+                      dtype=_u8, returned=False)
     wp, wn = _workspace(ws, dev)
     a.n_seq, a.T, a.n_k, a.n_v, a.dk, a.dv = s, t, n_k, n_v, dk, dv
     a.scale = dk ** -0.5 if scale is None else scale

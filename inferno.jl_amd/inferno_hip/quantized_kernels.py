@@ -14,6 +14,7 @@ all M verify tokens against one pass over the weights.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -100,6 +101,34 @@ def _stream(stream=None) -> int:
             _raw = _raw_stream()
         return _raw(torch.cuda.current_device())
     return getattr(stream, "cuda_stream", stream)
+
+
+def working_on(stream):
+    """A context in which torch allocates for, fills on and waits for the
+    stream that a call was given (nothing changes for None or the current
+    one)."""
+    import torch
+    handle = None if stream is None else getattr(stream, "cuda_stream", stream)
+    if handle is None or handle == _stream():
+        return contextlib.nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(handle))
+
+
+def made_for(stream, make, *args, returned: bool = True, **kw):
+    """make(*args, **kw): a tensor for the kernels that a call launches on
+    `stream`. It is allocated on that stream: memory that the current stream
+    still reads is not taken for it, and its own is not given to the current
+    stream's next tensor while the kernels run. A tensor that goes back to the
+    caller is also recorded for the current stream, where it is likely read."""
+    if stream is None:
+        return make(*args, **kw)
+    import torch
+    there = working_on(stream)
+    with there:
+        t = make(*args, **kw)
+    if returned and not isinstance(there, contextlib.nullcontext):
+        t.record_stream(torch.cuda.current_stream())
+    return t
 
 
 def _ptr(t) -> int:
