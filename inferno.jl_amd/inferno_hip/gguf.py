@@ -102,7 +102,7 @@ class GGUFFile:
         """The tensor on the GPU as a uint8 tensor: GGUF bytes, or (packed) the
         layout of pack_weights for a 2-D Q4_K/Q5_K/Q6_K/Q8_0 matrix."""
         import torch
-        from .quantized_kernels import _stream, packed_bytes
+        from .quantized_kernels import _stream, made_for, packed_bytes
         info = self.tensors[name]
         if packed:
             if len(info.dimensions) > 2:
@@ -113,7 +113,7 @@ class GGUFFile:
         else:
             nb = info.nbytes
         if out is None:
-            out = torch.empty(max(nb, 1), dtype=torch.uint8, device="cuda")
+            out = made_for(stream, torch.empty, max(nb, 1), dtype=torch.uint8, device="cuda")
         _lib.check(self._L.ihip_gguf_upload(self._h, self.index(name), out.data_ptr(), out.numel(),
                                             1 if packed else 0, _stream(stream)))
         return out

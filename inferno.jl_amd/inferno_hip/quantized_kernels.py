@@ -177,12 +177,12 @@ def gemm_q(qtype: int, w_dev, x, n: int, k: int, flags: int = GEMM_AUTO, out=Non
     m = x.shape[0]
     _check_weights(qtype, w_dev, n, k, flags)
     if out is None:
-        out = torch.empty((m, n), dtype=torch.float32, device=x.device)
+        out = made_for(stream, torch.empty, (m, n), dtype=torch.float32, device=x.device)
     check_tensor(out, "out", torch.float32, (m, n))
     L = _lib.load()
     need = gemm_ws_bytes(qtype, m, n, k, flags)
     if ws is None:
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        ws = made_for(stream, torch.empty, need, dtype=torch.uint8, device=x.device, returned=False)
     check_tensor(ws, "ws", torch.uint8, min_numel=need)
     _lib.check(L.ihip_gemm_q(qtype, _ptr(w_dev), _ptr(x), _ptr(out), m, n, k, flags, _ptr(ws), ws.numel(),
                              _stream(stream)))
@@ -221,13 +221,13 @@ def gemm_q_ex(qtype: int, w_dev, x, n: int, k: int, act: int = ACT_PLAIN, norm_w
     if norm_w is not None:
         check_tensor(norm_w, "norm_w", torch.float32, min_numel=k)
     if out is None and not (flags & GEMM_DEFER):
-        out = torch.empty((m, n), dtype=torch.float32, device=dev)
+        out = made_for(stream, torch.empty, (m, n), dtype=torch.float32, device=dev)
     if out is not None:
         check_tensor(out, "out", torch.float32, (m, n))
     L = _lib.load()
     need = gemm_ws_bytes(qtype, m, n, k, flags)
     if ws is None:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = made_for(stream, torch.empty, need, dtype=torch.uint8, device=dev, returned=False)
     check_tensor(ws, "ws", torch.uint8, min_numel=need)
     gi = _lib.GemmInput(xp, ldx, act, None if norm_w is None else _ptr(norm_w), eps,
                         None if add is None else add[0], 0 if add is None else add[1],
@@ -355,7 +355,7 @@ def gemm_q_chain(qtype: int, w_packed, n: int, k: int, m: int, x=None, act: int 
                             0 if add is None else add[2])
     need = gemm_ws_bytes(qtype, m, n, k, GEMM_F32 | GEMM_PACKED)
     if ws is None:  # (zeroed: a K-split chained epilogue's per-tile counts start at zero)
-        ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+        ws = made_for(stream, torch.zeros, need, dtype=torch.uint8, device="cuda")
     check_tensor(ws, "ws", torch.uint8, min_numel=need)
     _lib.check(_lib.load().ihip_gemm_q_chain(qtype, _ptr(w_packed), None if gi is None else C.byref(gi),
                                              None if cin is None else C.byref(cin),
@@ -371,7 +371,8 @@ def pack_weights_gated(qtype: int, w_gate_up_dev, f: int, k: int, out=None, stre
     check_tensor(w_gate_up_dev, "w_gate_up_dev", torch.uint8,
                  min_numel=2 * f * (k // BLOCK_ELEMS[qtype]) * BLOCK_BYTES[qtype])
     if out is None:
-        out = torch.empty(packed_bytes(qtype, 2 * f, k), dtype=torch.uint8, device=w_gate_up_dev.device)
+        out = made_for(stream, torch.empty, packed_bytes(qtype, 2 * f, k), dtype=torch.uint8,
+                       device=w_gate_up_dev.device)
     _lib.check(_lib.load().ihip_pack_weights_gated(qtype, _ptr(w_gate_up_dev), _ptr(out), f, k, _stream(stream)))
     return out
 
@@ -394,7 +395,8 @@ def mlp_forward_(qt_gate_up: int, w_gate_up, qt_down: int, w_down, x, h: int, f:
         raise ValueError("x must be a contiguous float32 [M, h] tensor")
     m = x.shape[0]
     if ws is None:
-        ws = torch.empty(mlp_ws_bytes(qt_gate_up, qt_down, m, h, f, flags), dtype=torch.uint8, device=x.device)
+        ws = made_for(stream, torch.empty, mlp_ws_bytes(qt_gate_up, qt_down, m, h, f, flags), dtype=torch.uint8,
+                      device=x.device, returned=False)
     _lib.check(_lib.load().ihip_mlp_forward(qt_gate_up, _ptr(w_gate_up), qt_down, _ptr(w_down), _ptr(x),
                                             None if norm_w is None else _ptr(norm_w), eps, m, h, f, flags,
                                             _ptr(ws), ws.numel(), _stream(stream)))
@@ -434,7 +436,7 @@ def pack_weights(qtype: int, w_dev, n: int, k: int, out=None, stream=None):
     that gemm_q reads with GEMM_PACKED (done once, at model load)."""
     import torch
     if out is None:
-        out = torch.empty(packed_bytes(qtype, n, k), dtype=torch.uint8, device=w_dev.device)
+        out = made_for(stream, torch.empty, packed_bytes(qtype, n, k), dtype=torch.uint8, device=w_dev.device)
     _lib.check(_lib.load().ihip_pack_weights(qtype, _ptr(w_dev), _ptr(out), n, k, _stream(stream)))
     return out
 
@@ -442,7 +444,7 @@ def pack_weights(qtype: int, w_dev, n: int, k: int, out=None, stream=None):
 def dequant(qtype: int, w_dev, n_elems: int, stream=None):
     """Bit-exact fp32 dequantization of the first n_elems weights."""
     import torch
-    out = torch.empty(n_elems, dtype=torch.float32, device=w_dev.device)
+    out = made_for(stream, torch.empty, n_elems, dtype=torch.float32, device=w_dev.device)
     _lib.check(_lib.load().ihip_dequant(qtype, _ptr(w_dev), _ptr(out), n_elems, _stream(stream)))
     return out
 
@@ -452,7 +454,7 @@ def rmsnorm(x, eps: float = 1e-6, weight=None, out=None, stream=None):
     import torch
     if x.dim() == 1:
         x = x.view(1, -1)
-    out = torch.empty_like(x) if out is None else out
+    out = made_for(stream, torch.empty_like, x) if out is None else out
     wp = None if weight is None else _ptr(weight)
     _lib.check(_lib.load().ihip_rmsnorm(_ptr(x), wp, _ptr(out), x.shape[0], x.shape[1], eps, _stream(stream)))
     return out
@@ -462,7 +464,7 @@ def synth_blocks(qtype: int, stream_id: int, n_blocks: int, first_block: int = 0
     """Seeded GGUF blocks generated on the device (same bytes as synth.blocks)."""
     import torch
     if out is None:
-        out = torch.empty(n_blocks * BLOCK_BYTES[qtype], dtype=torch.uint8, device="cuda")
+        out = made_for(stream, torch.empty, n_blocks * BLOCK_BYTES[qtype], dtype=torch.uint8, device="cuda")
     _lib.check(_lib.load().ihip_synth_blocks(qtype, C.c_uint64(stream_id), first_block, n_blocks, _ptr(out),
                                              _stream(stream)))
     return out
@@ -471,7 +473,7 @@ def synth_blocks(qtype: int, stream_id: int, n_blocks: int, first_block: int = 0
 def synth_gaussian(stream_id: int, n: int, scale: float = 1.0, add=None, out=None, stream=None):
     import torch
     if out is None:
-        out = torch.empty(n, dtype=torch.float32, device="cuda")
+        out = made_for(stream, torch.empty, n, dtype=torch.float32, device="cuda")
     ap = None if add is None else _ptr(add)
     _lib.check(_lib.load().ihip_synth_gaussian(C.c_uint64(stream_id), n, scale, ap, _ptr(out), _stream(stream)))
     return out
@@ -482,7 +484,7 @@ def stream_read(buf, out=None, stream=None):
     read-bandwidth probe); returns the XOR sink (one word per workgroup)."""
     import torch
     if out is None:
-        out = torch.zeros(2048, dtype=torch.int32, device=buf.device)
+        out = made_for(stream, torch.zeros, 2048, dtype=torch.int32, device=buf.device)
     if out.numel() < 2048:
         raise ValueError("stream_read: out needs 2048 words")
     _lib.check(_lib.load().ihip_stream_read(_ptr(buf), buf.numel() // 16 * 16, _ptr(out), _stream(stream)))
@@ -493,7 +495,7 @@ def silu_mul(gu, f: int, out=None, stream=None):
     """silu(gate) * up for rows of gu = [gate | up] (src/ModelCPU.jl:447-473)."""
     import torch
     m = gu.shape[0]
-    out = torch.empty((m, f), dtype=torch.float32, device=gu.device) if out is None else out
+    out = made_for(stream, torch.empty, (m, f), dtype=torch.float32, device=gu.device) if out is None else out
     _lib.check(_lib.load().ihip_silu_mul(_ptr(gu), m, f, _ptr(out), _stream(stream)))
     return out
 

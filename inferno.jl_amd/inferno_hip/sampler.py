@@ -13,7 +13,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
-from .quantized_kernels import _ptr, _stream
+from .quantized_kernels import _ptr, _stream, made_for, working_on
 
 
 @_lib.kept_by_size
@@ -40,7 +40,7 @@ def softmax_sample(logits, u, temperature: float = 1.0, top_p: float = 1.0, top_
     if not u.is_cuda or u.dtype != torch.float32 or u.numel() < rows:
         raise ValueError("u must be a float32 GPU tensor with one uniform per row")
     if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        out = made_for(stream, torch.empty, rows, dtype=torch.int32, device=logits.device)
     elif not out.is_cuda or out.dtype != torch.int32 or out.numel() < rows:
         raise ValueError("out must be an int32 GPU tensor with one entry per row")
     if not spread:
@@ -49,7 +49,7 @@ def softmax_sample(logits, u, temperature: float = 1.0, top_p: float = 1.0, top_
         return out
     need = sample_ws_bytes(rows, V)
     if ws is None:
-        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        ws = made_for(stream, torch.empty, need, dtype=torch.uint8, device=logits.device, returned=False)
     elif not ws.is_cuda or ws.dtype != torch.uint8 or ws.numel() < need:
         raise ValueError(f"ws must be a uint8 GPU tensor of at least {need} bytes")
     _lib.check(_lib.load().ihip_sample_ex(_ptr(logits), rows, V, float(temperature), int(top_k), float(top_p),
@@ -67,7 +67,8 @@ def apply_penalties_(logits, token_ids, presence: float = 0.0, repetition: float
     if logits.dtype != torch.float32 or not logits.is_contiguous() or not logits.is_cuda:
         raise ValueError("logits must be a contiguous float32 GPU tensor")
     rows, V = logits.shape
-    ids = torch.as_tensor(token_ids).to(device=logits.device, dtype=torch.int32).contiguous()
+    with working_on(stream):
+        ids = torch.as_tensor(token_ids).to(device=logits.device, dtype=torch.int32).contiguous()
     n = ids.shape[-1] if ids.numel() else 0
     stride = 0 if ids.dim() == 1 else ids.stride(0)
     if ids.dim() == 2 and ids.shape[0] != rows:

@@ -15,15 +15,15 @@ import ctypes as C
 from dataclasses import dataclass
 
 from . import _lib
-from .quantized_kernels import _ptr, _stream, check_tensor
+from .quantized_kernels import _ptr, _stream, check_tensor, made_for, working_on
 
 MODE_STANDARD = 0   # p, q at temperature T; residual max(0, p - q)
 MODE_REFERENCE = 1  # src/SpeculativeDecoding.jl:61-63,79-93 as written
 
 
-def _ws(nbytes: int, device):
+def _ws(nbytes: int, device, stream):
     import torch
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    return made_for(stream, torch.empty, max(nbytes, 16), dtype=torch.uint8, device=device, returned=False)
 
 
 # (Workspace sizes: functions of their numbers alone, asked once a shape.)
@@ -46,9 +46,8 @@ def softmax_stats(logits, temperature: float, stream=None):
     import torch
     rows, V = logits.shape
     L = _lib.load()
-    ws = _ws(_accept_ws_bytes(rows, V), logits.device)
-    zmax = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    zsum = torch.empty_like(zmax)
+    ws = _ws(_accept_ws_bytes(rows, V), logits.device, stream)
+    zmax, zsum = (made_for(stream, torch.empty, rows, dtype=torch.float32, device=logits.device) for _ in range(2))
     _lib.check(L.ihip_softmax_stats(_ptr(logits), rows, V, temperature, _ptr(zmax), _ptr(zsum), _ptr(ws),
                                     ws.numel(), _stream(stream)))
     return zmax, zsum
@@ -92,12 +91,12 @@ def spec_accept(target_logits, draft_logits, draft_tokens, temperature: float, u
     need = _spec_accept_ws_bytes(S, k, V, top_k, float(top_p), float(min_p))
     dev = target_logits.device
     if ws is None:
-        ws = _ws(need, dev)
+        ws = _ws(need, dev, stream)
     check_tensor(ws, "ws", torch.uint8, min_numel=need)
     if out_tok is None:
-        out_tok = torch.zeros((S, k + 1), dtype=torch.int32, device=dev)
+        out_tok = made_for(stream, torch.zeros, (S, k + 1), dtype=torch.int32, device=dev)
     if out_n is None:
-        out_n = torch.zeros(S, dtype=torch.int32, device=dev)
+        out_n = made_for(stream, torch.zeros, S, dtype=torch.int32, device=dev)
     check_tensor(out_tok, "out_tok", torch.int32, (S, k + 1))
     check_tensor(out_n, "out_n", torch.int32, (S,))
     _lib.check(L.ihip_spec_accept_ex(_ptr(target_logits), _ptr(draft_logits), _ptr(draft_tokens), S, k, V,
@@ -129,9 +128,9 @@ def greedy_verify(logits, draft_tokens, stream=None):
     k = k1 - 1
     check_tensor(draft_tokens, "draft_tokens", torch.int32, (S, k))
     L = _lib.load()
-    ws = _ws(_accept_ws_bytes(S * k1, V), logits.device)
-    out_n = torch.empty(S, dtype=torch.int32, device=logits.device)  # (both written in full)
-    am = torch.empty((S, k1), dtype=torch.int32, device=logits.device)
+    ws = _ws(_accept_ws_bytes(S * k1, V), logits.device, stream)
+    out_n = made_for(stream, torch.empty, S, dtype=torch.int32, device=logits.device)  # (both written in full)
+    am = made_for(stream, torch.empty, (S, k1), dtype=torch.int32, device=logits.device)
     _lib.check(L.ihip_greedy_verify(_ptr(logits), _ptr(draft_tokens) if k else None, S, k, V, _ptr(out_n),
                                     _ptr(am), _ptr(ws), ws.numel(), _stream(stream)))
     return out_n, am
@@ -142,7 +141,8 @@ def mtp_verify_step(logits, draft_tokens, stream=None):
     the verify forward: rows 0..k for tokens [last, d_1..d_k]; draft_tokens
     are d_1..d_k. Returns (accepted_count, logits)."""
     n, _ = greedy_verify(logits, draft_tokens, stream)
-    return int(n[0].item()), logits
+    with working_on(stream):  # (waits for that stream)
+        return int(n[0].item()), logits
 
 
 def tree_accept(target_logits, draft_logits, node_tokens, parent, temperature: float, u, stream=None):
@@ -158,13 +158,15 @@ def tree_accept(target_logits, draft_logits, node_tokens, parent, temperature: f
     check_tensor(parent, "parent", torch.int32, (n,))
     check_tensor(u, "u", torch.float32, (n,))
     L = _lib.load()
-    ws = _ws(_accept_ws_bytes(3 * n, V), target_logits.device)
-    path = torch.empty(n, dtype=torch.int32, device=target_logits.device)  # (written up to the length)
-    ln = torch.empty(1, dtype=torch.int32, device=target_logits.device)
+    ws = _ws(_accept_ws_bytes(3 * n, V), target_logits.device, stream)
+    # (written up to the length)
+    path = made_for(stream, torch.empty, n, dtype=torch.int32, device=target_logits.device)
+    ln = made_for(stream, torch.empty, 1, dtype=torch.int32, device=target_logits.device, returned=False)
     _lib.check(L.ihip_tree_accept(_ptr(target_logits), _ptr(draft_logits), _ptr(node_tokens), _ptr(parent), n, V,
                                   temperature, _ptr(u), _ptr(path), _ptr(ln), _ptr(ws), ws.numel(),
                                   _stream(stream)))
-    n_path = int(ln.item())
+    with working_on(stream):  # (waits for that stream)
+        n_path = int(ln.item())
     if n_path < 0:
         raise ValueError("tree_accept: malformed tree (parent[i] must lie in [0, i), tokens in [0, V))")
     return path[:n_path]

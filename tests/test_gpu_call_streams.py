@@ -78,3 +78,33 @@ def test_the_default_stream_from_another(ih):  # noqa: F811
             s.synchronize()
             assert torch.equal(read, want)
     torch.cuda.synchronize()
+
+
+def test_accept_and_matmul_beside_the_current_stream(ih):  # noqa: F811
+    """The other wrappers: a matmul and an accept step, and a count that is waited for on its own stream."""
+    import torch
+    F = ih.formats
+    n, k = 512, 1024
+    w = ih.quantized_kernels.synth_blocks(F.Q4_K, 11, n * k // F.BLOCK_ELEMS[F.Q4_K])
+    x = torch.randn(5, k, device="cuda")
+    logits = torch.randn(3, 5, 9000, device="cuda")
+    tok = logits.argmax(-1).int()[:, :4].contiguous()
+    tok[1, 2] = 5
+    want, (count, am) = ih.gemm_q(F.Q4_K, w, x, n, k), ih.greedy_verify(logits, tok)
+    assert count.tolist()[0] == 4 and count.tolist()[1] <= 2
+    nb = ih.quantized_kernels.gemm_ws_bytes(F.Q4_K, 5, n, k)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(WAIT)
+        y = ih.gemm_q(F.Q4_K, w, x, n, k, stream=s)
+        c, a = ih.greedy_verify(logits, tok, stream=s)
+        others = crowd([(nb,), (5 * n * 4,), (12,), (60,)])
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(y, want) and torch.equal(c, count) and torch.equal(a, am)
+        assert all(bool((t == 255).all()) for t in others)
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(WAIT)
+        assert ih.mtp_verify_step(logits, tok, stream=s)[0] == 4
+        del y, c, a, others
