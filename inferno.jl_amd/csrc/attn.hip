@@ -530,6 +530,9 @@ __global__ __launch_bounds__(512) void attn_part_kernel(AttnArgs a, AttnSplit pr
     else attn_part<TYPE, D, S, true>(a, own, (int)blockIdx.x - n_pre, lds, sh, opart, ml);
 }
 
+// Ranges of keys that a prefix and a sequence's own entries are cut into at most.
+constexpr int MOST_PRE = 128, MOST_OWN = 64;
+
 // The parts' results of a row, each times 2^(its reference - the largest), over their sum: W waves a row, each taking every W-th
 // part, four loads in flight. Bound by reading the parts (256 rows of a tree, 256 wide, 64 parts: 67 MB). With W = 4 and 1
 // (us, the whole call, 8 heads of D = 128): 16 query heads and 4 parts 10.4, 10.2, 16 parts 11.1, 12.8; 1024 and 4 25.3, 24.1,
@@ -537,7 +540,7 @@ __global__ __launch_bounds__(512) void attn_part_kernel(AttnArgs a, AttnSplit pr
 template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int parts, const float *__restrict__ opart,
                                                                               const float2 *__restrict__ ml) {
     constexpr int E = D / 64, ROWS = 4 / W, LANES = W * 64;
-    __shared__ float weight[ROWS][256];
+    __shared__ float weight[ROWS][MOST_PRE + MOST_OWN];
     __shared__ float4 red[4][64];
     __shared__ float tops[4], sums[4];
     typedef float ve __attribute__((ext_vector_type(E)));
@@ -594,8 +597,6 @@ template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(
 
 // ---- launch shapes ----
 
-constexpr int MOST_PARTS = 256;
-
 // The shape for `rows` query rows that meet `keys` keys in each of `units` heads (of sequences), and its rows a block. Blocks
 // of 32 rows are the quickest to finish, and where they are many take the fewest ranges of keys, whose results cost a pass of
 // their own; blocks of 64 and 256 (D = 256: 64 and 128) read less LDS for a product. Measured over a prefix in 2 or 8 heads
@@ -636,7 +637,7 @@ AttnPlan plan_of(const AttnArgs &a) {
     p.own.blocks = (int)((own_rows + own_block - 1) / own_block);
     const int64_t units = (int64_t)p.own.blocks * a.n_kv * a.n_seq;
     int64_t splits = (a.P > 0 ? 128 : 256) / units;
-    splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
+    splits = splits < 1 ? 1 : splits > MOST_OWN ? MOST_OWN : splits;
     const int64_t most = (a.capacity + 127) / 128;
     p.own.splits = (int)(splits < most ? splits : most);
     p.pre_shape = p.own_shape;
@@ -649,7 +650,7 @@ AttnPlan plan_of(const AttnArgs &a) {
         p.pre.blocks = (int)((rows + block - 1) / block);
         const int64_t beside = units * p.own.splits, room = beside <= 128 ? 256 - beside : 256;
         int64_t n = room / ((int64_t)p.pre.blocks * a.n_kv);
-        n = n < 1 ? 1 : n > 128 ? 128 : n;
+        n = n < 1 ? 1 : n > MOST_PRE ? MOST_PRE : n;
         const int64_t top = (a.P + 127) / 128;
         n = n < top ? n : top;
         p.pre.per = ((a.P + n - 1) / n + 31) / 32 * 32;
@@ -702,7 +703,6 @@ size_t attn_ws(const AttnArgs &a) {
 
 hipError_t launch_attn(const AttnArgs &a, void *ws, hipStream_t st) {
     const AttnPlan p = plan_of(a);
-    if (p.parts > MOST_PARTS) return hipErrorInvalidValue;
     if (a.type == KV_F16)
         return a.head_dim == 64    ? launch_all<KV_F16, 64>(a, p, ws, st)
                : a.head_dim == 128 ? launch_all<KV_F16, 128>(a, p, ws, st)
