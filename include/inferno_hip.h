@@ -473,7 +473,9 @@ typedef struct ihip_kv {
  *     the model was trained on; keep = clamp((r - beta_slow) / (beta_fast -
  *     beta_slow), 0, 1); theta_i' = theta_i (keep + (1 - keep) / factor).
  * freq_factors_dev (a device array [rot_dim / 2], NULL: none; a GGUF file's
- * rope_freqs) divides each theta_i; not with IHIP_ROPE_BY_PARTS.
+ * rope_freqs) divides each theta_i; not with IHIP_ROPE_BY_PARTS. A ramp that is
+ * linear in the pair's index instead of its turns is given by them, as
+ * theta_i / theta_i' with IHIP_ROPE_PLAIN.
  * Angles are formed in fp64 and reduced to a turn before sine and cosine, so
  * far positions lose nothing. ihip_rope_init fills the caller's ihip_rope
  * (host memory, kept with the model; no GPU work); the calls below copy it
@@ -553,7 +555,9 @@ int ihip_attn_prefix(const float *q_dev, int64_t ldq, float *out_dev,
  *   S  = exp(g_t) S
  *   S += k_t (beta_t (v_t - S^T k_t))^T
  *   o_t = scale S^T q_t
- * with the q and k of key head h / (n_v / n_k); with IHIP_DELTA_L2NORM q and k
+ * with the q and k of key head h / (n_v / n_k) (value heads that a checkpoint
+ * keeps in another order, h mod n_k, are put in this one with their weights);
+ * with IHIP_DELTA_L2NORM q and k
  * are first divided by sqrt(sum x^2 + 1e-6). Row s T + t holds token t of
  * sequence s: heads of dk (q, k) or dv (v, o) values, ldq .. ldo values
  * between rows; g and beta one value a head, ldg and ldb between rows. The

@@ -21,14 +21,16 @@
 //
 // What bounds it, and what it measured (the parts, then the join):
 //   64 sequences of 5 tokens, 32 query heads over 8 of 128, 16384 shared f16
-//     entries: the matrix cores, 186 + 10 us; the limbs' products are 176 GFLOP,
-//     0.95 PFLOP/s (a large f16 matrix product reaches 1.17 here), the softmax
-//     between them is most of the rest;
+//     entries: the matrix cores and the vector work between their products, 186
+//     + 10 us; the limbs' products are 176 GFLOP, 0.95 PFLOP/s (a large f16
+//     matrix product reaches 1.17 here), and 4 vector instructions (softmax,
+//     limbs) go with each MFMA, two waves a SIMD: about as long to issue;
 //   one row of each of 32 query heads over 131072 entries: reading them, 537 MB
 //     in 101 + 4 us, 5.3 TB/s;
 //   a tree of 64 nodes, 16 query heads over 4 of 256, 6001 bf16 entries: 31 + 7
 //     us: three limbs' products at half their rate, and 30 MB of parts written
-//     and read (1024 rows of 256 values for each of 28 ranges of keys);
+//     and read (1024 rows of 256 values for each of 27 ranges of keys, 24 of them
+//     the prefix's);
 //   9 sequences of 5 tokens over 4099 bf16 entries of 64: 11 + 4 us, and one row
 //     over 777 entries: 7 + 4 us: two launches, a few tiles one after the other.
 #include "common.h"
@@ -457,7 +459,8 @@ __device__ __forceinline__ void attn_part(const AttnArgs &a, const AttnSplit &sp
                 __syncthreads();
             }
         }
-        // (the last tiles' loads and stores of a tile that is not there repeat the first: no branch, no use)
+        // (the last tiles' loads and stores of a tile that is not there repeat the first: no branch, but a range of one tile
+        // waits for such a load before its products)
         const int64_t k1 = k0 + KB < end ? k0 + KB : begin, k2 = k0 + 2 * KB < end ? k0 + 2 * KB : begin;
 #pragma unroll
         for (int part = 0; part < ST; part++) {
@@ -599,13 +602,15 @@ template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(
 
 // The shape for `rows` query rows that meet `keys` keys in each of `units` heads (of sequences), and its rows a block. Blocks
 // of 32 rows are the quickest to finish, and where they are many take the fewest ranges of keys, whose results cost a pass of
-// their own; blocks of 64 and 256 (D = 256: 64 and 128) read less LDS for a product. Measured over a prefix in 2 or 8 heads
-// (us: blocks of 32, 64, 256; f16, D = 128): 256 rows, 4000 keys, 2 heads (2^21) 16.2, 19.6, 25.6; 512 rows, 4000, 8 (2^24)
+// their own; blocks of 64 and 256 (D = 256: 64 and 128) read less LDS for a product. Measured over a prefix in 2 or 8 heads,
+// rows / 4 sequences of one token and 4 query heads a key head, with 20 own entries each, whose workgroups (1024 rows, 8 heads:
+// 2048) are in the times (us: blocks of 32, 64, 256; f16, D = 128): 256 rows, 4000 keys, 2 heads (2^21) 16.2, 19.6, 25.6; 512 rows, 4000, 8 (2^24)
 // 58.5, 57.5, 61.2; 1024, 4000, 8 (2^25) 105.5, 97.5, 99.3; 2048, 16000, 8 (2^28) 455, 361, 327; 2048, 1000, 2 (2^22) 51.6,
 // 44.2, 52.0. Of sequences' own entries (D = 64, bf16): 16 heads of 256 rows, 2064 keys 19.7, -, 28.9; 128 of 48 rows, 2012
 // keys 32.3, 25.9. D = 256 (blocks of 64, 128): 256 rows, 4000 keys, 2 heads (2^21) 25.6, 29.7; 16 heads of 256 rows, 2064 keys
-// (2^23) 59.6, 50.2. With what 256 rows leave empty counted (f16, D = 128, 32000 keys, 8 heads; blocks of 64, 256): 256 rows
-// 135, 112, 320 rows 174, 202, 640 rows 190, 172. bf16 at D = 128 spills registers in blocks of 64: 1024 rows, 4000, 8 113, 117, 111.
+// (2^23) 59.6, 50.2. With what 256 rows leave empty counted (f16, D = 128, 32000 keys, 8 heads; one sequence of 64 tokens, 16 and 32 of
+// 5, 300 own entries each; blocks of 64, 256): 256 rows 135, 112, 320 rows 174, 202, 640 rows 190, 172. Sizes between these were not
+// measured. bf16 at D = 128 spills registers in blocks of 64: 1024 rows, 4000, 8 113, 117, 111.
 int shape_for(const AttnArgs &a, int64_t rows, int64_t units, int64_t keys) {
     const double work = (double)rows * (double)units * (double)keys;
     if (a.head_dim == 256) return rows <= 64 || work <= 1 << 22 ? 1 : 2;
@@ -626,7 +631,8 @@ struct AttnPlan {
 // that beside a prefix. The prefix: as many ranges (of 128 keys or more) as fill the chip beside them, or once over where they
 // are many. Half and all of the chip for the own entries (us, 8 heads of D = 128, 4 rows a token, 1024 to 4096 entries of
 // capacity): 4 sequences of 5 tokens, 777 shared entries 14.4, 21.0; 8, 1500 17.7, 23.6; 9, 4099 25.7, 29.8; 16 of one token,
-// 8000 23.5, 27.8; 16 of 5, 8000 55, 49. Ranges of 128 and of 64: one row a head over 777 entries 10.6, 11.1, at D = 256 over
+// 8000 23.5, 27.8; 16 of 5, 8000 55, 49. The host knows capacities, not lengths: a cache with room to spare gives its own entries
+// ranges that are empty, and the prefix as many workgroups fewer. Ranges of 128 and of 64: one row a head over 777 entries 10.6, 11.1, at D = 256 over
 // 3000 14.8, 17.0.
 AttnPlan plan_of(const AttnArgs &a) {
     AttnPlan p{};

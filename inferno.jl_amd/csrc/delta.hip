@@ -17,7 +17,7 @@ constexpr float UNDER = 0x1p-32f, UNDER_EPS = 1e-6f * 0x1p-64f;
 // Bound by the states' bytes where there are many (16 sequences of 5 tokens, 32
 // heads of 128 x 128, the state after every token kept: 205 MB in 37.3 us, 5.5
 // TB/s), by one pass of loads, sums over the row groups and stores for one token
-// of one sequence: 4.7 us.
+// of one sequence: 4.8 us.
 template <int DK> __global__ __launch_bounds__(64) void delta_token_kernel(DeltaArgs a) {
     constexpr int R = DK / 8;
     const int lane = threadIdx.x, g = lane >> 3;
@@ -89,7 +89,8 @@ template <int DK> __global__ __launch_bounds__(64) void delta_token_kernel(Delta
         for (int i = 0; i < R; i++) S[i] = decay * S[i] + (k[i] * nk) * u;
         if (in && g == 0)
             *(f4 *)(a.o + row * a.ldo + (int64_t)hv * a.dv + c0) = (a.scale * nq) * (decay * r + (kq * nk) * u);
-        if (in && a.snap) {  // (past the caches: they would only push each other out; 46.4 us through them, 37.3 so)
+        if (in && a.snap) {  // (past the caches: 165 MB would only push each other out, 46.4 us through them, 37.5 so; a few MB,
+                                // which what commits one of them could find there, were not timed)
             float *to = a.snap + (row * a.n_v + hv) * DK * a.dv + mine;
 #pragma unroll
             for (int i = 0; i < R; i++) __builtin_nontemporal_store(S[i], (f4 *)(to + (int64_t)i * a.dv));
@@ -1007,7 +1008,7 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
     }
 }
 
-// Chunks where no snapshots are asked for and there are tokens enough: a chunk costs as much with one token as with 64, the
+// Chunks where no snapshots are asked for and there are tokens enough (sizes between the measured ones follow their line): a chunk costs as much with one token as with 64, the
 // recurrence as many times more as there are tokens. Where the two meet, by the number of 16-column groups there are to carry,
 // in microseconds (recurrence, chunks) at dk = dv = 128, 32 heads: 1 sequence (256 groups) 16 tokens 22.9, 19.3; 4 (1024)
 // 20 tokens 31.6, 34.9 and 24 tokens 37.0, 35; 16 (4096) 40 tokens 78, 87 and 64 tokens 118, 89. dk = dv = 64, 16 heads: 1

@@ -143,7 +143,7 @@ hipError_t launch_rope(const RopeArgs &a, const RopeTable &tab, int64_t rows, bo
     if (split > 8) split = 8;
     const dim3 grid((unsigned)rows, (unsigned)(split < 1 ? 1 : split));
     // past the caches from 32 MB of rows on, what the eight L2s hold: 8190 rows of 201 MB 73.5 us, 77.5 through them (fewer are
-    // read again by what comes next)
+    // read again by what comes next; timed by itself, at this size, not with the projection before it and the attention behind)
     const bool stream = rows * units * per * 4 >= (int64_t)32 << 20;
     if (vec && stream) rope_kernel<4, true><<<grid, 256, 0, st>>>(a, tab);
     else if (vec) rope_kernel<4, false><<<grid, 256, 0, st>>>(a, tab);

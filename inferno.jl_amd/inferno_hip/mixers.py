@@ -269,8 +269,9 @@ def gated_delta_rule(q, k, v, g, beta, state, new_state=None, snapshots=None, le
     with unit q and k where l2norm is set. new_state receives the last state
     (may be `state`), snapshots [sequences, T, n_v, dk, dv] the state after
     every token (T <= 64; commit_state_ picks from them). lengths int32
-    [sequences]: tokens of each, rows past them left as they were. Returns
-    out [sequences, T, n_v, dv]."""
+    [sequences]: tokens of each, rows past them left as they were. Value head
+    h reads key head h // (n_v // n_k). out overlaps none of the inputs.
+    Returns out [sequences, T, n_v, dv]."""
     if _f32 is None:
         _torch()
     dev = _device_of(q, "q")
