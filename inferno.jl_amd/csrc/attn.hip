@@ -604,13 +604,14 @@ template <int D, int W> __global__ __launch_bounds__(256) void attn_join_kernel(
 // of 32 rows are the quickest to finish, and where they are many take the fewest ranges of keys, whose results cost a pass of
 // their own; blocks of 64 and 256 (D = 256: 64 and 128) read less LDS for a product. Measured over a prefix in 2 or 8 heads,
 // rows / 4 sequences of one token and 4 query heads a key head, with 20 own entries each, whose workgroups (1024 rows, 8 heads:
-// 2048) are in the times (us: blocks of 32, 64, 256; f16, D = 128): 256 rows, 4000 keys, 2 heads (2^21) 16.2, 19.6, 25.6; 512 rows, 4000, 8 (2^24)
-// 58.5, 57.5, 61.2; 1024, 4000, 8 (2^25) 105.5, 97.5, 99.3; 2048, 16000, 8 (2^28) 455, 361, 327; 2048, 1000, 2 (2^22) 51.6,
-// 44.2, 52.0. Of sequences' own entries (D = 64, bf16): 16 heads of 256 rows, 2064 keys 19.7, -, 28.9; 128 of 48 rows, 2012
-// keys 32.3, 25.9. D = 256 (blocks of 64, 128): 256 rows, 4000 keys, 2 heads (2^21) 25.6, 29.7; 16 heads of 256 rows, 2064 keys
-// (2^23) 59.6, 50.2. With what 256 rows leave empty counted (f16, D = 128, 32000 keys, 8 heads; one sequence of 64 tokens, 16 and 32 of
-// 5, 300 own entries each; blocks of 64, 256): 256 rows 135, 112, 320 rows 174, 202, 640 rows 190, 172. Sizes between these were not
-// measured. bf16 at D = 128 spills registers in blocks of 64: 1024 rows, 4000, 8 113, 117, 111.
+// 2048) are in the times (us: blocks of 32, 64, 256; f16, D = 128): 256 rows, 4000 keys, 2 heads (2^21) 16.2, 19.6, 25.6; 512
+// rows, 4000, 8 (2^24) 58.5, 57.5, 61.2; 1024, 4000, 8 (2^25) 105.5, 97.5, 99.3; 2048, 16000, 8 (2^28) 455, 361, 327; 2048,
+// 1000, 2 (2^22) 51.6, 44.2, 52.0. Of sequences' own entries (D = 64, bf16): 16 heads of 256 rows, 2064 keys 19.7, -, 28.9; 128
+// of 48 rows, 2012 keys 32.3, 25.9. D = 256 (blocks of 64, 128): 256 rows, 4000 keys, 2 heads (2^21) 25.6, 29.7; 16 heads of
+// 256 rows, 2064 keys (2^23) 59.6, 50.2. With what 256 rows leave empty counted (f16, D = 128, 32000 keys, 8 heads; one
+// sequence of 64 tokens, 16 and 32 of 5, 300 own entries each; blocks of 64, 256): 256 rows 135, 112, 320 rows 174, 202, 640
+// rows 190, 172. Sizes between these were not measured. bf16 at D = 128 spills registers in blocks of 64: 1024 rows, 4000, 8
+// 113, 117, 111.
 int shape_for(const AttnArgs &a, int64_t rows, int64_t units, int64_t keys) {
     const double work = (double)rows * (double)units * (double)keys;
     if (a.head_dim == 256) return rows <= 64 || work <= 1 << 22 ? 1 : 2;
@@ -626,14 +627,14 @@ struct AttnPlan {
     int parts, pre_shape, own_shape;
 };
 
-// One workgroup fills a CU. The sequences' own entries: ranges of 128 keys or more, up to 256 workgroups (5 tokens, 4 heads of 4
-// rows each, D = 128: 16 sequences of 4000 entries 29.5 us, 56.9 unsplit, 38.0 with up to 512; 4 of 200 12.7, 13.1, 21.3), half
-// that beside a prefix. The prefix: as many ranges (of 128 keys or more) as fill the chip beside them, or once over where they
-// are many. Half and all of the chip for the own entries (us, 8 heads of D = 128, 4 rows a token, 1024 to 4096 entries of
+// One workgroup fills a CU. The sequences' own entries: ranges of 128 keys or more, up to 256 workgroups (5 tokens, 4 heads of
+// 4 rows each, D = 128: 16 sequences of 4000 entries 29.5 us, 56.9 unsplit, 38.0 with up to 512; 4 of 200 12.7, 13.1, 21.3),
+// half that beside a prefix. The prefix: as many ranges (of 128 keys or more) as fill the chip beside them, or once over where
+// they are many. Half and all of the chip for the own entries (us, 8 heads of D = 128, 4 rows a token, 1024 to 4096 entries of
 // capacity): 4 sequences of 5 tokens, 777 shared entries 14.4, 21.0; 8, 1500 17.7, 23.6; 9, 4099 25.7, 29.8; 16 of one token,
-// 8000 23.5, 27.8; 16 of 5, 8000 55, 49. The host knows capacities, not lengths: a cache with room to spare gives its own entries
-// ranges that are empty, and the prefix as many workgroups fewer. Ranges of 128 and of 64: one row a head over 777 entries 10.6, 11.1, at D = 256 over
-// 3000 14.8, 17.0.
+// 8000 23.5, 27.8; 16 of 5, 8000 55, 49. The host knows capacities, not lengths: a cache with room to spare gives its own
+// entries ranges that are empty, and the prefix as many workgroups fewer. Ranges of 128 and of 64: one row a head over 777
+// entries 10.6, 11.1, at D = 256 over 3000 14.8, 17.0.
 AttnPlan plan_of(const AttnArgs &a) {
     AttnPlan p{};
     const int64_t G = a.n_q / a.n_kv, own_rows = a.M * G;

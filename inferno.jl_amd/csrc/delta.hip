@@ -1008,11 +1008,11 @@ template <int DK> __global__ __launch_bounds__(DK * 4, 2) void delta_chunk_kerne
     }
 }
 
-// Chunks where no snapshots are asked for and there are tokens enough (sizes between the measured ones follow their line): a chunk costs as much with one token as with 64, the
+// Chunks where no snapshots are asked for and there are tokens enough: a chunk costs as much with one token as with 64, the
 // recurrence as many times more as there are tokens. Where the two meet, by the number of 16-column groups there are to carry,
 // in microseconds (recurrence, chunks) at dk = dv = 128, 32 heads: 1 sequence (256 groups) 16 tokens 22.9, 19.3; 4 (1024)
 // 20 tokens 31.6, 34.9 and 24 tokens 37.0, 35; 16 (4096) 40 tokens 78, 87 and 64 tokens 118, 89. dk = dv = 64, 16 heads: 1
-// sequence (64) 16 tokens 17.4, 15.6; 16 (1024) 20 tokens 23.7, 27.2 and 28 tokens 31.5, 27.2.
+// sequence (64) 16 tokens 17.4, 15.6; 16 (1024) 20 tokens 23.7, 27.2 and 28 tokens 31.5, 27.2. The rule is a line between these.
 bool chunked(const DeltaArgs &a, bool snapshots) {
     const int64_t groups = (int64_t)a.n_seq * a.n_v * ((a.dv + 15) / 16);
     return !snapshots && a.T >= 14 + (groups < 4096 ? groups / 128 : 32);
