@@ -604,6 +604,53 @@ int ihip_delta_ws_bytes(int n_seq, int T, int n_k, int n_v, int dk, int dv,
 int ihip_gated_delta_rule(const ihip_delta *a, void *ws, size_t ws_bytes,
                           void *stream);
 
+/* ---- 8-bit projections: prompts of any length, and single tokens
+ *      (csrc/quant8.hip, csrc/gemm8.hip) ----
+ * ihip_gemm_q takes up to 64 rows; a prompt's projections run on 8-bit codes
+ * with a scale for each token and each channel:
+ *   ihip_quantize_i8 (RMSNORM) -> ihip_gemm_i8 [q; k; v] -> the token mixers ->
+ *   ihip_quantize_i8 (PLAIN) -> ihip_gemm_i8 o (ACCUM: the residual) ->
+ *   ihip_quantize_i8 (RMSNORM) -> ihip_gemm_i8 [gate; up] ->
+ *   ihip_quantize_i8 (SILU_MUL) -> ihip_gemm_i8 down (ACCUM).
+ * A weight matrix is quantized the same way, once: ihip_dequant gives its rows
+ * (the channels) in fp32, ihip_quantize_i8 (PLAIN) their codes and scales. */
+
+/* M rows of K values as codes q (int8, -127 .. 127; rows ldq values apart) and a
+ * scale a row. Of row m, with x' = in->x + the in->add slices (fp32 sums in
+ * slice order, stored back into x; rows of the slices K values apart), or with
+ * in->x NULL the slices' sum (rows of the slices in->ldx values apart, nothing
+ * is stored back):
+ *   t    = x' (IHIP_ACT_PLAIN), x' norm_w (IHIP_ACT_RMSNORM; norm_w NULL: 1), or
+ *          silu(x'[:K]) x'[K:2K] (IHIP_ACT_SILU_MUL; add only with x NULL);
+ *   top  = max_k |t_k|;  q_k = 127 t_k / top rounded to the nearest, ties to even;
+ *   scale = r top / 127, r = 1, or 1 / sqrt(mean(x'^2) + eps) for IHIP_ACT_RMSNORM.
+ * The codes are those of the exact t (formed in fp64 where fp32 cannot tell), so
+ * they do not depend on how fp32 arithmetic is ordered. A row of zeros has scale
+ * 0 and codes 0; a row with a value that is not finite, or whose scale passes
+ * fp32, has scale NaN and codes 0 (its products are NaN). K a multiple of 16 up
+ * to 65536, M up to 2^23; x, norm_w, add and q 16-byte aligned, ldx and add_stride
+ * multiples of 4, ldq of 16 and at least K (values past K are left as they were).
+ * q and scale overlap none of the inputs. No workspace. */
+int ihip_quantize_i8(const ihip_gemm_input *in, int M, int K, int8_t *q_dev,
+                     int64_t ldq, float *scale_dev, void *stream);
+
+/* y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k], or with IHIP_GEMM_ACCUM
+ * that added to y[m, n]. x: M rows of K codes, w: N rows (channels) of K codes,
+ * ldx / ldw values between rows; y fp32, ldy values between rows (columns past N
+ * are left as they were). The sums are 32-bit integers and exact; the sum is
+ * rounded to fp32 once and multiplied by x_scale, then by w_scale (a scale that
+ * is not finite gives its row or column what fp32 products give). Any M and N
+ * from 1 to 2^23 with M N up to 2^38; K a multiple of 16 up to 65536; x and w
+ * 16-byte aligned, ldx and ldw multiples of 16. y overlaps none of the inputs.
+ * ws: ihip_gemm_i8_ws_bytes (may be 0: then NULL is allowed), 16-byte aligned,
+ * any contents, not shared by calls that overlap in time. The batched form of
+ * the reference's projections (src/ModelCPU.jl:284-378) past 64 tokens. */
+int ihip_gemm_i8_ws_bytes(int M, int N, int K, int flags, size_t *bytes);
+int ihip_gemm_i8(const int8_t *x_dev, int64_t ldx, const float *x_scale_dev,
+                 const int8_t *w_dev, int64_t ldw, const float *w_scale_dev,
+                 float *y_dev, int64_t ldy, int M, int N, int K, int flags,
+                 void *ws, size_t ws_bytes, void *stream);
+
 /* ---- draft-side sampler (csrc/sample.hip) ---- */
 
 /* softmax_sample (src/ModelCPU.jl:1123-1200) on each row of logits

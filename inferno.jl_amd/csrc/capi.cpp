@@ -14,6 +14,7 @@
 
 #include "../../include/inferno_hip.h"
 #include "chain.h"
+#include "int8.h"
 #include "mixer.h"
 
 // kernels (gemm.hip, dequant.hip, accept.hip, misc.hip)
@@ -76,6 +77,10 @@ size_t attn_ws(const AttnArgs &a);
 hipError_t launch_attn(const AttnArgs &a, void *ws, hipStream_t st);
 size_t delta_ws(const DeltaArgs &a, bool snapshots);
 hipError_t launch_delta(const DeltaArgs &a, void *ws, hipStream_t st);
+// 8-bit projections (quant8.hip, gemm8.hip)
+hipError_t launch_quant8(const Quant8Args &a, int act, hipStream_t st);
+size_t gemm8_ws(const Gemm8Args &a);
+hipError_t launch_gemm8(const Gemm8Args &a, void *ws, hipStream_t st);
 size_t noalloc_scratch_bytes();
 hipError_t noalloc_scratch(void **out);
 hipError_t noalloc_prepare(int device);
@@ -1217,6 +1222,91 @@ int ihip_gated_delta_rule(const ihip_delta *d, void *ws, size_t ws_bytes, void *
     if (ws_bytes < need) return fail(IHIP_ENOMEM, "ihip_gated_delta_rule: workspace %zu < %zu bytes", ws_bytes, need);
     const hipError_t e = launch_delta(a, ws, S(stream));
     return e == hipSuccess ? ok() : hip_fail(e, "ihip_gated_delta_rule");
+}
+
+// ---- 8-bit projections ----
+int ihip_quantize_i8(const ihip_gemm_input *in, int M, int K, int8_t *q_dev, int64_t ldq, float *scale_dev, void *stream) {
+    const char *fn = "ihip_quantize_i8";
+    if (!in || !q_dev || !scale_dev) return fail(IHIP_EFAULT, "%s: NULL pointer", fn);
+    if (!in->x && !in->add) return fail(IHIP_EFAULT, "%s: NULL x without add slices", fn);
+    const int act = in->act;
+    if (act < IHIP_ACT_PLAIN || act > IHIP_ACT_SILU_MUL) return fail(IHIP_EINVAL, "%s: act=%d", fn, act);
+    if (M < 1 || M > 1 << 23) return fail(IHIP_EINVAL, "%s: M=%d outside 1..2^23", fn, M);
+    if (K < 16 || K > 65536 || K % 16) return fail(IHIP_EINVAL, "%s: K=%d (a multiple of 16 up to 65536)", fn, K);
+    if (ldq < K || ldq % 16 || !aligned16(q_dev))
+        return fail(IHIP_EINVAL, "%s: ldq=%lld (need >= %d, a multiple of 16; q 16-byte aligned)", fn, (long long)ldq, K);
+    if ((uintptr_t)scale_dev & 3) return fail(IHIP_EINVAL, "%s: scale must be 4-byte aligned", fn);
+    const int min_ld = act == IHIP_ACT_SILU_MUL ? 2 * K : K;
+    if (in->ldx < min_ld || (in->ldx & 3) || (in->x && !aligned16(in->x)))
+        return fail(IHIP_EINVAL, "%s: ldx=%d (need >= %d, a multiple of 4; x 16-byte aligned)", fn, in->ldx, min_ld);
+    if (act == IHIP_ACT_RMSNORM && !(in->eps >= 0.f)) return fail(IHIP_EINVAL, "%s: eps=%g", fn, in->eps);
+    if (act == IHIP_ACT_RMSNORM && in->norm_w && !aligned16(in->norm_w))
+        return fail(IHIP_EINVAL, "%s: norm_w must be 16-byte aligned", fn);
+    if (in->add) {
+        if (act == IHIP_ACT_SILU_MUL && in->x)
+            return fail(IHIP_EINVAL, "%s: add with SILU_MUL needs x = NULL (the slices are the input)", fn);
+        const int64_t slice = (int64_t)M * (in->x ? K : in->ldx);
+        if (in->n_add < 1 || (in->n_add > 1 && in->add_stride < slice) || (in->add_stride & 3) || !aligned16(in->add))
+            return fail(IHIP_EINVAL, "%s: add slices n=%d stride=%lld", fn, in->n_add, (long long)in->add_stride);
+    }
+    Quant8Args a{};
+    a.x = const_cast<float *>(in->x);
+    a.norm_w = act == IHIP_ACT_RMSNORM ? in->norm_w : nullptr;
+    a.add = in->add;
+    a.q = q_dev, a.scale = scale_dev;
+    a.ldx = in->ldx, a.ldq = ldq, a.add_stride = in->add_stride;
+    a.M = M, a.K = K, a.n_add = in->add ? in->n_add : 0;
+    a.eps = in->eps;
+    const hipError_t e = launch_quant8(a, act, S(stream));
+    return e == hipSuccess ? ok() : hip_fail(e, fn);
+}
+
+namespace {
+int check_gemm8_shape(const char *fn, int M, int N, int K, int flags) {
+    if (M < 1 || M > 1 << 23 || N < 1 || N > 1 << 23 || (int64_t)M * N > (int64_t)1 << 38)
+        return fail(IHIP_EINVAL, "%s: M=%d N=%d (each 1..2^23, the product up to 2^38)", fn, M, N);
+    if (K < 16 || K > 65536 || K % 16) return fail(IHIP_EINVAL, "%s: K=%d (a multiple of 16 up to 65536)", fn, K);
+    if (flags & ~IHIP_GEMM_ACCUM) return fail(IHIP_EINVAL, "%s: flags 0x%x (IHIP_GEMM_ACCUM or 0)", fn, flags);
+    return IHIP_OK;
+}
+}  // namespace
+
+int ihip_gemm_i8_ws_bytes(int M, int N, int K, int flags, size_t *bytes) {
+    const char *fn = "ihip_gemm_i8_ws_bytes";
+    if (!bytes) return fail(IHIP_EFAULT, "%s: NULL pointer", fn);
+    const int rc = check_gemm8_shape(fn, M, N, K, flags);
+    if (rc != IHIP_OK) return rc;
+    Gemm8Args a{};
+    a.M = M, a.N = N, a.K = K, a.accum = flags & IHIP_GEMM_ACCUM ? 1 : 0;
+    *bytes = gemm8_ws(a);
+    return ok();
+}
+
+int ihip_gemm_i8(const int8_t *x_dev, int64_t ldx, const float *x_scale_dev, const int8_t *w_dev, int64_t ldw,
+                 const float *w_scale_dev, float *y_dev, int64_t ldy, int M, int N, int K, int flags, void *ws,
+                 size_t ws_bytes, void *stream) {
+    const char *fn = "ihip_gemm_i8";
+    if (!x_dev || !x_scale_dev || !w_dev || !w_scale_dev || !y_dev) return fail(IHIP_EFAULT, "%s: NULL pointer", fn);
+    const int rc = check_gemm8_shape(fn, M, N, K, flags);
+    if (rc != IHIP_OK) return rc;
+    if (ldx < K || ldx % 16 || !aligned16(x_dev) || ldw < K || ldw % 16 || !aligned16(w_dev))
+        return fail(IHIP_EINVAL, "%s: ldx=%lld ldw=%lld (need >= %d, multiples of 16; x and w 16-byte aligned)", fn,
+                    (long long)ldx, (long long)ldw, K);
+    if (ldy < N) return fail(IHIP_EINVAL, "%s: ldy=%lld (need >= %d)", fn, (long long)ldy, N);
+    if (((uintptr_t)x_scale_dev | (uintptr_t)w_scale_dev | (uintptr_t)y_dev) & 3)
+        return fail(IHIP_EINVAL, "%s: scales and y must be 4-byte aligned", fn);
+    Gemm8Args a{};
+    a.x = x_dev, a.w = w_dev, a.x_scale = x_scale_dev, a.w_scale = w_scale_dev, a.y = y_dev;
+    a.ldx = ldx, a.ldw = ldw, a.ldy = ldy;
+    a.M = M, a.N = N, a.K = K, a.accum = flags & IHIP_GEMM_ACCUM ? 1 : 0;
+    const size_t need = gemm8_ws(a);
+    if (need) {
+        if (!ws) return fail(IHIP_EFAULT, "%s: NULL workspace (%zu bytes needed)", fn, need);
+        if (ws_bytes < need) return fail(IHIP_ENOMEM, "%s: workspace %zu < %zu bytes", fn, ws_bytes, need);
+        if (!aligned16(ws)) return fail(IHIP_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+    }
+    const hipError_t e = launch_gemm8(a, ws, S(stream));
+    return e == hipSuccess ? ok() : hip_fail(e, fn);
 }
 
 int ihip_sample(const float *logits_dev, int rows, int V, float T, int top_k, float top_p, float min_p,

@@ -1,0 +1,271 @@
+// Rows of fp32 values as 8-bit codes with a scale a row: the input of the 8-bit
+// products (gemm8.hip), from the residual stream (the residual's addition and
+// the RMSNorm of src/ModelCPU.jl:110-122, :870-891), from [gate | up] (:447-473)
+// or from rows as they are.
+//
+//   t = x | x w | silu(gate) up;  top = max |t|;  code = rint(127 t / top)
+//   scale = top / 127, times 1 / sqrt(mean(x^2) + eps) for the norm
+//
+// The norm's factor is one number a row, so it cancels in the codes and enters
+// the scale alone: codes need the row's largest |t| and nothing else, and a row
+// is read once, held in registers, and its codes written once.
+//
+// Codes are those of the exact t, not of its fp32 rounding: t and 127 / top are
+// formed in fp32, and where 127 t / top comes nearer to a tie than their error
+// (a value in ten thousand) that one value is formed again in fp64. So codes do
+// not depend on how the fp32 arithmetic was ordered or contracted.
+#include "common.h"
+#include "int8.h"
+
+namespace {
+
+constexpr int WAVES = 16;  // of the largest workgroup
+
+struct Quant8Shared {
+    uint32_t top[WAVES];
+    float ssq[WAVES];
+    uint64_t dtop[WAVES];
+    double dssq[WAVES];
+    uint64_t most;
+};
+
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t w = __shfl_xor(v, o);
+        v = v > w ? v : w;
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint64_t dbits(double v) { return (uint64_t)__double_as_longlong(fabs(v)); }
+
+__device__ __forceinline__ double silu_mul(double g, double u) { return g / (1.0 + exp(-g)) * u; }
+
+// 4 values at column c of a row as the input has them after its additions
+__device__ __forceinline__ f4 input4(const Quant8Args &a, int64_t row, int c) {
+    if (a.x) return *(const f4 *)(a.x + row * a.ldx + c);
+    f4 v = *(const f4 *)(a.add + row * a.ldx + c);
+    for (int s = 1; s < a.n_add; s++) v += *(const f4 *)(a.add + s * a.add_stride + row * a.ldx + c);
+    return v;
+}
+
+template <int ACT> __device__ __forceinline__ double exact1(float x, float w_or_up) {
+    if constexpr (ACT == Q8_PLAIN) return (double)x;
+    else if constexpr (ACT == Q8_RMSNORM) return (double)x * (double)w_or_up;
+    else return silu_mul((double)x, (double)w_or_up);
+}
+
+// the second factor of 4 values at column c (norm_w, up)
+template <int ACT> __device__ __forceinline__ f4 second4(const Quant8Args &a, int64_t row, int c) {
+    if constexpr (ACT == Q8_RMSNORM) return a.norm_w ? *(const f4 *)(a.norm_w + c) : f4{1, 1, 1, 1};
+    else if constexpr (ACT == Q8_SILU_MUL) return input4(a, row, a.K + c);
+    else return f4{0, 0, 0, 0};
+}
+
+__device__ __forceinline__ float row_scale(double top, double ssq, bool norm, int K, float eps) {
+    if (top == 0.0) return 0.f;
+    const double s = top / 127.0;
+    return (float)(norm ? s / sqrt(ssq / (double)K + (double)eps) : s);
+}
+
+// A row whose values leave the range in which fp32 serves: all of it in fp64. (Rows of zeros, of values past 1e30 or
+// below 1e-20, and rows with a value that is not finite, whose codes are 0 and whose scale is NaN.)
+template <int ACT> __device__ __forceinline__ void wide_row(const Quant8Args &a, int64_t row, Quant8Shared &sh) {
+    const int tid = threadIdx.x, n4 = a.K / 4;
+    uint64_t top = 0;
+    double ssq = 0.0;
+    for (int c = tid; c < n4; c += blockDim.x) {
+        const f4 x = input4(a, row, 4 * c), w = second4<ACT>(a, row, 4 * c);
+        for (int j = 0; j < 4; j++) {
+            const uint64_t b = dbits(exact1<ACT>(x[j], w[j]));
+            top = top > b ? top : b;
+            ssq += (double)x[j] * (double)x[j];
+        }
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint64_t w = __shfl_xor((unsigned long long)top, o);
+        top = top > w ? top : w;
+        ssq += __shfl_xor(ssq, o);
+    }
+    if ((tid & 63) == 0) sh.dtop[tid >> 6] = top, sh.dssq[tid >> 6] = ssq;
+    __syncthreads();
+    top = sh.dtop[0], ssq = sh.dssq[0];
+    for (int i = 1; i < (int)(blockDim.x >> 6); i++) {
+        top = top > sh.dtop[i] ? top : sh.dtop[i];
+        ssq += sh.dssq[i];
+    }
+    const double most = __longlong_as_double((long long)top);
+    const float scale = row_scale(most, ssq, ACT == Q8_RMSNORM, a.K, a.eps);
+    const bool fine = top < 0x7ff0000000000000ull && scale < __builtin_inff();
+    uint32_t *q = (uint32_t *)(a.q + row * a.ldq);
+    for (int c = tid; c < n4; c += blockDim.x) {
+        uint32_t word = 0;
+        if (fine && top) {
+            const f4 x = input4(a, row, 4 * c), w = second4<ACT>(a, row, 4 * c);
+            for (int j = 0; j < 4; j++) {
+                const int code = (int)rint(exact1<ACT>(x[j], w[j]) * 127.0 / most);
+                word |= (uint32_t)(code & 255) << (8 * j);
+            }
+        }
+        q[c] = word;
+    }
+    if (tid == 0) a.scale[row] = fine ? scale : __builtin_nanf("");
+}
+
+// how far 127 t / top in fp32 may be off: t to 1 (norm) or 7 (silu: exp 2, 1 + exp 1, reciprocal 2, two products) halves of
+// 2^-23, top as much, its reciprocal and the product one each: 127 (1 + 1 + 2) 2^-24 = 3.1e-5, 127 (7 + 7 + 2) 2^-24 = 1.2e-4
+template <int ACT> constexpr float NEAR = ACT == Q8_SILU_MUL ? 2e-4f : 4e-5f;
+
+// 4 values at column c of a row, the residual's additions made and stored
+__device__ __forceinline__ f4 take4(const Quant8Args &a, int64_t row, int c, bool adds) {
+    f4 v = input4(a, row, c);
+    if (adds) {
+        const float *add = a.add + row * a.K + c;
+        f4 s = *(const f4 *)add;
+        for (int k = 1; k < a.n_add; k++) s += *(const f4 *)(add + k * a.add_stride);
+        v += s;
+        *(f4 *)(a.x + row * a.ldx + c) = v;
+    }
+    return v;
+}
+
+// x to t in fp32, with the sum of squares of x and the largest |t|, as bits (as whole numbers NaN is the largest)
+template <int ACT> __device__ __forceinline__ f4 to_t(f4 x, f4 w, float &ssq, uint32_t &top) {
+    f4 t = x;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if constexpr (ACT == Q8_RMSNORM) {
+            ssq = __builtin_fmaf(x[j], x[j], ssq);
+            t[j] = x[j] * w[j];
+        } else if constexpr (ACT == Q8_SILU_MUL) {
+            t[j] = x[j] * __builtin_amdgcn_rcpf(1.f + expf(-x[j])) * w[j];
+            // (exp(-x) passes fp32 there; what is lost counts only beside so large an up)
+            if (x[j] < -80.f && fabsf(w[j]) > 1e8f) top = 0x7fffffffu;
+        }
+        const uint32_t b = __float_as_uint(t[j]) & 0x7fffffffu;
+        top = top > b ? top : b;
+    }
+    return t;
+}
+
+template <int ACT>
+__device__ __forceinline__ void raise_most(const Quant8Args &a, int64_t row, int c, f4 t, float from, Quant8Shared &sh) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (fabsf(t[j]) >= from) {
+            const f4 x = input4(a, row, c), w = second4<ACT>(a, row, c);
+            atomicMax((unsigned long long *)&sh.most, (unsigned long long)dbits(exact1<ACT>(x[j], w[j])));
+        }
+}
+
+template <int ACT>
+__device__ __forceinline__ uint32_t codes4(const Quant8Args &a, int64_t row, int c, f4 t, float inv, double most) {
+    int r[4];
+    bool near = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float v = t[j] * inv, n = rintf(v);
+        near |= fabsf(v - n) > 0.5f - NEAR<ACT>;
+        r[j] = (int)n;
+    }
+    if (near) {
+        const f4 x = input4(a, row, c), w = second4<ACT>(a, row, c);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (fabsf(t[j] * inv - (float)r[j]) > 0.5f - NEAR<ACT>) r[j] = (int)rint(exact1<ACT>(x[j], w[j]) * 127.0 / most);
+    }
+    return (uint32_t)(r[0] & 255) | (uint32_t)(r[1] & 255) << 8 | (uint32_t)(r[2] & 255) << 16 | (uint32_t)r[3] << 24;
+}
+
+// One workgroup a row, V x 4 values a thread kept in registers; V = 0: rows of any length, read a second time for the codes.
+template <int ACT, int V> __global__ __launch_bounds__(1024) void quant8_kernel(Quant8Args a) {
+    __shared__ Quant8Shared sh;
+    constexpr int KEPT = V ? V : 1;
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, n4 = a.K / 4, nt = blockDim.x;
+    const bool adds = ACT != Q8_SILU_MUL && a.x && a.add;
+    f4 t[KEPT];
+    uint32_t top = 0;
+    float ssq = 0.f;
+    if constexpr (V > 0) {
+        f4 w[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int c = tid + i * nt;
+            t[i] = c < n4 ? take4(a, row, 4 * c, adds) : f4{0, 0, 0, 0};
+            w[i] = c < n4 ? second4<ACT>(a, row, 4 * c) : f4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) t[i] = to_t<ACT>(t[i], w[i], ssq, top);
+    } else {
+        for (int c = tid; c < n4; c += nt) {
+            const f4 x = take4(a, row, 4 * c, adds);
+            to_t<ACT>(x, second4<ACT>(a, row, 4 * c), ssq, top);
+        }
+    }
+    auto again = [&](int c) __attribute__((always_inline)) {
+        float s = 0.f;
+        uint32_t b = 0;
+        return to_t<ACT>(input4(a, row, 4 * c), second4<ACT>(a, row, 4 * c), s, b);
+    };
+    top = wave_umax(top);
+    if (ACT == Q8_RMSNORM) ssq = wave_sum(ssq);
+    if ((tid & 63) == 0) sh.top[tid >> 6] = top, sh.ssq[tid >> 6] = ssq;
+    if (tid == 0) sh.most = 0;
+    __syncthreads();
+    top = sh.top[0], ssq = sh.ssq[0];
+    for (int i = 1; i < (nt >> 6); i++) {
+        top = top > sh.top[i] ? top : sh.top[i];
+        ssq += sh.ssq[i];
+    }
+    const float ftop = __uint_as_float(top);
+    if (!(ftop > 1e-20f && ftop < 1e30f) || (ACT == Q8_RMSNORM && !(ssq > 1e-30f && ssq < 1e30f))) {
+        wide_row<ACT>(a, row, sh);
+        return;
+    }
+    double most = (double)ftop;
+    if (ACT == Q8_SILU_MUL || (ACT == Q8_RMSNORM && a.norm_w)) {
+        // the exact largest |t|: among those whose fp32 value is the largest (a product's rounding keeps the order), or within
+        // twice the gate's error of it
+        const float from = ACT == Q8_SILU_MUL ? ftop * (1.f - 0x1p-18f) : ftop;
+        if constexpr (V > 0) {
+#pragma unroll
+            for (int i = 0; i < V; i++) raise_most<ACT>(a, row, 4 * (tid + i * nt), t[i], from, sh);
+        } else {
+            for (int c = tid; c < n4; c += nt) raise_most<ACT>(a, row, 4 * c, again(c), from, sh);
+        }
+        __syncthreads();
+        most = __longlong_as_double((long long)sh.most);
+    }
+    const float inv = 127.f / ftop;
+    uint32_t *q = (uint32_t *)(a.q + row * a.ldq);
+    if constexpr (V > 0) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int c = tid + i * nt;
+            if (c < n4) q[c] = codes4<ACT>(a, row, 4 * c, t[i], inv, most);
+        }
+    } else {
+        for (int c = tid; c < n4; c += nt) q[c] = codes4<ACT>(a, row, 4 * c, again(c), inv, most);
+    }
+    if (tid == 0) a.scale[row] = row_scale(most, (double)ssq, ACT == Q8_RMSNORM, a.K, a.eps);
+}
+
+template <int ACT> void launch(const Quant8Args &a, hipStream_t st) {
+    const int n4 = a.K / 4;
+    const int v = n4 > 4096 ? 0 : a.M > 256 || n4 > 2048 ? 4 : n4 > 1024 ? 2 : 1;
+    const int nt = v ? ((n4 + v - 1) / v + 63) / 64 * 64 : 1024;
+    if (v == 1) quant8_kernel<ACT, 1><<<a.M, nt, 0, st>>>(a);
+    else if (v == 2) quant8_kernel<ACT, 2><<<a.M, nt, 0, st>>>(a);
+    else if (v == 4) quant8_kernel<ACT, 4><<<a.M, nt, 0, st>>>(a);
+    else quant8_kernel<ACT, 0><<<a.M, nt, 0, st>>>(a);
+}
+
+}  // namespace
+
+hipError_t launch_quant8(const Quant8Args &a, int act, hipStream_t st) {
+    if (act == Q8_PLAIN) launch<Q8_PLAIN>(a, st);
+    else if (act == Q8_RMSNORM) launch<Q8_RMSNORM>(a, st);
+    else launch<Q8_SILU_MUL>(a, st);
+    return hipGetLastError();
+}

@@ -7,6 +7,7 @@ lib/libinferno_hip.so. There is no CPU fallback.
 """
 from . import formats, gguf, synth
 from ._lib import HipError, load
+from .int8 import gemm_i8, gemm_i8_ws_bytes, quantize_i8, quantize_weights_i8, rmsnorm_i8, silu_mul_i8
 from .mixers import (KVCache, RopeParams, attn_prefix, attn_prefix_ws_bytes, gated_delta_rule, gated_delta_rule_ws_bytes,
                      rope, rope_append)
 from .quantized_kernels import (ACT_PLAIN, ACT_RMSNORM, ACT_SILU_MUL, EPI_GATE, EPI_RESID, EPI_STATS, EPI_STORE,
@@ -28,5 +29,5 @@ __all__ = [
     "greedy_verify", "mtp_verify_step", "n_tokens", "softmax_stats", "spec_accept", "tree_accept",
     "softmax_sample", "sample_ws_bytes", "apply_penalties_", "commit_state_", "advance_len_",
     "KVCache", "RopeParams", "rope", "rope_append", "attn_prefix", "attn_prefix_ws_bytes", "gated_delta_rule",
-    "gated_delta_rule_ws_bytes",
+    "gated_delta_rule_ws_bytes", "quantize_i8", "rmsnorm_i8", "silu_mul_i8", "quantize_weights_i8", "gemm_i8", "gemm_i8_ws_bytes",
 ]

@@ -93,6 +93,9 @@ SIGNATURES = {
     "ihip_attn_prefix": (_i, [_vp, _i64, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _f, _vp, _sz, _vp]),
     "ihip_delta_ws_bytes": (_i, [_i, _i, _i, _i, _i, _i, _i, C.POINTER(_sz)]),
     "ihip_gated_delta_rule": (_i, [_vp, _vp, _sz, _vp]),
+    "ihip_quantize_i8": (_i, [_vp, _i, _i, _vp, _i64, _vp, _vp]),
+    "ihip_gemm_i8_ws_bytes": (_i, [_i, _i, _i, _i, C.POINTER(_sz)]),
+    "ihip_gemm_i8": (_i, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
     "ihip_sample": (_i, [_vp, _i, _i, _f, _i, _f, _f, _vp, _vp, _vp]),
     "ihip_sample_ws_bytes": (_i, [_i, _i, C.POINTER(_sz)]),
     "ihip_sample_ex": (_i, [_vp, _i, _i, _f, _i, _f, _f, _vp, _vp, _vp, _sz, _vp]),

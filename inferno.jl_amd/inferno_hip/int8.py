@@ -1,0 +1,154 @@
+"""The 8-bit projections of prompts and single tokens: rows of the residual
+stream, of [gate | up] or of the mixers' output as 8-bit codes with a scale for
+each row (the RMSNorm, gating and residual adds of src/ModelCPU.jl:110-122,
+:447-473, :870-891), and their products with 8-bit weights (:284-378), past the
+64 rows that gemm_q takes.
+
+Kernels run on `stream` (default: torch's current one). What a call allocates
+itself (codes, scales, out, ws) is made for that stream; its inputs have to be
+ready there, and other streams wait for it before they read its outputs. A
+workspace that is given serves one call at a time.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _lib, mixers
+from .formats import BLOCK_BYTES, BLOCK_ELEMS
+from .mixers import _call, _device_of, _on, _refuse, _rows, _torch, _whole, _workspace
+from .quantized_kernels import ACT_PLAIN, ACT_RMSNORM, ACT_SILU_MUL, GEMM_ACCUM, check_tensor, dequant, made_for
+
+_i8 = None
+
+
+def _names():
+    """torch's names, looked up once."""
+    global _i8
+    import torch
+    _torch()
+    _i8 = torch.int8
+
+
+def _codes(t, name: str, rows: int | None, k: int | None, dev: int):
+    """t as int8 [rows, k or more] with unit column stride on device dev; its address, rows, columns and row stride."""
+    if not isinstance(t, mixers._Tensor) or t.dtype is not _i8 or t.get_device() != dev:
+        _refuse(t, name, _i8, None, False, dev)
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] < 1 or (rows is not None and shape[0] != rows) or shape[1] < (k or 1) or stride[1] != 1:
+        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {'k' if k is None else f'>= {k}'}] int8 with "
+                         f"unit column stride, got {tuple(shape)} of strides {stride}")
+    return t.data_ptr(), shape[0], shape[1], stride[0] if shape[0] > 1 else max(stride[0], (shape[1] + 15) // 16 * 16)
+
+
+def _quantize(x, act: int, k: int, norm_w, eps: float, add, out, scales, stream):
+    dev = _device_of(x, "x")
+    xp, rows, ldx = _rows(x, "x", 2 * k if act == ACT_SILU_MUL else k, None, dev)
+    a = _lib.GemmInput(xp, ldx, act, None, eps, None, 0, 0)
+    if norm_w is not None:
+        a.norm_w = _whole(norm_w, "norm_w", mixers._f32, (k,), dev)
+    if add is not None:
+        if isinstance(add, mixers._Tensor) and add.dim() == 2:
+            add = add[None]
+        n = add.shape[0] if isinstance(add, mixers._Tensor) and add.dim() == 3 else 1
+        a.add, a.n_add, a.add_stride = _whole(add, "add", mixers._f32, (n, rows, k), dev), n, rows * k
+    if out is None:
+        out = made_for(stream, x.new_empty, (rows, k), dtype=_i8)
+    if scales is None:
+        scales = made_for(stream, x.new_empty, rows)
+    qp, _, _, ldq = _codes(out, "out", rows, k, dev)
+    sp = _whole(scales, "scales", mixers._f32, (rows,), dev)
+    _lib.check(_call("ihip_quantize_i8")(C.byref(a), rows, k, qp, ldq, sp, _on(stream, dev)))
+    return out, scales
+
+
+def quantize_i8(x, out=None, scales=None, stream=None):
+    """Rows x [M, K] float32 (unit column stride, K a multiple of 16) as int8
+    codes [M, K] and float32 scales [M]: scales[m] = max |x[m]| / 127, codes
+    the nearest, ties to even. A row of zeros has scale 0, one with a value
+    that is not finite scale NaN, both codes 0."""
+    if _i8 is None:
+        _names()
+    return _quantize(x, ACT_PLAIN, _columns(x), None, 0.0, None, out, scales, stream)
+
+
+def rmsnorm_i8(x, norm_w=None, eps: float = 1e-6, add=None, out=None, scales=None, stream=None):
+    """RMSNorm(x) * norm_w of rows x [M, K] as codes and scales. add, [M, K] or
+    [n, M, K]: the slices are added to x first, in place."""
+    if _i8 is None:
+        _names()
+    return _quantize(x, ACT_RMSNORM, _columns(x), norm_w, eps, add, out, scales, stream)
+
+
+def silu_mul_i8(gate_up, out=None, scales=None, stream=None):
+    """silu(gate) * up of rows [gate | up] (gate_up [M, 2 K]) as codes [M, K] and scales."""
+    if _i8 is None:
+        _names()
+    n = _columns(gate_up)
+    if n % 2:
+        raise ValueError(f"gate_up has {n} columns: gate, then up")
+    return _quantize(gate_up, ACT_SILU_MUL, n // 2, None, 0.0, None, out, scales, stream)
+
+
+def _columns(x) -> int:
+    if not isinstance(x, mixers._Tensor) or x.dim() != 2:
+        raise ValueError("rows must be a float32 GPU tensor [M, K]")
+    return x.shape[1]
+
+
+def quantize_weights_i8(qtype: int, w_dev, n: int, k: int, stream=None):
+    """A GGUF matrix [n, k] on the device as int8 codes [n, k] and a scale a
+    channel, once at load time: its rows dequantized, 64 Mi values at a time, then quantize_i8."""
+    import torch
+    if _i8 is None:
+        _names()
+    if qtype not in BLOCK_ELEMS or k % BLOCK_ELEMS[qtype]:
+        raise ValueError(f"qtype {qtype}, k={k}: not rows of whole blocks")
+    row = k // BLOCK_ELEMS[qtype] * BLOCK_BYTES[qtype]
+    check_tensor(w_dev, "w_dev", torch.uint8, min_numel=n * row)
+    codes = made_for(stream, torch.empty, (n, k), dtype=torch.int8, device=w_dev.device)
+    scales = made_for(stream, torch.empty, n, dtype=torch.float32, device=w_dev.device)
+    step = max(1, (64 << 20) // k)
+    flat = w_dev.view(-1)
+    for i in range(0, n, step):
+        rows = min(step, n - i)
+        x = dequant(qtype, flat[i * row:(i + rows) * row], rows * k, stream=stream).view(rows, k)
+        quantize_i8(x, out=codes[i:i + rows], scales=scales[i:i + rows], stream=stream)
+    return codes, scales
+
+
+@_lib.kept_by_size
+def _ws_bytes(m: int, n: int, k: int, flags: int) -> int:
+    nb = C.c_size_t()
+    _lib.check(_lib.load().ihip_gemm_i8_ws_bytes(m, n, k, flags, C.byref(nb)))
+    return int(nb.value)
+
+
+def gemm_i8_ws_bytes(m: int, n: int, k: int, accum: bool = False) -> int:
+    """Workspace bytes of gemm_i8 (0: none)."""
+    return _ws_bytes(m, n, k, GEMM_ACCUM if accum else 0)
+
+
+def gemm_i8(q, scales, w, w_scales, accum: bool = False, out=None, ws=None, stream=None):
+    """out [M, N] float32 = scales[m] * w_scales[n] * sum_k q[m, k] w[n, k], or
+    with accum that added to out (which is then given). q int8 [M, K or more
+    columns], w int8 [N, K] (unit column stride, rows a multiple of 16 values
+    apart, K a multiple of 16), scales float32 [M] and [N]. Any M and N."""
+    if _i8 is None:
+        _names()
+    dev = _device_of(q, "q")
+    wp, n, k, ldw = _codes(w, "w", None, None, dev)
+    qp, m, _, ldq = _codes(q, "q", None, k, dev)
+    sp = _whole(scales, "scales", mixers._f32, (m,), dev)
+    wsp = _whole(w_scales, "w_scales", mixers._f32, (n,), dev)
+    if out is None:
+        if accum:
+            raise ValueError("accum adds to out: pass it")
+        out = made_for(stream, scales.new_empty, (m, n))
+    yp, _, ldy = _rows(out, "out", n, m, dev)
+    flags = GEMM_ACCUM if accum else 0
+    if ws is None:
+        need = _ws_bytes(m, n, k, flags)
+        ws = made_for(stream, scales.new_empty, need, dtype=mixers._u8, returned=False) if need else None
+    tp, tn = (None, 0) if ws is None else _workspace(ws, dev)
+    _lib.check(_call("ihip_gemm_i8")(qp, ldq, sp, wp, ldw, wsp, yp, ldy, m, n, k, flags, tp, tn, _on(stream, dev)))
+    return out
