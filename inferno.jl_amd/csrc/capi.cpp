@@ -1289,8 +1289,8 @@ int ihip_gemm_i8(const int8_t *x_dev, int64_t ldx, const float *x_scale_dev, con
     if (!x_dev || !x_scale_dev || !w_dev || !w_scale_dev || !y_dev) return fail(IHIP_EFAULT, "%s: NULL pointer", fn);
     const int rc = check_gemm8_shape(fn, M, N, K, flags);
     if (rc != IHIP_OK) return rc;
-    if (ldx < K || ldx % 16 || !aligned16(x_dev) || ldw < K || ldw % 16 || !aligned16(w_dev))
-        return fail(IHIP_EINVAL, "%s: ldx=%lld ldw=%lld (need >= %d, multiples of 16; x and w 16-byte aligned)", fn,
+    if (ldx < K || ldx > 1 << 22 || ldx % 16 || !aligned16(x_dev) || ldw < K || ldw > 1 << 22 || ldw % 16 || !aligned16(w_dev))
+        return fail(IHIP_EINVAL, "%s: ldx=%lld ldw=%lld (%d..2^22, multiples of 16; x and w 16-byte aligned)", fn,
                     (long long)ldx, (long long)ldw, K);
     if (ldy < N) return fail(IHIP_EINVAL, "%s: ldy=%lld (need >= %d)", fn, (long long)ldy, N);
     if (((uintptr_t)x_scale_dev | (uintptr_t)w_scale_dev | (uintptr_t)y_dev) & 3)

@@ -10,90 +10,379 @@
 namespace {
 
 typedef int i4 __attribute__((ext_vector_type(4)));
+typedef int i16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(1))) const void global_void;
 
-__device__ const i4 zeros16 = {0, 0, 0, 0};  // what is loaded past K
+constexpr int KB = 128;  // bytes of K that a stage holds: a line of each row
 
-constexpr int KB = 128;  // bytes of K a tile holds
+// Which of the eight 16-byte places of a row its chunk c takes: c ^ turn_of(row). The 16 lanes that LDS serves at once in a load
+// of 32 rows' chunk c (lanes 0-7 with 16-23, 8-15 with 24-31: rows) then meet in no bank.
+__device__ __forceinline__ int turn_of(int row) { return (row & 6) | (row >> 4 & 1); }
 
-// Byte of 16-byte chunk c of row r: the chunks of a row are permuted by its number, so that the 16 rows of an operand load
-// (one chunk each) do not meet in a bank.
-__device__ __forceinline__ int tile_at(int r, int c) { return r * KB + ((c ^ (r & 7)) << 4); }
+// All but the last N loads of this wave are there, its LDS operations are done, and every wave is here.
+template <int N> __device__ __forceinline__ void meet() {
+    static_assert(N < 64, "the counter's range");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // vmcnt N, lgkmcnt 0
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
-// One tile of BM tokens x BN channels; WM x WN waves.
-template <int BM, int BN, int WM, int WN> __global__ __launch_bounds__(WM *WN * 64) void gemm8_tile(Gemm8Args a, int tiles_m) {
-    constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-    __shared__ char lds[(BM + BN) * KB];
+// Rows first .. of a matrix, as a buffer that ends behind its last row or behind `most` rows (empty past the last row).
+struct Rows {
+    const int8_t *p;
+    int bytes;
+};
+__device__ __forceinline__ Rows rows_at(const int8_t *p, int64_t ld, int first, int rows, int most) {
+    int n = rows - first < most ? rows - first : most;
+    n = __builtin_amdgcn_readfirstlane(n < 0 ? 0 : n);  // (a scalar, or the loads would loop over its lanes)
+    return Rows{p + first * ld, n * (int)ld};
+}
+
+// Tile number t of tiles_m x tiles_n: the eight XCDs (consecutive workgroups in turn) take a contiguous range each, in groups
+// of GROUP tiles of tokens, so that the tiles in flight on an XCD share rows and channels in its L2.
+constexpr int GROUP = 8;
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &tm, int &tn) {
+    const int total = tiles_m * tiles_n, q = total >> 3, r = total & 7, x = id & 7, i = id >> 3;
+    const int t = x * q + (x < r ? x : r) + i;
+    const int per = GROUP * tiles_n, group = t / per, first = group * GROUP;
+    const int size = tiles_m - first < GROUP ? tiles_m - first : GROUP, in = t - group * per;
+    tm = __builtin_amdgcn_readfirstlane(first + in % size), tn = __builtin_amdgcn_readfirstlane(in / size);
+}
+
+// How a product is cut: tiles of tokens and channels, `per` of K for each of the launch's y; with several of those their sums go
+// to `sums` (rows of ld, a multiple of 4) instead of y.
+struct Tiling {
+    int m, n, per, ld, stream;
+    int *sums;
+};
+
+// 4 channels of one token into y
+__device__ __forceinline__ void put(const Gemm8Args &a, int m, int n, f4 r, bool vec, bool stream) {
+    float *y = a.y + (int64_t)m * a.ldy + n;
+    if (vec && n + 4 <= a.N) {
+        if (a.accum) r += *(const f4 *)y;
+        if (stream) __builtin_nontemporal_store(r, (f4 *)y);
+        else *(f4 *)y = r;
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            if (n + c < a.N) y[c] = a.accum ? y[c] + r[c] : r[c];
+    }
+}
+
+// A tile of B tokens x B channels; WM x WN waves. H places in LDS, each for the tokens' or the channels' half of a stage.
+template <int B, int WM, int WN, int H, int EU>
+__global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU, EU))) void gemm8_tile(Gemm8Args a, Tiling t) {
+#if __HIP_DEVICE_COMPILE__  // (the host's pass over these builtins would leave the kernel without its launch stub)
+    constexpr int NW = WM * WN, TM = B / WM / 32, TN = B / WN / 32, NLH = B / 8 / NW, BYTES = B * KB;
+    static_assert(B % (8 * NW) == 0 && NW % 4 == 0, "rows of a load");
+    static_assert(H % 2 == 1 && H >= 5 && H <= 9 && H * BYTES <= 160 * 1024 && NW <= 2 * (BYTES / 4096), "places, and the results' way out");
+    // (an array each, so that the compiler sees which loads a read has to wait for)
+    __shared__ __attribute__((aligned(1024))) char lds0[BYTES], lds1[BYTES], lds2[BYTES], lds3[BYTES], lds4[BYTES];
+    __shared__ __attribute__((aligned(1024))) char lds5[H > 5 ? BYTES : 16], lds6[H > 6 ? BYTES : 16], lds7[H > 7 ? BYTES : 16], lds8[H > 8 ? BYTES : 16];
+    auto place = [&](int n) __attribute__((always_inline)) {
+        n %= H;
+        return n == 0 ? lds0 : n == 1 ? lds1 : n == 2 ? lds2 : n == 3 ? lds3 : n == 4 ? lds4 : n == 5 ? lds5 : n == 6 ? lds6 : n == 7 ? lds7 : lds8;
+    };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave / WN, wn = wave % WN, g = lane >> 4, col = lane & 15;
-    const int m0 = (blockIdx.x % tiles_m) * BM, n0 = (blockIdx.x / tiles_m) * BN;
-    i4 acc[TN][TM];
+    const int wm = wave / WN, wn = wave % WN, g = lane >> 5, col = lane & 31;
+    int tm, tn;
+    tile_of(blockIdx.x, t.m, t.n, tm, tn);
+    const int first = blockIdx.y * t.per, end = first + t.per < a.K ? first + t.per : a.K;  // of K
+
+    // this wave's loads of a stage: rows (i NW + wave) 8 .. + 7 each, tokens first; a lane brings 16 bytes of one row. Rows past
+    // the last and bytes past K are past the buffer's end: they read as zero.
+    const int lr = lane >> 3, lc = ((lane & 7) ^ turn_of(wave * 8 + lr)) * 16;
+    const Rows x = rows_at(a.x, a.ldx, tm * B, a.M, B), w = rows_at(a.w, a.ldw, tn * B, a.N, B);
+    const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc((void *)x.p, 0, x.bytes, 0x00027000);
+    const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc((void *)w.p, 0, w.bytes, 0x00027000);
+    uint32_t xat[NLH], wat[NLH];
+#pragma unroll
+    for (int i = 0; i < NLH; i++) {
+        xat[i] = (uint32_t)((i * NW + wave) * 8 + lr) * (uint32_t)a.ldx + lc;
+        wat[i] = (uint32_t)((i * NW + wave) * 8 + lr) * (uint32_t)a.ldw + lc;
+    }
+    auto fetch = [&](char *lds, bool tok, int k0) __attribute__((always_inline)) {
+        const uint32_t past = k0 + lc < end ? 0u : 1u << 31;
+#pragma unroll
+        for (int i = 0; i < NLH; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(tok ? xb : wb, (lds_void *)(lds + (i * NW + wave) * 8 * KB), 16,
+                                                     (tok ? xat[i] : wat[i]) | past, k0, 0, 0);
+    };
+    i16 acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; i++)
 #pragma unroll
-        for (int j = 0; j < TM; j++) acc[i][j] = i4{0, 0, 0, 0};
-    const int lr = lane >> 3, lc = (lane & 7) ^ lr;  // this lane's row of 8 and its 16-byte chunk
-    for (int k0 = 0; k0 < a.K; k0 += KB) {
-        __syncthreads();
+        for (int j = 0; j < TM; j++) acc[i][j] = i16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    struct Part {  // 32 bytes of K of this wave's rows
+        i4 w[TN], x[TM];
+    };
+    const int ax = (wm * TM * 32 + col) * KB, aw = (wn * TN * 32 + col) * KB, turn = turn_of(col) << 4;
+    auto read = [&](const char *lx, const char *lw, int s, Part &p) __attribute__((always_inline)) {
+        const int c = ((2 * s + g) << 4) ^ turn;
 #pragma unroll
-        for (int i = 0; i < (BM + BN) / 8 / NW; i++) {
-            const int r = (i * NW + wave) * 8;  // (uniform: rows r .. r + 7 of the tile, tokens first)
-            const bool tok = r < BM;
-            const int row = (tok ? m0 + r : n0 + r - BM) + lr, last = (tok ? a.M : a.N) - 1;
-            const int8_t *p = (tok ? a.x : a.w) + (int64_t)(row < last ? row : last) * (tok ? a.ldx : a.ldw) + k0 + lc * 16;
-            const void *src = k0 + lc * 16 < a.K ? (const void *)p : (const void *)&zeros16;
-            __builtin_amdgcn_global_load_lds((global_void *)src, (lds_void *)(lds + r * KB), 16, 0, 0);
+        for (int j = 0; j < TM; j++) p.x[j] = *(const i4 *)(lx + ax + c + j * 32 * KB);
+#pragma unroll
+        for (int i = 0; i < TN; i++) p.w[i] = *(const i4 *)(lw + aw + c + i * 32 * KB);
+    };
+    auto multiply = [&](const Part &p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < TN; i++)
+#pragma unroll
+            for (int j = 0; j < TM; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(p.w[i], p.x[j], acc[i][j], 0, 0, 0);
+    };
+    auto spread = [&]() __attribute__((always_inline)) {  // operand loads between the products
+#pragma unroll
+        for (int i = 0; i < TN * TM; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (i < TN + TM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-        __syncthreads();
+    };
+    Part p0, p1;
+    // A stage's products in four parts, the operands of each read during the one before. After the third the stage is read and
+    // its places are free; the loads into them go between the products of the fourth.
+    auto head = [&](const char *cx, const char *cw) __attribute__((always_inline)) {
+        read(cx, cw, 1, p1);
+        multiply(p0);
+        spread();
+        read(cx, cw, 2, p0);
+        multiply(p1);
+        spread();
+        read(cx, cw, 3, p1);
+        multiply(p0);
+        spread();
+        meet<(H - 4) * NLH>();  // (the next stage is there; a wave's loads end in the order in which they began)
+    };
+    auto tail = [&](char *cx, char *cw, const char *nx, const char *nw, int k0) __attribute__((always_inline)) {
+        fetch(cx, false, k0 + (H - 1) / 2 * KB);
+        fetch(cw, true, k0 + (H + 1) / 2 * KB);
+        read(nx, nw, 0, p0);
+        multiply(p1);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            i4 w[TN], x[TM];
-#pragma unroll
-            for (int i = 0; i < TN; i++) w[i] = *(const i4 *)(lds + tile_at(BM + (wn * TN + i) * 16 + col, 4 * h + g));
-#pragma unroll
-            for (int j = 0; j < TM; j++) x[j] = *(const i4 *)(lds + tile_at((wm * TM + j) * 16 + col, 4 * h + g));
-#pragma unroll
-            for (int i = 0; i < TN; i++)
-#pragma unroll
-                for (int j = 0; j < TM; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x[j], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < TN * TM; i++) {  // (a wave's loads queue behind each other: all at once they would hold up its products)
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (i < TN + TM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, (2 * NLH + TN * TM - 1) / (TN * TM), 0);
         }
+    };
+#pragma unroll
+    for (int h = 0; h < H; h++) fetch(place(h), h % 2 == 0, first + h / 2 * KB);
+    meet<(H - 2) * NLH>();
+    read(lds0, lds1, 0, p0);
+    head(lds0, lds1);
+    // (H stages, and each place has held every one of them; written out, for the places have to be known when it is compiled)
+    for (int k0 = first;;) {
+#define STAGE(i)                                                                          \
+    if (k0 + KB >= end) break;                                                            \
+    tail(place(2 * (i)), place(2 * (i) + 1), place(2 * (i) + 2), place(2 * (i) + 3), k0); \
+    k0 += KB;                                                                             \
+    head(place(2 * (i) + 2), place(2 * (i) + 3));
+        STAGE(0) STAGE(1) STAGE(2) STAGE(3) STAGE(4)
+        if constexpr (H > 5) {
+            STAGE(5) STAGE(6)
+        }
+        if constexpr (H > 7) {
+            STAGE(7) STAGE(8)
+        }
+#undef STAGE
     }
-    // a lane's accumulators are 4 channels of one token
+    multiply(p1);
+    // A part of 32 x 32 at a time through LDS (each wave its own 4 KiB): a lane's accumulators are 4 channels of one token, four
+    // times; rows of 128 bytes go to memory, 8 of them with an instruction. (Parts of lines cost as much as whole ones.)
+    meet<0>();
+    char *const own = wave < BYTES / 4096 ? lds0 + wave * 4096 : lds1 + (wave - BYTES / 4096) * 4096;
+    const int m0 = tm * B + wm * TM * 32, n0 = tn * B + wn * TN * 32;
+    const int er = lane >> 3, en = (lane & 7) * 4;  // this lane's row of 8, its 4 channels
     const bool vec = (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0;
+    int *const part = t.sums ? t.sums + (int64_t)blockIdx.y * a.M * t.ld : nullptr;
+    float xs[TM][4];
 #pragma unroll
-    for (int j = 0; j < TM; j++) {
-        const int m = m0 + (wm * TM + j) * 16 + col;
-        if (m >= a.M) continue;
-        const float xs = a.x_scale[m];
+    for (int j = 0; j < TM; j++)
 #pragma unroll
-        for (int i = 0; i < TN; i++) {
-            const int n = n0 + (wn * TN + i) * 16 + 4 * g;
-            float *y = a.y + (int64_t)m * a.ldy + n;
-            if (vec && n + 4 <= a.N) {
-                f4 v;
+        for (int u = 0; u < 4; u++) {
+            const int m = m0 + j * 32 + 8 * u + er;
+            xs[j][u] = m < a.M ? a.x_scale[m] : 0.f;
+        }
 #pragma unroll
-                for (int c = 0; c < 4; c++) v[c] = (float)acc[i][j][c] * xs * a.w_scale[n + c];
-                if (a.accum) v += *(const f4 *)y;
-                *(f4 *)y = v;
-            } else {
+    for (int i = 0; i < TN; i++) {
+        const int n = n0 + i * 32 + en;
+        f4 ws;
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (n + c < a.N) {
-                        const float v = (float)acc[i][j][c] * xs * a.w_scale[n + c];
-                        y[c] = a.accum ? y[c] + v : v;
-                    }
+        for (int c = 0; c < 4; c++) ws[c] = n + c < a.N ? a.w_scale[n + c] : 0.f;
+#pragma unroll
+        for (int j = 0; j < TM; j++) {
+            const i16 v = acc[i][j];
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                *(i4 *)(own + col * 128 + (((2 * q + g) ^ (col & 7)) << 4)) = i4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            i4 o[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) o[u] = *(const i4 *)(own + (8 * u + er) * 128 + (((lane & 7) ^ er) << 4));
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int m = m0 + j * 32 + 8 * u + er;
+                if (m >= a.M) continue;
+                if (part) {
+                    if (n < t.ld) *(i4 *)(part + (int64_t)m * t.ld + n) = o[u];
+                    continue;
+                }
+                f4 r;
+#pragma unroll
+                for (int c = 0; c < 4; c++) r[c] = (float)o[u][c] * xs[j][u] * ws[c];
+                put(a, m, n, r, vec, t.stream);
             }
         }
     }
+#endif
+}
+
+// The sums of P parts of K, four channels of a token a thread.
+template <int P> __global__ __launch_bounds__(256) void gemm8_join(Gemm8Args a, const int *sums, int ld) {
+    const int id = blockIdx.x * 256 + threadIdx.x, m = id / (ld / 4), n = (id - m * (ld / 4)) * 4;
+    if (m >= a.M) return;
+    const int *p = sums + (int64_t)m * ld + n;
+    i4 v[P];
+#pragma unroll
+    for (int i = 0; i < P; i++) v[i] = *(const i4 *)(p + (int64_t)i * a.M * ld);
+    const float xs = a.x_scale[m];
+    f4 ws, r;
+#pragma unroll
+    for (int c = 0; c < 4; c++) ws[c] = n + c < a.N ? a.w_scale[n + c] : 0.f;
+#pragma unroll
+    for (int i = 1; i < P; i++) v[0] += v[i];
+#pragma unroll
+    for (int c = 0; c < 4; c++) r[c] = (float)v[0][c] * xs * ws[c];
+    put(a, m, n, r, (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0, false);
+}
+
+template <int B, int WM, int WN, int H, int EU> void tiles(const Gemm8Args &a, int parts, int *sums, hipStream_t st) {
+    Tiling t{};
+    t.m = (a.M + B - 1) / B, t.n = (a.N + B - 1) / B;
+    t.ld = (a.N + 3) / 4 * 4;
+    t.per = ((a.K + KB - 1) / KB + parts - 1) / parts * KB;
+    t.sums = parts > 1 ? sums : nullptr;
+    // past the caches from 32 MB of results on, what the eight L2s hold
+    t.stream = (int64_t)a.M * a.N * 4 >= (int64_t)32 << 20;
+    gemm8_tile<B, WM, WN, H, EU><<<dim3(t.m * t.n, parts), WM * WN * 64, 0, st>>>(a, t);
+    const int blocks = (int)(((int64_t)a.M * (t.ld / 4) + 255) / 256);
+    if (parts == 2) gemm8_join<2><<<blocks, 256, 0, st>>>(a, sums, t.ld);
+    else if (parts == 3) gemm8_join<3><<<blocks, 256, 0, st>>>(a, sums, t.ld);
+    else if (parts == 4) gemm8_join<4><<<blocks, 256, 0, st>>>(a, sums, t.ld);
+    else if (parts == 6) gemm8_join<6><<<blocks, 256, 0, st>>>(a, sums, t.ld);
+    else if (parts == 8) gemm8_join<8><<<blocks, 256, 0, st>>>(a, sums, t.ld);
+}
+
+// Few tokens: 16 tokens x 16 channels a workgroup, K over its W waves. Operands go from memory to the products' registers, U units
+// of 64 bytes of K ahead; the waves' sums meet in LDS.
+template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm8Args a) {
+#if __HIP_DEVICE_COMPILE__
+    __shared__ i4 sums[W][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+    const Rows x = rows_at(a.x, a.ldx, m0, a.M, 16), w = rows_at(a.w, a.ldw, n0, a.N, 16);
+    const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc((void *)x.p, 0, x.bytes, 0x00027000);
+    const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc((void *)w.p, 0, w.bytes, 0x00027000);
+    const uint32_t xat = (uint32_t)col * (uint32_t)a.ldx + g * 16, wat = (uint32_t)col * (uint32_t)a.ldw + g * 16;
+    struct Part {
+        i4 w[U], x[U];
+    };
+    const int units = (a.K + 63) / 64, per = (units + W - 1) / W, first = wave * per;
+    const int end = first + per < units ? first + per : units;
+    auto load = [&](int u0, Part &p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = (u0 + u) * 64;
+            const uint32_t past = u0 + u < end && k + g * 16 < a.K ? 0u : 1u << 31;  // (of another wave, or past K: zeros)
+            p.w[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(wb, wat | past, k, 0));
+            p.x[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(xb, xat | past, k, 0));
+        }
+    };
+    i4 acc = {0, 0, 0, 0};
+    auto multiply = [&](const Part &p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(p.w[u], p.x[u], acc, 0, 0, 0);
+    };
+    Part p0, p1;
+    load(first, p0);
+    for (int u = first; u < end; u += 2 * U) {
+        load(u + U, p1);
+        multiply(p0);
+        load(u + 2 * U, p0);
+        multiply(p1);
+    }
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int i = 1; i < W; i++) acc += sums[i][lane];
+    const int m = m0 + col, n = n0 + 4 * g;  // (a lane's sums are 4 channels of one token)
+    if (m >= a.M || n >= a.N) return;
+    const float xs = a.x_scale[m];
+    f4 r;
+#pragma unroll
+    for (int c = 0; c < 4; c++) r[c] = n + c < a.N ? (float)acc[c] * xs * a.w_scale[n + c] : 0.f;
+    put(a, m, n, r, (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0, false);
+#endif
+}
+
+template <int W, int U> void few(const Gemm8Args &a, hipStream_t st) {
+    gemm8_few<W, U><<<dim3((a.N + 15) / 16, (a.M + 15) / 16), W * 64, 0, st>>>(a);
+}
+
+// Which kernel, and into how many parts K goes: the one whose time comes out shortest. A launch is rounds of workgroups; a round
+// takes `start` for its first loads and its results, and for each stage `alone` where it leaves most of the chip's memory paths
+// to few workgroups, `full` where it fills the chip (us, fitted to 20 products of 16 to 4096 tokens, 1024 to 24576 channels, K
+// 2048 to 12288: the choice is at most 18% behind the best of these kernels there, mostly below 5).
+struct Shape {
+    int tile, at_once;
+    double start, alone, full;
+};
+constexpr Shape shapes[] = {
+    {64, 512, 3.5, 0.18, 0.39},   // 9 places of 8 KiB, two workgroups a CU
+    {128, 256, 5.0, 0.36, 0.58},  // 9 places of 16 KiB
+    {128, 512, 4.5, 0.50, 1.09},  // 5 places of 16 KiB, two workgroups a CU
+    {256, 256, 9.4, 0.95, 1.60},  // 5 places of 32 KiB
+};
+struct Plan {
+    int shape, parts;  // shape -1: gemm8_few
+};
+Plan plan_of(const Gemm8Args &a) {
+    const double weights = 1.0 + (double)a.N * a.K / 5.0e6;  // reading them, at 5 TB/s
+    const int64_t few_wgs = (int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16);
+    const double few_us = 2.5 + (double)few_wgs * (16 + (a.M < 16 ? a.M : 16)) * a.K / 8.5e6;  // operands through the L2s at 8.5 TB/s
+    Plan best{-1, 1};
+    double best_us = few_us > weights ? few_us : weights;
+    for (int i = 0; i < 4; i++)
+        for (const int parts : {1, 2, 3, 4, 6, 8}) {
+            const Shape &s = shapes[i];
+            const int64_t wgs = (int64_t)((a.M + s.tile - 1) / s.tile) * ((a.N + s.tile - 1) / s.tile) * parts;
+            const int stages = ((a.K + KB - 1) / KB + parts - 1) / parts;
+            const int64_t bytes = (int64_t)parts * a.M * ((a.N + 3) / 4 * 4) * 4;
+            if (parts > 1 && (stages < 8 || bytes > (int64_t)64 << 20)) break;
+            const double rest = (double)(wgs % s.at_once) / s.at_once;
+            double us = (double)(wgs / s.at_once) * (s.start + stages * s.full);
+            if (rest > 0) us += s.start + stages * (s.alone + (s.full - s.alone) * rest);
+            if (us < weights) us = weights;
+            if (parts > 1) us += 2.5 + 2.0 * (double)bytes / 8.0e6;  // (sums written and read, and a launch more)
+            if (us < best_us) best_us = us, best = Plan{i, parts};
+        }
+    return best;
 }
 
 }  // namespace
 
-size_t gemm8_ws(const Gemm8Args &) { return 0; }
+size_t gemm8_ws(const Gemm8Args &a) {
+    const Plan p = plan_of(a);
+    return p.parts > 1 ? (size_t)p.parts * a.M * ((a.N + 3) / 4 * 4) * 4 : 0;
+}
 
-hipError_t launch_gemm8(const Gemm8Args &a, void *, hipStream_t st) {
-    const int tm = (a.M + 63) / 64, tn = (a.N + 127) / 128;
-    gemm8_tile<64, 128, 2, 2><<<tm * tn, 256, 0, st>>>(a, tm);
+hipError_t launch_gemm8(const Gemm8Args &a, void *ws, hipStream_t st) {
+    const Plan p = plan_of(a);
+    if (p.shape < 0) few<8, 2>(a, st);
+    else if (p.shape == 0) tiles<64, 2, 2, 9, 2>(a, p.parts, (int *)ws, st);
+    else if (p.shape == 1) tiles<128, 2, 4, 9, 2>(a, p.parts, (int *)ws, st);
+    else if (p.shape == 2) tiles<128, 2, 4, 5, 4>(a, p.parts, (int *)ws, st);
+    else tiles<256, 2, 4, 5, 2>(a, p.parts, (int *)ws, st);
     return hipGetLastError();
 }
