@@ -117,7 +117,13 @@ template <int ACT> __device__ __forceinline__ void wide_row(const Quant8Args &a,
 template <int ACT> constexpr float NEAR = ACT == Q8_SILU_MUL ? 2e-4f : 4e-5f;
 
 // 4 values at column c of a row, the residual's additions made and stored
-__device__ __forceinline__ f4 take4(const Quant8Args &a, int64_t row, int c, bool adds) {
+template <bool STREAM> __device__ __forceinline__ f4 take4(const Quant8Args &a, int64_t row, int c, bool adds) {
+    if constexpr (STREAM) {  // (x and one slice)
+        f4 *x = (f4 *)(a.x + row * a.ldx + c);
+        const f4 v = __builtin_nontemporal_load(x) + __builtin_nontemporal_load((const f4 *)(a.add + row * a.K + c));
+        __builtin_nontemporal_store(v, x);
+        return v;
+    }
     f4 v = input4(a, row, c);
     if (adds) {
         const float *add = a.add + row * a.K + c;
@@ -129,21 +135,30 @@ __device__ __forceinline__ f4 take4(const Quant8Args &a, int64_t row, int c, boo
     return v;
 }
 
-// x to t in fp32, with the sum of squares of x and the largest |t|, as bits (as whole numbers NaN is the largest)
-template <int ACT> __device__ __forceinline__ f4 to_t(f4 x, f4 w, float &ssq, uint32_t &top) {
+// What a thread has found of its row: the sum of squares of x, and the largest |t| in fp32, as bits (as whole numbers NaN is the
+// largest); for a norm with weights the largest exact product besides.
+struct Found {
+    float ssq = 0.f;
+    uint32_t top = 0;
+    double most = 0.0;
+};
+
+// x to t in fp32
+template <int ACT> __device__ __forceinline__ f4 to_t(f4 x, f4 w, bool weights, Found &f) {
     f4 t = x;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         if constexpr (ACT == Q8_RMSNORM) {
-            ssq = __builtin_fmaf(x[j], x[j], ssq);
+            f.ssq = __builtin_fmaf(x[j], x[j], f.ssq);
             t[j] = x[j] * w[j];
+            if (weights) f.most = fmax(f.most, fabs((double)x[j] * (double)w[j]));
         } else if constexpr (ACT == Q8_SILU_MUL) {
             t[j] = x[j] * __builtin_amdgcn_rcpf(1.f + expf(-x[j])) * w[j];
             // (exp(-x) passes fp32 there; what is lost counts only beside so large an up)
-            if (x[j] < -80.f && fabsf(w[j]) > 1e8f) top = 0x7fffffffu;
+            if (x[j] < -80.f && fabsf(w[j]) > 1e8f) f.top = 0x7fffffffu;
         }
         const uint32_t b = __float_as_uint(t[j]) & 0x7fffffffu;
-        top = top > b ? top : b;
+        f.top = f.top > b ? f.top : b;
     }
     return t;
 }
@@ -178,55 +193,65 @@ __device__ __forceinline__ uint32_t codes4(const Quant8Args &a, int64_t row, int
 }
 
 // One workgroup a row, V x 4 values a thread kept in registers; V = 0: rows of any length, read a second time for the codes.
-template <int ACT, int V> __global__ __launch_bounds__(1024) void quant8_kernel(Quant8Args a) {
+template <int ACT, int V, bool STREAM = false> __global__ __launch_bounds__(1024) void quant8_kernel(Quant8Args a) {
     __shared__ Quant8Shared sh;
     constexpr int KEPT = V ? V : 1;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, n4 = a.K / 4, nt = blockDim.x;
     const bool adds = ACT != Q8_SILU_MUL && a.x && a.add;
+    // (the norm's exact largest: on the way where a row is a workgroup's latency, of the candidates alone where rows are many:
+    // 8190 rows of 4096 36.3 us and 34.0)
+    constexpr bool DIRECT = ACT == Q8_RMSNORM && (V == 1 || V == 2);
+    const bool weights = DIRECT && a.norm_w;
     f4 t[KEPT];
-    uint32_t top = 0;
-    float ssq = 0.f;
+    Found f;
     if constexpr (V > 0) {
         f4 w[V];
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const int c = tid + i * nt;
-            t[i] = c < n4 ? take4(a, row, 4 * c, adds) : f4{0, 0, 0, 0};
+            t[i] = c < n4 ? take4<STREAM>(a, row, 4 * c, adds) : f4{0, 0, 0, 0};
             w[i] = c < n4 ? second4<ACT>(a, row, 4 * c) : f4{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int i = 0; i < V; i++) t[i] = to_t<ACT>(t[i], w[i], ssq, top);
+        for (int i = 0; i < V; i++) t[i] = to_t<ACT>(t[i], w[i], weights, f);
     } else {
         for (int c = tid; c < n4; c += nt) {
-            const f4 x = take4(a, row, 4 * c, adds);
-            to_t<ACT>(x, second4<ACT>(a, row, 4 * c), ssq, top);
+            const f4 x = take4<STREAM>(a, row, 4 * c, adds);
+            to_t<ACT>(x, second4<ACT>(a, row, 4 * c), weights, f);
         }
     }
     auto again = [&](int c) __attribute__((always_inline)) {
-        float s = 0.f;
-        uint32_t b = 0;
-        return to_t<ACT>(input4(a, row, 4 * c), second4<ACT>(a, row, 4 * c), s, b);
+        Found none;
+        return to_t<ACT>(input4(a, row, 4 * c), second4<ACT>(a, row, 4 * c), false, none);
     };
-    top = wave_umax(top);
-    if (ACT == Q8_RMSNORM) ssq = wave_sum(ssq);
-    if ((tid & 63) == 0) sh.top[tid >> 6] = top, sh.ssq[tid >> 6] = ssq;
+    f.top = wave_umax(f.top);
+    if constexpr (ACT == Q8_RMSNORM) {
+        f.ssq = wave_sum(f.ssq);
+        if (weights)
+            for (int o = 32; o > 0; o >>= 1) f.most = fmax(f.most, __shfl_xor(f.most, o));
+    }
+    if ((tid & 63) == 0) sh.top[tid >> 6] = f.top, sh.ssq[tid >> 6] = f.ssq, sh.dssq[tid >> 6] = f.most;
     if (tid == 0) sh.most = 0;
     __syncthreads();
-    top = sh.top[0], ssq = sh.ssq[0];
+    uint32_t top = sh.top[0];
+    float ssq = sh.ssq[0];
+    double most = sh.dssq[0];
     for (int i = 1; i < (nt >> 6); i++) {
         top = top > sh.top[i] ? top : sh.top[i];
         ssq += sh.ssq[i];
+        most = fmax(most, sh.dssq[i]);
     }
     const float ftop = __uint_as_float(top);
     if (!(ftop > 1e-20f && ftop < 1e30f) || (ACT == Q8_RMSNORM && !(ssq > 1e-30f && ssq < 1e30f))) {
+        __syncthreads();  // (sh is read)
         wide_row<ACT>(a, row, sh);
         return;
     }
-    double most = (double)ftop;
-    if (ACT == Q8_SILU_MUL || (ACT == Q8_RMSNORM && a.norm_w)) {
-        // the exact largest |t|: among those whose fp32 value is the largest (a product's rounding keeps the order), or within
-        // twice the gate's error of it
+    if (!weights) most = (double)ftop;
+    if (ACT == Q8_SILU_MUL || (!DIRECT && ACT == Q8_RMSNORM && a.norm_w)) {
+        // the exact largest |t| is among those whose fp32 value is the largest (a product's rounding keeps the order), or within
+        // twice the fp32 gate's error of it
         const float from = ACT == Q8_SILU_MUL ? ftop * (1.f - 0x1p-18f) : ftop;
         if constexpr (V > 0) {
 #pragma unroll
@@ -253,8 +278,18 @@ template <int ACT, int V> __global__ __launch_bounds__(1024) void quant8_kernel(
 
 template <int ACT> void launch(const Quant8Args &a, hipStream_t st) {
     const int n4 = a.K / 4;
-    const int v = n4 > 4096 ? 0 : a.M > 256 || n4 > 2048 ? 4 : n4 > 1024 ? 2 : 1;
+    // few values a thread where rows are few and a row's time is latency; four times 4 where they are many (8190 rows of 4096: 34 us,
+    // with one 83), as far as a wave has them
+    const int v = n4 > 4096 ? 0 : n4 > 2048 ? 4 : a.M <= 256 ? (n4 > 1024 ? 2 : 1) : n4 > 128 ? 4 : n4 > 64 ? 2 : 1;
     const int nt = v ? ((n4 + v - 1) / v + 63) / 64 * 64 : 1024;
+    if constexpr (ACT == Q8_RMSNORM) {
+        // rows that are read, added to and written past the caches, from 64 MB of them on (8190 of 4096: 75.7 us, 81.4 through them;
+        // 515: 9.0 and 8.1)
+        if (v == 4 && a.x && a.n_add == 1 && (int64_t)a.M * a.K >= (int64_t)16 << 20) {
+            quant8_kernel<ACT, 4, true><<<a.M, nt, 0, st>>>(a);
+            return;
+        }
+    }
     if (v == 1) quant8_kernel<ACT, 1><<<a.M, nt, 0, st>>>(a);
     else if (v == 2) quant8_kernel<ACT, 2><<<a.M, nt, 0, st>>>(a);
     else if (v == 4) quant8_kernel<ACT, 4><<<a.M, nt, 0, st>>>(a);

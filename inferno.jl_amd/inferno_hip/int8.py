@@ -12,52 +12,90 @@ workspace that is given serves one call at a time.
 from __future__ import annotations
 
 import ctypes as C
+from struct import Struct
 
-from . import _lib, mixers
+from . import _lib
 from .formats import BLOCK_BYTES, BLOCK_ELEMS
-from .mixers import _call, _device_of, _on, _refuse, _rows, _torch, _whole, _workspace
-from .quantized_kernels import ACT_PLAIN, ACT_RMSNORM, ACT_SILU_MUL, GEMM_ACCUM, check_tensor, dequant, made_for
+from .mixers import _device_of, _refuse, _rows, _torch, _whole, _workspace
+from .quantized_kernels import ACT_PLAIN, ACT_RMSNORM, ACT_SILU_MUL, GEMM_ACCUM, _raw_stream, check_tensor, dequant, made_for
 
-_i8 = None
+_i8 = _u8 = _f32 = _Tensor = _current_device = _stream_of = _c_quantize = _c_gemm = None
+_INPUT = Struct("@PiiPfPiq").pack  # ihip_gemm_input (a call's host time is most of a small one's: a ctypes Structure takes longer)
 
 
 def _names():
-    """torch's names, looked up once."""
-    global _i8
+    """torch's and the library's names, looked up once."""
+    global _i8, _u8, _f32, _Tensor, _current_device, _stream_of, _c_quantize, _c_gemm
     import torch
     _torch()
-    _i8 = torch.int8
+    lib = _lib.load()
+    _c_quantize, _c_gemm = lib.ihip_quantize_i8, lib.ihip_gemm_i8
+    _current_device, _stream_of, _Tensor = torch.cuda.current_device, _raw_stream(), torch.Tensor
+    _u8, _f32 = torch.uint8, torch.float32
+    _i8 = torch.int8  # (last: what the calls look at)
+
+
+def _on(stream, dev: int) -> int:
+    return _stream_of(dev) if stream is None else getattr(stream, "cuda_stream", stream)
+
+
+def _refuse_codes(t, name: str, rows, k, dev: int):
+    if not isinstance(t, _Tensor) or t.dtype is not _i8 or t.get_device() != dev:
+        _refuse(t, name, _i8, None, False, dev)
+    raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {'k' if k is None else f'>= {k}'}] int8 with "
+                     f"unit column stride, got {tuple(t.shape)} of strides {t.stride()}")
 
 
 def _codes(t, name: str, rows: int | None, k: int | None, dev: int):
     """t as int8 [rows, k or more] with unit column stride on device dev; its address, rows, columns and row stride."""
-    if not isinstance(t, mixers._Tensor) or t.dtype is not _i8 or t.get_device() != dev:
-        _refuse(t, name, _i8, None, False, dev)
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or shape[0] < 1 or (rows is not None and shape[0] != rows) or shape[1] < (k or 1) or stride[1] != 1:
-        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {'k' if k is None else f'>= {k}'}] int8 with "
-                         f"unit column stride, got {tuple(shape)} of strides {stride}")
-    return t.data_ptr(), shape[0], shape[1], stride[0] if shape[0] > 1 else max(stride[0], (shape[1] + 15) // 16 * 16)
+    if not isinstance(t, _Tensor) or t.dtype is not _i8 or t.get_device() != dev or t.dim() != 2:
+        _refuse_codes(t, name, rows, k, dev)
+    m, n = t.shape
+    ld, one = t.stride()
+    if one != 1 or m < 1 or (rows is not None and m != rows) or n < (k or 1):
+        _refuse_codes(t, name, rows, k, dev)
+    return t.data_ptr(), m, n, ld if m > 1 else (n + 15) // 16 * 16
 
 
-def _quantize(x, act: int, k: int, norm_w, eps: float, add, out, scales, stream):
-    dev = _device_of(x, "x")
-    xp, rows, ldx = _rows(x, "x", 2 * k if act == ACT_SILU_MUL else k, None, dev)
-    a = _lib.GemmInput(xp, ldx, act, None, eps, None, 0, 0)
-    if norm_w is not None:
-        a.norm_w = _whole(norm_w, "norm_w", mixers._f32, (k,), dev)
-    if add is not None:
-        if isinstance(add, mixers._Tensor) and add.dim() == 2:
-            add = add[None]
-        n = add.shape[0] if isinstance(add, mixers._Tensor) and add.dim() == 3 else 1
-        a.add, a.n_add, a.add_stride = _whole(add, "add", mixers._f32, (n, rows, k), dev), n, rows * k
+def _quantize(x, act: int, norm_w, eps: float, add, out, scales, stream):
+    if _i8 is None:
+        _names()
+    if not isinstance(x, _Tensor) or x.dim() != 2:
+        raise ValueError("rows must be a float32 GPU tensor [M, K]")
+    rows, k = x.shape
+    if act == ACT_SILU_MUL:
+        if k % 2:
+            raise ValueError(f"gate_up has {k} columns: gate, then up")
+        k //= 2
+    dev = x.get_device()
+    if dev < 0 or dev != _current_device():
+        _device_of(x, "x")
+    ldx, one = x.stride()
+    if x.dtype is not _f32 or one != 1 or rows < 1 or k < 1 or ldx > 0x7fffffff:
+        _rows(x, "x", k, None, dev)
+        raise ValueError(f"x of strides {x.stride()}: unit column stride, rows up to 2^31 values apart")
+    if rows == 1:
+        ldx = x.shape[1]
+    wp = 0 if norm_w is None else _whole(norm_w, "norm_w", _f32, (k,), dev)
+    if add is None:
+        ap, n = 0, 0
+    else:
+        if isinstance(add, _Tensor) and add.dim() == 2:
+            n, shape = 1, (rows, k)
+        else:
+            n = add.shape[0] if isinstance(add, _Tensor) and add.dim() == 3 else 1
+            shape = (n, rows, k)
+        ap = _whole(add, "add", _f32, shape, dev)
     if out is None:
         out = made_for(stream, x.new_empty, (rows, k), dtype=_i8)
     if scales is None:
         scales = made_for(stream, x.new_empty, rows)
     qp, _, _, ldq = _codes(out, "out", rows, k, dev)
-    sp = _whole(scales, "scales", mixers._f32, (rows,), dev)
-    _lib.check(_call("ihip_quantize_i8")(C.byref(a), rows, k, qp, ldq, sp, _on(stream, dev)))
+    sp = _whole(scales, "scales", _f32, (rows,), dev)
+    rc = _c_quantize(_INPUT(x.data_ptr(), ldx, act, wp, eps, ap, n, rows * k), rows, k, qp, ldq, sp,
+                     _stream_of(dev) if stream is None else _on(stream, dev))
+    if rc:
+        _lib.check(rc)
     return out, scales
 
 
@@ -66,33 +104,18 @@ def quantize_i8(x, out=None, scales=None, stream=None):
     codes [M, K] and float32 scales [M]: scales[m] = max |x[m]| / 127, codes
     the nearest, ties to even. A row of zeros has scale 0, one with a value
     that is not finite scale NaN, both codes 0."""
-    if _i8 is None:
-        _names()
-    return _quantize(x, ACT_PLAIN, _columns(x), None, 0.0, None, out, scales, stream)
+    return _quantize(x, ACT_PLAIN, None, 0.0, None, out, scales, stream)
 
 
 def rmsnorm_i8(x, norm_w=None, eps: float = 1e-6, add=None, out=None, scales=None, stream=None):
     """RMSNorm(x) * norm_w of rows x [M, K] as codes and scales. add, [M, K] or
     [n, M, K]: the slices are added to x first, in place."""
-    if _i8 is None:
-        _names()
-    return _quantize(x, ACT_RMSNORM, _columns(x), norm_w, eps, add, out, scales, stream)
+    return _quantize(x, ACT_RMSNORM, norm_w, eps, add, out, scales, stream)
 
 
 def silu_mul_i8(gate_up, out=None, scales=None, stream=None):
     """silu(gate) * up of rows [gate | up] (gate_up [M, 2 K]) as codes [M, K] and scales."""
-    if _i8 is None:
-        _names()
-    n = _columns(gate_up)
-    if n % 2:
-        raise ValueError(f"gate_up has {n} columns: gate, then up")
-    return _quantize(gate_up, ACT_SILU_MUL, n // 2, None, 0.0, None, out, scales, stream)
-
-
-def _columns(x) -> int:
-    if not isinstance(x, mixers._Tensor) or x.dim() != 2:
-        raise ValueError("rows must be a float32 GPU tensor [M, K]")
-    return x.shape[1]
+    return _quantize(gate_up, ACT_SILU_MUL, None, 0.0, None, out, scales, stream)
 
 
 def quantize_weights_i8(qtype: int, w_dev, n: int, k: int, stream=None):
@@ -135,11 +158,13 @@ def gemm_i8(q, scales, w, w_scales, accum: bool = False, out=None, ws=None, stre
     apart, K a multiple of 16), scales float32 [M] and [N]. Any M and N."""
     if _i8 is None:
         _names()
-    dev = _device_of(q, "q")
+    dev = q.get_device() if isinstance(q, _Tensor) else -1
+    if dev < 0 or dev != _current_device():
+        _device_of(q, "q")
     wp, n, k, ldw = _codes(w, "w", None, None, dev)
     qp, m, _, ldq = _codes(q, "q", None, k, dev)
-    sp = _whole(scales, "scales", mixers._f32, (m,), dev)
-    wsp = _whole(w_scales, "w_scales", mixers._f32, (n,), dev)
+    sp = _whole(scales, "scales", _f32, (m,), dev)
+    wsp = _whole(w_scales, "w_scales", _f32, (n,), dev)
     if out is None:
         if accum:
             raise ValueError("accum adds to out: pass it")
@@ -148,7 +173,9 @@ def gemm_i8(q, scales, w, w_scales, accum: bool = False, out=None, ws=None, stre
     flags = GEMM_ACCUM if accum else 0
     if ws is None:
         need = _ws_bytes(m, n, k, flags)
-        ws = made_for(stream, scales.new_empty, need, dtype=mixers._u8, returned=False) if need else None
+        ws = made_for(stream, scales.new_empty, need, dtype=_u8, returned=False) if need else None
     tp, tn = (None, 0) if ws is None else _workspace(ws, dev)
-    _lib.check(_call("ihip_gemm_i8")(qp, ldq, sp, wp, ldw, wsp, yp, ldy, m, n, k, flags, tp, tn, _on(stream, dev)))
+    rc = _c_gemm(qp, ldq, sp, wp, ldw, wsp, yp, ldy, m, n, k, flags, tp, tn, _stream_of(dev) if stream is None else _on(stream, dev))
+    if rc:
+        _lib.check(rc)
     return out
