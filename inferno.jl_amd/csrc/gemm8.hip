@@ -58,12 +58,11 @@ struct Tiling {
 };
 
 // 4 channels of one token into y
-__device__ __forceinline__ void put(const Gemm8Args &a, int m, int n, f4 r, bool vec, bool stream) {
+__device__ __forceinline__ void put(const Gemm8Args &a, int m, int n, f4 r, bool vec) {
     float *y = a.y + (int64_t)m * a.ldy + n;
     if (vec && n + 4 <= a.N) {
         if (a.accum) r += *(const f4 *)y;
-        if (stream) __builtin_nontemporal_store(r, (f4 *)y);
-        else *(f4 *)y = r;
+        *(f4 *)y = r;
     } else {
 #pragma unroll
         for (int c = 0; c < 4; c++)
@@ -190,47 +189,69 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
     multiply(p1);
     // A part of 32 x 32 at a time through LDS (each wave its own 4 KiB): a lane's accumulators are 4 channels of one token, four
     // times; rows of 128 bytes go to memory, 8 of them with an instruction. (Parts of lines cost as much as whole ones.)
-    meet<0>();
-    char *const own = wave < BYTES / 4096 ? lds0 + wave * 4096 : lds1 + (wave - BYTES / 4096) * 4096;
     const int m0 = tm * B + wm * TM * 32, n0 = tn * B + wn * TN * 32;
     const int er = lane >> 3, en = (lane & 7) * 4;  // this lane's row of 8, its 4 channels
     const bool vec = (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0;
     int *const part = t.sums ? t.sums + (int64_t)blockIdx.y * a.M * t.ld : nullptr;
     float xs[TM][4];
+    f4 ws[TN];
 #pragma unroll
-    for (int j = 0; j < TM; j++)
+    for (int j = 0; j < TM; j++)  // (all on their way at once; past the ends the last)
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int m = m0 + j * 32 + 8 * u + er;
-            xs[j][u] = m < a.M ? a.x_scale[m] : 0.f;
+            xs[j][u] = a.x_scale[m < a.M ? m : a.M - 1];
         }
 #pragma unroll
-    for (int i = 0; i < TN; i++) {
-        const int n = n0 + i * 32 + en;
-        f4 ws;
+    for (int i = 0; i < TN; i++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) ws[c] = n + c < a.N ? a.w_scale[n + c] : 0.f;
+        for (int c = 0; c < 4; c++) {
+            const int n = n0 + i * 32 + en + c;
+            ws[i][c] = a.w_scale[n < a.N ? n : a.N - 1];
+        }
+    // what is added to, a part ahead of its sums
+    f4 was[2][4];
+    auto ahead = [&](int part_no) __attribute__((always_inline)) {
+        const int i = part_no / TM, j = part_no % TM, n = n0 + i * 32 + en;
 #pragma unroll
-        for (int j = 0; j < TM; j++) {
-            const i16 v = acc[i][j];
+        for (int u = 0; u < 4; u++) {
+            const int m = m0 + j * 32 + 8 * u + er;
+            was[part_no & 1][u] = f4{0, 0, 0, 0};
+            if (a.accum && vec && !part && m < a.M && n + 4 <= a.N) was[part_no & 1][u] = *(const f4 *)(a.y + (int64_t)m * a.ldy + n);
+        }
+    };
+    ahead(0);
+    meet<0>();
+    char *const own = wave < BYTES / 4096 ? lds0 + wave * 4096 : lds1 + (wave - BYTES / 4096) * 4096;
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-                *(i4 *)(own + col * 128 + (((2 * q + g) ^ (col & 7)) << 4)) = i4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-            i4 o[4];
+    for (int p = 0; p < TN * TM; p++) {
+        const int i = p / TM, j = p % TM, n = n0 + i * 32 + en;
+        if (p + 1 < TN * TM) ahead(p + 1);
+        const i16 v = acc[i][j];
 #pragma unroll
-            for (int u = 0; u < 4; u++) o[u] = *(const i4 *)(own + (8 * u + er) * 128 + (((lane & 7) ^ er) << 4));
+        for (int q = 0; q < 4; q++)
+            *(i4 *)(own + col * 128 + (((2 * q + g) ^ (col & 7)) << 4)) = i4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        i4 o[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int m = m0 + j * 32 + 8 * u + er;
-                if (m >= a.M) continue;
-                if (part) {
-                    if (n < t.ld) *(i4 *)(part + (int64_t)m * t.ld + n) = o[u];
-                    continue;
-                }
-                f4 r;
+        for (int u = 0; u < 4; u++) o[u] = *(const i4 *)(own + (8 * u + er) * 128 + (((lane & 7) ^ er) << 4));
 #pragma unroll
-                for (int c = 0; c < 4; c++) r[c] = (float)o[u][c] * xs[j][u] * ws[c];
-                put(a, m, n, r, vec, t.stream);
+        for (int u = 0; u < 4; u++) {
+            const int m = m0 + j * 32 + 8 * u + er;
+            if (m >= a.M) continue;
+            if (part) {
+                if (n < t.ld) *(i4 *)(part + (int64_t)m * t.ld + n) = o[u];
+                continue;
+            }
+            f4 r;
+#pragma unroll
+            for (int c = 0; c < 4; c++) r[c] = (float)o[u][c] * xs[j][u] * ws[i][c];
+            if (vec && n + 4 <= a.N) {
+                r += was[p & 1][u];
+                f4 *y = (f4 *)(a.y + (int64_t)m * a.ldy + n);
+                if (t.stream) __builtin_nontemporal_store(r, y);
+                else *y = r;
+            } else {
+                put(a, m, n, r, false);
             }
         }
     }
@@ -253,7 +274,7 @@ template <int P> __global__ __launch_bounds__(256) void gemm8_join(Gemm8Args a, 
     for (int i = 1; i < P; i++) v[0] += v[i];
 #pragma unroll
     for (int c = 0; c < 4; c++) r[c] = (float)v[0][c] * xs * ws[c];
-    put(a, m, n, r, (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0, false);
+    put(a, m, n, r, (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0);
 }
 
 template <int B, int WM, int WN, int H, int EU> void tiles(const Gemm8Args &a, int parts, int *sums, hipStream_t st) {
@@ -287,6 +308,17 @@ template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm
     struct Part {
         i4 w[U], x[U];
     };
+    // the first wave's scales and what it adds to, on their way first
+    const int m = m0 + col, n = n0 + 4 * g;
+    const bool there = m < a.M && n < a.N, vec = (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0 && n + 4 <= a.N;
+    float xs = 0.f;
+    f4 ws = {0, 0, 0, 0}, was = {0, 0, 0, 0};
+    if (wave == 0 && there) {
+        xs = a.x_scale[m];
+#pragma unroll
+        for (int c = 0; c < 4; c++) ws[c] = a.w_scale[n + c < a.N ? n + c : a.N - 1];
+        if (a.accum && vec) was = *(const f4 *)(a.y + (int64_t)m * a.ldy + n);
+    }
     const int units = (a.K + 63) / 64, per = (units + W - 1) / W, first = wave * per;
     const int end = first + per < units ? first + per : units;
     auto load = [&](int u0, Part &p) __attribute__((always_inline)) {
@@ -316,13 +348,12 @@ template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm
     if (wave) return;
 #pragma unroll
     for (int i = 1; i < W; i++) acc += sums[i][lane];
-    const int m = m0 + col, n = n0 + 4 * g;  // (a lane's sums are 4 channels of one token)
-    if (m >= a.M || n >= a.N) return;
-    const float xs = a.x_scale[m];
-    f4 r;
+    if (!there) return;
+    f4 r;  // (a lane's sums are 4 channels of one token)
 #pragma unroll
-    for (int c = 0; c < 4; c++) r[c] = n + c < a.N ? (float)acc[c] * xs * a.w_scale[n + c] : 0.f;
-    put(a, m, n, r, (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0, false);
+    for (int c = 0; c < 4; c++) r[c] = (float)acc[c] * xs * ws[c];
+    if (vec) *(f4 *)(a.y + (int64_t)m * a.ldy + n) = r + was;
+    else put(a, m, n, r, false);
 #endif
 }
 
@@ -379,7 +410,7 @@ size_t gemm8_ws(const Gemm8Args &a) {
 
 hipError_t launch_gemm8(const Gemm8Args &a, void *ws, hipStream_t st) {
     const Plan p = plan_of(a);
-    if (p.shape < 0) few<8, 2>(a, st);
+    if (p.shape < 0) few<4, 2>(a, st);
     else if (p.shape == 0) tiles<64, 2, 2, 9, 2>(a, p.parts, (int *)ws, st);
     else if (p.shape == 1) tiles<128, 2, 4, 9, 2>(a, p.parts, (int *)ws, st);
     else if (p.shape == 2) tiles<128, 2, 4, 5, 4>(a, p.parts, (int *)ws, st);

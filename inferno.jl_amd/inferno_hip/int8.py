@@ -90,9 +90,18 @@ def _quantize(x, act: int, norm_w, eps: float, add, out, scales, stream):
         out = made_for(stream, x.new_empty, (rows, k), dtype=_i8)
     if scales is None:
         scales = made_for(stream, x.new_empty, rows)
-    qp, _, _, ldq = _codes(out, "out", rows, k, dev)
-    sp = _whole(scales, "scales", _f32, (rows,), dev)
-    rc = _c_quantize(_INPUT(x.data_ptr(), ldx, act, wp, eps, ap, n, rows * k), rows, k, qp, ldq, sp,
+    try:
+        (m, kq), (ldq, q1) = out.shape, out.stride()
+        fine = (out.dtype is _i8 and m == rows and kq >= k and q1 == 1 and out.get_device() == dev and scales.dtype is _f32
+                and scales.shape == (rows,) and scales.get_device() == dev and scales.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        fine = False
+    if not fine:  # (which of them is not, by name)
+        _, _, kq, ldq = _codes(out, "out", rows, k, dev)
+        _whole(scales, "scales", _f32, (rows,), dev)
+    if rows == 1:  # (a single row's stride has no meaning)
+        ldq = (kq + 15) // 16 * 16
+    rc = _c_quantize(_INPUT(x.data_ptr(), ldx, act, wp, eps, ap, n, rows * k), rows, k, out.data_ptr(), ldq, scales.data_ptr(),
                      _stream_of(dev) if stream is None else _on(stream, dev))
     if rc:
         _lib.check(rc)
@@ -158,13 +167,23 @@ def gemm_i8(q, scales, w, w_scales, accum: bool = False, out=None, ws=None, stre
     apart, K a multiple of 16), scales float32 [M] and [N]. Any M and N."""
     if _i8 is None:
         _names()
-    dev = q.get_device() if isinstance(q, _Tensor) else -1
-    if dev < 0 or dev != _current_device():
-        _device_of(q, "q")
-    wp, n, k, ldw = _codes(w, "w", None, None, dev)
-    qp, m, _, ldq = _codes(q, "q", None, k, dev)
-    sp = _whole(scales, "scales", _f32, (m,), dev)
-    wsp = _whole(w_scales, "w_scales", _f32, (n,), dev)
+    try:
+        (n, k), (m, kq), (ldw, w1), (ldq, q1) = w.shape, q.shape, w.stride(), q.stride()
+        dev = q.get_device()
+        fine = (dev >= 0 and dev == _current_device() and q.dtype is _i8 and w.dtype is _i8 and w1 == 1 and q1 == 1 and kq >= k > 0
+                and w.get_device() == dev and m > 0 and n > 0 and scales.dtype is _f32 and scales.shape == (m,)
+                and scales.get_device() == dev and scales.is_contiguous() and w_scales.dtype is _f32 and w_scales.shape == (n,)
+                and w_scales.get_device() == dev and w_scales.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        fine = False
+    if not fine:  # (which of them is not, by name)
+        dev = _device_of(q, "q")
+        _, n, k, ldw = _codes(w, "w", None, None, dev)
+        _, m, _, ldq = _codes(q, "q", None, k, dev)
+        _whole(scales, "scales", _f32, (m,), dev)
+        _whole(w_scales, "w_scales", _f32, (n,), dev)
+    elif m == 1:  # (a single row's stride has no meaning)
+        ldq = (kq + 15) // 16 * 16
     if out is None:
         if accum:
             raise ValueError("accum adds to out: pass it")
@@ -175,7 +194,8 @@ def gemm_i8(q, scales, w, w_scales, accum: bool = False, out=None, ws=None, stre
         need = _ws_bytes(m, n, k, flags)
         ws = made_for(stream, scales.new_empty, need, dtype=_u8, returned=False) if need else None
     tp, tn = (None, 0) if ws is None else _workspace(ws, dev)
-    rc = _c_gemm(qp, ldq, sp, wp, ldw, wsp, yp, ldy, m, n, k, flags, tp, tn, _stream_of(dev) if stream is None else _on(stream, dev))
+    rc = _c_gemm(q.data_ptr(), ldq, scales.data_ptr(), w.data_ptr(), ldw, w_scales.data_ptr(), yp, ldy, m, n, k, flags, tp, tn,
+                 _stream_of(dev) if stream is None else _on(stream, dev))
     if rc:
         _lib.check(rc)
     return out
