@@ -339,8 +339,10 @@ template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm
     load(first, p0);
     for (int u = first; u < end; u += 2 * U) {
         load(u + U, p1);
+        __builtin_amdgcn_sched_barrier(0);  // (the loads before the products that wait for the others)
         multiply(p0);
         load(u + 2 * U, p0);
+        __builtin_amdgcn_sched_barrier(0);
         multiply(p1);
     }
     sums[wave][lane] = acc;
