@@ -4,6 +4,8 @@
 // Sums are 32-bit integers and exact (K <= 65536: below 2^30 for codes of +-127,
 // 2^30 for -128), so their order has no effect on the result; they are rounded
 // to fp32 once and multiplied by the two scales.
+#include <type_traits>
+
 #include "common.h"
 #include "int8.h"
 
@@ -187,8 +189,7 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
 #undef STAGE
     }
     multiply(p1);
-    // A part of 32 x 32 at a time through LDS (each wave its own 4 KiB): a lane's accumulators are 4 channels of one token, four
-    // times; rows of 128 bytes go to memory, 8 of them with an instruction. (Parts of lines cost as much as whole ones.)
+    // the results' places and scales
     const int m0 = tm * B + wm * TM * 32, n0 = tn * B + wn * TN * 32;
     const int er = lane >> 3, en = (lane & 7) * 4;  // this lane's row of 8, its 4 channels
     const bool vec = (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0;
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
     float xs[TM][4];
     f4 ws[TN];
 #pragma unroll
-    for (int j = 0; j < TM; j++)  // (all on their way at once; past the ends the last)
+    for (int j = 0; j < TM; j++)  // (past the ends the last)
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int m = m0 + j * 32 + 8 * u + er;
@@ -209,52 +210,74 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
             const int n = n0 + i * 32 + en + c;
             ws[i][c] = a.w_scale[n < a.N ? n : a.N - 1];
         }
-    // what is added to, a part ahead of its sums
-    f4 was[2][4];
-    auto ahead = [&](int part_no) __attribute__((always_inline)) {
-        const int i = part_no / TM, j = part_no % TM, n = n0 + i * 32 + en;
+    // Parts of 32 x 32 through LDS, PB at a time (each wave its own 4 KiB for each): a lane's accumulators are 4 channels of one
+    // token, four times; rows of 128 bytes go to memory, 8 of them with an instruction. (Parts of lines cost as much as whole ones.)
+    constexpr int PB = TN * TM < 2 ? 1 : 2;
+    static_assert(2 * PB * 4096 <= BYTES && NW / 2 <= H && TN * TM % PB == 0, "two waves a place");
+    auto results = [&](auto adds, auto inside) __attribute__((always_inline)) {  // inside: the whole tile is, its rows 16-byte aligned
+        constexpr bool ADDS = decltype(adds)::value, INSIDE = decltype(inside)::value;
+        f4 was[PB][4];
+        char *const own = place(wave >> 1) + (wave & 1) * (PB * 4096);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int m = m0 + j * 32 + 8 * u + er;
-            was[part_no & 1][u] = f4{0, 0, 0, 0};
-            if (a.accum && vec && !part && m < a.M && n + 4 <= a.N) was[part_no & 1][u] = *(const f4 *)(a.y + (int64_t)m * a.ldy + n);
+        for (int p0 = 0; p0 < TN * TM; p0 += PB) {
+            if constexpr (ADDS) {  // what is added to, on its way
+#pragma unroll
+                for (int p = 0; p < PB; p++)
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int m = m0 + (p0 + p) % TM * 32 + 8 * u + er, n = n0 + (p0 + p) / TM * 32 + en;
+                        if constexpr (!INSIDE) was[p][u] = f4{0, 0, 0, 0};
+                        if (INSIDE || (vec && m < a.M && n + 4 <= a.N)) was[p][u] = *(const f4 *)(a.y + (int64_t)m * a.ldy + n);
+                    }
+            }
+            if (p0 == 0) meet<0>();
+#pragma unroll
+            for (int p = 0; p < PB; p++) {
+                const i16 v = acc[(p0 + p) / TM][(p0 + p) % TM];
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    *(i4 *)(own + p * 4096 + col * 128 + (((2 * q + g) ^ (col & 7)) << 4)) = i4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            }
+#pragma unroll
+            for (int p = 0; p < PB; p++) {
+                const int i = (p0 + p) / TM, j = (p0 + p) % TM, n = n0 + i * 32 + en;
+                i4 o[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) o[u] = *(const i4 *)(own + p * 4096 + (8 * u + er) * 128 + (((lane & 7) ^ er) << 4));
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int m = m0 + j * 32 + 8 * u + er;
+                    if constexpr (!INSIDE) {
+                        if (m >= a.M) continue;
+                        if (part) {
+                            if (n < t.ld) *(i4 *)(part + (int64_t)m * t.ld + n) = o[u];
+                            continue;
+                        }
+                    }
+                    f4 r;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) r[c] = (float)o[u][c] * xs[j][u] * ws[i][c];
+                    if (INSIDE || (vec && n + 4 <= a.N)) {
+                        if constexpr (ADDS) r += was[p][u];
+                        f4 *y = (f4 *)(a.y + (int64_t)m * a.ldy + n);
+                        if (t.stream) __builtin_nontemporal_store(r, y);
+                        else *y = r;
+                    } else {
+                        put(a, m, n, r, false);
+                    }
+                }
+            }
         }
     };
-    ahead(0);
-    meet<0>();
-    char *const own = wave < BYTES / 4096 ? lds0 + wave * 4096 : lds1 + (wave - BYTES / 4096) * 4096;
-#pragma unroll
-    for (int p = 0; p < TN * TM; p++) {
-        const int i = p / TM, j = p % TM, n = n0 + i * 32 + en;
-        if (p + 1 < TN * TM) ahead(p + 1);
-        const i16 v = acc[i][j];
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-            *(i4 *)(own + col * 128 + (((2 * q + g) ^ (col & 7)) << 4)) = i4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-        i4 o[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) o[u] = *(const i4 *)(own + (8 * u + er) * 128 + (((lane & 7) ^ er) << 4));
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int m = m0 + j * 32 + 8 * u + er;
-            if (m >= a.M) continue;
-            if (part) {
-                if (n < t.ld) *(i4 *)(part + (int64_t)m * t.ld + n) = o[u];
-                continue;
-            }
-            f4 r;
-#pragma unroll
-            for (int c = 0; c < 4; c++) r[c] = (float)o[u][c] * xs[j][u] * ws[i][c];
-            if (vec && n + 4 <= a.N) {
-                r += was[p & 1][u];
-                f4 *y = (f4 *)(a.y + (int64_t)m * a.ldy + n);
-                if (t.stream) __builtin_nontemporal_store(r, y);
-                else *y = r;
-            } else {
-                put(a, m, n, r, false);
-            }
+    if constexpr (TN * TM <= 2) {  // (the largest tile has no registers for a way of its own)
+        if (!part && vec && m0 + TM * 32 <= a.M && n0 + TN * 32 <= a.N) {
+            if (a.accum) results(std::true_type{}, std::true_type{});
+            else results(std::false_type{}, std::true_type{});
+            return;
         }
     }
+    if (a.accum && !part) results(std::true_type{}, std::false_type{});
+    else results(std::false_type{}, std::false_type{});
 #endif
 }
 
