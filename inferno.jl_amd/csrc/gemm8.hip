@@ -42,8 +42,8 @@ __device__ __forceinline__ Rows rows_at(const int8_t *p, int64_t ld, int first, 
 }
 
 // Tile number t of tiles_m x tiles_n: the eight XCDs (consecutive workgroups in turn) take a contiguous range each, in groups
-// of GROUP tiles of tokens, so that the tiles in flight on an XCD share rows and channels in its L2.
-constexpr int GROUP = 8;
+// of GROUP tiles of tokens, so that the tiles in flight on an XCD share rows and channels in its L2. (Groups of 4, 8, 16: 4096 x 4096 x 12288 166, 169, -- us.)
+constexpr int GROUP = 4;
 __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &tm, int &tn) {
     const int total = tiles_m * tiles_n, q = total >> 3, r = total & 7, x = id & 7, i = id >> 3;
     const int t = x * q + (x < r ? x : r) + i;
