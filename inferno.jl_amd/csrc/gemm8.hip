@@ -13,6 +13,7 @@ namespace {
 
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef int i16 __attribute__((ext_vector_type(16)));
+typedef f4 f4u __attribute__((aligned(4)));  // (rows of y begin at any value)
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int KB = 128;  // bytes of K that a stage holds: a line of each row
@@ -60,11 +61,11 @@ struct Tiling {
 };
 
 // 4 channels of one token into y
-__device__ __forceinline__ void put(const Gemm8Args &a, int m, int n, f4 r, bool vec) {
+__device__ __forceinline__ void put(const Gemm8Args &a, int m, int n, f4 r) {
     float *y = a.y + (int64_t)m * a.ldy + n;
-    if (vec && n + 4 <= a.N) {
-        if (a.accum) r += *(const f4 *)y;
-        *(f4 *)y = r;
+    if (n + 4 <= a.N) {
+        if (a.accum) r += *(const f4u *)y;
+        *(f4u *)y = r;
     } else {
 #pragma unroll
         for (int c = 0; c < 4; c++)
@@ -192,7 +193,6 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
     // the results' places and scales
     const int m0 = tm * B + wm * TM * 32, n0 = tn * B + wn * TN * 32;
     const int er = lane >> 3, en = (lane & 7) * 4;  // this lane's row of 8, its 4 channels
-    const bool vec = (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0;
     int *const part = t.sums ? t.sums + (int64_t)blockIdx.y * a.M * t.ld : nullptr;
     float xs[TM][4];
     f4 ws[TN];
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
     // token, four times; rows of 128 bytes go to memory, 8 of them with an instruction. (Parts of lines cost as much as whole ones.)
     constexpr int PB = TN * TM < 2 ? 1 : 2;
     static_assert(2 * PB * 4096 <= BYTES && NW / 2 <= H && TN * TM % PB == 0, "two waves a place");
-    auto results = [&](auto adds, auto inside) __attribute__((always_inline)) {  // inside: the whole tile is, its rows 16-byte aligned
+    auto results = [&](auto adds, auto inside) __attribute__((always_inline)) {  // inside: the whole tile is
         constexpr bool ADDS = decltype(adds)::value, INSIDE = decltype(inside)::value;
         f4 was[PB][4];
         char *const own = place(wave >> 1) + (wave & 1) * (PB * 4096);
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
                     for (int u = 0; u < 4; u++) {
                         const int m = m0 + (p0 + p) % TM * 32 + 8 * u + er, n = n0 + (p0 + p) / TM * 32 + en;
                         if constexpr (!INSIDE) was[p][u] = f4{0, 0, 0, 0};
-                        if (INSIDE || (vec && m < a.M && n + 4 <= a.N)) was[p][u] = *(const f4 *)(a.y + (int64_t)m * a.ldy + n);
+                        if (INSIDE || (m < a.M && n + 4 <= a.N)) was[p][u] = *(const f4u *)(a.y + (int64_t)m * a.ldy + n);
                     }
             }
             if (p0 == 0) meet<0>();
@@ -257,20 +257,20 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
                     f4 r;
 #pragma unroll
                     for (int c = 0; c < 4; c++) r[c] = (float)o[u][c] * xs[j][u] * ws[i][c];
-                    if (INSIDE || (vec && n + 4 <= a.N)) {
+                    if (INSIDE || n + 4 <= a.N) {
                         if constexpr (ADDS) r += was[p][u];
-                        f4 *y = (f4 *)(a.y + (int64_t)m * a.ldy + n);
+                        f4u *y = (f4u *)(a.y + (int64_t)m * a.ldy + n);
                         if (t.stream) __builtin_nontemporal_store(r, y);
                         else *y = r;
                     } else {
-                        put(a, m, n, r, false);
+                        put(a, m, n, r);
                     }
                 }
             }
         }
     };
     if constexpr (TN * TM <= 2) {  // (the largest tile has no registers for a way of its own)
-        if (!part && vec && m0 + TM * 32 <= a.M && n0 + TN * 32 <= a.N) {
+        if (!part && m0 + TM * 32 <= a.M && n0 + TN * 32 <= a.N) {
             if (a.accum) results(std::true_type{}, std::true_type{});
             else results(std::false_type{}, std::true_type{});
             return;
@@ -297,7 +297,7 @@ template <int P> __global__ __launch_bounds__(256) void gemm8_join(Gemm8Args a, 
     for (int i = 1; i < P; i++) v[0] += v[i];
 #pragma unroll
     for (int c = 0; c < 4; c++) r[c] = (float)v[0][c] * xs * ws[c];
-    put(a, m, n, r, (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0);
+    put(a, m, n, r);
 }
 
 template <int B, int WM, int WN, int H, int EU> void tiles(const Gemm8Args &a, int parts, int *sums, hipStream_t st) {
@@ -333,14 +333,14 @@ template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm
     };
     // the first wave's scales and what it adds to, on their way first
     const int m = m0 + col, n = n0 + 4 * g;
-    const bool there = m < a.M && n < a.N, vec = (a.ldy & 3) == 0 && ((uintptr_t)a.y & 15) == 0 && n + 4 <= a.N;
+    const bool there = m < a.M && n < a.N, whole = n + 4 <= a.N;
     float xs = 0.f;
     f4 ws = {0, 0, 0, 0}, was = {0, 0, 0, 0};
     if (wave == 0 && there) {
         xs = a.x_scale[m];
 #pragma unroll
         for (int c = 0; c < 4; c++) ws[c] = a.w_scale[n + c < a.N ? n + c : a.N - 1];
-        if (a.accum && vec) was = *(const f4 *)(a.y + (int64_t)m * a.ldy + n);
+        if (a.accum && whole) was = *(const f4u *)(a.y + (int64_t)m * a.ldy + n);
     }
     const int units = (a.K + 63) / 64, per = (units + W - 1) / W, first = wave * per;
     const int end = first + per < units ? first + per : units;
@@ -377,8 +377,8 @@ template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm
     f4 r;  // (a lane's sums are 4 channels of one token)
 #pragma unroll
     for (int c = 0; c < 4; c++) r[c] = (float)acc[c] * xs * ws[c];
-    if (vec) *(f4 *)(a.y + (int64_t)m * a.ldy + n) = r + was;
-    else put(a, m, n, r, false);
+    if (whole) *(f4u *)(a.y + (int64_t)m * a.ldy + n) = r + was;
+    else put(a, m, n, r);
 #endif
 }
 
