@@ -80,7 +80,7 @@ hipError_t launch_delta(const DeltaArgs &a, void *ws, hipStream_t st);
 // 8-bit projections (quant8.hip, gemm8.hip)
 hipError_t launch_quant8(const Quant8Args &a, int act, hipStream_t st);
 size_t gemm8_ws(const Gemm8Args &a);
-hipError_t launch_gemm8(const Gemm8Args &a, void *ws, hipStream_t st);
+hipError_t launch_gemm8(const Gemm8Args &a, void *ws, size_t ws_bytes, size_t *need, hipStream_t st);
 size_t noalloc_scratch_bytes();
 hipError_t noalloc_scratch(void **out);
 hipError_t noalloc_prepare(int device);
@@ -1299,13 +1299,13 @@ int ihip_gemm_i8(const int8_t *x_dev, int64_t ldx, const float *x_scale_dev, con
     a.x = x_dev, a.w = w_dev, a.x_scale = x_scale_dev, a.w_scale = w_scale_dev, a.y = y_dev;
     a.ldx = ldx, a.ldw = ldw, a.ldy = ldy;
     a.M = M, a.N = N, a.K = K, a.accum = flags & IHIP_GEMM_ACCUM ? 1 : 0;
-    const size_t need = gemm8_ws(a);
+    size_t need = 0;
+    const hipError_t e = launch_gemm8(a, ws, ws_bytes, &need, S(stream));
     if (need) {
         if (!ws) return fail(IHIP_EFAULT, "%s: NULL workspace (%zu bytes needed)", fn, need);
         if (ws_bytes < need) return fail(IHIP_ENOMEM, "%s: workspace %zu < %zu bytes", fn, ws_bytes, need);
         if (!aligned16(ws)) return fail(IHIP_EINVAL, "%s: workspace must be 16-byte aligned", fn);
     }
-    const hipError_t e = launch_gemm8(a, ws, S(stream));
     return e == hipSuccess ? ok() : hip_fail(e, fn);
 }
 

@@ -386,19 +386,21 @@ template <int W, int U> void few(const Gemm8Args &a, hipStream_t st) {
     gemm8_few<W, U><<<dim3((a.N + 15) / 16, (a.M + 15) / 16), W * 64, 0, st>>>(a);
 }
 
-// Which kernel, and into how many parts K goes: the one whose time comes out shortest. A launch is rounds of workgroups; a round
-// takes `start` for its first loads and its results, and for each stage `alone` where it leaves most of the chip's memory paths
-// to few workgroups, `full` where it fills the chip (us, fitted to 20 products of 16 to 4096 tokens, 1024 to 24576 channels, K
-// 2048 to 12288: the choice is at most 18% behind the best of these kernels there, mostly below 5).
+// Which kernel, and into how many parts K goes: the one whose time comes out shortest. A launch is rounds of workgroups. A round
+// takes `fill` for its first loads, for each stage `alone` where it leaves most of the chip's memory paths to few workgroups and
+// `full` where it fills the chip, and the time of its results, by a CU's rate or by the chip's. (us, fitted to 33 products of 16 to
+// 4096 tokens, 140 to 24576 channels, K 288 to 12288; there the choice is mostly within 5% of the best of these kernels, at
+// worst 13% behind it.)
 struct Shape {
     int tile, at_once;
-    double start, alone, full;
+    double fill, alone, full;
+    bool late;  // (nears `full` with the square of the round's part)
 };
 constexpr Shape shapes[] = {
-    {64, 512, 3.5, 0.18, 0.39},   // 9 places of 8 KiB, two workgroups a CU
-    {128, 256, 5.0, 0.36, 0.58},  // 9 places of 16 KiB
-    {128, 512, 4.5, 0.50, 1.09},  // 5 places of 16 KiB, two workgroups a CU
-    {256, 256, 9.4, 0.95, 1.60},  // 5 places of 32 KiB
+    {64, 512, 1.2, 0.18, 0.39, false},   // 9 places of 8 KiB, two workgroups a CU
+    {128, 256, 2.0, 0.36, 0.56, true},   // 9 places of 16 KiB
+    {128, 512, 1.2, 0.50, 1.09, false},  // 5 places of 16 KiB, two workgroups a CU
+    {256, 256, 5.0, 0.95, 1.60, false},  // 5 places of 32 KiB
 };
 struct Plan {
     int shape, parts;  // shape -1: gemm8_few
@@ -409,18 +411,23 @@ Plan plan_of(const Gemm8Args &a) {
     const double few_us = 2.5 + (double)few_wgs * (16 + (a.M < 16 ? a.M : 16)) * a.K / 8.5e6;  // operands through the L2s at 8.5 TB/s
     Plan best{-1, 1};
     double best_us = few_us > weights ? few_us : weights;
+    if (best_us <= weights) return best;  // (no other is faster than reading the weights)
     for (int i = 0; i < 4; i++)
         for (const int parts : {1, 2, 3, 4, 6, 8}) {
             const Shape &s = shapes[i];
             const int64_t wgs = (int64_t)((a.M + s.tile - 1) / s.tile) * ((a.N + s.tile - 1) / s.tile) * parts;
             const int stages = ((a.K + KB - 1) / KB + parts - 1) / parts;
-            const int64_t bytes = (int64_t)parts * a.M * ((a.N + 3) / 4 * 4) * 4;
-            if (parts > 1 && (stages < 8 || bytes > (int64_t)64 << 20)) break;
+            const double y = 4.0 * a.M * ((a.N + 3) / 4 * 4), touched = a.accum ? 2.0 : 1.0;
+            if (parts > 1 && (stages < 8 || parts * y > (double)(64 << 20))) break;
+            const double bytes = 4.0 * s.tile * s.tile * (parts > 1 ? 1.0 : touched), one = bytes / 60e3, all = s.at_once * bytes / 5.0e6;
+            auto round = [&](double part) {
+                const double results = part < 1 ? one + (all > one ? all - one : 0.0) * part : all;
+                return s.fill + results + stages * (s.alone + (s.full - s.alone) * (s.late ? part * part : part));
+            };
             const double rest = (double)(wgs % s.at_once) / s.at_once;
-            double us = (double)(wgs / s.at_once) * (s.start + stages * s.full);
-            if (rest > 0) us += s.start + stages * (s.alone + (s.full - s.alone) * rest);
+            double us = 2.0 + (double)(wgs / s.at_once) * round(1.0) + (rest > 0 ? round(rest) : 0.0);
             if (us < weights) us = weights;
-            if (parts > 1) us += 2.5 + 2.0 * (double)bytes / 8.0e6;  // (sums written and read, and a launch more)
+            if (parts > 1) us += 2.5 + y * (parts + touched) / 8.0e6;  // (the sums read again, and a launch more)
             if (us < best_us) best_us = us, best = Plan{i, parts};
         }
     return best;
@@ -428,13 +435,17 @@ Plan plan_of(const Gemm8Args &a) {
 
 }  // namespace
 
-size_t gemm8_ws(const Gemm8Args &a) {
-    const Plan p = plan_of(a);
+static size_t sums_bytes(const Gemm8Args &a, const Plan &p) {
     return p.parts > 1 ? (size_t)p.parts * a.M * ((a.N + 3) / 4 * 4) * 4 : 0;
 }
 
-hipError_t launch_gemm8(const Gemm8Args &a, void *ws, hipStream_t st) {
+size_t gemm8_ws(const Gemm8Args &a) { return sums_bytes(a, plan_of(a)); }
+
+// need: the workspace's bytes; with fewer given nothing is launched.
+hipError_t launch_gemm8(const Gemm8Args &a, void *ws, size_t ws_bytes, size_t *need, hipStream_t st) {
     const Plan p = plan_of(a);
+    *need = sums_bytes(a, p);
+    if (*need && (!ws || ws_bytes < *need || ((uintptr_t)ws & 15))) return hipErrorInvalidValue;
     if (p.shape < 0) few<4, 2>(a, st);
     else if (p.shape == 0) tiles<64, 2, 2, 9, 2>(a, p.parts, (int *)ws, st);
     else if (p.shape == 1) tiles<128, 2, 4, 9, 2>(a, p.parts, (int *)ws, st);
