@@ -641,7 +641,8 @@ int ihip_quantize_i8(const ihip_gemm_input *in, int M, int K, int8_t *q_dev,
  * rounded to fp32 once and multiplied by x_scale, then by w_scale (a scale that
  * is not finite gives its row or column what fp32 products give). Any M and N
  * from 1 to 2^23 with M N up to 2^38; K a multiple of 16 up to 65536; x and w
- * 16-byte aligned, ldx and ldw multiples of 16 up to 2^22. y overlaps none of the inputs.
+ * 16-byte aligned, ldx and ldw multiples of 16 up to 2^22 (of 128, with x and w
+ * so aligned, rows are read fastest). y overlaps none of the inputs.
  * ws: ihip_gemm_i8_ws_bytes (may be 0: then NULL is allowed), 16-byte aligned,
  * any contents, not shared by calls that overlap in time. The batched form of
  * the reference's projections (src/ModelCPU.jl:284-378) past 64 tokens. */

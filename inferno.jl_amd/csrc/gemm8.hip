@@ -107,10 +107,11 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
     }
     auto fetch = [&](char *lds, bool tok, int k0) __attribute__((always_inline)) {
         const uint32_t past = k0 + lc < end ? 0u : 1u << 31;
+        const int from = k0 < a.K ? k0 : a.K;  // (within a row, and so within the buffer, where all of it is past)
 #pragma unroll
         for (int i = 0; i < NLH; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(tok ? xb : wb, (lds_void *)(lds + (i * NW + wave) * 8 * KB), 16,
-                                                     (tok ? xat[i] : wat[i]) | past, k0, 0, 0);
+                                                     (tok ? xat[i] : wat[i]) | past, from, 0, 0);
     };
     i16 acc[TN][TM];
 #pragma unroll
@@ -349,8 +350,9 @@ template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm
         for (int u = 0; u < U; u++) {
             const int k = (u0 + u) * 64;
             const uint32_t past = u0 + u < end && k + g * 16 < a.K ? 0u : 1u << 31;  // (of another wave, or past K: zeros)
-            p.w[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(wb, wat | past, k, 0));
-            p.x[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(xb, xat | past, k, 0));
+            const int from = k < a.K ? k : a.K;
+            p.w[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(wb, wat | past, from, 0));
+            p.x[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(xb, xat | past, from, 0));
         }
     };
     i4 acc = {0, 0, 0, 0};
@@ -408,7 +410,8 @@ struct Plan {
 Plan plan_of(const Gemm8Args &a) {
     const double weights = 1.0 + (double)a.N * a.K / 5.0e6;  // reading them, at 5 TB/s
     const int64_t few_wgs = (int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16);
-    const double few_us = 2.5 + (double)few_wgs * (16 + (a.M < 16 ? a.M : 16)) * a.K / 8.5e6;  // operands through the L2s at 8.5 TB/s
+    const double few_us = a.M > 16 * 65535 ? 1e9 : 2.5 + (double)few_wgs * (16 + (a.M < 16 ? a.M : 16)) * a.K / 8.5e6;  // operands through the L2s at 8.5 TB/s
+    // (a launch holds 65535 of its rows of workgroups)
     Plan best{-1, 1};
     double best_us = few_us > weights ? few_us : weights;
     if (best_us <= weights) return best;  // (no other is faster than reading the weights)

@@ -129,15 +129,20 @@ def silu_mul_i8(gate_up, out=None, scales=None, stream=None):
 
 def quantize_weights_i8(qtype: int, w_dev, n: int, k: int, stream=None):
     """A GGUF matrix [n, k] on the device as int8 codes [n, k] and a scale a
-    channel, once at load time: its rows dequantized, 64 Mi values at a time, then quantize_i8."""
+    channel, once at load time: its rows dequantized, 64 Mi values at a time,
+    then quantize_i8. The codes' rows begin at multiples of 128 bytes, which
+    gemm_i8 reads fastest (512 x 4096 x 2880: 14.5 us, with rows of 2880 bytes 16.0)."""
     import torch
     if _i8 is None:
         _names()
     if qtype not in BLOCK_ELEMS or k % BLOCK_ELEMS[qtype]:
         raise ValueError(f"qtype {qtype}, k={k}: not rows of whole blocks")
     row = k // BLOCK_ELEMS[qtype] * BLOCK_BYTES[qtype]
+    if n < 1:
+        raise ValueError(f"n={n} channels")
     check_tensor(w_dev, "w_dev", torch.uint8, min_numel=n * row)
-    codes = made_for(stream, torch.empty, (n, k), dtype=torch.int8, device=w_dev.device)
+    _device_of(w_dev, "w_dev")
+    codes = made_for(stream, torch.empty, (n, (k + 127) // 128 * 128), dtype=torch.int8, device=w_dev.device)[:, :k]
     scales = made_for(stream, torch.empty, n, dtype=torch.float32, device=w_dev.device)
     step = max(1, (64 << 20) // k)
     flat = w_dev.view(-1)
@@ -182,8 +187,10 @@ def gemm_i8(q, scales, w, w_scales, accum: bool = False, out=None, ws=None, stre
         _, m, _, ldq = _codes(q, "q", None, k, dev)
         _whole(scales, "scales", _f32, (m,), dev)
         _whole(w_scales, "w_scales", _f32, (n,), dev)
-    elif m == 1:  # (a single row's stride has no meaning)
+    if m == 1:  # (a single row's stride has no meaning)
         ldq = (kq + 15) // 16 * 16
+    if n == 1:
+        ldw = (k + 15) // 16 * 16
     if out is None:
         if accum:
             raise ValueError("accum adds to out: pass it")

@@ -236,6 +236,13 @@ def test_product_large(ih, m, n, k):
     near(ih.gemm_i8(*map(cu, a)), R.product(*a))
 
 
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_product_of_a_million_tokens(ih, n):
+    """More tokens than 65535 groups of 16, few channels."""
+    a = operands(rng(20, n), 16 * 65535 + 19, n, 16)
+    near(ih.gemm_i8(*map(cu, a)), R.product(*a))
+
+
 @pytest.mark.parametrize("m", [1, 40, 130])
 def test_largest_sums(ih, m):
     """K = 65536 of the extreme codes, -128 among them: sums up to 2^30."""
@@ -326,6 +333,88 @@ def test_repeats_are_equal(ih):
             assert torch.equal(ih.gemm_i8(*a), first)
 
 
+def in_parts(ih):
+    """Products whose K goes in parts through a workspace."""
+    found = [(m, n, k) for m, n, k in ((130, 517, 8192), (300, 1000, 4096), (300, 257, 8208), (515, 1030, 12288), (515, 4096, 4096))
+             if ih.gemm_i8_ws_bytes(m, n, k)]
+    assert len(found) >= 3
+    return found
+
+
+@pytest.mark.parametrize("accum", [False, True])
+def test_workspace_ends(ih, accum):
+    """A workspace of just its size, any bytes in it, with bytes behind it that stay; rows of y of any length."""
+    import torch
+    for m, n, k in in_parts(ih):
+        r = rng(21, m, n, k)
+        a = operands(r, m, n, k)
+        need = ih.gemm_i8_ws_bytes(m, n, k, accum)
+        space = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+        space[:need].random_()
+        y = r.standard_normal((m, n + 3)).astype(np.float32)
+        out = cu(y)
+        ih.gemm_i8(*map(cu, a), accum=accum, out=out[:, 1:n + 1], ws=space[:need])
+        want = R.product(*a)
+        total = want + y[:, 1:n + 1] if accum else want
+        near(out[:, 1:n + 1], total, R.PRODUCT_TOL * np.abs(want) + R.HALF * np.abs(total) if accum else 0.0)
+        assert bool((space[need:] == 0x5a).all())
+        out = out.cpu().numpy()
+        assert np.array_equal(out[:, 0], y[:, 0]) and np.array_equal(out[:, n + 1:], y[:, n + 1:])
+        with pytest.raises(ih.HipError):
+            ih.gemm_i8(*map(cu, a), ws=space[:need - 1] if not accum else space[:16])
+
+
+def test_two_streams_at_once(ih):
+    """Calls that overlap in time, each with its own workspace or one that it makes itself."""
+    import torch
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for m, n, k in in_parts(ih):
+        ops = [[cu(v) for v in operands(rng(22, m, i), m, n, k)] for i in range(2)]
+        want = [ih.gemm_i8(*o) for o in ops]
+        outs = [[], []]
+        for side in sides:
+            side.wait_stream(torch.cuda.current_stream())
+        for _ in range(8):
+            for i in range(2):
+                outs[i].append(ih.gemm_i8(*ops[i], stream=sides[i]))
+        for side in sides:
+            torch.cuda.current_stream().wait_stream(side)
+        for i in range(2):
+            assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+def test_captured_with_its_own_workspace(ih):
+    """Two graphs of calls that make codes, scales, results and workspace themselves, replayed in turn with eager calls between."""
+    import torch
+    (m, n, k), (m2, n2, k2) = in_parts(ih)[:2]
+    r = rng(23)
+    w, w2 = (ih.quantize_i8(cu(r.standard_normal(s).astype(np.float32))) for s in ((n, k), (n2, k2)))
+    x, x2 = (torch.zeros(s, device="cuda") for s in ((m, k), (m2, k2)))
+    graphs, outs = [], []
+    for a, b in ((x, w), (x2, w2)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ih.gemm_i8(*ih.quantize_i8(a), *b))
+        graphs.append(g)
+    for i in range(3):
+        x.copy_(cu(rows(r, m, k))), x2.copy_(cu(rows(r, m2, k2)))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for a, b, o in ((x, w, outs[0]), (x2, w2, outs[1])):
+            assert torch.equal(o, ih.gemm_i8(*ih.quantize_i8(a), *b)), i
+
+
+def test_single_rows_of_any_stride(ih):
+    """A single token's, a single channel's row: its stride has no meaning."""
+    r = rng(24)
+    a = operands(r, 1, 1, 48)
+    q, s, w, ws = map(cu, a)
+    near(ih.gemm_i8(q.as_strided((1, 48), (1, 1)), s, w.as_strided((1, 48), (7, 1)), ws), R.product(*a))
+    x = rows(r, 1, 48)
+    same(ih.quantize_i8(cu(x).as_strided((1, 48), (5, 1))), R.quantize(x), R.HALF)
+
+
 def test_python_refusals(ih):
     import torch
     x = torch.zeros((4, 64), device="cuda")
@@ -354,6 +443,25 @@ def test_weights(ih, name):
     d = cu(w)
     codes, scales = ih.quantize_weights_i8(qt, d, n, k)
     same((codes, scales), R.quantize(ih.dequant(qt, d, n * k).view(n, k).cpu().numpy()), R.HALF)
+
+
+@pytest.mark.parametrize("name,k", [("Q6_K", 768), ("Q8_0", 32 * 27)])
+def test_weights_of_several_pieces(ih, name, k):
+    """More values than are dequantized at a time; pieces whose blocks begin at any 2 bytes, rows not a multiple of 128."""
+    from inferno_hip import formats as F
+    from inferno_hip.quantized_kernels import synth_blocks
+    qt, step = getattr(F, name), (64 << 20) // k
+    n, row = step + 300, k // F.BLOCK_ELEMS[getattr(F, name)] * F.BLOCK_BYTES[getattr(F, name)]
+    d = synth_blocks(qt, 0x1F3E0002, n * row // F.BLOCK_BYTES[qt])
+    codes, scales = ih.quantize_weights_i8(qt, d, n, k)
+    assert codes.shape == (n, k) and codes.stride(0) % 128 == 0
+    for i in (0, step - 40, n - 40):
+        x = ih.dequant(qt, d[i * row:(i + 40) * row].clone(), 40 * k).view(40, k).cpu().numpy()
+        same((codes[i:i + 40], scales[i:i + 40]), R.quantize(x), R.HALF)
+    for i in range(0, n, 1 << 15):  # (the rows between: no code differs from those of the whole matrix in one piece)
+        j = min(n, i + (1 << 15))
+        q, s = ih.quantize_i8(ih.dequant(qt, d[i * row:j * row].clone(), (j - i) * k).view(j - i, k))
+        assert bool((q == codes[i:j]).all()) and bool((s == scales[i:j]).all())
 
 
 @pytest.mark.parametrize("m,start", [(150, 0), (1, 37), (5, 3)])
