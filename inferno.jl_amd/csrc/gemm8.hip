@@ -42,13 +42,18 @@ __device__ __forceinline__ Rows rows_at(const int8_t *p, int64_t ld, int first, 
     return Rows{p + first * ld, n * (int)ld};
 }
 
-// Tile number t of tiles_m x tiles_n: the eight XCDs (consecutive workgroups in turn) take a contiguous range each, in groups
-// of GROUP tiles of tokens, so that the tiles in flight on an XCD share rows and channels in its L2. (Groups of 4, 8, 16: 4096 x 4096 x 12288 166, 169, -- us.)
+// The place of workgroup `id` in an order of `total` of which each of the eight XCDs (consecutive workgroups in turn) takes a
+// contiguous range.
+__device__ __forceinline__ int place_of(int id, int total) {
+    const int q = total >> 3, r = total & 7, x = id & 7;
+    return x * q + (x < r ? x : r) + (id >> 3);
+}
+
+// The tile of workgroup `id`, in groups of GROUP tiles of tokens, so that the tiles in flight on an XCD share rows and channels
+// in its L2. (Groups of 4, 8 and 16: 4096 x 24576 x 4096 377, 379 and 400 us.)
 constexpr int GROUP = 4;
 __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &tm, int &tn) {
-    const int total = tiles_m * tiles_n, q = total >> 3, r = total & 7, x = id & 7, i = id >> 3;
-    const int t = x * q + (x < r ? x : r) + i;
-    const int per = GROUP * tiles_n, group = t / per, first = group * GROUP;
+    const int t = place_of(id, tiles_m * tiles_n), per = GROUP * tiles_n, group = t / per, first = group * GROUP;
     const int size = tiles_m - first < GROUP ? tiles_m - first : GROUP, in = t - group * per;
     tm = __builtin_amdgcn_readfirstlane(first + in % size), tn = __builtin_amdgcn_readfirstlane(in / size);
 }
@@ -318,20 +323,22 @@ template <int B, int WM, int WN, int H, int EU> void tiles(const Gemm8Args &a, i
     else if (parts == 8) gemm8_join<8><<<blocks, 256, 0, st>>>(a, sums, t.ld);
 }
 
-// Few tokens: 16 tokens x 16 channels a workgroup, K over its W waves. Operands go from memory to the products' registers, U units
-// of 64 bytes of K ahead; the waves' sums meet in LDS.
-template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm8Args a) {
+// Few tokens: 16 tokens x 16 channels a workgroup, K over its W waves. A wave brings 128 bytes of K of its 32 rows at a time, whole
+// lines (loads of half lines, as the products' registers would take them, reach 40 GB/s a CU, these 112), to places of its own in
+// LDS, two ahead; the waves' sums meet at the end.
+template <int W> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm8Args a, int tiles_m, int tiles_n) {
 #if __HIP_DEVICE_COMPILE__
+    constexpr int D = 3, UNIT = 4096;  // places a wave; 16 rows of w, then of x, with the turns of tile rows
+    __shared__ __attribute__((aligned(1024))) char lds[W * D * UNIT];
     __shared__ i4 sums[W][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+    const int t = place_of(blockIdx.x, tiles_m * tiles_n), tn = __builtin_amdgcn_readfirstlane(t / tiles_m);
+    const int n0 = tn * 16, m0 = (t - tn * tiles_m) * 16;  // (the tokens of the same channels one after another, on one XCD)
     const Rows x = rows_at(a.x, a.ldx, m0, a.M, 16), w = rows_at(a.w, a.ldw, n0, a.N, 16);
     const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc((void *)x.p, 0, x.bytes, 0x00027000);
     const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc((void *)w.p, 0, w.bytes, 0x00027000);
-    const uint32_t xat = (uint32_t)col * (uint32_t)a.ldx + g * 16, wat = (uint32_t)col * (uint32_t)a.ldw + g * 16;
-    struct Part {
-        i4 w[U], x[U];
-    };
+    const int lr = lane >> 3, lc = ((lane & 7) ^ (lr & 6)) * 16;
+    const uint32_t xat = (uint32_t)lr * (uint32_t)a.ldx + lc, wat = (uint32_t)lr * (uint32_t)a.ldw + lc;
     // the first wave's scales and what it adds to, on their way first
     const int m = m0 + col, n = n0 + 4 * g;
     const bool there = m < a.M && n < a.N, whole = n + 4 <= a.N;
@@ -343,39 +350,46 @@ template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm
         for (int c = 0; c < 4; c++) ws[c] = a.w_scale[n + c < a.N ? n + c : a.N - 1];
         if (a.accum && whole) was = *(const f4u *)(a.y + (int64_t)m * a.ldy + n);
     }
-    const int units = (a.K + 63) / 64, per = (units + W - 1) / W, first = wave * per;
+    const int units = (a.K + KB - 1) / KB, per = (units + W - 1) / W, first = wave * per;
     const int end = first + per < units ? first + per : units;
-    auto load = [&](int u0, Part &p) __attribute__((always_inline)) {
+    char *const own = lds + wave * D * UNIT;
+    auto fetch = [&](int at, int u) __attribute__((always_inline)) {
+        const int k = u * KB, from = k < a.K ? k : a.K;
+        const uint32_t past = u < end && k + lc < a.K ? 0u : 1u << 31;  // (of another wave, or past K: zeros)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k = (u0 + u) * 64;
-            const uint32_t past = u0 + u < end && k + g * 16 < a.K ? 0u : 1u << 31;  // (of another wave, or past K: zeros)
-            const int from = k < a.K ? k : a.K;
-            p.w[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(wb, wat | past, from, 0));
-            p.x[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(xb, xat | past, from, 0));
-        }
+        for (int i = 0; i < 2; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (lds_void *)(own + at + i * 1024), 16, (wat + i * 8 * (uint32_t)a.ldw) | past, from, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void *)(own + at + 2048 + i * 1024), 16, (xat + i * 8 * (uint32_t)a.ldx) | past, from, 0, 0);
     };
     i4 acc = {0, 0, 0, 0};
-    auto multiply = [&](const Part &p) __attribute__((always_inline)) {
+    const uint32_t row = (uint32_t)(uintptr_t)(lds_void *)own + col * KB, c0 = row + ((g << 4) ^ (col & 6) << 4), c1 = row + ((64 + (g << 4)) ^ (col & 6) << 4);
 #pragma unroll
-        for (int u = 0; u < U; u++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(p.w[u], p.x[u], acc, 0, 0, 0);
-    };
-    Part p0, p1;
-    load(first, p0);
-    for (int u = first; u < end; u += 2 * U) {
-        load(u + U, p1);
-        __builtin_amdgcn_sched_barrier(0);  // (the loads before the products that wait for the others)
-        multiply(p0);
-        load(u + 2 * U, p0);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(p1);
+    for (int d = 0; d < D; d++) fetch(d * UNIT, first + d);
+    int at = 0;
+    for (int u = first; u < end; u++) {
+        i4 w0, x0, w1, x1;
+        // the oldest place's loads are there; it is read, and free. (Of reads that it sees the compiler makes each wait for all loads.)
+        asm volatile("s_waitcnt vmcnt(%6)\n\t"
+                     "ds_read_b128 %0, %4\n\t"
+                     "ds_read_b128 %1, %4 offset:2048\n\t"
+                     "ds_read_b128 %2, %5\n\t"
+                     "ds_read_b128 %3, %5 offset:2048\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(w0), "=&v"(x0), "=&v"(w1), "=&v"(x1)
+                     : "v"(c0 + at), "v"(c1 + at), "n"((D - 1) * 4)
+                     : "memory");
+        fetch(at, u + D);
+        at = at == (D - 1) * UNIT ? 0 : at + UNIT;
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, x0, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, x1, acc, 0, 0, 0);
     }
     sums[wave][lane] = acc;
     __syncthreads();
-    if (wave) return;
+    if (wave || !there) return;
 #pragma unroll
     for (int i = 1; i < W; i++) acc += sums[i][lane];
-    if (!there) return;
     f4 r;  // (a lane's sums are 4 channels of one token)
 #pragma unroll
     for (int c = 0; c < 4; c++) r[c] = (float)acc[c] * xs * ws[c];
@@ -384,8 +398,9 @@ template <int W, int U> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm
 #endif
 }
 
-template <int W, int U> void few(const Gemm8Args &a, hipStream_t st) {
-    gemm8_few<W, U><<<dim3((a.N + 15) / 16, (a.M + 15) / 16), W * 64, 0, st>>>(a);
+template <int W> void few(const Gemm8Args &a, hipStream_t st) {
+    const int tm = (a.M + 15) / 16, tn = (a.N + 15) / 16;
+    gemm8_few<W><<<tm * tn, W * 64, 0, st>>>(a, tm, tn);
 }
 
 // Which kernel, and into how many parts K goes: the one whose time comes out shortest. A launch is rounds of workgroups. A round
@@ -410,10 +425,11 @@ struct Plan {
 Plan plan_of(const Gemm8Args &a) {
     const double weights = 1.0 + (double)a.N * a.K / 5.0e6;  // reading them, at 5 TB/s
     const int64_t few_wgs = (int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16);
-    const double few_us = a.M > 16 * 65535 ? 1e9 : 2.5 + (double)few_wgs * (16 + (a.M < 16 ? a.M : 16)) * a.K / 8.5e6;  // operands through the L2s at 8.5 TB/s
-    // (a launch holds 65535 of its rows of workgroups)
+    // a CU takes in 98 GB/s; weights that several workgroups take come more slowly (a launch holds 2^32 threads)
+    const double a_cu = (few_wgs > 256 ? (double)few_wgs : 256.0) / 256.0, few_us = 2.5 + a_cu * (0.2 + (16 + (a.M < 16 ? a.M : 16)) * a.K / 98e3);
+    const double few_weights = weights + (a.M > 16 ? 0.7 * a_cu : 0.0);
     Plan best{-1, 1};
-    double best_us = few_us > weights ? few_us : weights;
+    double best_us = few_wgs > 1 << 24 ? 1e9 : few_us > few_weights ? few_us : few_weights;
     if (best_us <= weights) return best;  // (no other is faster than reading the weights)
     for (int i = 0; i < 4; i++)
         for (const int parts : {1, 2, 3, 4, 6, 8}) {
@@ -449,7 +465,12 @@ hipError_t launch_gemm8(const Gemm8Args &a, void *ws, size_t ws_bytes, size_t *n
     const Plan p = plan_of(a);
     *need = sums_bytes(a, p);
     if (*need && (!ws || ws_bytes < *need || ((uintptr_t)ws & 15))) return hipErrorInvalidValue;
-    if (p.shape < 0) few<4, 2>(a, st);
+    if (p.shape < 0) {
+        // four waves where half of the CUs or more have no workgroup and K is long (5 x 2048 x 12288: 6.2 us, with two 8.8; 1 x 2048
+        // x 4096: 4.4 and 4.1; 17 x 4096 x 4096: 6.0 and 5.3)
+        if ((int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16) <= 128 && a.K >= 8192) few<4>(a, st);
+        else few<2>(a, st);
+    }
     else if (p.shape == 0) tiles<64, 2, 2, 9, 2>(a, p.parts, (int *)ws, st);
     else if (p.shape == 1) tiles<128, 2, 4, 9, 2>(a, p.parts, (int *)ws, st);
     else if (p.shape == 2) tiles<128, 2, 4, 5, 4>(a, p.parts, (int *)ws, st);

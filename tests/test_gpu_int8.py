@@ -335,8 +335,8 @@ def test_repeats_are_equal(ih):
 
 def in_parts(ih):
     """Products whose K goes in parts through a workspace."""
-    found = [(m, n, k) for m, n, k in ((130, 517, 8192), (300, 1000, 4096), (300, 257, 8208), (515, 1030, 12288), (515, 4096, 4096))
-             if ih.gemm_i8_ws_bytes(m, n, k)]
+    shapes = ((515, 1030, 12288), (700, 1000, 8192), (300, 2001, 8208), (500, 1500, 16400), (100, 2050, 16400), (200, 2048, 16384))
+    found = [s for s in shapes if ih.gemm_i8_ws_bytes(*s)]  # (2 to 8 parts)
     assert len(found) >= 3
     return found
 

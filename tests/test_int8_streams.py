@@ -26,12 +26,12 @@ def on8(world, monkeypatch):  # noqa: F811
 def calls(w):
     f = lambda *s: Tensor(w, s, torch.float32)  # noqa: E731
     c = lambda *s: Tensor(w, s, torch.int8)  # noqa: E731
-    assert int8.gemm_i8_ws_bytes(130, 517, 8192)
+    assert int8.gemm_i8_ws_bytes(515, 1030, 12288)
     return {  # the call, what it returns, what it makes
         "quantize_i8": (lambda **kw: int8.quantize_i8(f(6, 64), **kw), 2, 2),
         "rmsnorm_i8": (lambda **kw: int8.rmsnorm_i8(f(6, 64), f(64), add=f(2, 6, 64), **kw), 2, 2),
         "silu_mul_i8": (lambda **kw: int8.silu_mul_i8(f(6, 128), **kw), 2, 2),
-        "gemm_i8": (lambda **kw: int8.gemm_i8(c(130, 8192), f(130), c(517, 8192), f(517), **kw), 1, 2),
+        "gemm_i8": (lambda **kw: int8.gemm_i8(c(515, 12288), f(515), c(1030, 12288), f(1030), **kw), 1, 2),
         "gemm_i8 without parts": (lambda **kw: int8.gemm_i8(c(1, 64), f(1), c(64, 64), f(64), **kw), 1, 1),
     }
 
