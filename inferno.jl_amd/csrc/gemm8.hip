@@ -4,6 +4,14 @@
 // Sums are 32-bit integers and exact (K <= 65536: below 2^30 for codes of +-127,
 // 2^30 for -128), so their order has no effect on the result; they are rounded
 // to fp32 once and multiplied by the two scales.
+//
+// What bounds it. Few tokens: reading the weights (gemm8_few: 1 x 24576 x 4096
+// in 16.8 us, 6.0 TB/s; 5 x 4096 x 12288 added to y 9.3 us, 5.4). Many: the
+// matrix cores and the clock that they leave (gemm8_tile: 4096 x 24576 x 4096 in
+// 376 to 382 us, 2.2 PFLOP/s at 1.9 GHz; their instructions alone would take 222
+// at 2.4). Between, what a CU takes in, 100 to 125 GB/s, and the rounds of
+// workgroups: 515 x 4096 x 4096 19 us, 64 x 12288 x 2048 7.4. Rows that do not
+// begin at multiples of 128 bytes cost the tiles 5 to 12 % (2 lines for 1).
 #include <type_traits>
 
 #include "common.h"
@@ -18,8 +26,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int KB = 128;  // bytes of K that a stage holds: a line of each row
 
-// Which of the eight 16-byte places of a row its chunk c takes: c ^ turn_of(row). The 16 lanes that LDS serves at once in a load
-// of 32 rows' chunk c (lanes 0-7 with 16-23, 8-15 with 24-31: rows) then meet in no bank.
+// Which of the eight 16-byte places of a row its chunk c takes: c ^ turn_of(row). The 16 lanes that LDS serves at once in a
+// load of 32 rows' chunk c (lanes 0-7 with 16-23, 8-15 with 24-31: rows) then meet in no bank (no conflicts counted).
 __device__ __forceinline__ int turn_of(int row) { return (row & 6) | (row >> 4 & 1); }
 
 // All but the last N loads of this wave are there, its LDS operations are done, and every wave is here.
@@ -58,10 +66,10 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &t
     tm = __builtin_amdgcn_readfirstlane(first + in % size), tn = __builtin_amdgcn_readfirstlane(in / size);
 }
 
-// How a product is cut: tiles of tokens and channels, `per` of K for each of the launch's y; with several of those their sums go
-// to `sums` (rows of ld, a multiple of 4) instead of y.
+// How a product is cut: tiles of tokens and channels, `per` of K for each of the launch's y; with several of those their
+// sums go to `sums` (rows of ld, a multiple of 4) instead of y.
 struct Tiling {
-    int m, n, per, ld, stream;
+    int m, n, per, ld;
     int *sums;
 };
 
@@ -78,19 +86,27 @@ __device__ __forceinline__ void put(const Gemm8Args &a, int m, int n, f4 r) {
     }
 }
 
-// A tile of B tokens x B channels; WM x WN waves. H places in LDS, each for the tokens' or the channels' half of a stage.
+// A tile of B tokens x B channels; WM x WN waves. H places in LDS, each for the tokens' or the channels' half of a stage: while
+// a stage is multiplied, (H - 2) / 2 stages are on their way, straight to LDS (no registers, no LDS stores by the waves).
+// Products 32x32x32, which take half the operand reads of 16x16x64; a wave's rows of w are the first operand, so that a lane's
+// accumulators are 4 neighbouring channels of one token.
+// (4096 x 24576 x 4096: 376 to 382 us in tiles of 256, 573 of 128. In tiles of 256 with stages of 64 bytes 420, four waves of
+// 128 x 128 416, workgroups that go on to further tiles 408, as a tile's first wait then includes the last one's stores.)
 template <int B, int WM, int WN, int H, int EU>
-__global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU, EU))) void gemm8_tile(Gemm8Args a, Tiling t) {
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
+void gemm8_tile(Gemm8Args a, Tiling t) {
 #if __HIP_DEVICE_COMPILE__  // (the host's pass over these builtins would leave the kernel without its launch stub)
     constexpr int NW = WM * WN, TM = B / WM / 32, TN = B / WN / 32, NLH = B / 8 / NW, BYTES = B * KB;
     static_assert(B % (8 * NW) == 0 && NW % 4 == 0, "rows of a load");
-    static_assert(H % 2 == 1 && H >= 5 && H <= 9 && H * BYTES <= 160 * 1024 && NW <= 2 * (BYTES / 4096), "places, and the results' way out");
+    static_assert(H % 2 == 1 && H >= 5 && H <= 9 && H * BYTES <= 160 * 1024, "places");
     // (an array each, so that the compiler sees which loads a read has to wait for)
+    constexpr int MORE = H > 5 ? BYTES : 16, MOST = H > 7 ? BYTES : 16;
     __shared__ __attribute__((aligned(1024))) char lds0[BYTES], lds1[BYTES], lds2[BYTES], lds3[BYTES], lds4[BYTES];
-    __shared__ __attribute__((aligned(1024))) char lds5[H > 5 ? BYTES : 16], lds6[H > 6 ? BYTES : 16], lds7[H > 7 ? BYTES : 16], lds8[H > 8 ? BYTES : 16];
+    __shared__ __attribute__((aligned(1024))) char lds5[MORE], lds6[MORE], lds7[MOST], lds8[MOST];
     auto place = [&](int n) __attribute__((always_inline)) {
         n %= H;
-        return n == 0 ? lds0 : n == 1 ? lds1 : n == 2 ? lds2 : n == 3 ? lds3 : n == 4 ? lds4 : n == 5 ? lds5 : n == 6 ? lds6 : n == 7 ? lds7 : lds8;
+        return n == 0 ? lds0 : n == 1 ? lds1 : n == 2 ? lds2 : n == 3 ? lds3 : n == 4 ? lds4 : n == 5 ? lds5 : n == 6 ? lds6
+               : n == 7 ? lds7 : lds8;
     };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN, g = lane >> 5, col = lane & 31;
@@ -98,8 +114,8 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
     tile_of(blockIdx.x, t.m, t.n, tm, tn);
     const int first = blockIdx.y * t.per, end = first + t.per < a.K ? first + t.per : a.K;  // of K
 
-    // this wave's loads of a stage: rows (i NW + wave) 8 .. + 7 each, tokens first; a lane brings 16 bytes of one row. Rows past
-    // the last and bytes past K are past the buffer's end: they read as zero.
+    // this wave's loads of a stage: rows (i NW + wave) 8 .. + 7 each; a lane brings 16 bytes of one row. Rows past the last and
+    // bytes past K are past the buffer's end: they read as zero.
     const int lr = lane >> 3, lc = ((lane & 7) ^ turn_of(wave * 8 + lr)) * 16;
     const Rows x = rows_at(a.x, a.ldx, tm * B, a.M, B), w = rows_at(a.w, a.ldw, tn * B, a.N, B);
     const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc((void *)x.p, 0, x.bytes, 0x00027000);
@@ -168,7 +184,7 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
         read(nx, nw, 0, p0);
         multiply(p1);
 #pragma unroll
-        for (int i = 0; i < TN * TM; i++) {  // (a wave's loads queue behind each other: all at once they would hold up its products)
+        for (int i = 0; i < TN * TM; i++) {  // (a wave's loads queue behind each other: all at once would hold up its products)
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             if (i < TN + TM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x020, (2 * NLH + TN * TM - 1) / (TN * TM), 0);
@@ -216,11 +232,12 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
             const int n = n0 + i * 32 + en + c;
             ws[i][c] = a.w_scale[n < a.N ? n : a.N - 1];
         }
-    // Parts of 32 x 32 through LDS, PB at a time (each wave its own 4 KiB for each): a lane's accumulators are 4 channels of one
-    // token, four times; rows of 128 bytes go to memory, 8 of them with an instruction. (Parts of lines cost as much as whole ones.)
+    // Parts of 32 x 32 through LDS, PB at a time (each wave its own 4 KiB for each): a lane's accumulators are 4 channels of
+    // one token, four times; rows of 128 bytes go to memory, 8 of them with an instruction. (Parts of lines cost as much as
+    // whole ones. One part at a time 64 x 12288 x 2048 added to y 8.9 us, two 7.9, four spill.)
     constexpr int PB = TN * TM < 2 ? 1 : 2;
     static_assert(2 * PB * 4096 <= BYTES && NW / 2 <= H && TN * TM % PB == 0, "two waves a place");
-    auto results = [&](auto adds, auto inside) __attribute__((always_inline)) {  // inside: the whole tile is
+    auto results = [&](auto adds, auto inside) __attribute__((always_inline)) {  // inside: all of this wave's tile is
         constexpr bool ADDS = decltype(adds)::value, INSIDE = decltype(inside)::value;
         f4 was[PB][4];
         char *const own = place(wave >> 1) + (wave & 1) * (PB * 4096);
@@ -233,7 +250,8 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
                     for (int u = 0; u < 4; u++) {
                         const int m = m0 + (p0 + p) % TM * 32 + 8 * u + er, n = n0 + (p0 + p) / TM * 32 + en;
                         if constexpr (!INSIDE) was[p][u] = f4{0, 0, 0, 0};
-                        if (INSIDE || (m < a.M && n + 4 <= a.N)) was[p][u] = *(const f4u *)(a.y + (int64_t)m * a.ldy + n);
+                        if (INSIDE || (m < a.M && n + 4 <= a.N))
+                            was[p][u] = *(const f4u *)(a.y + (int64_t)m * a.ldy + n);
                     }
             }
             if (p0 == 0) meet<0>();
@@ -241,15 +259,18 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
             for (int p = 0; p < PB; p++) {
                 const i16 v = acc[(p0 + p) / TM][(p0 + p) % TM];
 #pragma unroll
-                for (int q = 0; q < 4; q++)
-                    *(i4 *)(own + p * 4096 + col * 128 + (((2 * q + g) ^ (col & 7)) << 4)) = i4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                for (int q = 0; q < 4; q++) {
+                    i4 *const to = (i4 *)(own + p * 4096 + col * 128 + (((2 * q + g) ^ (col & 7)) << 4));
+                    *to = i4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                }
             }
 #pragma unroll
             for (int p = 0; p < PB; p++) {
                 const int i = (p0 + p) / TM, j = (p0 + p) % TM, n = n0 + i * 32 + en;
                 i4 o[4];
 #pragma unroll
-                for (int u = 0; u < 4; u++) o[u] = *(const i4 *)(own + p * 4096 + (8 * u + er) * 128 + (((lane & 7) ^ er) << 4));
+                for (int u = 0; u < 4; u++)
+                    o[u] = *(const i4 *)(own + p * 4096 + (8 * u + er) * 128 + (((lane & 7) ^ er) << 4));
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const int m = m0 + j * 32 + 8 * u + er;
@@ -265,9 +286,7 @@ __global__ __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(EU,
                     for (int c = 0; c < 4; c++) r[c] = (float)o[u][c] * xs[j][u] * ws[i][c];
                     if (INSIDE || n + 4 <= a.N) {
                         if constexpr (ADDS) r += was[p][u];
-                        f4u *y = (f4u *)(a.y + (int64_t)m * a.ldy + n);
-                        if (t.stream) __builtin_nontemporal_store(r, y);
-                        else *y = r;
+                        *(f4u *)(a.y + (int64_t)m * a.ldy + n) = r;
                     } else {
                         put(a, m, n, r);
                     }
@@ -312,8 +331,6 @@ template <int B, int WM, int WN, int H, int EU> void tiles(const Gemm8Args &a, i
     t.ld = (a.N + 3) / 4 * 4;
     t.per = ((a.K + KB - 1) / KB + parts - 1) / parts * KB;
     t.sums = parts > 1 ? sums : nullptr;
-    // past the caches from 32 MB of results on, what the eight L2s hold
-    t.stream = (int64_t)a.M * a.N * 4 >= (int64_t)32 << 20;
     gemm8_tile<B, WM, WN, H, EU><<<dim3(t.m * t.n, parts), WM * WN * 64, 0, st>>>(a, t);
     const int blocks = (int)(((int64_t)a.M * (t.ld / 4) + 255) / 256);
     if (parts == 2) gemm8_join<2><<<blocks, 256, 0, st>>>(a, sums, t.ld);
@@ -323,17 +340,22 @@ template <int B, int WM, int WN, int H, int EU> void tiles(const Gemm8Args &a, i
     else if (parts == 8) gemm8_join<8><<<blocks, 256, 0, st>>>(a, sums, t.ld);
 }
 
-// Few tokens: 16 tokens x 16 channels a workgroup, K over its W waves. A wave brings 128 bytes of K of its 32 rows at a time, whole
-// lines (loads of half lines, as the products' registers would take them, reach 40 GB/s a CU, these 112), to places of its own in
-// LDS, two ahead; the waves' sums meet at the end.
+// Few tokens: 16 tokens x 16 channels a workgroup, K over its W waves. A wave brings 128 bytes of K of its 32 rows at a time,
+// whole lines (loads of half lines, as the products' registers would take them, reach 40 GB/s a CU, these 112), to places of
+// its own in LDS, two ahead; the waves' sums meet at the end. Bound by the weights' bytes where channels are many, else by what
+// a CU takes in. (W = 2: 16 x 24576 x 4096 19.9 us, 33 x 4096 x 4096 6.5; with 4 places 22.4 and 6.4, with 8 25.1 and 9.9, as
+// fewer workgroups fit on a CU. With 32 tokens a workgroup 64 x 4096 x 4096 6.9 and 16 x 512 x 8192 7.1, with 16 7.8 and 6.2.)
 template <int W> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm8Args a, int tiles_m, int tiles_n) {
 #if __HIP_DEVICE_COMPILE__
     constexpr int D = 3, UNIT = 4096;  // places a wave; 16 rows of w, then of x, with the turns of tile rows
     __shared__ __attribute__((aligned(1024))) char lds[W * D * UNIT];
     __shared__ i4 sums[W][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, col = lane & 15;
+    // the tokens of the same channels one after another, on one XCD (50 x 2880 x 5760: 7.9 us, channels first 9.1;
+    // 33 x 4096 x 4096: 6.5 and 6.0)
     const int t = place_of(blockIdx.x, tiles_m * tiles_n), tn = __builtin_amdgcn_readfirstlane(t / tiles_m);
-    const int n0 = tn * 16, m0 = (t - tn * tiles_m) * 16;  // (the tokens of the same channels one after another, on one XCD)
+    const int n0 = tn * 16, m0 = (t - tn * tiles_m) * 16;
     const Rows x = rows_at(a.x, a.ldx, m0, a.M, 16), w = rows_at(a.w, a.ldw, n0, a.N, 16);
     const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc((void *)x.p, 0, x.bytes, 0x00027000);
     const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc((void *)w.p, 0, w.bytes, 0x00027000);
@@ -356,21 +378,21 @@ template <int W> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm8Args a
     auto fetch = [&](int at, int u) __attribute__((always_inline)) {
         const int k = u * KB, from = k < a.K ? k : a.K;
         const uint32_t past = u < end && k + lc < a.K ? 0u : 1u << 31;  // (of another wave, or past K: zeros)
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (lds_void *)(own + at + i * 1024), 16, (wat + i * 8 * (uint32_t)a.ldw) | past, from, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void *)(own + at + 2048 + i * 1024), 16, (xat + i * 8 * (uint32_t)a.ldx) | past, from, 0, 0);
+        const uint32_t w8 = 8 * (uint32_t)a.ldw, x8 = 8 * (uint32_t)a.ldx;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (lds_void *)(own + at), 16, wat | past, from, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (lds_void *)(own + at + 1024), 16, (wat + w8) | past, from, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void *)(own + at + 2048), 16, xat | past, from, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void *)(own + at + 3072), 16, (xat + x8) | past, from, 0, 0);
     };
     i4 acc = {0, 0, 0, 0};
-    const uint32_t row = (uint32_t)(uintptr_t)(lds_void *)own + col * KB, c0 = row + ((g << 4) ^ (col & 6) << 4), c1 = row + ((64 + (g << 4)) ^ (col & 6) << 4);
+    const uint32_t row = (uint32_t)(uintptr_t)(lds_void *)own + col * KB, turn = (col & 6) << 4;
+    const uint32_t c0 = row + ((uint32_t)(g << 4) ^ turn), c1 = row + ((uint32_t)(64 + (g << 4)) ^ turn);
 #pragma unroll
     for (int d = 0; d < D; d++) fetch(d * UNIT, first + d);
     int at = 0;
     for (int u = first; u < end; u++) {
         i4 w0, x0, w1, x1;
-        // the oldest place's loads are there; it is read, and free. (Of reads that it sees the compiler makes each wait for all loads.)
+        // the oldest place's loads are there; it is read, and free. (A read that the compiler sees it lets wait for all loads.)
         asm volatile("s_waitcnt vmcnt(%6)\n\t"
                      "ds_read_b128 %0, %4\n\t"
                      "ds_read_b128 %1, %4 offset:2048\n\t"
@@ -403,11 +425,11 @@ template <int W> void few(const Gemm8Args &a, hipStream_t st) {
     gemm8_few<W><<<tm * tn, W * 64, 0, st>>>(a, tm, tn);
 }
 
-// Which kernel, and into how many parts K goes: the one whose time comes out shortest. A launch is rounds of workgroups. A round
-// takes `fill` for its first loads, for each stage `alone` where it leaves most of the chip's memory paths to few workgroups and
-// `full` where it fills the chip, and the time of its results, by a CU's rate or by the chip's. (us, fitted to 33 products of 16 to
-// 4096 tokens, 140 to 24576 channels, K 288 to 12288; there the choice is mostly within 5% of the best of these kernels, at
-// worst 13% behind it.)
+// Which kernel, and into how many parts K goes: the one whose time comes out shortest. A launch is rounds of workgroups. A
+// round takes `fill` for its first loads, for each stage `alone` where it leaves most of the chip's memory paths to few
+// workgroups and `full` where it fills the chip, and the time of its results, by a CU's rate or by the chip's. (us, fitted to
+// 60 products of 1 to 4096 tokens, 17 to 24576 channels, K 128 to 12288; there the choice is mostly within 5% of the best of
+// these kernels, at worst 13% behind it.)
 struct Shape {
     int tile, at_once;
     double fill, alone, full;
@@ -426,7 +448,8 @@ Plan plan_of(const Gemm8Args &a) {
     const double weights = 1.0 + (double)a.N * a.K / 5.0e6;  // reading them, at 5 TB/s
     const int64_t few_wgs = (int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16);
     // a CU takes in 98 GB/s; weights that several workgroups take come more slowly (a launch holds 2^32 threads)
-    const double a_cu = (few_wgs > 256 ? (double)few_wgs : 256.0) / 256.0, few_us = 2.5 + a_cu * (0.2 + (16 + (a.M < 16 ? a.M : 16)) * a.K / 98e3);
+    const double a_cu = (few_wgs > 256 ? (double)few_wgs : 256.0) / 256.0;
+    const double few_us = 2.5 + a_cu * (0.2 + (16.0 + (a.M < 16 ? a.M : 16)) * a.K / 98e3);
     const double few_weights = weights + (a.M > 16 ? 0.7 * a_cu : 0.0);
     Plan best{-1, 1};
     double best_us = few_wgs > 1 << 24 ? 1e9 : few_us > few_weights ? few_us : few_weights;
@@ -438,7 +461,8 @@ Plan plan_of(const Gemm8Args &a) {
             const int stages = ((a.K + KB - 1) / KB + parts - 1) / parts;
             const double y = 4.0 * a.M * ((a.N + 3) / 4 * 4), touched = a.accum ? 2.0 : 1.0;
             if (parts > 1 && (stages < 8 || parts * y > (double)(64 << 20))) break;
-            const double bytes = 4.0 * s.tile * s.tile * (parts > 1 ? 1.0 : touched), one = bytes / 60e3, all = s.at_once * bytes / 5.0e6;
+            const double bytes = 4.0 * s.tile * s.tile * (parts > 1 ? 1.0 : touched);
+            const double one = bytes / 60e3, all = s.at_once * bytes / 5.0e6;
             auto round = [&](double part) {
                 const double results = part < 1 ? one + (all > one ? all - one : 0.0) * part : all;
                 return s.fill + results + stages * (s.alone + (s.full - s.alone) * (s.late ? part * part : part));
@@ -466,8 +490,8 @@ hipError_t launch_gemm8(const Gemm8Args &a, void *ws, size_t ws_bytes, size_t *n
     *need = sums_bytes(a, p);
     if (*need && (!ws || ws_bytes < *need || ((uintptr_t)ws & 15))) return hipErrorInvalidValue;
     if (p.shape < 0) {
-        // four waves where half of the CUs or more have no workgroup and K is long (5 x 2048 x 12288: 6.2 us, with two 8.8; 1 x 2048
-        // x 4096: 4.4 and 4.1; 17 x 4096 x 4096: 6.0 and 5.3)
+        // four waves where half of the CUs or more have no workgroup and K is long (5 x 2048 x 12288: 6.2 us, with two 8.8;
+        // 1 x 2048 x 4096: 4.4 and 4.1; 17 x 4096 x 4096: 6.0 and 5.3)
         if ((int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16) <= 128 && a.K >= 8192) few<4>(a, st);
         else few<2>(a, st);
     }

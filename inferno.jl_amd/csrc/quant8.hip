@@ -14,6 +14,13 @@
 // formed in fp32, and where 127 t / top comes nearer to a tie than their error
 // (a value in ten thousand) that one value is formed again in fp64. So codes do
 // not depend on how the fp32 arithmetic was ordered or contracted.
+//
+// What bounds it. Many rows: memory. 8190 rows of 4096, the residual added and
+// stored, in 72 us (268 MB read, 168 written: 6.1 TB/s; a copy reaches 5.2),
+// 4096 plain rows of 12288 in 51 (5.0), 4097 gates of 6144 in 51 (4.5: the
+// exponentials and divisions beside). Few: a launch and one row's way, 3.5 to
+// 4.5 us (a gate of 12288 7.5). One workgroup a row, for a row's largest is one
+// exchange through LDS then, and its values wait for it in registers.
 #include "common.h"
 #include "int8.h"
 
@@ -135,8 +142,8 @@ template <bool STREAM> __device__ __forceinline__ f4 take4(const Quant8Args &a, 
     return v;
 }
 
-// What a thread has found of its row: the sum of squares of x, and the largest |t| in fp32, as bits (as whole numbers NaN is the
-// largest); for a norm with weights the largest exact product besides.
+// What a thread has found of its row: the sum of squares of x, and the largest |t| in fp32, as bits (as whole numbers NaN is
+// the largest); for a norm with weights the largest exact product besides.
 struct Found {
     float ssq = 0.f;
     uint32_t top = 0;
@@ -250,8 +257,8 @@ template <int ACT, int V, bool STREAM = false> __global__ __launch_bounds__(1024
     }
     if (!weights) most = (double)ftop;
     if (ACT == Q8_SILU_MUL || (!DIRECT && ACT == Q8_RMSNORM && a.norm_w)) {
-        // the exact largest |t| is among those whose fp32 value is the largest (a product's rounding keeps the order), or within
-        // twice the fp32 gate's error of it
+        // the exact largest |t| is among those whose fp32 value is the largest (a product's rounding keeps the order), or
+        // within twice the fp32 gate's error of it
         const float from = ACT == Q8_SILU_MUL ? ftop * (1.f - 0x1p-18f) : ftop;
         if constexpr (V > 0) {
 #pragma unroll
@@ -278,13 +285,13 @@ template <int ACT, int V, bool STREAM = false> __global__ __launch_bounds__(1024
 
 template <int ACT> void launch(const Quant8Args &a, hipStream_t st) {
     const int n4 = a.K / 4;
-    // few values a thread where rows are few and a row's time is latency; four times 4 where they are many (8190 rows of 4096: 34 us,
-    // with one 83), as far as a wave has them
+    // few values a thread where rows are few and a row's time is latency; four times 4 where they are many (8190 rows of 4096,
+    // plain: 34 us, with one 83), as far as a wave has them
     const int v = n4 > 4096 ? 0 : n4 > 2048 ? 4 : a.M <= 256 ? (n4 > 1024 ? 2 : 1) : n4 > 128 ? 4 : n4 > 64 ? 2 : 1;
     const int nt = v ? ((n4 + v - 1) / v + 63) / 64 * 64 : 1024;
     if constexpr (ACT == Q8_RMSNORM) {
-        // rows that are read, added to and written past the caches, from 64 MB of them on (8190 of 4096: 75.7 us, 81.4 through them;
-        // 515: 9.0 and 8.1)
+        // rows that are read, added to and written past the caches, from 64 MB of them on (8190 of 4096: 75.7 us, 81.4 through
+        // them; 515: 9.0 and 8.1)
         if (v == 4 && a.x && a.n_add == 1 && (int64_t)a.M * a.K >= (int64_t)16 << 20) {
             quant8_kernel<ACT, 4, true><<<a.M, nt, 0, st>>>(a);
             return;

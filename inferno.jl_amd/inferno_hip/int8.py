@@ -20,7 +20,7 @@ from .mixers import _device_of, _refuse, _rows, _torch, _whole, _workspace
 from .quantized_kernels import ACT_PLAIN, ACT_RMSNORM, ACT_SILU_MUL, GEMM_ACCUM, _raw_stream, check_tensor, dequant, made_for
 
 _i8 = _u8 = _f32 = _Tensor = _current_device = _stream_of = _c_quantize = _c_gemm = None
-_INPUT = Struct("@PiiPfPiq").pack  # ihip_gemm_input (a call's host time is most of a small one's: a ctypes Structure takes longer)
+_INPUT = Struct("@PiiPfPiq").pack  # ihip_gemm_input (host time is most of a small call: a ctypes Structure takes longer)
 
 
 def _names():
@@ -175,8 +175,8 @@ def gemm_i8(q, scales, w, w_scales, accum: bool = False, out=None, ws=None, stre
     try:
         (n, k), (m, kq), (ldw, w1), (ldq, q1) = w.shape, q.shape, w.stride(), q.stride()
         dev = q.get_device()
-        fine = (dev >= 0 and dev == _current_device() and q.dtype is _i8 and w.dtype is _i8 and w1 == 1 and q1 == 1 and kq >= k > 0
-                and w.get_device() == dev and m > 0 and n > 0 and scales.dtype is _f32 and scales.shape == (m,)
+        fine = (dev >= 0 and dev == _current_device() and q.dtype is _i8 and w.dtype is _i8 and w1 == 1 and q1 == 1
+                and kq >= k > 0 and w.get_device() == dev and m > 0 and n > 0 and scales.dtype is _f32 and scales.shape == (m,)
                 and scales.get_device() == dev and scales.is_contiguous() and w_scales.dtype is _f32 and w_scales.shape == (n,)
                 and w_scales.get_device() == dev and w_scales.is_contiguous())
     except (AttributeError, TypeError, ValueError):

@@ -11,7 +11,8 @@ from test_call_streams import HERE, THERE, Lib, Stream, Tensor, Waiting, world  
 @pytest.fixture
 def on8(world, monkeypatch):  # noqa: F811
     real = _lib.load()
-    made = lambda shape, dtype=None, device=None: Waiting(world, (shape,) if isinstance(shape, int) else shape, dtype, world.current)  # noqa: E731
+    size = lambda s: (s,) if isinstance(s, int) else s  # noqa: E731
+    made = lambda shape, dtype=None, device=None: Waiting(world, size(shape), dtype, world.current)  # noqa: E731
     for name, value in (("_i8", torch.int8), ("_u8", torch.uint8), ("_f32", torch.float32), ("_Tensor", Tensor),
                         ("_current_device", lambda: 0), ("_stream_of", lambda device: world.current),
                         ("_c_quantize", lambda *a: world.launched.append(("quantize", a)) or 0),
