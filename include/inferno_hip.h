@@ -640,7 +640,7 @@ int ihip_quantize_i8(const ihip_gemm_input *in, int M, int K, int8_t *q_dev,
  * are left as they were). The sums are 32-bit integers and exact; the sum is
  * rounded to fp32 once and multiplied by x_scale, then by w_scale (a scale that
  * is not finite gives its row or column what fp32 products give). Any M and N
- * from 1 to 2^23 with M N up to 2^38; K a multiple of 16 up to 65536; x and w
+ * from 1 to 2^23 with M N up to 2^36; K a multiple of 16 up to 65536; x and w
  * 16-byte aligned, ldx and ldw multiples of 16 up to 2^22 (of 128, with x and w
  * so aligned, rows are read fastest). y overlaps none of the inputs.
  * ws: ihip_gemm_i8_ws_bytes (may be 0: then NULL is allowed), 16-byte aligned,

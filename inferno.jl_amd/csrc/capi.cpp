@@ -1263,8 +1263,8 @@ int ihip_quantize_i8(const ihip_gemm_input *in, int M, int K, int8_t *q_dev, int
 
 namespace {
 int check_gemm8_shape(const char *fn, int M, int N, int K, int flags) {
-    if (M < 1 || M > 1 << 23 || N < 1 || N > 1 << 23 || (int64_t)M * N > (int64_t)1 << 38)
-        return fail(IHIP_EINVAL, "%s: M=%d N=%d (each 1..2^23, the product up to 2^38)", fn, M, N);
+    if (M < 1 || M > 1 << 23 || N < 1 || N > 1 << 23 || (int64_t)M * N > (int64_t)1 << 36)
+        return fail(IHIP_EINVAL, "%s: M=%d N=%d (each 1..2^23, the product up to 2^36)", fn, M, N);
     if (K < 16 || K > 65536 || K % 16) return fail(IHIP_EINVAL, "%s: K=%d (a multiple of 16 up to 65536)", fn, K);
     if (flags & ~IHIP_GEMM_ACCUM) return fail(IHIP_EINVAL, "%s: flags 0x%x (IHIP_GEMM_ACCUM or 0)", fn, flags);
     return IHIP_OK;

@@ -188,7 +188,7 @@ def gemm_i8(q, scales, w, w_scales, accum: bool = False, out=None, ws=None, stre
         _whole(scales, "scales", _f32, (m,), dev)
         _whole(w_scales, "w_scales", _f32, (n,), dev)
     if m == 1:  # (a single row's stride has no meaning)
-        ldq = (kq + 15) // 16 * 16
+        ldq = (k + 15) // 16 * 16
     if n == 1:
         ldw = (k + 15) // 16 * 16
     if out is None:

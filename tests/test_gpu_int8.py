@@ -415,6 +415,39 @@ def test_single_rows_of_any_stride(ih):
     same(ih.quantize_i8(cu(x).as_strided((1, 48), (5, 1))), R.quantize(x), R.HALF)
 
 
+def test_offsets_past_32_bits(ih):
+    """Codes, weights, rows and results of more than 2^32 bytes or 2^31 values: the last rows are those of a call on them alone."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(25)
+    codes = lambda m, k: torch.randint(-127, 128, (m, k), dtype=torch.int8, device="cuda", generator=g)  # noqa: E731
+    ones = lambda m: torch.rand(m, device="cuda", generator=g)  # noqa: E731
+    big, small, sb, ss = codes(600000, 8192), codes(40, 8192), ones(600000), ones(40)  # 4.9 GB
+    y = ih.gemm_i8(small[:3], ss[:3], big, sb)
+    assert torch.equal(y[:, -70:], ih.gemm_i8(small[:3], ss[:3], big[-70:].clone(), sb[-70:].clone()))
+    y = ih.gemm_i8(big, sb, small, ss)
+    assert torch.equal(y[-70:], ih.gemm_i8(big[-70:].clone(), sb[-70:].clone(), small, ss))
+    del big, y
+    q, w, s, ws = codes(80000, 64), codes(30001, 64), ones(80000), ones(30001)
+    y = ih.gemm_i8(q, s, w, ws)  # 2.4e9 values
+    assert torch.equal(y[-70:], ih.gemm_i8(q[-70:].clone(), s[-70:].clone(), w, ws))
+    before = y[-70:].clone()
+    ih.gemm_i8(q, s, w, ws, accum=True, out=y)
+    assert torch.equal(y[-70:], before + before)
+    del y
+    x = torch.randn((300000, 8192), device="cuda", generator=g)  # 2.5e9 values
+    # (a norm's sum of squares is added in an order that depends on the number of rows: each of the two scales is within
+    # norm_tol of the exact one, so they are within twice that of each other)
+    alike = lambda s, rs: bool(((s[-70:].double() - rs).abs() <= 2 * R.norm_tol(8192) * rs).all())  # noqa: E731
+    for call in (ih.quantize_i8, ih.silu_mul_i8, ih.rmsnorm_i8):
+        (c, s), (rc, rs) = call(x), call(x[-70:].clone())
+        assert torch.equal(c[-70:], rc) and (alike(s, rs) if call is ih.rmsnorm_i8 else torch.equal(s[-70:], rs))
+    add = torch.full_like(x, 0.5)
+    last = x[-70:] + 0.5
+    c, s = ih.rmsnorm_i8(x, add=add)
+    rc, rs = ih.rmsnorm_i8(last.clone())
+    assert torch.equal(x[-70:], last) and torch.equal(c[-70:], rc) and alike(s, rs)
+
+
 def test_python_refusals(ih):
     import torch
     x = torch.zeros((4, 64), device="cuda")
