@@ -145,8 +145,8 @@ template <int ACT> __device__ __forceinline__ void wide_row(const Quant8Args &a,
     if (tid == 0) a.scale[row] = fine ? scale : __builtin_nanf("");
 }
 
-// how far 127 t / top in fp32 may be off: t to 1 (norm) or 7 (silu: exp 2, 1 + exp 1, reciprocal 2, two products) halves of
-// 2^-23, top as much, its reciprocal and the product one each: 127 (1 + 1 + 2) 2^-24 = 3.1e-5, 127 (7 + 7 + 2) 2^-24 = 1.2e-4
+// how far 127 t / top in fp32 may be off: t to 1 (norm) or 8 (silu: exp 3, 1 + exp 1, reciprocal 2, two products) halves of
+// 2^-23, top as much, its reciprocal and the product one each: 127 (1 + 1 + 2) 2^-24 = 3.1e-5, 127 (8 + 8 + 2) 2^-24 = 1.4e-4
 template <int ACT> constexpr float NEAR = ACT == Q8_SILU_MUL ? 2e-4f : 4e-5f;
 
 // 4 values at column c of a row, the residual's additions made and stored
@@ -176,6 +176,14 @@ struct Found {
     double most = 0.0;
 };
 
+// exp(x) for x up to 88: 2^(x log2 e), the exponent's rest (its rounding and log2 e's second part) to first order
+__device__ __forceinline__ float exp_to_88(float x) {
+    const float y = x * 0x1.715476p+0f;
+    const float rest = __builtin_fmaf(x, 0x1.4ae0cp-26f, __builtin_fmaf(x, 0x1.715476p+0f, -y));
+    const float e = __builtin_amdgcn_exp2f(y);
+    return __builtin_fmaf(e, rest * 0x1.62e43p-1f, e);
+}
+
 // x to t in fp32
 template <int ACT> __device__ __forceinline__ f4 to_t(f4 x, f4 w, bool weights, Found &f) {
     f4 t = x;
@@ -186,8 +194,8 @@ template <int ACT> __device__ __forceinline__ f4 to_t(f4 x, f4 w, bool weights, 
             t[j] = x[j] * w[j];
             if (weights) f.most = fmax(f.most, fabs((double)x[j] * (double)w[j]));
         } else if constexpr (ACT == Q8_SILU_MUL) {
-            t[j] = x[j] * __builtin_amdgcn_rcpf(1.f + expf(-x[j])) * w[j];
-            // (exp(-x) passes fp32 there; what is lost counts only beside so large an up)
+            t[j] = x[j] * __builtin_amdgcn_rcpf(1.f + exp_to_88(fminf(-x[j], 88.f))) * w[j];
+            // (exp(-x) stops there; what is lost counts only beside so large an up)
             if (x[j] < -80.f && fabsf(w[j]) > 1e8f) f.top = 0x7fffffffu;
         }
         const uint32_t b = __float_as_uint(t[j]) & 0x7fffffffu;
@@ -208,21 +216,25 @@ __device__ __forceinline__ void raise_most(const Quant8Args &a, int64_t row, int
 
 template <int ACT>
 __device__ __forceinline__ uint32_t codes4(const Quant8Args &a, int64_t row, int c, f4 t, float inv, double most) {
-    int r[4];
-    bool near = false;
+    constexpr float WHOLE = 0x1.8p23f;  // v + WHOLE: v rounded, ties to even, in the low bits
+    uint32_t r[4];
+    bool near[4], any = false;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const float v = t[j] * inv, n = rintf(v);
-        near |= fabsf(v - n) > 0.5f - NEAR<ACT>;
-        r[j] = (int)n;
+        const float v = t[j] * inv, n = v + WHOLE;
+        near[j] = fabsf(v - (n - WHOLE)) > 0.5f - NEAR<ACT>;
+        any |= near[j];
+        r[j] = __float_as_uint(n);
     }
-    if (near) {
+    if (any) {
         const f4 x = input4(a, row, c), w = second4<ACT>(a, row, c);
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (fabsf(t[j] * inv - (float)r[j]) > 0.5f - NEAR<ACT>) r[j] = (int)rint(exact1<ACT>(x[j], w[j]) * 127.0 / most);
+            if (near[j]) r[j] = (uint32_t)(int)rint(exact1<ACT>(x[j], w[j]) * 127.0 / most);
     }
-    return (uint32_t)(r[0] & 255) | (uint32_t)(r[1] & 255) << 8 | (uint32_t)(r[2] & 255) << 16 | (uint32_t)r[3] << 24;
+    // (bytes 0 of four words: two of the first two, two of the last two, those of both)
+    const uint32_t lo = __builtin_amdgcn_perm(r[1], r[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(r[3], r[2], 0x0c0c0400);
+    return lo | hi << 16;
 }
 
 // One workgroup a row, V x 4 values a thread kept in registers; V = 0: rows of any length, read a second time for the codes.
