@@ -16,11 +16,12 @@
 // not depend on how the fp32 arithmetic was ordered or contracted.
 //
 // What bounds it. Many rows: memory. 8190 rows of 4096, the residual added and
-// stored, in 72 us (268 MB read, 168 written: 6.1 TB/s; a copy reaches 5.2),
-// 4096 plain rows of 12288 in 51 (5.0), 4097 gates of 6144 in 51 (4.5: the
-// exponentials and divisions beside). Few: a launch and one row's way, 3.5 to
-// 4.5 us (a gate of 12288 7.5). One workgroup a row, for a row's largest is one
-// exchange through LDS then, and its values wait for it in registers.
+// stored, in 71 us (268 MB read, 168 written: 6.1 TB/s; a copy reaches 5.2),
+// 4096 plain rows of 12288 in 41 (6.2), 4097 gates of 6144 in 45 (5.1). Few: a
+// launch and one row's way, 2 us plain, 3.1 with the norm and the residual, and
+// a gate's vector instructions, 5.5 us for 12288 on one CU. One workgroup a row,
+// for a row's largest is one exchange through LDS then, and its values wait for
+// it in registers.
 #include "common.h"
 #include "int8.h"
 
@@ -36,8 +37,8 @@ struct Quant8Shared {
     uint64_t most;
 };
 
-// The lanes' values joined by op from neighbour to neighbour (DPP: 0.8 us less for a row of 4096 than through LDS), 0 standing
-// for lanes that there are not: the 16 of a row of lanes in its last, then the rows in the last of all.
+// The lanes' values joined by op from neighbour to neighbour (DPP, where a shuffle goes by way of LDS), 0 standing for lanes
+// that there are not: the 16 of a row of lanes in its last, then the rows in the last of all.
 template <int CTRL, class T> __device__ __forceinline__ T from_lane(T v) {
     if constexpr (sizeof(T) == 8) {
         const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -270,7 +271,8 @@ template <int ACT, int V, bool STREAM = false> __global__ __launch_bounds__(1024
         Found none;
         return to_t<ACT>(input4(a, row, 4 * c), second4<ACT>(a, row, 4 * c), false, none);
     };
-    // the waves' findings, then those of all waves: a lane for each
+    // the waves' findings, then those of all waves: a lane for each (one row of 4096 3.1 us; by shuffles, and every thread over
+    // all waves, 4.3)
     auto umax = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
     auto dmax = [](double a, double b) { return fmax(a, b); };
     auto sum = [](float a, float b) { return a + b; };
