@@ -347,7 +347,8 @@ template <int B, int WM, int WN, int H, int EU> void tiles(const Gemm8Args &a, i
 // fewer workgroups fit on a CU. With 32 tokens a workgroup 64 x 4096 x 4096 6.9 and 16 x 512 x 8192 7.1, with 16 7.8 and 6.2.)
 template <int W> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm8Args a, int tiles_m, int tiles_n) {
 #if __HIP_DEVICE_COMPILE__
-    constexpr int D = 3, UNIT = 4096;  // places a wave; 16 rows of w, then of x, with the turns of tile rows
+    // D places a wave, each 16 rows of w, then of x, with turns as a tile's rows; ROWS: bytes of the 8 rows of a load
+    constexpr int D = 3, ROWS = 8 * KB, UNIT = 4 * ROWS;
     __shared__ __attribute__((aligned(1024))) char lds[W * D * UNIT];
     __shared__ i4 sums[W][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -380,9 +381,9 @@ template <int W> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm8Args a
         const uint32_t past = u < end && k + lc < a.K ? 0u : 1u << 31;  // (of another wave, or past K: zeros)
         const uint32_t w8 = 8 * (uint32_t)a.ldw, x8 = 8 * (uint32_t)a.ldx;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (lds_void *)(own + at), 16, wat | past, from, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (lds_void *)(own + at + 1024), 16, (wat + w8) | past, from, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void *)(own + at + 2048), 16, xat | past, from, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void *)(own + at + 3072), 16, (xat + x8) | past, from, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (lds_void *)(own + at + ROWS), 16, (wat + w8) | past, from, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void *)(own + at + 2 * ROWS), 16, xat | past, from, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void *)(own + at + 3 * ROWS), 16, (xat + x8) | past, from, 0, 0);
     };
     i4 acc = {0, 0, 0, 0};
     const uint32_t row = (uint32_t)(uintptr_t)(lds_void *)own + col * KB, turn = (col & 6) << 4;

@@ -64,7 +64,8 @@ template <class T, class Op> __device__ __forceinline__ T join64(T v, Op op) {
 template <class T> __device__ __forceinline__ T of_lane15(T v) {
     if constexpr (sizeof(T) == 8) {
         const uint64_t b = __builtin_bit_cast(uint64_t, v);
-        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, 15), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 15);
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, 15);
+        const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 15);
         return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
     } else {
         return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 15));
