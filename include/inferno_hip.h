@@ -625,7 +625,8 @@ int ihip_gated_delta_rule(const ihip_delta *a, void *ws, size_t ws_bytes,
  *   top  = max_k |t_k|;  q_k = 127 t_k / top rounded to the nearest, ties to even;
  *   scale = r top / 127, r = 1, or 1 / sqrt(mean(x'^2) + eps) for IHIP_ACT_RMSNORM.
  * The codes are those of the exact t (formed in fp64 where fp32 cannot tell), so
- * they do not depend on how fp32 arithmetic is ordered. A row of zeros has scale
+ * they do not depend on how fp32 arithmetic is ordered; a norm's scale may differ
+ * in its last places with M, as mean(x'^2) is summed in fp32. A row of zeros has scale
  * 0 and codes 0; a row with a value that is not finite, or whose scale passes
  * fp32, has scale NaN and codes 0 (its products are NaN). K a multiple of 16 up
  * to 65536, M up to 2^23; x, norm_w, add and q 16-byte aligned, ldx and add_stride
@@ -639,7 +640,8 @@ int ihip_quantize_i8(const ihip_gemm_input *in, int M, int K, int8_t *q_dev,
  * ldx / ldw values between rows; y fp32, ldy values between rows (columns past N
  * are left as they were). The sums are 32-bit integers and exact; the sum is
  * rounded to fp32 once and multiplied by x_scale, then by w_scale (a scale that
- * is not finite gives its row or column what fp32 products give). Any M and N
+ * is not finite gives its row or column what fp32 products give): the same bits
+ * for a row and a channel, whatever M, N and the kernel that takes them. Any M and N
  * from 1 to 2^23 with M N up to 2^36; K a multiple of 16 up to 65536; x and w
  * 16-byte aligned, ldx and ldw multiples of 16 up to 2^22 (of 128, with x and w
  * so aligned, rows are read fastest). y overlaps none of the inputs.

@@ -278,6 +278,17 @@ def test_product_strides(ih, m, n, k):
         assert bool((rest == 5.0).all())
 
 
+def test_a_rows_results_are_its_own(ih):
+    """The same bits for a row and a channel from every kernel, alone or among others, added to y or not."""
+    import torch
+    q, s, w, ws = (cu(v) for v in operands(rng(26), 700, 1540, 8208))
+    y = ih.gemm_i8(q, s, w, ws)
+    for m, n in ((1, 1540), (5, 1540), (64, 1540), (130, 700), (300, 1540), (700, 16), (700, 1)):
+        assert torch.equal(ih.gemm_i8(q[:m], s[:m], w[:n], ws[:n]), y[:m, :n]), (m, n)
+        out = torch.ones((m, n), device="cuda")
+        assert torch.equal(ih.gemm_i8(q[:m], s[:m], w[:n], ws[:n], accum=True, out=out), y[:m, :n] + 1), (m, n)
+
+
 def test_scales_not_finite(ih):
     """A row of scale NaN is NaN, the others are not."""
     m, n, k = 70, 40, 64
