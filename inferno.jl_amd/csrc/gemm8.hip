@@ -17,6 +17,8 @@
 #include "common.h"
 #include "int8.h"
 
+#pragma clang fp contract(off)  // (the addition to y after the product's own rounding, in every kernel)
+
 namespace {
 
 typedef int i4 __attribute__((ext_vector_type(4)));

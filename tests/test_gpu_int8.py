@@ -289,6 +289,20 @@ def test_a_rows_results_are_its_own(ih):
         assert torch.equal(ih.gemm_i8(q[:m], s[:m], w[:n], ws[:n], accum=True, out=out), y[:m, :n] + 1), (m, n)
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 300, 272), (491, 668, 32), (385, 1923, 2576), (1012, 1860, 176), (300, 2001, 8208), (700, 1540, 8208)])
+def test_added_after_its_rounding(ih, m, n, k):
+    """The product's roundings, then that of the addition, each by itself: the same bits as the four steps one by one."""
+    import torch
+    q, s, w, ws = (cu(v) for v in operands(rng(27, m), m, n, k))
+    y = cu(rng(28, m).standard_normal((m, n)).astype(np.float32)) * 1e4
+    want = torch.from_numpy(R.product(*(a.cpu().numpy() for a in (q, s, w, ws)))).cuda()
+    steps = (q.double() @ w.double().T).float() * s[:, None] * ws
+    near(steps, want.cpu().numpy())
+    assert torch.equal(ih.gemm_i8(q, s, w, ws), steps)
+    want = steps + y
+    assert torch.equal(ih.gemm_i8(q, s, w, ws, accum=True, out=y), want)
+
+
 def test_scales_not_finite(ih):
     """A row of scale NaN is NaN, the others are not."""
     m, n, k = 70, 40, 64
