@@ -418,8 +418,12 @@ template <int W> __global__ __launch_bounds__(W * 64) void gemm8_few(Gemm8Args a
     f4 r;  // (a lane's sums are 4 channels of one token)
 #pragma unroll
     for (int c = 0; c < 4; c++) r[c] = (float)acc[c] * xs * ws[c];
-    if (whole) *(f4u *)(a.y + (int64_t)m * a.ldy + n) = r + was;
-    else put(a, m, n, r);
+    if (whole) {
+        if (a.accum) r += was;  // (not without: -0 + 0 is +0)
+        *(f4u *)(a.y + (int64_t)m * a.ldy + n) = r;
+    } else {
+        put(a, m, n, r);
+    }
 #endif
 }
 
