@@ -103,8 +103,8 @@ __device__ __forceinline__ float row_scale(double top, double ssq, bool norm, in
     return (float)(norm ? s / sqrt(ssq / (double)K + (double)eps) : s);
 }
 
-// A row whose values leave the range in which fp32 serves: all of it in fp64. (Rows of zeros, of values past 1e30 or
-// below 1e-20, and rows with a value that is not finite, whose codes are 0 and whose scale is NaN.)
+// A row whose values leave the range in which fp32 serves: all of it in fp64. (Rows of zeros, of values past most_of or
+// below 1e-20, and rows with a value that is not finite or a scale past fp32, whose codes are 0 and whose scale is NaN.)
 template <int ACT> __device__ __forceinline__ void wide_row(const Quant8Args &a, int64_t row, Quant8Shared &sh) {
     const int tid = threadIdx.x, n4 = a.K / 4;
     uint64_t top = 0;
@@ -146,6 +146,10 @@ template <int ACT> __device__ __forceinline__ void wide_row(const Quant8Args &a,
     }
     if (tid == 0) a.scale[row] = fine ? scale : __builtin_nanf("");
 }
+
+// Up to which largest |t| fp32 serves. The norm's: its scale top / 127 / sqrt(mean(x^2) + eps) can pass fp32 where the row is all
+// but empty and a weight is large, with the sum of squares past 1e-30 and K up to 65536 only from a top of 1.6e23 on.
+template <int ACT> constexpr float most_of = ACT == Q8_RMSNORM ? 1e23f : 1e30f;
 
 // how far 127 t / top in fp32 may be off: t to 1 (norm) or 8 (silu: exp 3, 1 + exp 1, reciprocal 2, two products) halves of
 // 2^-23, top as much, its reciprocal and the product one each: 127 (1 + 1 + 2) 2^-24 = 3.1e-5, 127 (8 + 8 + 2) 2^-24 = 1.4e-4
@@ -290,7 +294,7 @@ template <int ACT, int V, bool STREAM = false> __global__ __launch_bounds__(1024
     if constexpr (ACT == Q8_RMSNORM) ssq = of_lane15(join16(is ? sh.ssq[wave] : 0.f, sum));
     double most = weights ? of_lane15(join16(is ? sh.dssq[wave] : 0.0, dmax)) : 0.0;
     const float ftop = __uint_as_float(top);
-    if (!(ftop > 1e-20f && ftop < 1e30f) || (ACT == Q8_RMSNORM && !(ssq > 1e-30f && ssq < 1e30f))) {
+    if (!(ftop > 1e-20f && ftop < most_of<ACT>) || (ACT == Q8_RMSNORM && !(ssq > 1e-30f && ssq < 1e30f))) {
         __syncthreads();  // (sh is read)
         wide_row<ACT>(a, row, sh);
         return;

@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from test_gpu_int8 import cu, ih, operands, rng  # noqa: F401  (ih: the fixture)
+import _i8ref as R
+from test_gpu_int8 import cu, ih, operands, rng, rows, same  # noqa: F401  (ih: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +30,20 @@ def test_signs_of_zero(ih, m, n, k):  # noqa: F811
     got = ih.gemm_i8(*map(cu, (q, s, w, ws))).cpu().numpy()
     bad = np.argwhere(got.view(np.int32) != want.view(np.int32))
     assert not len(bad), (len(bad), bad[:4].tolist())
+
+
+@pytest.mark.parametrize("k", [16160, 16384, 16400, 65536])
+def test_scales_past_fp32(ih, k):  # noqa: F811
+    """A norm's scale can pass fp32 where neither the row's largest value nor its sum of squares is out of the ordinary: one value
+    that is not zero, eps 0 and a large weight. Such a row has scale NaN and codes 0, its neighbours what they have."""
+    x = np.zeros((6, k), np.float32)
+    x[0, 5], x[1, k - 9], x[4, 5] = 1e-13, -1e-10, 2e-15
+    x[3, 77], x[5, 77] = 1e-13, -1e-3
+    x[2] = rows(rng(31, k), 1, k)[0]
+    w = np.ones(k, np.float32)
+    w[[5, k - 9]] = np.finfo(np.float32).max  # (sqrt(K) / 127 of it: past fp32 from K = 16130 on)
+    w[77] = 1e30
+    want = R.rmsnorm(x, w, 0.0)
+    past = np.isin(np.arange(6), (0, 1, 4))
+    assert np.isnan(want[1][past]).all() and np.isfinite(want[1][~past]).all()
+    same(ih.rmsnorm_i8(cu(x), cu(w), 0.0), want, R.norm_tol(k))
