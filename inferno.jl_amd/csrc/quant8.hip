@@ -200,9 +200,11 @@ template <int ACT> __device__ __forceinline__ f4 to_t(f4 x, f4 w, bool weights, 
             t[j] = x[j] * w[j];
             if (weights) f.most = fmax(f.most, fabs((double)x[j] * (double)w[j]));
         } else if constexpr (ACT == Q8_SILU_MUL) {
-            t[j] = x[j] * __builtin_amdgcn_rcpf(1.f + exp_to_88(fminf(-x[j], 88.f))) * w[j];
-            // (exp(-x) stops there; what is lost counts only beside so large an up)
-            if (x[j] < -80.f && fabsf(w[j]) > 1e8f) f.top = 0x7fffffffu;
+            const float silu = x[j] * __builtin_amdgcn_rcpf(1.f + exp_to_88(fminf(-x[j], 88.f)));
+            t[j] = silu * w[j];
+            // (a silu next to nothing has few bits, of a subnormal gate, or none, as exp(-x) stops at 88 and its reciprocal is 0;
+            // what is lost counts only beside so large an up)
+            if (fabsf(silu) < 1e-30f && fabsf(w[j]) > 1e8f) f.top = 0x7fffffffu;
         }
         const uint32_t b = __float_as_uint(t[j]) & 0x7fffffffu;
         f.top = f.top > b ? f.top : b;

@@ -47,3 +47,27 @@ def test_scales_past_fp32(ih, k):  # noqa: F811
     past = np.isin(np.arange(6), (0, 1, 4))
     assert np.isnan(want[1][past]).all() and np.isfinite(want[1][~past]).all()
     same(ih.rmsnorm_i8(cu(x), cu(w), 0.0), want, R.norm_tol(k))
+
+
+@pytest.mark.parametrize("m,k", [(3, 512), (300, 1040), (2, 16400)])
+def test_gates_below_the_normal_numbers(ih, m, k):  # noqa: F811
+    """Gates whose half is a subnormal number, with ups so large that their product is an ordinary one."""
+    r = rng(32, m, k)
+    for gate, up in ((1e-42, 1e25), (1e-40, 1e37), (3e-38, 1e20), (1e-44, 5e37), (1e-39, 1e9)):
+        g, u = (r.uniform(-1, 1, (m, k)) * gate).astype(np.float32), (r.standard_normal((m, k)) * up).astype(np.float32)
+        g[0, 3:], u[m - 1, 0] = 0, 0
+        gu = np.concatenate([g, u], 1)
+        same(ih.silu_mul_i8(cu(gu)), R.quantize(R.silu_mul(gu)), 2 * R.HALF)
+
+
+@pytest.mark.parametrize("far", [-89.0, -1e3, -9e5, -2e6, -1e12, -1e30, -3e38])
+@pytest.mark.parametrize("m,k", [(3, 512), (300, 1040), (2, 16400)])
+def test_gates_far_below_zero(ih, m, k, far):  # noqa: F811
+    """A finite gate far below zero has a product of nothing, beside products of any size."""
+    r = rng(33, m, k)
+    for up in (1.0, 1e-3, 1e-16, 1e4, 1e12):
+        gu = (2 * r.standard_normal((m, 2 * k))).astype(np.float32)
+        gu[:, k:] *= up
+        gu[:, 1:k:9] = far
+        gu[m - 1, k + 1::9] *= 1e3
+        same(ih.silu_mul_i8(cu(gu)), R.quantize(R.silu_mul(gu)), 2 * R.HALF)
