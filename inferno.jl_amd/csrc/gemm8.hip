@@ -15,18 +15,19 @@
 #include <type_traits>
 
 #include "common.h"
+#include "gemm8_plan.h"
 #include "int8.h"
 
 #pragma clang fp contract(off)  // (the addition to y after the product's own rounding, in every kernel)
 
 namespace {
 
+constexpr int KB = GEMM8_KB;
+
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef int i16 __attribute__((ext_vector_type(16)));
 typedef f4 f4u __attribute__((aligned(4)));  // (rows of y begin at any value)
 typedef __attribute__((address_space(3))) void lds_void;
-
-constexpr int KB = 128;  // bytes of K that a stage holds: a line of each row
 
 // Which of the eight 16-byte places of a row its chunk c takes: c ^ turn_of(row). The 16 lanes that LDS serves at once in a
 // load of 32 rows' chunk c (lanes 0-7 with 16-23, 8-15 with 24-31: rows) then meet in no bank (no conflicts counted).
@@ -432,68 +433,19 @@ template <int W> void few(const Gemm8Args &a, hipStream_t st) {
     gemm8_few<W><<<tm * tn, W * 64, 0, st>>>(a, tm, tn);
 }
 
-// Which kernel, and into how many parts K goes: the one whose time comes out shortest. A launch is rounds of workgroups. A
-// round takes `fill` for its first loads, for each stage `alone` where it leaves most of the chip's memory paths to few
-// workgroups and `full` where it fills the chip, and the time of its results, by a CU's rate or by the chip's. (us, fitted to
-// 60 products of 1 to 4096 tokens, 17 to 24576 channels, K 128 to 12288; there the choice is mostly within 5% of the best of
-// these kernels, at worst 13% behind it.)
-struct Shape {
-    int tile, at_once;
-    double fill, alone, full;
-    bool late;  // (nears `full` with the square of the round's part)
-};
-constexpr Shape shapes[] = {
-    {64, 512, 1.2, 0.18, 0.39, false},   // 9 places of 8 KiB, two workgroups a CU
-    {128, 256, 2.0, 0.36, 0.56, true},   // 9 places of 16 KiB
-    {128, 512, 1.2, 0.50, 1.09, false},  // 5 places of 16 KiB, two workgroups a CU
-    {256, 256, 5.0, 0.95, 1.60, false},  // 5 places of 32 KiB
-};
-struct Plan {
-    int shape, parts;  // shape -1: gemm8_few
-};
-Plan plan_of(const Gemm8Args &a) {
-    const double weights = 1.0 + (double)a.N * a.K / 5.0e6;  // reading them, at 5 TB/s
-    const int64_t few_wgs = (int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16);
-    // a CU takes in 98 GB/s; weights that several workgroups take come more slowly (a launch holds 2^32 threads)
-    const double a_cu = (few_wgs > 256 ? (double)few_wgs : 256.0) / 256.0;
-    const double few_us = 2.5 + a_cu * (0.2 + (16.0 + (a.M < 16 ? a.M : 16)) * a.K / 98e3);
-    const double few_weights = weights + (a.M > 16 ? 0.7 * a_cu : 0.0);
-    Plan best{-1, 1};
-    double best_us = few_wgs > 1 << 24 ? 1e9 : few_us > few_weights ? few_us : few_weights;
-    if (best_us <= weights) return best;  // (no other is faster than reading the weights)
-    for (int i = 0; i < 4; i++)
-        for (const int parts : {1, 2, 3, 4, 6, 8}) {
-            const Shape &s = shapes[i];
-            const int64_t wgs = (int64_t)((a.M + s.tile - 1) / s.tile) * ((a.N + s.tile - 1) / s.tile) * parts;
-            const int stages = ((a.K + KB - 1) / KB + parts - 1) / parts;
-            const double y = 4.0 * a.M * ((a.N + 3) / 4 * 4), touched = a.accum ? 2.0 : 1.0;
-            if (parts > 1 && (stages < 8 || parts * y > (double)(64 << 20))) break;
-            const double bytes = 4.0 * s.tile * s.tile * (parts > 1 ? 1.0 : touched);
-            const double one = bytes / 60e3, all = s.at_once * bytes / 5.0e6;
-            auto round = [&](double part) {
-                const double results = part < 1 ? one + (all > one ? all - one : 0.0) * part : all;
-                return s.fill + results + stages * (s.alone + (s.full - s.alone) * (s.late ? part * part : part));
-            };
-            const double rest = (double)(wgs % s.at_once) / s.at_once;
-            double us = 2.0 + (double)(wgs / s.at_once) * round(1.0) + (rest > 0 ? round(rest) : 0.0);
-            if (us < weights) us = weights;
-            if (parts > 1) us += 2.5 + y * (parts + touched) / 8.0e6;  // (the sums read again, and a launch more)
-            if (us < best_us) best_us = us, best = Plan{i, parts};
-        }
-    return best;
-}
-
 }  // namespace
 
-static size_t sums_bytes(const Gemm8Args &a, const Plan &p) {
+static size_t sums_bytes(const Gemm8Args &a, const Gemm8Plan &p) {
     return p.parts > 1 ? (size_t)p.parts * a.M * ((a.N + 3) / 4 * 4) * 4 : 0;
 }
+
+static Gemm8Plan plan_of(const Gemm8Args &a) { return gemm8_plan(a.M, a.N, a.K, a.accum); }
 
 size_t gemm8_ws(const Gemm8Args &a) { return sums_bytes(a, plan_of(a)); }
 
 // need: the workspace's bytes; with fewer given nothing is launched.
 hipError_t launch_gemm8(const Gemm8Args &a, void *ws, size_t ws_bytes, size_t *need, hipStream_t st) {
-    const Plan p = plan_of(a);
+    const Gemm8Plan p = plan_of(a);
     *need = sums_bytes(a, p);
     if (*need && (!ws || ws_bytes < *need || ((uintptr_t)ws & 15))) return hipErrorInvalidValue;
     if (p.shape < 0) {

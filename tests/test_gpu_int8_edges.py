@@ -3,9 +3,15 @@ import numpy as np
 import pytest
 
 import _i8ref as R
+from _i8plans import PLANS, TILE128X2
 from test_gpu_int8 import cu, ih, operands, rng, rows, same  # noqa: F401  (ih: the fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+def bits(t):
+    import torch
+    return t.contiguous().view(torch.int32)
 
 
 def rounded(q, s, w, ws):
@@ -71,3 +77,41 @@ def test_gates_far_below_zero(ih, m, k, far):  # noqa: F811
         gu[:, 1:k:9] = far
         gu[m - 1, k + 1::9] *= 1e3
         same(ih.silu_mul_i8(cu(gu)), R.quantize(R.silu_mul(gu)), 2 * R.HALF)
+
+
+@pytest.mark.parametrize("m,n,k,accum,kernel,parts", PLANS)
+def test_every_kernel_and_number_of_parts(ih, m, n, k, accum, kernel, parts):  # noqa: F811
+    """Products that end inside the tiles of each kernel, over K of several times its places in LDS, into rows that begin at any
+    value: the bits of the sum's rounding, the two scales' and the addition's. What lies beside the results stays."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(35 + m + k)
+    codes = lambda *s: torch.randint(-128, 128, s, dtype=torch.int8, device="cuda", generator=g)  # noqa: E731
+    scale = lambda c: torch.rand(c, device="cuda", generator=g) + 0.01  # noqa: E731
+    # (rows beside K: operands lie in wider ones, whose other values count for nothing)
+    q, w, s, ws = codes(m, k + 48)[:, 16:16 + k], codes(n, k + 16)[:, :k], scale(m), scale(n)
+    sums = torch.empty((m, n), device="cuda")
+    wt = w.double().T.contiguous()
+    for i in range(0, m, 512):
+        sums[i:i + 512] = (q[i:i + 512].double() @ wt).float()  # (whole numbers below 2^53: exact)
+    y = 1e4 * torch.randn((m + 2, n + 5), device="cuda", generator=g)
+    want = y.clone()
+    steps = sums * s[:, None] * ws
+    want[1:m + 1, 1:n + 1] = steps + y[1:m + 1, 1:n + 1] if accum else steps
+    space = torch.full((ih.gemm_i8_ws_bytes(m, n, k, accum) + 256,), 0x5a, dtype=torch.uint8, device="cuda")
+    ih.gemm_i8(q, s, w, ws, accum=accum, out=y[1:m + 1, 1:n + 1], ws=space[:-256])
+    assert (space.numel() > 256) == (parts > 1) and bool((space[-256:] == 0x5a).all())
+    bad = (bits(y) != bits(want)).nonzero()
+    assert not len(bad), (len(bad), bad[0].tolist(), bad[-1].tolist())
+
+
+def test_rows_alone_and_from_the_large_tiles(ih):  # noqa: F811
+    """A row's and a channel's results in tiles of 128 and 256 are the bits of calls on them alone."""
+    import torch
+    for m, n, k, accum, kernel, parts in PLANS:
+        if kernel < TILE128X2 or accum:
+            continue
+        q, s, w, ws = (cu(v) for v in operands(rng(36, m, k), m, n, k))
+        y = ih.gemm_i8(q, s, w, ws)
+        for i, j in ((1, n), (5, 700), (64, 1030), (300, 333), (m, 1)):
+            got = ih.gemm_i8(q[m - i:], s[m - i:], w[n - j:], ws[n - j:])
+            assert torch.equal(bits(got), bits(y[m - i:, n - j:])), (m, n, k, i, j)
