@@ -42,14 +42,13 @@ template <int N> __device__ __forceinline__ void meet() {
     asm volatile("" ::: "memory");
 }
 
-// Rows first .. of a matrix, as a buffer that ends behind its last row or behind `most` rows (empty past the last row).
+// Rows first .. of a matrix, as a buffer that ends behind its last row or behind `most` rows (first is one of its rows).
 struct Rows {
     const int8_t *p;
     int bytes;
 };
 __device__ __forceinline__ Rows rows_at(const int8_t *p, int64_t ld, int first, int rows, int most) {
-    int n = rows - first < most ? rows - first : most;
-    n = __builtin_amdgcn_readfirstlane(n < 0 ? 0 : n);  // (a scalar, or the loads would loop over its lanes)
+    const int n = __builtin_amdgcn_readfirstlane(rows - first < most ? rows - first : most);  // (or the loads would loop over lanes)
     return Rows{p + first * ld, n * (int)ld};
 }
 
