@@ -115,3 +115,43 @@ def test_rows_alone_and_from_the_large_tiles(ih):  # noqa: F811
         for i, j in ((1, n), (5, 700), (64, 1030), (300, 333), (m, 1)):
             got = ih.gemm_i8(q[m - i:], s[m - i:], w[n - j:], ws[n - j:])
             assert torch.equal(bits(got), bits(y[m - i:, n - j:])), (m, n, k, i, j)
+
+
+@pytest.mark.parametrize("m,k,weight", [(4200, 4112, True), (4200, 4112, False), (1027, 16384, True), (8200, 2064, True)])
+def test_norm_past_the_caches(ih, m, k, weight):  # noqa: F811
+    """The residual's addition and the norm of so many rows that they are read and written past the caches: every row's sums,
+    codes and scales. Among them rows whose values lie next to a tie, and rows whose largest products are equal in fp32 and not
+    in truth, made of halves that only the sum puts together."""
+    import torch
+    assert m * k >= 16 << 20
+    r = rng(34, m, k)
+    w = (1 + 0.3 * r.standard_normal(k)).astype(np.float32)
+    w[np.abs(w) < 0.05] = 1
+    if not weight:
+        w[:] = 1
+    x = rows(r, m, k)
+    add = r.standard_normal((m, k), dtype=np.float32)
+    planted = np.arange(3, m, m // 60)
+    for i in planted:
+        if i % 2:
+            top = np.float32(r.uniform(0.5, 200.0))
+            y = ((r.integers(-127, 127, k) + 0.5) * np.float64(top) / 127.0 / w).astype(np.float32)
+            y += (r.integers(-2, 3, k) * np.spacing(np.abs(y))).astype(np.float32)
+            y[7] = top / w[7]
+        else:
+            y = (np.float32(3.0) / w).astype(np.float32) * (r.integers(0, 2, k) * 2 - 1).astype(np.float32)
+        x[i] = add[i] = y / 2
+    xd, wd = cu(x), cu(w)
+    want_x = torch.from_numpy(x + add).cuda()
+    q, s = ih.rmsnorm_i8(xd, wd if weight else None, 1e-5, add=cu(add))
+    assert torch.equal(bits(xd), bits(want_x))
+    for i in range(0, m, 512):
+        t = want_x[i:i + 512].double()
+        factor = 1.0 / torch.sqrt((t * t).mean(-1) + 1e-5)
+        t = t * wd.double()
+        top = t.abs().amax(-1)
+        code = torch.round(t * 127.0 / top[:, None])
+        bad = (code != q[i:i + 512]).nonzero()
+        assert not len(bad), (len(bad), bad[0].tolist(), (bad[0] + torch.tensor([i, 0], device="cuda")).tolist())
+        scale = top / 127.0 * factor
+        assert bool(((s[i:i + 512].double() - scale).abs() <= R.norm_tol(k) * scale).all()), i
