@@ -629,8 +629,9 @@ int ihip_gated_delta_rule(const ihip_delta *a, void *ws, size_t ws_bytes,
  * in its last places with M, as mean(x'^2) is summed in fp32. A row of zeros has scale
  * 0 and codes 0; a row with a value that is not finite, or whose scale passes
  * fp32, has scale NaN and codes 0 (its products are NaN). K a multiple of 16 up
- * to 65536, M up to 2^23; x, norm_w, add and q 16-byte aligned, ldx and add_stride
- * multiples of 4, ldq of 16 and at least K (values past K are left as they were).
+ * to 65536, M up to 2^23 (past M K = 2^36 - 2^33 rows that take 2^32 threads are
+ * refused); x, norm_w, add and q 16-byte aligned, ldx and add_stride multiples of
+ * 4, ldq of 16 and at least K (values past K are left as they were).
  * q and scale overlap none of the inputs. No workspace. */
 int ihip_quantize_i8(const ihip_gemm_input *in, int M, int K, int8_t *q_dev,
                      int64_t ldq, float *scale_dev, void *stream);

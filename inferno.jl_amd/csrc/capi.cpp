@@ -78,6 +78,7 @@ hipError_t launch_attn(const AttnArgs &a, void *ws, hipStream_t st);
 size_t delta_ws(const DeltaArgs &a, bool snapshots);
 hipError_t launch_delta(const DeltaArgs &a, void *ws, hipStream_t st);
 // 8-bit projections (quant8.hip, gemm8.hip)
+bool quant8_fits(int M, int K);
 hipError_t launch_quant8(const Quant8Args &a, int act, hipStream_t st);
 size_t gemm8_ws(const Gemm8Args &a);
 hipError_t launch_gemm8(const Gemm8Args &a, void *ws, size_t ws_bytes, size_t *need, hipStream_t st);
@@ -1233,6 +1234,7 @@ int ihip_quantize_i8(const ihip_gemm_input *in, int M, int K, int8_t *q_dev, int
     if (act < IHIP_ACT_PLAIN || act > IHIP_ACT_SILU_MUL) return fail(IHIP_EINVAL, "%s: act=%d", fn, act);
     if (M < 1 || M > 1 << 23) return fail(IHIP_EINVAL, "%s: M=%d outside 1..2^23", fn, M);
     if (K < 16 || K > 65536 || K % 16) return fail(IHIP_EINVAL, "%s: K=%d (a multiple of 16 up to 65536)", fn, K);
+    if (!quant8_fits(M, K)) return fail(IHIP_EINVAL, "%s: M=%d rows of K=%d take 2^32 threads or more", fn, M, K);
     if (ldq < K || ldq % 16 || !aligned16(q_dev))
         return fail(IHIP_EINVAL, "%s: ldq=%lld (need >= %d, a multiple of 16; q 16-byte aligned)", fn, (long long)ldq, K);
     if ((uintptr_t)scale_dev & 3) return fail(IHIP_EINVAL, "%s: scale must be 4-byte aligned", fn);

@@ -329,12 +329,21 @@ template <int ACT, int V, bool STREAM = false> __global__ __launch_bounds__(1024
     if (tid == 0) a.scale[row] = row_scale(most, (double)ssq, ACT == Q8_RMSNORM, a.K, a.eps);
 }
 
-template <int ACT> void launch(const Quant8Args &a, hipStream_t st) {
-    const int n4 = a.K / 4;
+// How M rows of K values are cut: v times 4 values a thread (0: any number, read twice), nt threads a row.
+struct Cut {
+    int v, nt;
+};
+Cut cut_of(int M, int K) {
+    const int n4 = K / 4;
     // few values a thread where rows are few and a row's time is latency; four times 4 where they are many (8190 rows of 4096,
     // plain: 34 us, with one 83), as far as a wave has them
-    const int v = n4 > 4096 ? 0 : n4 > 2048 ? 4 : a.M <= 256 ? (n4 > 1024 ? 2 : 1) : n4 > 128 ? 4 : n4 > 64 ? 2 : 1;
-    const int nt = v ? ((n4 + v - 1) / v + 63) / 64 * 64 : 1024;
+    const int v = n4 > 4096 ? 0 : n4 > 2048 ? 4 : M <= 256 ? (n4 > 1024 ? 2 : 1) : n4 > 128 ? 4 : n4 > 64 ? 2 : 1;
+    return Cut{v, v ? ((n4 + v - 1) / v + 63) / 64 * 64 : 1024};
+}
+
+template <int ACT> void launch(const Quant8Args &a, hipStream_t st) {
+    const Cut cut = cut_of(a.M, a.K);
+    const int v = cut.v, nt = cut.nt;
     if constexpr (ACT == Q8_RMSNORM) {
         // rows that are read, added to and written past the caches, from 64 MB of them on (8190 of 4096: 75.7 us, 81.4 through
         // them; 515: 9.0 and 8.1)
@@ -350,6 +359,8 @@ template <int ACT> void launch(const Quant8Args &a, hipStream_t st) {
 }
 
 }  // namespace
+
+bool quant8_fits(int M, int K) { return (int64_t)M * cut_of(M, K).nt < (int64_t)1 << 32; }
 
 hipError_t launch_quant8(const Quant8Args &a, int act, hipStream_t st) {
     if (act == Q8_PLAIN) launch<Q8_PLAIN>(a, st);

@@ -82,3 +82,18 @@ def test_launches_at_the_limits(plan):
         wgs = -(-m // 16) * -(-n // 16) if kernel == FEW else -(-m // TILE[kernel]) * -(-n // TILE[kernel])
         assert wgs * (128 if kernel == FEW else 512) < 1 << 32, (m, n, k)
         assert parts == 1 or parts * m * ((n + 3) // 4) < 1 << 31, (m, n, k)
+
+
+def test_rows_at_the_limits():
+    """Rows of codes that a launch does not hold are refused by name, before any launch; those that it holds pass that check (and
+    are refused for a stride here)."""
+    lib, at = L.load(), (C.c_uint8 * 64)()
+    p = (C.addressof(at) + 15) & ~15
+    for m, k, fits in ((1 << 23, 7184, False), (1 << 23, 65536, False), (1 << 22, 16400, False), ((1 << 23) - 1, 7184, True),
+                       (1 << 23, 7168, True), (1 << 23, 16, True), ((1 << 22) - 1, 65536, True), (4300000, 14400, True)):
+        for act in (0, 1, 2):
+            a = L.GemmInput(p, 4, act, None, 1e-6, None, 0, 0)
+            assert lib.ihip_quantize_i8(C.byref(a), m, k, p, k, p, None) == -22
+            assert (b"2^32 threads" in lib.ihip_last_error()) == (not fits), (m, k, lib.ihip_last_error())
+            assert fits == (b"ldx=4" in lib.ihip_last_error())
+            assert fits or m * k > (1 << 36) - (1 << 33)
