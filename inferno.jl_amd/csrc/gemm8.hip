@@ -6,12 +6,14 @@
 // to fp32 once and multiplied by the two scales.
 //
 // What bounds it. Few tokens: reading the weights (gemm8_few: 1 x 24576 x 4096
-// in 16.8 us, 6.0 TB/s; 5 x 4096 x 12288 added to y 9.3 us, 5.4). Many: the
-// matrix cores and the clock that they leave (gemm8_tile: 4096 x 24576 x 4096 in
-// 376 to 382 us, 2.2 PFLOP/s at 1.9 GHz; their instructions alone would take 222
-// at 2.4). Between, what a CU takes in, 100 to 125 GB/s, and the rounds of
-// workgroups: 515 x 4096 x 4096 19 us, 64 x 12288 x 2048 7.4. Rows that do not
-// begin at multiples of 128 bytes cost the tiles 5 to 12 % (2 lines for 1).
+// in 16.8 us, 6.0 TB/s; 5 x 4096 x 12288 added to y 9.3 us, 5.4). Many: products,
+// at the rate of the library's (gemm8_tile: 4096 x 24576 x 4096 in 376 to 382 us,
+// the library 382, 2.2 PFLOP/s at 1.9 GHz). Their instructions hold a SIMD's
+// matrix core for 393216 cycles, 207 us at that clock and 164 at 2.4 GHz: it is
+// busy 56 % of the time, and what fills the rest was not found. Between, what a CU
+// takes in, 100 to 125 GB/s, and the rounds of workgroups: 515 x 4096 x 4096 19 us,
+// 64 x 12288 x 2048 7.4. Rows that do not begin at multiples of 128 bytes cost the
+// tiles 5 to 12 % (2 lines for 1).
 #include <type_traits>
 
 #include "common.h"

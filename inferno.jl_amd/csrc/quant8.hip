@@ -12,16 +12,18 @@
 //
 // Codes are those of the exact t, not of its fp32 rounding: t and 127 / top are
 // formed in fp32, and where 127 t / top comes nearer to a tie than their error
-// (a value in ten thousand) that one value is formed again in fp64. So codes do
-// not depend on how the fp32 arithmetic was ordered or contracted.
+// (a value in ten thousand, four of the gate's) that one value is formed again in
+// fp64. So codes do not depend on how the fp32 arithmetic was ordered or contracted.
 //
 // What bounds it. Many rows: memory. 8190 rows of 4096, the residual added and
 // stored, in 71 us (268 MB read, 168 written: 6.1 TB/s; a copy reaches 5.2),
 // 4096 plain rows of 12288 in 41 (6.2), 4097 gates of 6144 in 45 (5.1). Few: a
-// launch and one row's way, 2 us plain, 3.1 with the norm and the residual, and
-// a gate's vector instructions, 5.5 us for 12288 on one CU. One workgroup a row,
-// for a row's largest is one exchange through LDS then, and its values wait for
-// it in registers.
+// launch and one row's way, 2 us plain, 3.1 with the norm and the residual, 5.5
+// with 12288 gates on one CU. A gate's waves wait 71 % of their time and issue
+// vector instructions in 12 % (5 rows of 12288): for their loads, at two barriers,
+// and for gate and up read again behind the row's largest, where its exact value or
+// a code next to a tie is formed in fp64. One workgroup a row, for a row's largest
+// is one exchange through LDS then, and its values wait for it in registers.
 #include "common.h"
 #include "int8.h"
 

@@ -2,7 +2,8 @@
 stream, of [gate | up] or of the mixers' output as 8-bit codes with a scale for
 each row (the RMSNorm, gating and residual adds of src/ModelCPU.jl:110-122,
 :447-473, :870-891), and their products with 8-bit weights (:284-378), past the
-64 rows that gemm_q takes.
+64 rows that gemm_q takes. (Up to those, gemm_q on GGUF weights is about as fast
+or faster and more exact; these calls take any number of rows.)
 
 Kernels run on `stream` (default: torch's current one). What a call allocates
 itself (codes, scales, out, ws) is made for that stream; its inputs have to be
